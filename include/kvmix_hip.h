@@ -47,8 +47,14 @@ extern "C" {
 #define KVMIX_ERR_STATIC_SCRATCH (-13) /* kvmix_quantized_gemv_static: problem beyond the built-in buffer */
 #define KVMIX_ERR_STATIC_LOOKUP (-14)  /* kvmix_quantized_gemv_static: the built-in buffer's address could not be obtained */
 
+#define KVMIX_ERR_PAGE (-15)       /* a page number outside its pool */
+#define KVMIX_ERR_PAGE_ORDER (-16) /* kvmix_paged_copy: a page written twice, or written and read */
+#define KVMIX_ERR_LENGTHS (-17)    /* kvmix_paged_plan: lengths that do not fit one another or the table */
+#define KVMIX_ERR_MEMORY (-18)     /* host memory could not be had */
+
 #define KVMIX_F16 0
 #define KVMIX_F32 1
+#define KVMIX_BF16 2 /* kvmix_token_logprobs only */
 
 #define KVMIX_FMT_REF 0
 #define KVMIX_FMT_DENSE3 1
@@ -509,6 +515,124 @@ int kvmix_copy_rows(const kvmix_copy_rows_t *items, int count, kvmix_stream_t st
  */
 int kvmix_grow(const kvmix_copy_rows_t *copies, int count, const kvmix_key_flush_t *keys, const kvmix_value_flush_t *values,
                kvmix_stream_t stream);
+
+/*
+ * A cache in pages (no counterpart in the reference, whose cache is one batch of equal length grown by concatenation).
+ * A page holds page_size tokens (32, 64, ... 1024) of one layer for all kv heads; head_dim is 64 or 128.
+ *   rows    fp16 pages: [row_pages, kv_heads, 2, page_size * head_dim] halves: the keys [page_size][head_dim], and the values
+ *           as one [head_dim][32] matrix for every 32 tokens
+ *   packed  packed pages: [packed_pages, kv_heads, page_size / 32 blocks, head_dim * (k_bits + v_bits + 2)] 32-bit words.  A
+ *           block holds 32 tokens: key codes (head_dim * k_bits words), value codes (head_dim * v_bits words), then halves: the
+ *           keys' scale and minimum per channel (head_dim each), the values' scale and minimum per token and 32 channels
+ *           ([head_dim / 32][32 tokens] each).  Codes lie in the order of 64 lanes: lane 16 g + m has, of the keys, as piece
+ *           u * head_dim / 32 + s the channels 32 s + 8 g + (0..7) of token 8 (m / 4) + 4 u + m % 4, and of the values, as
+ *           piece t, the tokens 8 g + (0..7) of channel 16 t + m.  A lane's codes, piece by piece and two by two, fill
+ *           head_dim * bits / 64 words: pair p of a word has its codes at bits p * bits and p * bits + 16; with 3 bits five
+ *           pairs to a word, and pair 5 n + r (n words) takes bits 15 and 31 of the words 3 r, 3 r + 1, 3 r + 2, lowest first.
+ *           The words lie in runs of 4 (2, 1) per lane, as n is a multiple of 4 (2, 1).
+ * Codes, scales and minima are those of kvmix_quant_pack_last_dim in groups of 32 with KVMIX_SCALE_RECIPROCAL (3 bits: 0..7).
+ * Pool pointers are 16-byte aligned.  Lists of pages are host memory and travel with the launch.
+ */
+typedef struct kvmix_paged_pool {
+    void *rows;
+    int64_t row_pages;
+    void *packed;
+    int64_t packed_pages;
+    int64_t kv_heads, page_size, head_dim;
+    int k_bits, v_bits;         /* not read where only fp16 pages are meant */
+} kvmix_paged_pool_t;
+
+/* New tokens into fp16 pages: k, v [tokens, kv_heads, head_dim] fp16 (strides in elements, multiples of 8; 16-byte aligned),
+ * slots [tokens] device memory: page * page_size + place; a token whose slot is negative or outside the pool is not stored. */
+int kvmix_paged_append(const kvmix_paged_pool_t *pool, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                       int64_t v_token_stride, int64_t v_head_stride, const int32_t *slots, int64_t tokens, kvmix_stream_t stream);
+
+/* fp16 pages to packed pages: pairs [count][2] = (fp16 page, packed page); a packed page is named once at most
+ * (KVMIX_ERR_PAGE_ORDER). */
+int kvmix_paged_quantize(const kvmix_paged_pool_t *pool, const int32_t *pairs, int64_t count, kvmix_stream_t stream);
+
+/* The values of pages, packed ones or fp16 ones: k, v [count, page_size, kv_heads, head_dim] fp16, code * scale + minimum
+ * rounded once. */
+int kvmix_paged_read(const kvmix_paged_pool_t *pool, int packed, const int32_t *pages, int64_t count, void *k, void *v, kvmix_stream_t stream);
+
+/* Pages copied, the same pairs [count][2] = (source, destination) in every pool: pool i is [pages, page_bytes[i]] (multiples of
+ * 8).  No page may be written twice, or written and read (KVMIX_ERR_PAGE_ORDER): the copies are done in no order. */
+int kvmix_paged_copy(void *const *pools, const int64_t *page_bytes, int64_t n_pools, int64_t pages, const int32_t *pairs, int64_t count,
+                     kvmix_stream_t stream);
+
+/*
+ * The plan of one step of a batch, made on the host from its lengths and page tables and used by every layer of the step: which
+ * block of which launch takes which queries and keys, and where the new tokens go.
+ *   table [sequences][table_stride]: a sequence's pages; token t lies in page table[t / page_size], which is a packed page for
+ *   t < packed_lens (a multiple of page_size), an fp16 page from there on.  kv_lens: tokens with the new ones, the q_lens newest.
+ * With words NULL only `plan` is filled (its `words` is the capacity that is needed); with words the list as well, which the
+ * caller copies to the device.  Sequences of no tokens, and of no new ones, are allowed.
+ */
+typedef struct kvmix_paged_batch {
+    const int32_t *table;
+    int64_t table_stride;
+    const int64_t *kv_lens, *packed_lens, *q_lens;
+    int64_t sequences, heads, kv_heads, head_dim, page_size;
+} kvmix_paged_batch_t;
+
+typedef struct kvmix_paged_plan {
+    int64_t words;                               /* 32-bit words of the list */
+    int64_t tokens;                              /* new tokens of all sequences */
+    int64_t heads, kv_heads, head_dim, page_size, table_stride;
+    int64_t row_pages, packed_pages;             /* pages that the pools must have at least */
+    int64_t slots_at, seqs_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
+    int64_t few, tiles, joins;                   /* items per kv head: of a few query rows, of many, rows to be joined */
+    int64_t few_rows;                            /* query rows of an item of few: 16 or 32 */
+    int64_t part_rows;                           /* rows of partial results per kv head */
+} kvmix_paged_plan_t;
+int kvmix_paged_plan(const kvmix_paged_batch_t *batch, int32_t *words, int64_t capacity, kvmix_paged_plan_t *plan);
+
+/*
+ * Attention of a batch's new tokens over its pages:  out[i, h] = sum_{j <= pos(i)} softmax_j(scale q[i, h] . k[j, h']) v[j, h'],
+ * h' = h / (heads / kv_heads), over the tokens of i's own sequence up to itself (the new tokens' keys and values are in their
+ * pages already).  Packed values are taken as fp16 (code * scale + minimum, rounded once), logits, softmax and sums in fp32,
+ * probabilities rounded to fp16 for the product with the values and for its sum alike.
+ *   q, out [plan.tokens, heads, head_dim] fp16, unit stride along head_dim, strides in elements, multiples of 8; 16-byte aligned
+ *   list: the plan's words in device memory;  scale > 0
+ * What pages hold behind a sequence's last token is not used, whatever it is.
+ */
+typedef struct kvmix_paged_attn {
+    const void *q;
+    int64_t q_token_stride, q_head_stride;
+    void *out;
+    int64_t out_token_stride, out_head_stride;
+    const int32_t *list;
+    float scale;
+} kvmix_paged_attn_t;
+int64_t kvmix_paged_attention_workspace_bytes(const kvmix_paged_plan_t *plan);
+int kvmix_paged_attention(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t *plan, const kvmix_paged_attn_t *call, void *workspace,
+                          int64_t workspace_bytes, kvmix_stream_t stream);
+
+/*
+ * Log probabilities of given tokens under rows of logits (no counterpart in the reference):
+ *   logprob[r] = x[r, targets[r]] - lse_r,  entropy[r] = lse_r - sum_i p_i x[r, i],  lse_r = log sum_i exp x[r, i]
+ * and, where top > 0 (at most 64), the `top` most likely tokens of a row with their log probabilities, equal logits in the order
+ * of their indexes, NaN first.  A negative target is none: its log probability is 0; one past the vocabulary gives NaN.
+ * Statistics in fp32.  A row of -inf only, or with NaN or +inf, gives NaN.
+ *   logits [rows, vocab] fp16, bf16 or fp32, rows row_stride elements apart;  stats: NULL, or [rows, 4] for the gradient
+ * kvmix_token_logprobs_grad: the logits' gradient, in their type, from those of logprob and entropy (either may be NULL: zero);
+ * of `p` it reads logits, row_stride, targets, rows, vocab, dtype and stats.
+ */
+typedef struct kvmix_token_logprobs {
+    const void *logits;
+    int64_t row_stride, rows, vocab;
+    int dtype;
+    const int64_t *targets;
+    float *logprob, *entropy;
+    int64_t top;
+    float *top_logprob;  /* [rows, top] */
+    int64_t *top_id;     /* [rows, top] */
+    float *stats;
+} kvmix_token_logprobs_t;
+int64_t kvmix_token_logprobs_workspace_bytes(const kvmix_token_logprobs_t *p);
+int kvmix_token_logprobs(const kvmix_token_logprobs_t *p, void *workspace, int64_t workspace_bytes, kvmix_stream_t stream);
+int kvmix_token_logprobs_grad(const kvmix_token_logprobs_t *p, const float *grad_logprob, const float *grad_entropy, void *grad_logits,
+                              int64_t grad_row_stride, kvmix_stream_t stream);
 
 /*
  * Measurement support, no counterpart in the reference and not called by any operator: a kernel

@@ -47,6 +47,16 @@ EXPORTS = (
     "kvmix_copy_rows",
     "kvmix_grow",
     "kvmix_probe_stream_read",
+    "kvmix_paged_append",
+    "kvmix_paged_quantize",
+    "kvmix_paged_read",
+    "kvmix_paged_copy",
+    "kvmix_paged_plan",
+    "kvmix_paged_attention_workspace_bytes",
+    "kvmix_paged_attention",
+    "kvmix_token_logprobs_workspace_bytes",
+    "kvmix_token_logprobs",
+    "kvmix_token_logprobs_grad",
 )
 
 _lib = None
@@ -127,6 +137,20 @@ class PrefillAttn(ctypes.Structure):
         ("mask", _vp), ("mask_batch_stride", _i64), ("mask_head_stride", _i64), ("mask_row_stride", _i64), ("mask_batch", _i64),
         ("mask_heads", _i64), ("mask_dtype", _i32), ("batch", _i64), ("heads", _i64),
         ("kv_heads", _i64), ("q_len", _i64), ("kv_len", _i64), ("head_dim", _i64), ("scale", ctypes.c_float)]
+
+
+class PagedBatch(ctypes.Structure):
+    """kvmix_paged_batch_t"""
+    _i64, _vp = ctypes.c_int64, ctypes.c_void_p
+    _fields_ = [("table", _vp), ("table_stride", _i64), ("kv_lens", _vp), ("packed_lens", _vp), ("q_lens", _vp),
+                ("sequences", _i64), ("heads", _i64), ("kv_heads", _i64), ("head_dim", _i64), ("page_size", _i64)]
+
+
+class PagedPlan(ctypes.Structure):
+    """kvmix_paged_plan_t"""
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "words", "tokens", "heads", "kv_heads", "head_dim", "page_size", "table_stride", "row_pages", "packed_pages", "slots_at",
+        "seqs_at", "table_at", "few_at", "tile_at", "join_at", "few", "tiles", "joins", "few_rows", "part_rows")]
 
 
 LINEAR_PLAIN, LINEAR_FLOAT, LINEAR_RESIDUAL, LINEAR_SWIGLU, LINEAR_ROPE_APPEND = range(5)
@@ -219,6 +243,8 @@ def load() -> ctypes.CDLL:
     L.kvmix_copy_rows.argtypes = [vp, i32, vp]
     L.kvmix_grow.restype = i32
     L.kvmix_grow.argtypes = [vp, i32, ctypes.POINTER(KeyFlush), ctypes.POINTER(ValueFlush), vp]
+    L.kvmix_paged_plan.restype = i32
+    L.kvmix_paged_plan.argtypes = [ctypes.POINTER(PagedBatch), vp, i64, ctypes.POINTER(PagedPlan)]
     L.kvmix_probe_stream_read.restype = i32
     L.kvmix_probe_stream_read.argtypes = [vp, i32, i64, i64, i32, i32, i32, i32, i32, vp, vp]
     _lib = L
@@ -289,6 +315,23 @@ def attn_plan(step: DecodeAttn) -> dict:
             "slab_positions": plan.slab_positions, "slab_begin": plan.slab_begin, "slabs": plan.slabs,
             "slab_blocks": plan.slab_blocks, "matrix_grid": tuple(plan.matrix_grid),
             "matrix_block": tuple(plan.matrix_block)}
+
+
+def paged_plan(table, kv_lens, packed_lens, q_lens, heads: int, kv_heads: int, head_dim: int, page_size: int):
+    """kvmix_paged_plan: (the plan's fields as a dict, its words as a list of int).  table: one list of pages per sequence, all of
+    one length.  Needs no GPU."""
+    n, stride = len(table), len(table[0]) if table else 0
+    cells = [c for row in table for c in row]
+    lens = [(ctypes.c_int64 * max(n, 1))(*x) for x in (kv_lens, packed_lens, q_lens)]
+    batch, plan = PagedBatch(), PagedPlan()
+    pages = (ctypes.c_int32 * max(len(cells), 1))(*cells)
+    batch.table, batch.table_stride = ctypes.addressof(pages), stride
+    batch.kv_lens, batch.packed_lens, batch.q_lens = (ctypes.addressof(x) for x in lens)
+    batch.sequences, batch.heads, batch.kv_heads, batch.head_dim, batch.page_size = n, heads, kv_heads, head_dim, page_size
+    check(load().kvmix_paged_plan(ctypes.byref(batch), None, 0, ctypes.byref(plan)))
+    words = (ctypes.c_int32 * max(plan.words, 1))()
+    check(load().kvmix_paged_plan(ctypes.byref(batch), words, plan.words, ctypes.byref(plan)))
+    return {name: getattr(plan, name) for name, _ in PagedPlan._fields_}, list(words)
 
 
 def flush_batch(keys, values, stream) -> int:

@@ -28,6 +28,12 @@ extern "C" const char *kvmix_strerror(int code)
     case KVMIX_ERR_STATIC_LOOKUP:
         return "the address of kvmix_quantized_gemv_static's built-in buffer could not be obtained on this device "
                "(hipGetSymbolAddress failed): use kvmix_quantized_gemv with a caller-owned workspace";
+    case KVMIX_ERR_PAGE: return "a page number lies outside its pool";
+    case KVMIX_ERR_PAGE_ORDER: return "pages are copied in no order: a page must not be written twice, or written and read";
+    case KVMIX_ERR_LENGTHS:
+        return "lengths of a sequence do not fit: 0 <= new tokens <= tokens, 0 <= packed tokens <= tokens in whole pages, new tokens "
+               "not packed, pages for all tokens in the table";
+    case KVMIX_ERR_MEMORY: return "host memory could not be had";
     default: return "unknown kvmix error";
     }
 }

@@ -44,6 +44,16 @@ struct Api {
     decltype(&kvmix_copy_rows) copy_rows;
     decltype(&kvmix_grow) grow;
     decltype(&kvmix_linear_rows) linear_rows;
+    decltype(&kvmix_paged_append) paged_append;
+    decltype(&kvmix_paged_quantize) paged_quantize;
+    decltype(&kvmix_paged_read) paged_read;
+    decltype(&kvmix_paged_copy) paged_copy;
+    decltype(&kvmix_paged_plan) paged_plan;
+    decltype(&kvmix_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
+    decltype(&kvmix_paged_attention) paged_attention;
+    decltype(&kvmix_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
+    decltype(&kvmix_token_logprobs) token_logprobs;
+    decltype(&kvmix_token_logprobs_grad) token_logprobs_grad;
 } api;
 
 void bind(const std::unordered_map<std::string, uintptr_t> &at)
@@ -66,6 +76,16 @@ void bind(const std::unordered_map<std::string, uintptr_t> &at)
     KVMIX_BIND(copy_rows);
     KVMIX_BIND(grow);
     KVMIX_BIND(linear_rows);
+    KVMIX_BIND(paged_append);
+    KVMIX_BIND(paged_quantize);
+    KVMIX_BIND(paged_read);
+    KVMIX_BIND(paged_copy);
+    KVMIX_BIND(paged_plan);
+    KVMIX_BIND(paged_attention_workspace_bytes);
+    KVMIX_BIND(paged_attention);
+    KVMIX_BIND(token_logprobs_workspace_bytes);
+    KVMIX_BIND(token_logprobs);
+    KVMIX_BIND(token_logprobs_grad);
 #undef KVMIX_BIND
 }
 
@@ -760,6 +780,8 @@ Tensor qkv_rope_append(const Tensor &x_in, const std::vector<Tensor> &ws, int64_
     return q;
 }
 
+#include "host_paged.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m)
@@ -780,4 +802,17 @@ PYBIND11_MODULE(_host, m)
     m.def("linear_rows", &linear_rows, NoGil());
     m.def("swiglu_rows", &swiglu_rows, NoGil());
     m.def("qkv_rope_append", &qkv_rope_append, NoGil());
+    py::class_<PagedPlan>(m, "PagedPlan", "The plan of one step of a batch (ops.paged_plan).")
+        .def_property_readonly("tokens", [](const PagedPlan &p) { return p.c.tokens; })
+        .def_property_readonly("slots", [](const PagedPlan &p) { return p.slots(); })
+        .def_property_readonly("device", [](const PagedPlan &p) { return p.list.device(); })
+        .def_property_readonly("launches", [](const PagedPlan &p) { return std::make_tuple(p.c.few, p.c.tiles, p.c.joins); });
+    m.def("paged_plan", &paged_plan, NoGil());
+    m.def("paged_append", &paged_append, NoGil());
+    m.def("paged_quantize", &paged_quantize, NoGil());
+    m.def("paged_read", &paged_read, NoGil());
+    m.def("paged_copy", &paged_copy, NoGil());
+    m.def("paged_attention", &paged_attention, NoGil());
+    m.def("token_logprobs", &token_logprobs, NoGil());
+    m.def("token_logprobs_grad", &token_logprobs_grad, NoGil());
 }

@@ -1,0 +1,717 @@
+// Attention of a batch's newest tokens, one or many of each sequence, over its paged cache: packed pages first, fp16 pages after
+// them (paged_common.h).  out_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j of i's sequence up to itself; one pass
+// over the tokens with a running maximum and sum, values of codes in registers or in the LDS only.
+//
+// The query heads of a kv head and the new tokens of a sequence are the rows of one problem: row r is token r / G, head r % G of
+// the group.  Sequences of few rows go to paged_few (bound by the reads of the cache), the others to paged_tile (bound by the
+// matrix cores and the vector ALU beside them); both take spans of a sequence, so that a long one with few rows fills the chip,
+// and paged_join puts the spans together.  Who takes what is decided on the host, once for all layers of a step
+// (kvmix_paged_plan): lengths that differ within a batch then cost no idle blocks.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "paged_common.h"
+
+namespace kvmix {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr int kItemWords = 6;  // sequence, first row, rows, first and last block (tile), part (-1: the whole sequence)
+constexpr int kSeqWords = 4;   // first new token, new tokens, tokens, packed tokens
+constexpr int kTileRows = 128, kTileKeys = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct PagedArgs {
+    const _Float16 *q;
+    _Float16 *out;
+    int64_t q_ts, q_hs, o_ts, o_hs;
+    const _Float16 *rows;
+    const uint32_t *packed;
+    const int32_t *seqs, *table, *items;
+    int table_stride, kv_heads, group, blocks_log2;  // blocks_log2: of 32 tokens to a page
+    float scale;                                     // with log2(e)
+    float *part;                                     // [kv heads][part_rows][D], relative to the maximum in part_ml
+    float2 *part_ml;                                 // [kv heads][part_rows] maximum (of log2) and sum
+    int64_t part_rows;
+};
+
+struct PagedItem {
+    int seq, row0, rows, begin, end, part;
+};
+
+__device__ __forceinline__ PagedItem item_of(const int32_t *items, int nth)
+{
+    const int32_t *p = items + nth * kItemWords;
+    return {p[0], p[1], p[2], p[3], p[4], p[5]};
+}
+
+// the larger of a lane's and those of the lanes with its place in the other rows of sixteen
+__device__ __forceinline__ float max_of_rows(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+__device__ __forceinline__ float sum_of_rows(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// A packed block as a lane holds it: its codes, and its share of the scales and minima, which go through the LDS to the lanes
+// that need them (each is wanted by sixteen).
+template <int D, int KB, int VB>
+struct PackedBlock {
+    uint32_t k[lane_words(D, KB)], v[lane_words(D, VB)], side[D / 32];
+};
+
+template <int D, int KB, int VB>
+__device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uint32_t *at, int lane)
+{
+    load_words<lane_words(D, KB)>(at, lane, b.k);
+    load_words<lane_words(D, VB)>(at + D * KB, lane, b.v);
+    load_words<D / 32>(at + D * (KB + VB), lane, b.side);
+}
+
+// Few rows.  Every wave of a block takes every fourth block of 32 tokens of the item's span, sixteen (NR times) rows of queries
+// at once, with v_mfma_f32_16x16x32: the logits transposed (tokens as rows of the result), so that a lane holds those of one query
+// and its probabilities are the operand of out^T = v^T p^T as they are.  Codes go from memory to registers, a block ahead, become
+// fp16 there and are used once.
+template <int D, int KB, int VB, int NR>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_few(PagedArgs a)
+{
+    constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
+    constexpr int kPad = D + 4;
+    __shared__ union {
+        uint32_t side[4][2 * D];
+        struct {
+            float out[4][16 * NR][kPad];
+            float2 ml[4][16 * NR];
+        } join;
+    } lds;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
+    const int head = blockIdx.x % a.kv_heads;
+    const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
+    const int32_t *seq = a.seqs + it.seq * kSeqWords;
+    const int q_start = seq[0], q_len = seq[1], kv_len = seq[2], packed = seq[3];
+    const int32_t *table = a.table + it.seq * a.table_stride;
+    const int per_page = 1 << a.blocks_log2;
+
+    half8v q[NR][KS];
+    int limit[NR];  // the row's own token
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const int r = it.row0 + min(16 * n + m, it.rows - 1), token = r / a.group;
+        limit[n] = kv_len - q_len + token;
+        const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * g;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[n][s] = *(const half8v *)(at + 32 * s);
+    }
+    const int first_limit = kv_len - q_len + it.row0 / a.group;
+
+    floatx4 acc[NR][DT];
+    float top[NR], sum[NR];
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        top[n] = -1e30f, sum[n] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; t++) acc[n][t] = floatx4{};
+    }
+
+    // a block's logits to probabilities; the maximum is moved when some row's has grown by more than 2^8 (they stay well inside
+    // fp16's range below that)
+    auto probabilities = [&](floatx4 (&x)[2][NR], half8v (&p)[NR], int block) {
+        if (block * kBlock + kBlock - 1 > first_limit) {
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (block * kBlock + 8 * g + i > limit[n]) x[i / 4][n][i % 4] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            float most = x[0][n][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) most = fmaxf(most, x[i / 4][n][i % 4]);
+            most *= a.scale;
+            if (__any(most > top[n] + 8.0f)) {
+                const float grown = fmaxf(top[n], max_of_rows(most));
+                const float shrink = __builtin_amdgcn_exp2f(top[n] - grown);
+                top[n] = grown;
+                sum[n] *= shrink;
+#pragma unroll
+                for (int t = 0; t < DT; t++) acc[n][t] *= shrink;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[i / 4][n][i % 4], a.scale, -top[n]));
+                if (i % 2) sum[n] = __builtin_amdgcn_fdot2(half2v{p[n][i - 1], p[n][i]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum[n], false);
+            }
+        }
+    };
+
+    auto take_packed = [&](const PackedBlock<D, KB, VB> &b, int block) {
+        uint32_t *side = lds.side[wave];
+        store_words<D / 32>(side, lane, b.side);
+        __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+        const _Float16 *sides = (const _Float16 *)side + 8 * g;
+        floatx4 x[2][NR] = {};
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const half8v scale = *(const half8v *)(sides + 32 * s), zero = *(const half8v *)(sides + D + 32 * s);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8v k = piece_values<KB, NK>(b.k, u * KS + s, scale, zero);
+#pragma unroll
+                for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+            }
+        }
+        half8v p[NR];
+        probabilities(x, p, block);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const half8v scale = *(const half8v *)(sides + 2 * D + 32 * s), zero = *(const half8v *)(sides + 3 * D + 32 * s);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8v v = piece_values<VB, NV>(b.v, 2 * s + u, scale, zero);
+#pragma unroll
+                for (int n = 0; n < NR; n++) acc[n][2 * s + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n], acc[n][2 * s + u], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+
+    const int packed_end = min(it.end, packed / kBlock);
+    auto packed_at = [&](int block) {
+        const int64_t page = table[block >> a.blocks_log2];
+        return a.packed + (((page * a.kv_heads + head) << a.blocks_log2) + (block & (per_page - 1))) * block_words(D, KB, VB);
+    };
+    int block = it.begin + wave;
+    if (block < packed_end) {
+        PackedBlock<D, KB, VB> one, two;
+        load_packed(one, packed_at(block), lane);
+        while (true) {
+            if (block + 4 < packed_end) load_packed(two, packed_at(block + 4), lane);
+            take_packed(one, block);
+            block += 4;
+            if (block >= packed_end) break;
+            if (block + 4 < packed_end) load_packed(one, packed_at(block + 4), lane);
+            take_packed(two, block);
+            block += 4;
+            if (block >= packed_end) break;
+        }
+    }
+    for (; block < it.end; block += 4) {
+        const int64_t page = table[block >> a.blocks_log2];
+        const int64_t P = kBlock << a.blocks_log2;
+        const _Float16 *keys = a.rows + (page * a.kv_heads + head) * 2 * P * D + (block & (per_page - 1)) * kBlock * D;
+        const _Float16 *values = keys + P * D;
+        floatx4 x[2][NR] = {};
+        half8v v[DT];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8v k = *(const half8v *)(keys + (8 * (m / 4) + 4 * u + m % 4) * D + 32 * s + 8 * g);
+                v[2 * s + u] = *(const half8v *)(values + (16 * (2 * s + u) + m) * kBlock + 8 * g);
+#pragma unroll
+                for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+            }
+        }
+        half8v p[NR];
+        probabilities(x, p, block);
+        if (block * kBlock + kBlock > kv_len) {  // (whatever lies behind the last token: zero times it may not be zero)
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (block * kBlock + 8 * g + j >= kv_len) v[t][j] = (_Float16)0.0f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < DT; t++) {
+#pragma unroll
+            for (int n = 0; n < NR; n++) acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], p[n], acc[n][t], 0, 0, 0);
+        }
+    }
+
+    // the four waves' sums together
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const float total = sum_of_rows(sum[n]);
+        if (g == 0) lds.join.ml[wave][16 * n + m] = make_float2(top[n], total);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        float most = top[n];
+#pragma unroll
+        for (int w = 0; w < 4; w++) most = fmaxf(most, lds.join.ml[w][16 * n + m].x);
+        const float shrink = __builtin_amdgcn_exp2f(top[n] - most);
+#pragma unroll
+        for (int t = 0; t < DT; t++) *(floatx4 *)&lds.join.out[wave][16 * n + m][16 * t + 4 * g] = acc[n][t] * shrink;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < it.rows * (D / 8); i += 256) {
+        const int r = i / (D / 8), c = i % (D / 8) * 8;
+        float most = lds.join.ml[0][r].x, total = 0.0f;
+#pragma unroll
+        for (int w = 1; w < 4; w++) most = fmaxf(most, lds.join.ml[w][r].x);
+        floatx4 o[2] = {};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            total += lds.join.ml[w][r].y * __builtin_amdgcn_exp2f(lds.join.ml[w][r].x - most);
+            o[0] += *(const floatx4 *)&lds.join.out[w][r][c];
+            o[1] += *(const floatx4 *)&lds.join.out[w][r][c + 4];
+        }
+        if (it.part >= 0) {
+            const int64_t to = head * a.part_rows + it.part + r;
+            *(floatx4 *)(a.part + to * D + c) = o[0];
+            *(floatx4 *)(a.part + to * D + c + 4) = o[1];
+            if (c == 0) a.part_ml[to] = make_float2(most, total);
+        } else {
+            const float inv = 1.0f / total;
+            half8v w;
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = (_Float16)(o[j / 4][j % 4] * inv);
+            const int token = (it.row0 + r) / a.group, h = head * a.group + (it.row0 + r) % a.group;
+            *(half8v *)(a.out + (int64_t)(q_start + token) * a.o_ts + (int64_t)h * a.o_hs + c) = w;
+        }
+    }
+}
+
+// Where the pieces of a tile lie in the LDS, so that neither side has bank conflicts: keys [64][D] and values [D][64], 16-byte
+// pieces exchanged by the row's low bits.
+template <int D>
+__device__ __forceinline__ int tile_key(int key, int c)
+{
+    return D == 128 ? key * 256 + ((c ^ (key & 15)) << 4) : key * 128 + ((c ^ ((key >> 1) & 7)) << 4);
+}
+
+__device__ __forceinline__ int tile_value(int channel, int c) { return channel * 128 + ((c ^ ((channel >> 1) & 7)) << 4); }
+
+// Many rows: 128 of them to a block, 32 to a wave, over tiles of 64 tokens.  A tile is four matrices of 32 tokens, keys and values
+// of two blocks; each wave turns one of them from codes to fp16, for all four.  Products with v_mfma_f32_32x32x16: logits
+// transposed, keys as rows in an order in which a lane's logits are those of eight tokens that follow one another, as the
+// values' pieces are.
+template <int D, int KB, int VB>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) paged_tile(PagedArgs a)
+{
+    constexpr int KS = D / 16, DT = D / 32, NP = D / 16;
+    constexpr int kBytes = kTileKeys * D * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kBytes];
+    __shared__ uint32_t sides[4][D];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane & 31, h2 = lane >> 5;
+    const int m = lane % 16, g = lane / 16;
+    const int head = blockIdx.x % a.kv_heads;
+    const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
+    const int32_t *seq = a.seqs + it.seq * kSeqWords;
+    const int q_start = seq[0], q_len = seq[1], kv_len = seq[2], packed_blocks = seq[3] / kBlock, blocks = (kv_len + kBlock - 1) / kBlock;
+    const int32_t *table = a.table + it.seq * a.table_stride;
+    const int per_page = 1 << a.blocks_log2;
+
+    const int own = 32 * wave + col, r = it.row0 + min(own, it.rows - 1), token = r / a.group, limit = kv_len - q_len + token;
+    const int wave_first = kv_len - q_len + (it.row0 + min(32 * wave, it.rows - 1)) / a.group;
+    const int wave_last = 32 * wave < it.rows ? kv_len - q_len + (it.row0 + min(32 * wave + 31, it.rows - 1)) / a.group : -1;
+    half8v q[KS];
+    {
+        const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * h2;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *(const half8v *)(at + 16 * s);
+    }
+
+    // This wave's matrix of a tile: on its way from memory in `held`, then into the LDS.
+    const int matrix = wave & 1, which = wave >> 1;
+    uint32_t held[4 * NP], side[D / 64];
+    auto fetch = [&](int tile) {
+        const int block = 2 * tile + which;
+        if (block >= blocks) return;
+        const int64_t page = table[block >> a.blocks_log2];
+        const int in_page = block & (per_page - 1);
+        if (block < packed_blocks) {
+            const uint32_t *at = a.packed + (((page * a.kv_heads + head) << a.blocks_log2) + in_page) * block_words(D, KB, VB);
+            if (matrix) load_words<lane_words(D, VB)>(at + D * KB, lane, held);
+            else load_words<lane_words(D, KB)>(at, lane, held);
+            load_words<D / 64>(at + D * (KB + VB) + matrix * D, lane, side);
+        } else {
+            const int64_t P = kBlock << a.blocks_log2;
+            const _Float16 *at = a.rows + (page * a.kv_heads + head) * 2 * P * D + (matrix ? P * D : 0) + (int64_t)in_page * kBlock * D;
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                const int off = matrix ? (16 * p + m) * kBlock + 8 * g : (8 * (m / 4) + 4 * (p / (D / 32)) + m % 4) * D + 32 * (p % (D / 32)) + 8 * g;
+                *(uint4v *)&held[4 * p] = *(const uint4v *)(at + off);
+            }
+        }
+    };
+    auto place = [&](int tile, int buf) {
+        const int block = 2 * tile + which;
+        uint8_t *to = lds[buf][matrix];
+        auto put = [&](int p, half8v x) {
+            const int at = matrix ? tile_value(16 * p + m, 4 * which + g)
+                                  : tile_key<D>(kBlock * which + 8 * (m / 4) + 4 * (p / (D / 32)) + m % 4, 4 * (p % (D / 32)) + g);
+            *(half8v *)(to + at) = x;
+        };
+        if (block < packed_blocks) {
+            store_words<D / 64>(sides[wave], lane, side);
+            __builtin_amdgcn_wave_barrier();
+            const _Float16 *s = (const _Float16 *)sides[wave] + 8 * g;
+            auto turn = [&](auto bits) {
+                constexpr int B = decltype(bits)::value;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    const int set = matrix ? p / 2 : p % (D / 32);
+                    put(p, piece_values<B, lane_words(D, B)>(held, p, *(const half8v *)(s + 32 * set), *(const half8v *)(s + D + 32 * set)));
+                }
+            };
+            if (matrix) turn(std::integral_constant<int, VB>());
+            else turn(std::integral_constant<int, KB>());
+            __builtin_amdgcn_wave_barrier();
+        } else if (block < blocks) {
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                half8v x = __builtin_bit_cast(half8v, *(const uint4v *)&held[4 * p]);
+                if (matrix && block * kBlock + kBlock > kv_len) {  // (zero times what lies behind the last token may not be zero)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (block * kBlock + 8 * g + j >= kv_len) x[j] = (_Float16)0.0f;
+                }
+                put(p, x);
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < NP; p++) put(p, half8v{});
+        }
+    };
+
+    // where a lane reads: keys row R of 32 as token R with its bits 2 and 3 exchanged
+    const int k_row = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
+    floatx16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = floatx16{};
+    float top = -1e30f, sum = 0.0f;
+
+    fetch(it.begin);
+    place(it.begin, 0);
+    if (it.begin + 1 < it.end) fetch(it.begin + 1);
+    __syncthreads();
+    int buf = 0;
+    for (int tile = it.begin; tile < it.end; tile++) {
+        if (tile + 1 < it.end) place(tile + 1, buf ^ 1);  // (that buffer was last read before the barrier that ended the turn before)
+        if (tile + 2 < it.end) fetch(tile + 2);
+        const int k0 = tile * kTileKeys;
+        if (k0 <= wave_last) {
+            floatx16 x[2] = {floatx16{}, floatx16{}};
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const half8v k = *(const half8v *)(lds[buf][0] + tile_key<D>(32 * t + k_row, 2 * s + h2));
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], x[t], 0, 0, 0);
+                }
+            }
+            // x[t][8 kk + j] is the logit of token 32 t + 16 kk + 8 h2 + j
+            if (k0 + kTileKeys - 1 > wave_first) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (k0 + 32 * (i / 16) + 16 * (i % 16 / 8) + 8 * h2 + i % 8 > limit) x[i / 16][i % 16] = -__builtin_inff();
+            }
+            float most = x[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; i++) most = fmaxf(most, x[i / 16][i % 16]);
+            {
+                const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+                most = fmaxf(__uint_as_float(e[0]), __uint_as_float(e[1])) * a.scale;
+            }
+            if (__any(most > top + 8.0f)) {
+                const float grown = fmaxf(top, most), shrink = __builtin_amdgcn_exp2f(top - grown);
+                top = grown;
+                sum *= shrink;
+#pragma unroll
+                for (int t = 0; t < DT; t++) o[t] *= shrink;
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) {
+                half8v p;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[j] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[kk / 2][8 * (kk % 2) + j], a.scale, -top));
+                    if (j % 2) sum = __builtin_amdgcn_fdot2(half2v{p[j - 1], p[j]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                }
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    const half8v v = *(const half8v *)(lds[buf][1] + tile_value(32 * t + col, 2 * kk + h2));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[t], 0, 0, 0);
+                }
+            }
+        }
+        buf ^= 1;
+        __syncthreads();
+    }
+    if (own >= it.rows) return;
+    {
+        const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(e[0]) + __uint_as_float(e[1]);
+    }
+    if (it.part >= 0) {
+        const int64_t to = head * a.part_rows + it.part + own;
+#pragma unroll
+        for (int t = 0; t < DT; t++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(floatx4 *)(a.part + to * D + 32 * t + 8 * i + 4 * h2) = floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+        }
+        if (h2 == 0) a.part_ml[to] = make_float2(top, sum);
+        return;
+    }
+    typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+    const float inv = 1.0f / sum;
+    _Float16 *to = a.out + (int64_t)(q_start + token) * a.o_ts + (int64_t)(head * a.group + r % a.group) * a.o_hs + 4 * h2;
+#pragma unroll
+    for (int t = 0; t < DT; t++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            half4v w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = (_Float16)(o[t][4 * i + j] * inv);
+            *(half4v *)(to + 32 * t + 8 * i) = w;
+        }
+    }
+}
+
+// The spans of one sequence's rows together: a row per wave; the item's `begin` is the number of spans, `end` the rows between them.
+template <int D>
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a)
+{
+    constexpr int PER = D / kWave;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int head = blockIdx.x % a.kv_heads;
+    const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
+    const int q_start = a.seqs[it.seq * kSeqWords];
+    for (int r = blockIdx.y * 4 + wave; r < it.rows; r += 4 * gridDim.y) {
+        const int64_t first = head * a.part_rows + it.part + r;
+        float most = -1e30f;
+        for (int i = lane; i < it.begin; i += kWave) most = fmaxf(most, a.part_ml[first + (int64_t)i * it.end].x);
+        most = wave_reduce<true>(most);
+        float total = 0.0f, o[PER] = {};
+        for (int i = 0; i < it.begin; i++) {
+            const int64_t at = first + (int64_t)i * it.end;
+            const float2 ml = a.part_ml[at];
+            const float w = __builtin_amdgcn_exp2f(ml.x - most);
+            total = fmaf(ml.y, w, total);
+#pragma unroll
+            for (int j = 0; j < PER; j++) o[j] = fmaf(a.part[at * D + PER * lane + j], w, o[j]);
+        }
+        const float inv = 1.0f / total;
+        const int row = it.row0 + r;
+        _Float16 *to = a.out + (int64_t)(q_start + row / a.group) * a.o_ts + (int64_t)(head * a.group + row % a.group) * a.o_hs + PER * lane;
+#pragma unroll
+        for (int j = 0; j < PER; j++) to[j] = (_Float16)(o[j] * inv);
+    }
+}
+
+namespace {
+
+constexpr int64_t kFewMost = 32;      // rows of a sequence and kv head that go to paged_few
+constexpr int64_t kFewLaunch = 1024;  // blocks that its launch aims at ...
+constexpr int64_t kFewSpan = 8;       // ... of that many blocks of tokens at least
+constexpr int64_t kTileLaunch = 1024;
+constexpr int64_t kTileSpan = 8;      // tiles
+
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+struct Span {
+    int32_t word[kItemWords];
+    int64_t cost;
+};
+
+int batch_check(const kvmix_paged_batch_t *b)
+{
+    if (!b) return KVMIX_ERR_NULL;
+    if (b->sequences < 0 || b->heads <= 0 || b->kv_heads <= 0 || b->table_stride < 0) return KVMIX_ERR_SHAPE;
+    if (b->heads % b->kv_heads != 0) return KVMIX_ERR_HEADS;
+    if ((b->head_dim != 64 && b->head_dim != 128) || !page_size_ok(b->page_size) || b->kv_heads > kMostHeads || b->heads > (1 << 20) ||
+        b->sequences > (1 << 20) || (__int128)b->sequences * b->table_stride > (1 << 28))
+        return KVMIX_ERR_UNSUPPORTED;
+    if (b->sequences && (!b->kv_lens || !b->packed_lens || !b->q_lens || (!b->table && b->table_stride))) return KVMIX_ERR_NULL;
+    return KVMIX_OK;
+}
+
+int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kvmix_paged_plan_t *plan)
+{
+    const int64_t G = b->heads / b->kv_heads, P = b->page_size, kMostTokens = int64_t(1) << 30;
+    *plan = kvmix_paged_plan_t{};
+    plan->heads = b->heads, plan->kv_heads = b->kv_heads, plan->head_dim = b->head_dim, plan->page_size = P;
+    plan->table_stride = b->table_stride;
+    int64_t few_cost = 0, tile_cost = 0;
+    plan->few_rows = 16;
+    for (int64_t s = 0; s < b->sequences; s++) {
+        const int64_t kv = b->kv_lens[s], pk = b->packed_lens[s], n = b->q_lens[s];
+        if (n < 0 || n > kv || pk < 0 || pk % P != 0 || pk > kv - n || (kv + P - 1) / P > b->table_stride) return KVMIX_ERR_LENGTHS;
+        if (kv > kMostTokens || n * G > kMostTokens || plan->tokens + n > kMostTokens) return KVMIX_ERR_UNSUPPORTED;
+        const int32_t *row = b->table + s * b->table_stride;
+        for (int64_t i = 0; i * P < kv; i++) {
+            if (row[i] < 0) return KVMIX_ERR_PAGE;
+            int64_t &most = i * P < pk ? plan->packed_pages : plan->row_pages;
+            most = std::max<int64_t>(most, row[i] + int64_t(1));
+        }
+        plan->tokens += n;
+        if (n * G <= kFewMost) {
+            few_cost += n ? (kv + kBlock - 1) / kBlock : 0;
+            if (n * G > 16) plan->few_rows = kFewMost;
+        } else {
+            for (int64_t r = 0; r < n * G; r += kTileRows)
+                tile_cost += (kv - n + std::min(n * G - 1, r + kTileRows - 1) / G) / kTileKeys + 1;
+        }
+    }
+    if ((__int128)plan->row_pages * P > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    const int64_t few_span = std::max(kFewSpan, up((few_cost * b->kv_heads + kFewLaunch - 1) / kFewLaunch, 4));
+    const int64_t tile_span = std::max(kTileSpan, (tile_cost * b->kv_heads + kTileLaunch - 1) / kTileLaunch);
+
+    std::vector<Span> few, tiles, joins;
+    int64_t part = 0;
+    auto cut = [&](std::vector<Span> &to, int64_t s, int64_t row0, int64_t rows, int64_t length, int64_t span, int64_t stride) {
+        const int64_t spans = (length + span - 1) / span, even = (length + spans - 1) / spans;
+        for (int64_t i = 0; i < spans; i++) {
+            const int64_t from = std::min(i * even, length), to_ = std::min(from + even, length);
+            to.push_back({{(int32_t)s, (int32_t)row0, (int32_t)rows, (int32_t)from, (int32_t)to_, spans > 1 ? (int32_t)(part + i * stride) : -1}, to_ - from});
+        }
+        if (spans > 1) {
+            joins.push_back({{(int32_t)s, (int32_t)row0, (int32_t)rows, (int32_t)spans, (int32_t)stride, (int32_t)part}, rows});
+            part += spans * stride;
+        }
+        return part <= kMostTokens;
+    };
+    for (int64_t s = 0; s < b->sequences; s++) {
+        const int64_t kv = b->kv_lens[s], n = b->q_lens[s], rows = n * G;
+        if (n == 0) continue;
+        if (rows <= kFewMost) {
+            if (!cut(few, s, 0, rows, (kv + kBlock - 1) / kBlock, up(few_span, 4), rows)) return KVMIX_ERR_UNSUPPORTED;
+        } else {
+            for (int64_t r = 0; r < rows; r += kTileRows) {
+                const int64_t here = std::min<int64_t>(kTileRows, rows - r);
+                if (!cut(tiles, s, r, here, (kv - n + (r + here - 1) / G) / kTileKeys + 1, tile_span, here)) return KVMIX_ERR_UNSUPPORTED;
+            }
+        }
+    }
+    if (std::max({few.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    // the longest first: what ends a launch is short then
+    for (auto *list : {&few, &tiles}) std::stable_sort(list->begin(), list->end(), [](const Span &x, const Span &y) { return x.cost > y.cost; });
+    plan->few = (int64_t)few.size(), plan->tiles = (int64_t)tiles.size(), plan->joins = (int64_t)joins.size(), plan->part_rows = part;
+    int64_t at = 0;
+    auto take = [&](int64_t n) {
+        const int64_t was = at;
+        at += up(n, 4);
+        return was;
+    };
+    plan->slots_at = take(plan->tokens);
+    plan->seqs_at = take(b->sequences * kSeqWords);
+    plan->table_at = take(b->sequences * b->table_stride);
+    plan->few_at = take(plan->few * kItemWords);
+    plan->tile_at = take(plan->tiles * kItemWords);
+    plan->join_at = take(plan->joins * kItemWords);
+    plan->words = at;
+    if (at > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    if (!words) return KVMIX_OK;
+    if (capacity < at) return KVMIX_ERR_WORKSPACE;
+    std::fill(words, words + at, 0);
+    int64_t token = 0;
+    for (int64_t s = 0; s < b->sequences; s++) {
+        const int64_t kv = b->kv_lens[s], n = b->q_lens[s];
+        const int32_t record[kSeqWords] = {(int32_t)token, (int32_t)n, (int32_t)kv, (int32_t)b->packed_lens[s]};
+        std::copy(record, record + kSeqWords, words + plan->seqs_at + s * kSeqWords);
+        for (int64_t t = kv - n; t < kv; t++) words[plan->slots_at + token++] = (int32_t)(b->table[s * b->table_stride + t / P] * P + t % P);
+    }
+    if (b->sequences && b->table_stride) std::copy(b->table, b->table + b->sequences * b->table_stride, words + plan->table_at);
+    auto write = [&](const std::vector<Span> &list, int64_t to) {
+        for (const Span &s : list) to = std::copy(s.word, s.word + kItemWords, words + to) - words;
+    };
+    write(few, plan->few_at), write(tiles, plan->tile_at), write(joins, plan->join_at);
+    return KVMIX_OK;
+}
+
+int attention_check(const kvmix_paged_pool_t *p, const kvmix_paged_plan_t *plan, const kvmix_paged_attn_t *c)
+{
+    int rc = pool_check(p);
+    if (rc == KVMIX_OK) rc = plan && c ? bits_check(p) : KVMIX_ERR_NULL;
+    if (rc != KVMIX_OK) return rc;
+    if (plan->kv_heads != p->kv_heads || plan->head_dim != p->head_dim || plan->page_size != p->page_size) return KVMIX_ERR_SHAPE;
+    if (plan->row_pages > p->row_pages || plan->packed_pages > p->packed_pages) return KVMIX_ERR_PAGE;
+    if (!(c->scale > 0.0f) || c->scale > 1e30f) return KVMIX_ERR_UNSUPPORTED;
+    for (int64_t s : {c->q_token_stride, c->q_head_stride, c->out_token_stride, c->out_head_stride})
+        if (s % 8 != 0) return KVMIX_ERR_UNSUPPORTED;
+    if (((uintptr_t)c->q | (uintptr_t)c->out) % 16 != 0 || (uintptr_t)c->list % 4 != 0) return KVMIX_ERR_UNSUPPORTED;
+    return KVMIX_OK;
+}
+
+}  // namespace
+}  // namespace kvmix
+
+using namespace kvmix;
+
+extern "C" int kvmix_paged_plan(const kvmix_paged_batch_t *batch, int32_t *words, int64_t capacity, kvmix_paged_plan_t *plan)
+{
+    const int rc = batch_check(batch);
+    if (rc != KVMIX_OK) return rc;
+    if (!plan) return KVMIX_ERR_NULL;
+    try {
+        return make_plan(batch, words, capacity, plan);
+    } catch (const std::bad_alloc &) {
+        return KVMIX_ERR_MEMORY;
+    }
+}
+
+extern "C" int64_t kvmix_paged_attention_workspace_bytes(const kvmix_paged_plan_t *plan)
+{
+    return plan ? plan->kv_heads * plan->part_rows * (plan->head_dim * 4 + 8) : 0;
+}
+
+extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_paged_plan_t *plan, const kvmix_paged_attn_t *c, void *workspace,
+                                     int64_t workspace_bytes, kvmix_stream_t stream)
+{
+    const int rc = attention_check(p, plan, c);
+    if (rc != KVMIX_OK) return rc;
+    if (plan->tokens == 0) return KVMIX_OK;
+    if (!c->q || !c->out || !c->list || (plan->row_pages && !p->rows) || (plan->packed_pages && !p->packed)) return KVMIX_ERR_NULL;
+    if (plan->part_rows && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < kvmix_paged_attention_workspace_bytes(plan)))
+        return KVMIX_ERR_WORKSPACE;
+    PagedArgs a;
+    a.q = (const _Float16 *)c->q, a.out = (_Float16 *)c->out;
+    a.q_ts = c->q_token_stride, a.q_hs = c->q_head_stride, a.o_ts = c->out_token_stride, a.o_hs = c->out_head_stride;
+    a.rows = (const _Float16 *)p->rows, a.packed = (const uint32_t *)p->packed;
+    a.seqs = c->list + plan->seqs_at, a.table = c->list + plan->table_at, a.items = nullptr;
+    a.table_stride = (int)plan->table_stride, a.kv_heads = (int)plan->kv_heads, a.group = (int)(plan->heads / plan->kv_heads);
+    a.blocks_log2 = __builtin_ctzll((uint64_t)plan->page_size / kBlock);
+    a.scale = c->scale * kLog2e;
+    a.part = (float *)workspace, a.part_rows = plan->part_rows;
+    a.part_ml = (float2 *)((float *)workspace + plan->kv_heads * plan->part_rows * plan->head_dim);
+    hipStream_t st = (hipStream_t)stream;
+    with_dim(p->head_dim, [&](auto D) {
+        with_bits(p->k_bits, [&](auto KB) {
+            with_bits(p->v_bits, [&](auto VB) {
+                if (plan->tiles) {
+                    a.items = c->list + plan->tile_at;
+                    paged_tile<D.value, KB.value, VB.value><<<(unsigned)(plan->tiles * plan->kv_heads), 256, 0, st>>>(a);
+                }
+                if (plan->few) {
+                    a.items = c->list + plan->few_at;
+                    const unsigned grid = (unsigned)(plan->few * plan->kv_heads);
+                    if (plan->few_rows > 16) paged_few<D.value, KB.value, VB.value, 2><<<grid, 256, 0, st>>>(a);
+                    else paged_few<D.value, KB.value, VB.value, 1><<<grid, 256, 0, st>>>(a);
+                }
+            });
+        });
+        if (plan->joins) {
+            a.items = c->list + plan->join_at;
+            const unsigned rows = plan->tiles ? kTileRows / 4 : (unsigned)(plan->few_rows + 3) / 4;
+            paged_join<D.value><<<dim3((unsigned)(plan->joins * plan->kv_heads), rows), 256, 0, st>>>(a);
+        }
+    });
+    return launch_status();
+}

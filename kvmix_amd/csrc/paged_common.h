@@ -1,0 +1,165 @@
+// What the kernels of the paged cache share: where things lie in a page, and codes to values and back.
+//
+// A page holds P tokens (a multiple of 32) of one layer, for every kv head.  Blocks of 32 tokens are the unit of everything:
+//   fp16 page      keys [P][D], then per block the values as [D][32] (what a matrix instruction wants of them is eight tokens
+//                  of one channel, so they are turned round when they are stored, once, and not at every read)
+//   packed page    per block D * (KB + VB + 2) words: key codes, value codes, then 4 D halves: the keys' scale and minimum per
+//                  channel, the values' per token, [D / 32 groups][32 tokens]
+// Codes lie in the order of the lanes of v_mfma_f32_16x16x32: lane 16 g + m has pieces of eight codes, of the keys piece
+// u * D / 32 + s = channels 32 s + 8 g + (0..7) of token 8 (m / 4) + 4 u + m % 4, of the values piece t = tokens 8 g + (0..7) of
+// channel 16 t + m.  With the keys' rows in that order the logits that a lane holds after q.K^T are those of tokens 8 g +
+// (0..7): they are its operand of p.V as they stand.  The D / 16 pieces of a lane fill D * bits / 64 words; a wave reads them
+// as whole runs of 16 (8, 4) bytes per lane.  Codes lie in the word so that two of them come out as a pair of halves with one
+// or two instructions: the pair's first code in the low half, its second at the same place in the high half.
+#pragma once
+
+#include <type_traits>
+
+#include "kvmix_common.h"
+
+namespace kvmix {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+
+constexpr int kBlock = 32;  // tokens
+
+__host__ __device__ constexpr int lane_words(int D, int bits) { return D * bits / 64; }
+__host__ __device__ constexpr int run_words(int words) { return words % 4 == 0 ? 4 : words % 2 == 0 ? 2 : 1; }
+__host__ __device__ constexpr int block_words(int D, int kb, int vb) { return D * (kb + vb + 2); }
+
+// A lane's words of one matrix of a block.
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t *at, int lane, uint32_t *w)
+{
+    constexpr int R = run_words(N);
+#pragma unroll
+    for (int i = 0; i < N / R; i++) {
+        const uint32_t *p = at + i * kWave * R + lane * R;
+        if constexpr (R == 4) {
+            const uint4v v = *(const uint4v *)p;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[4 * i + j] = v[j];
+        } else if constexpr (R == 2) {
+            const uint2v v = *(const uint2v *)p;
+            w[2 * i] = v[0], w[2 * i + 1] = v[1];
+        } else {
+            w[i] = *p;
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void store_words(uint32_t *at, int lane, const uint32_t *w)
+{
+    constexpr int R = run_words(N);
+#pragma unroll
+    for (int i = 0; i < N / R; i++) {
+        uint32_t *p = at + i * kWave * R + lane * R;
+        if constexpr (R == 4) *(uint4v *)p = uint4v{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        else if constexpr (R == 2) *(uint2v *)p = uint2v{w[2 * i], w[2 * i + 1]};
+        else *p = w[i];
+    }
+}
+
+// Where pair `t` of a lane's N words lies: word and bit (the second code 16 bits higher).  Three-bit pairs past 5 N take the top
+// bits of three words' halves, one bit from each.
+template <int BITS, int N>
+struct Pairs {
+    static constexpr int per = BITS == 3 ? 5 : 16 / BITS;
+    static constexpr bool whole(int t) { return t < N * per; }
+};
+
+// Pair `t` as two halves that hold the codes exactly.  A field at bit s of a half, under the exponent of 2^(10 - s), is the code
+// plus 2^(10 - s): the bits are masked in place and that is subtracted.
+template <int BITS, int N>
+__device__ __forceinline__ half2v code_pair(const uint32_t *w, int t)
+{
+    constexpr uint32_t ones = 0x00010001u;
+    constexpr uint32_t mask = (1u << BITS) - 1;
+    constexpr int per = Pairs<BITS, N>::per;
+    if (t >= N * per) {  // (3 bits only)
+        const int r = 3 * (t - N * per);
+        const uint32_t c = (w[r] >> 15 & ones) | (w[r + 1] >> 14 & 2 * ones) | (w[r + 2] >> 13 & 4 * ones) | 0x64006400u;
+        return __builtin_bit_cast(half2v, c) - half2v{(_Float16)1024.0f, (_Float16)1024.0f};
+    }
+    int s = t % per * BITS;
+    uint32_t v = w[t / per];
+    constexpr int shift = BITS == 4 ? 8 : BITS == 3 ? 9 : 10;  // fields that do not lie in the ten bits of a half's fraction
+    if (s + BITS > 10) v >>= shift, s -= shift;
+    const uint32_t c = (v & (mask * ones << s)) | (0x6400u - 0x400u * s) * ones;
+    const _Float16 base = (_Float16)(float)(1 << (10 - s));
+    return __builtin_bit_cast(half2v, c) - half2v{base, base};
+}
+
+// Codes (0 .. 2^BITS - 1) of pair t into the words (which start at zero).
+template <int BITS, int N>
+__device__ __forceinline__ void put_pair(uint32_t *w, int t, uint32_t first, uint32_t second)
+{
+    constexpr int per = Pairs<BITS, N>::per;
+    const uint32_t c = first | second << 16;
+    if (t >= N * per) {
+        const int r = 3 * (t - N * per);
+#pragma unroll
+        for (int i = 0; i < 3; i++) w[r + i] |= (c >> i & 0x00010001u) << 15;
+    } else {
+        w[t / per] |= c << (t % per * BITS);
+    }
+}
+
+// Piece `piece` of a lane's words as values: code * scale + zero, each rounded once, to fp16.
+template <int BITS, int N>
+__device__ __forceinline__ half8v piece_values(const uint32_t *w, int piece, half8v scale, half8v zero)
+{
+    half8v out;
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+        const half2v c = code_pair<BITS, N>(w, 4 * piece + p);
+        const half2v v = __builtin_elementwise_fma(c, half2v{scale[2 * p], scale[2 * p + 1]}, half2v{zero[2 * p], zero[2 * p + 1]});
+        out[2 * p] = v[0], out[2 * p + 1] = v[1];
+    }
+    return out;
+}
+
+constexpr int64_t kMost32 = 0x7fffffff;
+constexpr int64_t kMostHeads = 4096;
+
+inline bool page_size_ok(int64_t n) { return n >= kBlock && n <= 1024 && (n & (n - 1)) == 0; }
+
+// Sizes that every call on pages shares.
+inline int pool_check(const kvmix_paged_pool_t *p)
+{
+    if (!p) return KVMIX_ERR_NULL;
+    if (p->kv_heads <= 0 || p->row_pages < 0 || p->packed_pages < 0) return KVMIX_ERR_SHAPE;
+    if ((p->head_dim != 64 && p->head_dim != 128) || !page_size_ok(p->page_size) || p->kv_heads > kMostHeads)
+        return KVMIX_ERR_UNSUPPORTED;
+    if ((__int128)p->row_pages * p->page_size > kMost32 || p->packed_pages > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    if (((uintptr_t)p->rows | (uintptr_t)p->packed) % 16 != 0) return KVMIX_ERR_UNSUPPORTED;
+    return KVMIX_OK;
+}
+
+inline int bits_check(const kvmix_paged_pool_t *p)
+{
+    return p->k_bits < 1 || p->k_bits > 4 || p->v_bits < 1 || p->v_bits > 4 ? KVMIX_ERR_BITS : KVMIX_OK;
+}
+
+template <typename F>
+void with_dim(int64_t D, F f)
+{
+    if (D == 128) f(std::integral_constant<int, 128>());
+    else f(std::integral_constant<int, 64>());
+}
+
+template <typename F>
+__host__ __device__ __forceinline__ void with_bits(int bits, F f)
+{
+    if (bits == 1) f(std::integral_constant<int, 1>());
+    else if (bits == 2) f(std::integral_constant<int, 2>());
+    else if (bits == 3) f(std::integral_constant<int, 3>());
+    else f(std::integral_constant<int, 4>());
+}
+
+}  // namespace kvmix

@@ -1,0 +1,400 @@
+// The pages of a cache written, quantized, read back and copied (paged_common.h says what a page holds).  All of it is bound by
+// memory, or by the launch where there is little of it.
+#include <stdlib.h>
+
+#include <type_traits>
+
+#include "paged_common.h"
+
+namespace kvmix {
+
+constexpr int kStorePairs = 400;  // (source, destination) pages, or single pages, that travel as kernel arguments
+constexpr int kCopyPools = 32;
+
+struct PagePairs {
+    int2 at[kStorePairs];
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// append: thirty-two tokens of one head per block.  Keys are copied as they come; values go through the LDS, so that tokens
+// that follow one another in a page (a chunk's) are written as whole rows of it.  A single token's values touch D rows of 64
+// bytes: sixteen times the lines that it has to, for a store that is read at every step after it.
+
+struct AppendArgs {
+    const _Float16 *k, *v;
+    int64_t k_ts, k_hs, v_ts, v_hs;
+    _Float16 *rows;
+    const int32_t *slots;
+    int64_t pages;
+    int tokens, heads, page;
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) paged_append(AppendArgs a)
+{
+    constexpr int C = D / 8;  // 16-byte pieces of a token
+    __shared__ _Float16 values[kBlock][D + 2];
+    __shared__ int64_t to[kBlock];  // where the token's page and head begins, in halves; -1: nowhere
+    __shared__ int pos[kBlock];     // and the token's place in it
+    const int head = blockIdx.y, first = blockIdx.x * kBlock, n = a.tokens - first < kBlock ? a.tokens - first : kBlock;
+    if (threadIdx.x < kBlock) {
+        const int slot = (int)threadIdx.x < n ? a.slots[first + threadIdx.x] : -1;
+        const int page = slot / a.page;
+        to[threadIdx.x] = slot >= 0 && page < a.pages ? ((int64_t)page * a.heads + head) * 2 * a.page * D : -1;
+        pos[threadIdx.x] = slot - page * a.page;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * C; i += 256) {
+        const int t = i / C, c = i % C;
+        if (to[t] < 0) continue;
+        const half8v key = *(const half8v *)(a.k + (int64_t)(first + t) * a.k_ts + head * a.k_hs + 8 * c);
+        const half8v value = *(const half8v *)(a.v + (int64_t)(first + t) * a.v_ts + head * a.v_hs + 8 * c);
+        *(half8v *)(a.rows + to[t] + (int64_t)pos[t] * D + 8 * c) = key;
+#pragma unroll
+        for (int j = 0; j < 4; j++) *(half2v *)&values[t][8 * c + 2 * j] = half2v{value[2 * j], value[2 * j + 1]};
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBlock * D; i += 256) {
+        const int t = i % kBlock, d = i / kBlock;
+        if (t >= n || to[t] < 0) continue;
+        a.rows[to[t] + (int64_t)a.page * D + (int64_t)(pos[t] / kBlock) * kBlock * D + d * kBlock + pos[t] % kBlock] = values[t][d];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The pieces of one matrix of a block of an fp16 page, in the packed order: keys piece u * D / 32 + s, values piece t.
+
+template <int D, bool KEYS>
+__device__ __forceinline__ half8v row_piece(const _Float16 *page_head, int page, int block, int lane, int piece)
+{
+    const int m = lane % 16, g = lane / 16;
+    if constexpr (KEYS) {
+        const int u = piece / (D / 32), s = piece % (D / 32);
+        return *(const half8v *)(page_head + (int64_t)(block * kBlock + 8 * (m / 4) + 4 * u + m % 4) * D + 32 * s + 8 * g);
+    } else {
+        return *(const half8v *)(page_head + (int64_t)page * D + (int64_t)block * kBlock * D + (16 * piece + m) * kBlock + 8 * g);
+    }
+}
+
+struct QuantizeArgs {
+    const _Float16 *rows;
+    uint32_t *packed;
+    int heads, page, units;  // units: waves of work, pair by head by block by matrix
+    int k_bits, v_bits;
+};
+
+// One matrix of one block per wave.  A group's 32 values are two of a lane's (the keys' two tokens, the values' two channels)
+// and those of the sixteen lanes of a row: extremes by packed halves and exchanges within the row.  The codes are those of
+// kvmix_quant_pack_last_dim with KVMIX_SCALE_RECIPROCAL, bit for bit.
+template <int D, int BITS, bool KEYS>
+__device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, int block, uint32_t *to, _Float16 *side, int lane)
+{
+    constexpr int NP = D / 16, S = D / 32, N = lane_words(D, BITS);
+    constexpr int QMAX = (1 << BITS) - 1;
+    half8v x[NP];  // [set of eight groups][two of the group]
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+#pragma unroll
+        for (int w = 0; w < 2; w++) x[2 * s + w] = row_piece<D, KEYS>(from, page, block, lane, KEYS ? w * S + s : 2 * s + w);
+    }
+    uint32_t words[N] = {};
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        half2v lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const half2v a = {x[2 * s][2 * j], x[2 * s][2 * j + 1]}, b = {x[2 * s + 1][2 * j], x[2 * s + 1][2 * j + 1]};
+            lo[j] = __builtin_elementwise_min(a, b);
+            hi[j] = __builtin_elementwise_max(a, b);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            auto step = [&](half2v &v, bool most, float (*ror)(float)) {
+                const half2v o = __builtin_bit_cast(half2v, ror(__builtin_bit_cast(float, v)));
+                v = most ? __builtin_elementwise_max(v, o) : __builtin_elementwise_min(v, o);
+            };
+            step(lo[j], false, row_ror<8>), step(hi[j], true, row_ror<8>);
+            step(lo[j], false, row_ror<4>), step(hi[j], true, row_ror<4>);
+            step(lo[j], false, row_ror<2>), step(hi[j], true, row_ror<2>);
+            step(lo[j], false, row_ror<1>), step(hi[j], true, row_ror<1>);
+        }
+        half8v scales, zeros;
+        uint32_t q[2][8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float mn = (float)lo[j / 2][j % 2], range = (float)hi[j / 2][j % 2] - mn;
+            const float scale = range / (float)QMAX;
+            const float v[2] = {(float)x[2 * s][j], (float)x[2 * s + 1][j]};
+            uint32_t c[2];
+            quantize_codes<2>(v, mn, scale, quantize_rcp(scale), [](int) { return QMAX; }, c);
+            q[0][j] = c[0], q[1][j] = c[1];
+            scales[j] = (_Float16)scale_for_output(range, scale, 1.0f / (float)QMAX, KVMIX_SCALE_RECIPROCAL);
+            zeros[j] = (_Float16)mn;
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const int piece = KEYS ? w * S + s : 2 * s + w;
+#pragma unroll
+            for (int p = 0; p < 4; p++) put_pair<BITS, N>(words, 4 * piece + p, q[w][2 * p], q[w][2 * p + 1]);
+        }
+        if (lane % 16 == s) {
+            *(half8v *)(side + 32 * s + 8 * (lane / 16)) = scales;
+            *(half8v *)(side + D + 32 * s + 8 * (lane / 16)) = zeros;
+        }
+    }
+    store_words<N>(to, lane, words);
+}
+
+template <int D>
+__global__ void __launch_bounds__(256) paged_quantize(QuantizeArgs a, PagePairs pairs)
+{
+    const int lane = threadIdx.x % kWave;
+    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+    if (unit >= a.units) return;
+    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks % a.heads;
+    const int2 pair = pairs.at[unit / 2 / blocks / a.heads];
+    const _Float16 *from = a.rows + ((int64_t)pair.x * a.heads + head) * 2 * a.page * D;
+    uint32_t *to = a.packed + (((int64_t)pair.y * a.heads + head) * blocks + block) * block_words(D, a.k_bits, a.v_bits);
+    _Float16 *side = (_Float16 *)(to + D * (a.k_bits + a.v_bits));
+    if (values) with_bits(a.v_bits, [&](auto B) { quantize_matrix<D, B.value, false>(from, a.page, block, to + D * a.k_bits, side + 2 * D, lane); });
+    else with_bits(a.k_bits, [&](auto B) { quantize_matrix<D, B.value, true>(from, a.page, block, to, side, lane); });
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// read: the values of pages, token by token: [pages, P, heads, D].  A block of one head per wave pair, keys and values.
+
+struct ReadArgs {
+    const void *pool;
+    _Float16 *k, *v;
+    int heads, page, units;
+    int k_bits, v_bits;
+};
+
+template <int D, bool ROWS>
+__global__ void __launch_bounds__(256) paged_read(ReadArgs a, PagePairs ids)
+{
+    constexpr int NP = D / 16;
+    __shared__ _Float16 turned[4][kBlock][D + 8];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, m = lane % 16, g = lane / 16;
+    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
+    if (unit >= a.units) return;  // (waves share nothing but the array, of which each has its own part)
+    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks % a.heads, nth = unit / 2 / blocks / a.heads;
+    const int64_t id = nth % 2 ? ids.at[nth / 2].y : ids.at[nth / 2].x;
+    half8v x[NP];
+    if constexpr (ROWS) {
+        const _Float16 *from = (const _Float16 *)a.pool + (id * a.heads + head) * 2 * a.page * D;
+#pragma unroll
+        for (int p = 0; p < NP; p++) x[p] = values ? row_piece<D, false>(from, a.page, block, lane, p) : row_piece<D, true>(from, a.page, block, lane, p);
+    } else {
+        const uint32_t *from = (const uint32_t *)a.pool + ((id * a.heads + head) * blocks + block) * block_words(D, a.k_bits, a.v_bits);
+        const _Float16 *side = (const _Float16 *)(from + D * (a.k_bits + a.v_bits)) + (values ? 2 * D : 0) + 8 * g;
+        with_bits(values ? a.v_bits : a.k_bits, [&](auto B) {
+            constexpr int N = lane_words(D, B.value);
+            uint32_t w[N];
+            load_words<N>(values ? from + D * a.k_bits : from, lane, w);
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                const int s = values ? p / 2 : p % (D / 32);
+                x[p] = piece_values<B.value, N>(w, p, *(const half8v *)(side + 32 * s), *(const half8v *)(side + D + 32 * s));
+            }
+        });
+    }
+    const int64_t token0 = (int64_t)nth * a.page + block * kBlock;
+    if (!values) {
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const int u = p / (D / 32), s = p % (D / 32);
+            *(half8v *)(a.k + ((token0 + 8 * (m / 4) + 4 * u + m % 4) * a.heads + head) * D + 32 * s + 8 * g) = x[p];
+        }
+        return;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) turned[wave][8 * g + j][16 * p + m] = x[p][j];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < kBlock * D / 8 / kWave; i++) {
+        const int at = i * kWave + lane, t = at / (D / 8), c = at % (D / 8);
+        *(half8v *)(a.v + ((token0 + t) * a.heads + head) * D + 8 * c) = *(const half8v *)&turned[wave][t][8 * c];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// copy: pages of up to kCopyPools pools, the same pairs in all of them, 16 KiB to a block.
+
+constexpr int kCopyPieces = 4;  // of 16 bytes per thread
+constexpr uint32_t kCopyBytes = 256 * 16 * kCopyPieces;
+
+struct CopyArgs {
+    uint8_t *pool[kCopyPools];
+    uint32_t bytes[kCopyPools];      // of a page
+    uint32_t blocks[kCopyPools];     // up to and with this pool, per pair
+    int pools, pairs;
+};
+
+__global__ void __launch_bounds__(256) paged_copy(CopyArgs a, PagePairs pairs)
+{
+    const uint32_t per = a.blocks[a.pools - 1], nth = blockIdx.x / per, at = blockIdx.x % per;
+    int p = 0;
+    while (at >= a.blocks[p]) p++;
+    const uint32_t piece = at - (p ? a.blocks[p - 1] : 0);
+    const int2 pair = pairs.at[nth];
+    const uint32_t bytes = a.bytes[p];
+    const uint8_t *src = a.pool[p] + (int64_t)pair.x * bytes;
+    uint8_t *dst = a.pool[p] + (int64_t)pair.y * bytes;
+    if (__builtin_expect(bytes % 16 != 0, 0)) {  // (pages that begin between pieces of sixteen bytes)
+        for (uint32_t off = piece * kCopyBytes + threadIdx.x * 8; off < (piece + 1) * kCopyBytes && off < bytes; off += 256 * 8)
+            *(uint2v *)(dst + off) = *(const uint2v *)(src + off);
+        return;
+    }
+    uint4v v[kCopyPieces];
+#pragma unroll
+    for (int i = 0; i < kCopyPieces; i++) {
+        const uint32_t off = piece * kCopyBytes + (i * 256 + threadIdx.x) * 16;
+        if (off < bytes) v[i] = *(const uint4v *)(src + off);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopyPieces; i++) {
+        const uint32_t off = piece * kCopyBytes + (i * 256 + threadIdx.x) * 16;
+        if (off < bytes) *(uint4v *)(dst + off) = v[i];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+}  // namespace kvmix
+
+using namespace kvmix;
+
+namespace {
+
+// Whether no page of [0, pages) is written twice by these pairs, nor (`read_too`) written and read.
+int pairs_apart(const int32_t *pairs, int64_t count, int64_t pages, bool read_too)
+{
+    uint8_t *written = (uint8_t *)calloc((size_t)pages, 1);
+    if (!written) return KVMIX_ERR_MEMORY;
+    bool apart = true;
+    for (int64_t i = 0; i < count; i++) {
+        apart = apart && !written[pairs[2 * i + 1]];
+        written[pairs[2 * i + 1]] = 1;
+    }
+    for (int64_t i = 0; read_too && i < count; i++) apart = apart && !written[pairs[2 * i]];
+    free(written);
+    return apart ? KVMIX_OK : KVMIX_ERR_PAGE_ORDER;
+}
+
+}  // namespace
+
+extern "C" int kvmix_paged_append(const kvmix_paged_pool_t *p, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                                  int64_t v_token_stride, int64_t v_head_stride, const int32_t *slots, int64_t tokens, kvmix_stream_t stream)
+{
+    const int rc = pool_check(p);
+    if (rc != KVMIX_OK) return rc;
+    if (tokens < 0 || tokens > kMost32 - kBlock) return tokens < 0 ? KVMIX_ERR_SHAPE : KVMIX_ERR_UNSUPPORTED;
+    if (k_token_stride % 8 || k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8 || ((uintptr_t)k | (uintptr_t)v) % 16) return KVMIX_ERR_UNSUPPORTED;
+    if (tokens == 0) return KVMIX_OK;
+    if (!k || !v || !slots || !p->rows) return KVMIX_ERR_NULL;
+    const AppendArgs a = {(const _Float16 *)k, (const _Float16 *)v, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                          (_Float16 *)p->rows, slots, p->row_pages, (int)tokens, (int)p->kv_heads, (int)p->page_size};
+    const dim3 grid((unsigned)((tokens + kBlock - 1) / kBlock), (unsigned)p->kv_heads);
+    with_dim(p->head_dim, [&](auto D) { paged_append<D.value><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    return launch_status();
+}
+
+extern "C" int kvmix_paged_quantize(const kvmix_paged_pool_t *p, const int32_t *pairs, int64_t count, kvmix_stream_t stream)
+{
+    int rc = pool_check(p);
+    if (rc == KVMIX_OK) rc = bits_check(p);
+    if (rc != KVMIX_OK) return rc;
+    if (count < 0) return KVMIX_ERR_SHAPE;
+    if (count == 0) return KVMIX_OK;
+    if (!pairs || !p->rows || !p->packed) return KVMIX_ERR_NULL;
+    for (int64_t i = 0; i < count; i++)
+        if (pairs[2 * i] < 0 || pairs[2 * i] >= p->row_pages || pairs[2 * i + 1] < 0 || pairs[2 * i + 1] >= p->packed_pages) return KVMIX_ERR_PAGE;
+    rc = pairs_apart(pairs, count, p->packed_pages, false);
+    if (rc != KVMIX_OK) return rc;
+    const int64_t per = p->kv_heads * (p->page_size / kBlock) * 2;
+    for (int64_t first = 0; first < count; first += kStorePairs) {
+        const int n = (int)(count - first < kStorePairs ? count - first : kStorePairs);
+        PagePairs list{};
+        for (int i = 0; i < n; i++) list.at[i] = make_int2(pairs[2 * (first + i)], pairs[2 * (first + i) + 1]);
+        const QuantizeArgs a = {(const _Float16 *)p->rows, (uint32_t *)p->packed, (int)p->kv_heads, (int)p->page_size, (int)(n * per),
+                                p->k_bits, p->v_bits};
+        const unsigned grid = (unsigned)((n * per + 3) / 4);
+        with_dim(p->head_dim, [&](auto D) { paged_quantize<D.value><<<grid, 256, 0, (hipStream_t)stream>>>(a, list); });
+        if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
+    }
+    return KVMIX_OK;
+}
+
+extern "C" int kvmix_paged_read(const kvmix_paged_pool_t *p, int packed, const int32_t *pages, int64_t count, void *k, void *v, kvmix_stream_t stream)
+{
+    int rc = pool_check(p);
+    if (rc == KVMIX_OK && packed) rc = bits_check(p);
+    if (rc != KVMIX_OK) return rc;
+    if (count < 0) return KVMIX_ERR_SHAPE;
+    if (count == 0) return KVMIX_OK;
+    if (!pages || !k || !v || !(packed ? p->packed : p->rows)) return KVMIX_ERR_NULL;
+    if (((uintptr_t)k | (uintptr_t)v) % 16) return KVMIX_ERR_UNSUPPORTED;
+    for (int64_t i = 0; i < count; i++)
+        if (pages[i] < 0 || pages[i] >= (packed ? p->packed_pages : p->row_pages)) return KVMIX_ERR_PAGE;
+    const int64_t per = p->kv_heads * (p->page_size / kBlock) * 2, most = 2 * kStorePairs, size = p->page_size * p->kv_heads * p->head_dim;
+    for (int64_t first = 0; first < count; first += most) {
+        const int n = (int)(count - first < most ? count - first : most);
+        PagePairs list{};
+        for (int i = 0; i < n; i++) (i % 2 ? list.at[i / 2].y : list.at[i / 2].x) = pages[first + i];
+        const ReadArgs a = {packed ? p->packed : p->rows, (_Float16 *)k + first * size, (_Float16 *)v + first * size, (int)p->kv_heads,
+                            (int)p->page_size, (int)(n * per), p->k_bits, p->v_bits};
+        const unsigned grid = (unsigned)((n * per + 3) / 4);
+        with_dim(p->head_dim, [&](auto D) {
+            if (packed) paged_read<D.value, false><<<grid, 256, 0, (hipStream_t)stream>>>(a, list);
+            else paged_read<D.value, true><<<grid, 256, 0, (hipStream_t)stream>>>(a, list);
+        });
+        if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
+    }
+    return KVMIX_OK;
+}
+
+extern "C" int kvmix_paged_copy(void *const *pools, const int64_t *page_bytes, int64_t n_pools, int64_t pages, const int32_t *pairs, int64_t count,
+                                kvmix_stream_t stream)
+{
+    if (n_pools < 0 || count < 0 || pages < 0) return KVMIX_ERR_SHAPE;
+    if (n_pools == 0 || count == 0) return KVMIX_OK;
+    if (!pools || !page_bytes || !pairs) return KVMIX_ERR_NULL;
+    for (int64_t i = 0; i < n_pools; i++) {
+        if (page_bytes[i] < 0) return KVMIX_ERR_SHAPE;
+        if (page_bytes[i] % 8 != 0 || page_bytes[i] > (1 << 28) || (uintptr_t)pools[i] % 16 != 0) return KVMIX_ERR_UNSUPPORTED;
+        if (!pools[i] && page_bytes[i]) return KVMIX_ERR_NULL;
+    }
+    // Pairs are done in no particular order: a page is written once at most, and no page that is written is read.
+    if (pages > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    for (int64_t i = 0; i < 2 * count; i++)
+        if (pairs[i] < 0 || pairs[i] >= pages) return KVMIX_ERR_PAGE;
+    const int rc = pairs_apart(pairs, count, pages, true);
+    if (rc != KVMIX_OK) return rc;
+    for (int64_t p0 = 0; p0 < n_pools; p0 += kCopyPools) {
+        CopyArgs a{};
+        a.pools = (int)(n_pools - p0 < kCopyPools ? n_pools - p0 : kCopyPools);
+        uint32_t blocks = 0;
+        for (int i = 0; i < a.pools; i++) {
+            a.pool[i] = (uint8_t *)pools[p0 + i];
+            a.bytes[i] = (uint32_t)page_bytes[p0 + i];
+            blocks += (uint32_t)((page_bytes[p0 + i] + kCopyBytes - 1) / kCopyBytes);
+            a.blocks[i] = blocks;
+        }
+        if (blocks == 0) continue;
+        for (int64_t first = 0; first < count; first += kStorePairs) {
+            const int64_t n = count - first < kStorePairs ? count - first : kStorePairs;
+            PagePairs list{};
+            for (int64_t i = 0; i < n; i++) list.at[i] = make_int2(pairs[2 * (first + i)], pairs[2 * (first + i) + 1]);
+            a.pairs = (int)n;
+            paged_copy<<<(unsigned)(n * blocks), 256, 0, (hipStream_t)stream>>>(a, list);
+            if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
+        }
+    }
+    return KVMIX_OK;
+}

@@ -470,6 +470,84 @@ def grow_tuple(past, key_states, value_states, nk: int, nv: int, k_bits: int, k_
     return _host().grow_tuple(kc, k_tail, ks, km, vc, v_tail, vs, vm, key_states, value_states, nk, nv, k_bits, k_group, v_bits)
 
 
+def paged_plan(table: torch.Tensor, kv_lens, packed_lens, q_lens, heads: int, kv_heads: int, head_dim: int, page_size: int, device="cuda"):
+    """The plan of one step of a batch over a paged cache, for every layer of the step (kvmix_paged_plan): what each block of
+    the attention's launches takes, and where the new tokens go.
+
+    table: the sequences' pages, whole numbers in host memory [sequences, pages]: token t of a sequence lies in page
+    table[t // page_size], a packed page for t < packed_lens (whole pages), an fp16 page from there on.  kv_lens: tokens of each
+    sequence, the q_lens newest of them new (none of them packed).  The plan is made on torch's current stream of `device`."""
+    return _host().paged_plan(table, list(kv_lens), list(packed_lens), list(q_lens), heads, kv_heads, head_dim, page_size, _cuda(device))
+
+
+def _cuda(device) -> torch.device:
+    device = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, plan) -> None:
+    """Keys and values [plan.tokens, kv_heads, head_dim] fp16 of a step's new tokens, sequence after sequence, into the fp16
+    pages `rows` [pages, kv_heads, 2, page_size, head_dim]: the keys [page_size][head_dim] of a page and head, the values as one
+    [head_dim][32] matrix for every 32 tokens."""
+    _host().paged_append(k, v, rows, plan)
+
+
+def paged_quantize(rows: torch.Tensor, packed: torch.Tensor, pairs: torch.Tensor, k_bits: int, v_bits: int) -> None:
+    """fp16 pages to packed pages: pairs [n, 2] in host memory = (page of `rows`, page of `packed`); packed int32 [pages,
+    kv_heads, page_size / 32 * head_dim * (k_bits + v_bits + 2)].  Keys in groups of 32 tokens per channel, values in groups of 32
+    channels per token; codes, scales and minima are those of quantize_pack_last_dim_cuda (3 bits: of quantize_pack_dense3)."""
+    _host().paged_quantize(rows, packed, pairs, k_bits, v_bits)
+
+
+def paged_read(pool: torch.Tensor, pages: torch.Tensor, k_bits: int = None, v_bits: int = None, head_dim: int = None):
+    """The values that pages hold: (k, v) [n, page_size, kv_heads, head_dim] fp16 of the pages [n] (in host memory) of a pool of
+    fp16 pages or, with the widths and the head dimension, of packed ones."""
+    return _host().paged_read(pool, pages, k_bits, v_bits, head_dim)
+
+
+def paged_copy(pools, pairs: torch.Tensor) -> None:
+    """Pages copied within every pool of a sequence of pools (of all layers, say) of equally many pages: pairs [n, 2] in host
+    memory = (source, destination).  No page may be written twice, or written and read: the copies are done in no order."""
+    _host().paged_copy(list(pools), pairs)
+
+
+def paged_attention(q: torch.Tensor, rows: torch.Tensor, packed: torch.Tensor, plan, k_bits: int, v_bits: int, scale: float = None) -> torch.Tensor:
+    """Attention of a step's new tokens, one or many of each sequence, over the sequences' pages (kvmix_paged_attention): q
+    [plan.tokens, heads, head_dim] fp16 -> the same shape.  A token sees its own sequence up to itself; keys and values of the
+    new tokens are in their pages already (paged_append).  scale: head_dim ** -0.5 unless given."""
+    return _host().paged_attention(q, rows, packed, plan, k_bits, v_bits, scale)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top):
+        lp, entropy, top_lp, top_id, stats = _host().token_logprobs(logits, targets, top, True)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.set_materialize_grads(False)
+        if not top:
+            return lp, entropy
+        ctx.mark_non_differentiable(top_lp, top_id)
+        return lp, entropy, top_lp, top_id
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_lp, grad_entropy, *_):
+        if grad_lp is None and grad_entropy is None:
+            return None, None, None
+        return _host().token_logprobs_grad(*ctx.saved_tensors, grad_lp, grad_entropy), None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0):
+    """Log probabilities of given tokens: logits [..., vocabulary] fp16, bf16 or fp32, targets [...] int64 -> (log probability
+    of each target, entropy of each row) in fp32, and with top > 0 (at most 64) also (the log probabilities of the `top` most
+    likely tokens, their indexes) [..., top], equal logits in the order of their indexes.  A negative target is none (log
+    probability 0).  The first two are differentiable in the logits; their gradient is computed in the logits' type."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLogprobs.apply(logits, targets, top)
+    lp, entropy, top_lp, top_id, _ = _host().token_logprobs(logits, targets, top, False)
+    return (lp, entropy, top_lp, top_id) if top else (lp, entropy)
+
+
 def process_key_quantization_cuda(input: torch.Tensor, previous_code: torch.Tensor,
                                   previous_scale: torch.Tensor, previous_min: torch.Tensor,
                                   group_length: int, quant_bits: int):
