@@ -3,14 +3,14 @@
 //   lse = log sum_i exp(x_i),  logprob = x_t - lse,  entropy = lse - sum_i p_i x_i,  p_i = exp(x_i - lse)
 //   dx_i = a (1[i = t] - p_i) - b p_i (log p_i + entropy)   for the gradients a of logprob and b of entropy
 //
-// Bound by the reads: the logits are read once, with a running reference m, sum s = sum 2^d and sum u = sum 2^d d, where
-// d = (x - m) log2(e), from which lse - m = ln 2 log2 s and entropy = ln 2 (log2 s - u / s).  The reference is any value near the
-// largest: it is moved only when a value exceeds it by kStale.  The difference is taken before the product with log2(e): logits
-// far from zero lose nothing, and those at the type's lowest value, whose product would overflow, are as good as any.
+// Bound by the reads: a row (up to 128k values of 16 bits) is read once into registers by one block, and everything is made of it
+// there: the largest value, the sums s = sum 2^d and u = sum 2^d d with d = (x - m) log2(e), from which lse - m = ln 2 log2 s and
+// entropy = ln 2 (log2 s - u / s), and the most likely tokens.  Each wave sums relative to its own largest value.
 //
-// Most likely tokens: the k-th largest of the threads' own largest values is a lower bound of the row's k-th largest value, so
-// that few others reach it; those that do are collected in a second look at the row and put in order by counting.  Equal logits
-// come in the order of their indexes.  Rows in which too many reach the bound (constant ones) are searched value by value.
+// Most likely tokens: lanes of one number in all waves make a group, 64 of them; the k-th largest of the groups' largest values is
+// a lower bound of the row's k-th largest value that few others reach (25 values for k = 20).  It is found by bisection over
+// the lanes, by its upper sixteen bits; what reaches it is collected and put in order by counting.  Equal logits come in the
+// order of their indexes.  Rows in which too many reach it (constant ones), or with NaN, are searched value by value.
 #include <type_traits>
 
 #include "kvmix_common.h"
@@ -19,10 +19,9 @@ namespace kvmix {
 
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-constexpr int kScoreThreads = 256, kScoreWaves = kScoreThreads / kWave;
+constexpr int kPieces = 16;        // of sixteen bytes that a thread holds
 constexpr int kTopMost = 64, kCandidates = 1024;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
-constexpr float kStale = 20.0f;  // how far a value may exceed the reference: 2^d stays below 2^29
 
 struct ScoreStats {
     float m, s, u;  // reference (as a logit), sum of 2^d, sum of 2^d d
@@ -50,32 +49,46 @@ __device__ __forceinline__ float to_float(T v)
     return (float)v;
 }
 
-// Values of a row by sixteen bytes where it is aligned to them, one by one before and after: f(index, values, how many).
-template <typename T, typename F>
-__device__ __forceinline__ void each_value(const T *row, int begin, int end, F f)
+// A row's values from `begin` on as sixteen-byte pieces of memory: the first and the last may hold others, of no concern, beside
+// it (they lie in the same sixteen aligned bytes as values of the row do).
+template <typename T>
+struct Span {
+    static constexpr int PER = 16 / sizeof(T);
+    const uint4v *at;
+    int first, length, pieces;  // piece p holds values first + p * PER .. of [0, length)
+
+    __device__ __forceinline__ Span(const T *row, int begin, int end)
+    {
+        const int skew = (int)((uintptr_t)(row + begin) / sizeof(T) % PER);
+        at = (const uint4v *)(row + begin - skew);
+        first = -skew, length = max(end - begin, 0), pieces = length ? (length + skew + PER - 1) / PER : 0;
+    }
+};
+
+template <typename T>
+union Piece {
+    uint4v raw;
+    T t[16 / sizeof(T)];
+};
+
+// A piece of a span, with -inf for what is none of it.
+template <typename T>
+__device__ __forceinline__ Piece<T> span_piece(const Span<T> &span, int p)
 {
-    constexpr int PER = 16 / sizeof(T);
-    const int skew = (int)((uintptr_t)(row + begin) / sizeof(T) % PER);
-    const int body = min(end, begin + (skew ? PER - skew : 0)), tail = body + (end - body) / PER * PER;
-    float v[PER];
-    if (begin + (int)threadIdx.x < body) {
-        v[0] = to_float(row[begin + threadIdx.x]);
-        f(begin + (int)threadIdx.x, v, std::integral_constant<int, 1>());
-    }
-    for (int i = body + threadIdx.x * PER; i < tail; i += kScoreThreads * PER) {
-        union {
-            uint4v raw;
-            T t[PER];
-        } w;
-        w.raw = *(const uint4v *)(row + i);
+    constexpr int PER = Span<T>::PER;
+    constexpr uint32_t none = std::is_same<T, _Float16>::value ? 0xfc00fc00u : std::is_same<T, float>::value ? 0xff800000u : 0xff80ff80u;
+    Piece<T> w;
+    w.raw = uint4v{none, none, none, none};
+    if (p < span.pieces) {
+        w.raw = span.at[p];
+        const int i = span.first + p * PER;
+        if (__builtin_expect(i < 0 || i + PER > span.length, 0)) {
 #pragma unroll
-        for (int j = 0; j < PER; j++) v[j] = to_float(w.t[j]);
-        f(i, v, std::integral_constant<int, PER>());
+            for (int j = 0; j < PER; j++)
+                if (i + j < 0 || i + j >= span.length) w.t[j] = (T)-__builtin_inff();
+        }
     }
-    if (tail + (int)threadIdx.x < end) {
-        v[0] = to_float(row[tail + threadIdx.x]);
-        f(tail + (int)threadIdx.x, v, std::integral_constant<int, 1>());
-    }
+    return w;
 }
 
 __device__ __forceinline__ ScoreStats merged(ScoreStats a, ScoreStats b)
@@ -98,92 +111,69 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 
 __device__ __forceinline__ uint64_t full_key(float v, int index) { return (uint64_t)value_key(v) << 32 | (uint32_t)~index; }
 
+template <int NT>
 struct TopShared {
-    uint32_t most[kScoreThreads];
+    uint32_t most[NT];
     uint64_t key[kCandidates];
-    uint64_t best[kScoreWaves];
+    uint64_t best[NT / kWave];
     int count;
-    uint32_t bound;
 };
 
-// The `top` first keys among `count` in key[], in order, to out[] (padded with zeros).
-__device__ __forceinline__ void rank_keys(const uint64_t *key, int count, int top, uint64_t *out)
+// Calls f(rank, key) for the `top` first of `count` different keys, by the threads of a block.
+template <int NT, typename F>
+__device__ __forceinline__ void rank_keys(const uint64_t *key, int count, int top, F f)
 {
-    for (int i = threadIdx.x; i < count; i += kScoreThreads) {
+    for (int i = threadIdx.x; i < count; i += NT) {
         const uint64_t mine = key[i];
         int rank = 0;
-        for (int j = 0; j < count && rank < top; j++) rank += key[j] > mine;
-        if (rank < top) out[rank] = mine;
+#pragma unroll 8
+        for (int j = 0; j < count; j++) rank += key[j] > mine;
+        if (rank < top) f(rank, mine);
     }
-    for (int i = count + threadIdx.x; i < top; i += kScoreThreads) out[i] = 0;
 }
 
-// The `top` first keys of row[begin, end): to out[] (shared or global memory).  `largest`: this thread's largest value.
-template <typename T>
-__device__ void top_of(const T *row, int begin, int end, int top, float largest, TopShared &sh, uint64_t *out)
+// The `top` first keys of a span, one by one: for rows in which too many values are alike.
+template <typename T, int NT, typename F>
+__device__ void search_keys(const Span<T> &span, int begin, int top, uint64_t *shared, F f)
 {
-    sh.most[threadIdx.x] = value_key(largest);
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    // the top-th largest of the threads' largest: the value that fewer than `top` exceed
-    {
-        const uint32_t mine = sh.most[threadIdx.x];
-        int above = 0, equal = 0;
-        for (int j = 0; j < kScoreThreads; j++) {
-            above += sh.most[j] > mine;
-            equal += sh.most[j] == mine;
-        }
-        if (above < top && above + equal >= top) sh.bound = mine;
-    }
-    __syncthreads();
-    const uint32_t bound = sh.bound;
-    each_value(row, begin, end, [&](int i, const float *v, auto n) {
-#pragma unroll
-        for (int j = 0; j < n.value; j++) {
-            if (value_key(v[j]) >= bound) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kCandidates) sh.key[at] = full_key(v[j], i + j);
-            }
-        }
-    });
-    __syncthreads();
-    const int count = sh.count;
-    if (count <= kCandidates) {
-        rank_keys(sh.key, count, top, out);
-        return;
-    }
-    // too many: the next key below the last one, `top` times
+    constexpr int PER = Span<T>::PER;
     uint64_t last = ~(uint64_t)0;
     for (int k = 0; k < top; k++) {
         uint64_t best = 0;
-        each_value(row, begin, end, [&](int i, const float *v, auto n) {
+        for (int p = threadIdx.x; p < span.pieces; p += NT) {
+            const Piece<T> w = span_piece(span, p);
+            const int i = span.first + p * PER;
 #pragma unroll
-            for (int j = 0; j < n.value; j++) {
-                const uint64_t key = full_key(v[j], i + j);
-                if (key < last && key > best) best = key;
+            for (int j = 0; j < PER; j++) {
+                const uint64_t key = full_key(to_float(w.t[j]), begin + i + j);
+                if (i + j >= 0 && i + j < span.length && (key < last || k == 0) && key > best) best = key;
             }
-        });
+        }
         for (int o = 32; o; o /= 2) {
             const uint64_t other = __shfl_xor((unsigned long long)best, o);
             best = other > best ? other : best;
         }
         __syncthreads();
-        if (threadIdx.x % kWave == 0) sh.best[threadIdx.x / kWave] = best;
+        if (threadIdx.x % kWave == 0) shared[threadIdx.x / kWave] = best;
         __syncthreads();
-        for (int w = 0; w < kScoreWaves; w++) best = sh.best[w] > best ? sh.best[w] : best;
-        if (threadIdx.x == 0) out[k] = best;
+        for (int w = 0; w < NT / kWave; w++) best = shared[w] > best ? shared[w] : best;
+        if (threadIdx.x == 0 && best) f(k, best);
         last = best;
     }
 }
 
-// A row's results from its sums: by one thread.  x_t: the target's logit, read again.
+// The logit of a row's target (NaN if it is past the vocabulary).
 template <typename T>
-__device__ __forceinline__ float finish_row(const ScoreArgs &a, int row, ScoreStats t)
+__device__ __forceinline__ float target_logit(const ScoreArgs &a, int row, int64_t target)
+{
+    return target >= 0 && target < a.vocab ? to_float(((const T *)a.x)[row * a.row_stride + target]) : __builtin_nanf("");
+}
+
+// A row's results from its sums: by one thread.
+__device__ __forceinline__ float finish_row(const ScoreArgs &a, int row, ScoreStats t, int64_t target, float x)
 {
     float sum2 = log2f(t.s), entropy = kLn2 * (log2f(t.s) - t.u / t.s);
     if (t.m == __builtin_inff() || !(t.s > 0.0f)) sum2 = entropy = __builtin_nanf("");
-    const int64_t target = a.targets[row];
-    const float x = target >= 0 && target < a.vocab ? to_float(((const T *)a.x)[row * a.row_stride + target]) : __builtin_nanf("");
     a.logprob[row] = target < 0 ? 0.0f : (x - t.m) - kLn2 * sum2;
     a.entropy[row] = entropy;
     if (a.stats) {
@@ -193,138 +183,202 @@ __device__ __forceinline__ float finish_row(const ScoreArgs &a, int row, ScoreSt
     return sum2;
 }
 
-__device__ __forceinline__ void write_top(const ScoreArgs &a, int row, const uint64_t *keys, float m, float sum2)
+__device__ __forceinline__ void write_top(const ScoreArgs &a, int row, int rank, uint64_t key, float m, float sum2)
 {
-    for (int i = threadIdx.x; i < a.top; i += kScoreThreads) {
-        const uint64_t key = keys[i];
-        a.top_logprob[(int64_t)row * a.top + i] = (key_value((uint32_t)(key >> 32)) - m) - kLn2 * sum2;
-        a.top_id[(int64_t)row * a.top + i] = (int64_t)~(uint32_t)key;
-    }
+    a.top_logprob[(int64_t)row * a.top + rank] = (key_value((uint32_t)(key >> 32)) - m) - kLn2 * sum2;
+    a.top_id[(int64_t)row * a.top + rank] = (int64_t)~(uint32_t)key;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) score_rows(ScoreArgs a)
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
 {
-    __shared__ ScoreStats wave_stats[kScoreWaves];
-    __shared__ uint32_t wave_nan[kScoreWaves];
-    __shared__ TopShared sh;
-    __shared__ uint64_t best[kTopMost];
+    constexpr int PER = 16 / sizeof(T), W = NT / kWave;
+    __shared__ ScoreStats wave_stats[W];
+    __shared__ typename std::conditional<TOP, TopShared<NT>, int>::type sh;
     __shared__ float done[2];
-    const int row = blockIdx.x / a.chunks, nth = blockIdx.x % a.chunks;
+    const int row = blockIdx.x / a.chunks, nth = blockIdx.x % a.chunks, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int begin = nth * a.chunk, end = min(a.vocab, begin + a.chunk);
-    const T *x = (const T *)a.x + row * a.row_stride;
-    ScoreStats t = {-__builtin_inff(), 0.0f, 0.0f};
+    const Span<T> span((const T *)a.x + row * a.row_stride, begin, end);
+    Piece<T> x[kPieces];
+#pragma unroll
+    for (int r = 0; r < kPieces; r++)
+        if (r * NT < span.pieces) x[r] = span_piece(span, r * NT + (int)threadIdx.x);
+
+    const int64_t target = a.targets[row];
+    const float at_target = target_logit<T>(a, row, target);  // (here, so that it has arrived when it is wanted)
+
     float largest = -__builtin_inff();
-    bool nan = false;
-    each_value(x, begin, end, [&](int, const float *v, auto n) {
-        float most = v[0];
 #pragma unroll
-        for (int j = 0; j < n.value; j++) most = fmaxf(most, v[j]), nan |= v[j] != v[j];
-        if constexpr (TOP) largest = fmaxf(largest, most);
-        if (most > t.m + kStale) {  // (also what leaves -inf)
-            const float d = fmaxf((t.m - most) * kLog2e, -1e30f), f = __builtin_amdgcn_exp2f(d);
-            t.u = (t.u + t.s * d) * f, t.s *= f, t.m = most;
-        }
+    for (int r = 0; r < kPieces; r++) {
+        if (r * NT < span.pieces) {
 #pragma unroll
-        for (int j = 0; j < n.value; j++) {
-            const float d = fmaxf((v[j] - t.m) * kLog2e, -1e30f), e = __builtin_amdgcn_exp2f(d);  // (-inf, and -inf against -inf: nothing)
-            t.s += e;
-            t.u = fmaf(e, d, t.u);
+            for (int j = 0; j < PER; j++) largest = fmaxf(largest, to_float(x[r].t[j]));
         }
-    });
-    for (int o = 1; o < kWave; o *= 2) t = merged(t, {__shfl_xor(t.m, o), __shfl_xor(t.s, o), __shfl_xor(t.u, o)});
-    if (threadIdx.x % kWave == 0) wave_stats[threadIdx.x / kWave] = t;
-    const uint64_t any_nan = __ballot(nan);
-    if (threadIdx.x % kWave == 0) wave_nan[threadIdx.x / kWave] = any_nan != 0;
+    }
+    ScoreStats t = {wave_reduce<true>(largest), 0.0f, 0.0f};
+    // (a wave of -inf only sums nothing: against any finite reference.  NaN, and +inf against itself, make the sum NaN.)
+    const float m = t.m == -__builtin_inff() ? 0.0f : t.m;
+#pragma unroll
+    for (int r = 0; r < kPieces; r++) {
+        if (r * NT < span.pieces) {
+            asm volatile("" : "+v"(x[r].raw));  // (converted again: 128 floats do not stay)
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const float d = (to_float(x[r].t[j]) - m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+                t.s += e;
+                t.u = fmaf(e, fmaxf(d, -1e30f), t.u);  // (zero times -inf is to be zero)
+            }
+        }
+    }
+    t.s = wave_reduce<false>(t.s), t.u = wave_reduce<false>(t.u);
+    if (lane == 0) wave_stats[wave] = t;
+    if constexpr (TOP) {
+        sh.most[threadIdx.x] = value_key(largest);
+        if (threadIdx.x == 0) sh.count = 0;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kScoreWaves; w++) t = merged(t, wave_stats[w]), wave_nan[0] |= wave_nan[w];
-        if (wave_nan[0]) t.s = __builtin_nanf("");
-        if (a.chunks == 1) done[0] = t.m, done[1] = finish_row<T>(a, row, t);
-        else a.part[(int64_t)row * a.chunks + nth] = t;
+    if (!TOP || threadIdx.x == 0) {
+        if (threadIdx.x == 0) {
+            t = wave_stats[0];
+            for (int w = 1; w < W; w++) t = merged(t, wave_stats[w]);
+            if (a.chunks == 1) done[0] = t.m, done[1] = finish_row(a, row, t, target, at_target);
+            else a.part[(int64_t)row * a.chunks + nth] = t;
+        }
+        if (!TOP) return;
     }
     if constexpr (TOP) {
-        if (a.chunks > 1) {
-            top_of(x, begin, end, a.top, largest, sh, a.part_keys + ((int64_t)row * a.chunks + nth) * a.top);
+        // the lower bound: largest prefix of sixteen bits that `top` groups reach, found by every wave for itself
+        uint32_t group = sh.most[lane];
+#pragma unroll
+        for (int w = 1; w < W; w++) group = max(group, sh.most[w * kWave + lane]);
+        uint32_t bound = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 16; bit--) {
+            const uint32_t to = bound | 1u << bit;
+            if (__popcll(__ballot(group >= to)) >= a.top) bound = to;
+        }
+        bool nan = false;
+        for (int w = 0; w < W; w++) nan |= !(wave_stats[w].s >= 0.0f);
+        if (!nan) {
+#pragma unroll
+            for (int r = 0; r < kPieces; r++) {
+                if (r * NT >= span.pieces) break;
+                float most = to_float(x[r].t[0]);
+#pragma unroll
+                for (int j = 1; j < PER; j++) most = fmaxf(most, to_float(x[r].t[j]));
+                if (value_key(most) < bound) continue;
+                const int i = span.first + (r * NT + (int)threadIdx.x) * PER;
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const float v = to_float(x[r].t[j]);
+                    if (value_key(v) >= bound && i + j >= 0 && i + j < span.length) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kCandidates) sh.key[at] = full_key(v, begin + i + j);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const int count = sh.count;
+        uint64_t *part = a.part_keys + ((int64_t)row * a.chunks + nth) * a.top;
+        const float dm = done[0], sum2 = done[1];
+        auto found = [&](int rank, uint64_t key) {
+            if (a.chunks > 1) part[rank] = key;
+            else write_top(a, row, rank, key, dm, sum2);
+        };
+        if (!nan && count <= kCandidates) {
+            rank_keys<NT>(sh.key, count, a.top, found);
+            if (a.chunks > 1)  // (a chunk shorter than that)
+                for (int i = count + (int)threadIdx.x; i < a.top; i += NT) part[i] = 0;
         } else {
-            top_of(x, begin, end, a.top, largest, sh, best);
-            __syncthreads();
-            write_top(a, row, best, done[0], done[1]);
+            if (a.chunks > 1)
+                for (int i = span.length + (int)threadIdx.x; i < a.top; i += NT) part[i] = 0;
+            search_keys<T, NT>(span, begin, a.top, sh.best, found);
         }
     }
 }
 
 // The chunks of a row together.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) score_join(ScoreArgs a)
+__global__ void __launch_bounds__(256) score_join(ScoreArgs a)
 {
-    __shared__ uint64_t key[TOP ? kCandidates * 2 : 1], best[kTopMost];
+    __shared__ uint64_t key[TOP ? 2 * kCandidates : 1];  // (of 2^20 values in 32 bits there are 17 chunks)
     __shared__ float done[2];
     const int row = blockIdx.x;
-    if (threadIdx.x < kWave) {
-        ScoreStats t = {-__builtin_inff(), 0.0f, 0.0f};
-        for (int i = threadIdx.x; i < a.chunks; i += kWave) t = merged(t, a.part[(int64_t)row * a.chunks + i]);
-        for (int o = 1; o < kWave; o *= 2) t = merged(t, {__shfl_xor(t.m, o), __shfl_xor(t.s, o), __shfl_xor(t.u, o)});
-        if (threadIdx.x == 0) done[0] = t.m, done[1] = finish_row<T>(a, row, t);
+    if (threadIdx.x == 0) {
+        ScoreStats t = a.part[(int64_t)row * a.chunks];
+        for (int i = 1; i < a.chunks; i++) t = merged(t, a.part[(int64_t)row * a.chunks + i]);
+        const int64_t target = a.targets[row];
+        done[0] = t.m, done[1] = finish_row(a, row, t, target, target_logit<T>(a, row, target));
     }
     if constexpr (TOP) {
         const int count = a.chunks * a.top;
-        for (int i = threadIdx.x; i < count; i += kScoreThreads) key[i] = a.part_keys[(int64_t)row * count + i];
+        for (int i = threadIdx.x; i < count; i += 256) key[i] = a.part_keys[(int64_t)row * count + i];
         __syncthreads();
-        rank_keys(key, count, a.top, best);
-        __syncthreads();
-        write_top(a, row, best, done[0], done[1]);
+        rank_keys<256>(key, count, a.top, [&](int rank, uint64_t k) { write_top(a, row, rank, k, done[0], done[1]); });
     }
 }
 
+// The gradient, a piece per thread: pieces of dx lie as those of x do where their rows are aligned alike, else value by value.
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads) score_grad(ScoreArgs a)
+__global__ void __launch_bounds__(256) score_grad(ScoreArgs a)
 {
     constexpr int PER = 16 / sizeof(T);
     const int row = blockIdx.x / a.chunks, nth = blockIdx.x % a.chunks;
     const int begin = nth * a.chunk, end = min(a.vocab, begin + a.chunk);
-    const T *x = (const T *)a.x + row * a.row_stride;
-    T *dx = (T *)a.dx + row * a.dx_stride;
+    const Span<T> span((const T *)a.x + row * a.row_stride, begin, end);
+    T *dx = (T *)a.dx + row * a.dx_stride + begin;
     const float *s = a.stats + 4 * (int64_t)row;
     const float m = s[0], sum2 = s[1], entropy = s[2];
     const int64_t target = a.targets[row];
     const float ga = a.grad_logprob && target >= 0 ? a.grad_logprob[row] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[row] : 0.0f;
-    auto one = [&](int i, float v) {
-        const float q = fmaxf(fmaf(v - m, kLog2e, -sum2), -1e30f), p = __builtin_amdgcn_exp2f(q);
-        const float g = -p * (ga + gb * (q * kLn2 + entropy));
-        return i == target ? g + ga : g;
-    };
-    // (rows of dx and of x may be aligned differently: stores as wide as both allow)
-    const bool wide = (((uintptr_t)(x + begin) | (uintptr_t)(dx + begin)) & 15) == 0;
-    const int body = wide ? begin + (end - begin) / PER * PER : begin;
-    for (int i = begin + threadIdx.x * PER; i < body; i += kScoreThreads * PER) {
-        union {
-            uint4v raw;
-            T t[PER];
-        } w;
-        w.raw = *(const uint4v *)(x + i);
+    const int hit = target >= begin && target < end ? (int)target - begin : -PER;
+    const bool alike = (((uintptr_t)span.at ^ (uintptr_t)(dx + span.first)) & 15) == 0;
+    for (int p = threadIdx.x; p < span.pieces; p += 256) {
+        const int i = span.first + p * PER;
+        Piece<T> w = span_piece(span, p);
+        float g[PER];
 #pragma unroll
-        for (int j = 0; j < PER; j++) w.t[j] = (T)one(i + j, to_float(w.t[j]));
-        *(uint4v *)(dx + i) = w.raw;
+        for (int j = 0; j < PER; j++) {
+            const float q = fmaxf(fmaf(to_float(w.t[j]) - m, kLog2e, -sum2), -1e30f);
+            g[j] = -__builtin_amdgcn_exp2f(q) * (ga + gb * (q * kLn2 + entropy));
+        }
+        if (hit >= i && hit < i + PER) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) g[j] += i + j == hit ? ga : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; j++) w.t[j] = (T)g[j];
+        if (alike && i >= 0 && i + PER <= span.length) {
+            *(uint4v *)(dx + i) = w.raw;
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                if (i + j >= 0 && i + j < span.length) dx[i + j] = w.t[j];
+        }
     }
-    for (int i = body + threadIdx.x; i < end; i += kScoreThreads) dx[i] = (T)one(i, to_float(x[i]));
 }
 
 namespace {
 
-constexpr int64_t kScoreBlocks = 512;  // blocks that a launch over few rows is cut into ...
-constexpr int64_t kScoreChunk = 1024;  // ... of that many values at least
 constexpr int64_t kGradChunk = 8192;
 
-// Chunks of a row: one, as long as there are rows enough; as many as their most likely tokens' list holds at most.
-int64_t score_chunks(int64_t rows, int64_t vocab, int64_t top)
+// Threads to a row, and chunks of it.  Blocks of 256 threads, of which several share a CU, where there are rows enough for all CUs
+// and they fit; else of 1024: a row's latency is what counts, or its length.
+struct ScorePlan {
+    int threads;
+    int64_t chunks, chunk;
+};
+
+constexpr int64_t kManyRows = 512;
+
+ScorePlan score_plan(int64_t rows, int64_t vocab, int dtype)
 {
-    int64_t n = rows ? kScoreBlocks / rows : 1;
-    n = n < 1 ? 1 : n;
-    const int64_t most = (vocab + kScoreChunk - 1) / kScoreChunk;
-    n = n < most ? n : most;
-    if (top > 0 && n > 2 * kCandidates / top) n = 2 * kCandidates / top;
-    return n;
+    const int64_t per = dtype == KVMIX_F32 ? 4 : 8;
+    const int threads = rows >= kManyRows && vocab <= (256 * kPieces - 1) * per ? 256 : 1024;
+    const int64_t most = (threads * kPieces - 1) * per;  // (a piece for a row that is not aligned)
+    const int64_t chunks = (vocab + most - 1) / most;
+    return {threads, chunks, chunks > 1 ? ((vocab + chunks - 1) / chunks + 7) / 8 * 8 : vocab};
 }
 
 int64_t chunk_of(int64_t vocab, int64_t chunks) { return ((vocab + chunks - 1) / chunks + 7) / 8 * 8; }
@@ -334,8 +388,8 @@ int score_check(const kvmix_token_logprobs_t *p)
     if (!p) return KVMIX_ERR_NULL;
     if (p->dtype != KVMIX_F16 && p->dtype != KVMIX_F32 && p->dtype != KVMIX_BF16) return KVMIX_ERR_DTYPE;
     if (p->rows < 0 || p->vocab < 0 || p->top < 0 || (p->rows > 1 && p->row_stride < p->vocab)) return KVMIX_ERR_SHAPE;
-    if (p->top > kTopMost || p->top > p->vocab || p->vocab > (1 << 30) || p->vocab == 0) return KVMIX_ERR_UNSUPPORTED;
-    if ((__int128)p->rows * ((p->vocab + kScoreChunk - 1) / kScoreChunk) > 0x7fffffff) return KVMIX_ERR_UNSUPPORTED;
+    if (p->top > kTopMost || p->top > p->vocab || p->vocab > (1 << 20) || p->vocab == 0) return KVMIX_ERR_UNSUPPORTED;
+    if ((__int128)p->rows * ((p->vocab + kGradChunk - 1) / kGradChunk) > 0x7fffffff) return KVMIX_ERR_UNSUPPORTED;
     return KVMIX_OK;
 }
 
@@ -355,7 +409,7 @@ using namespace kvmix;
 extern "C" int64_t kvmix_token_logprobs_workspace_bytes(const kvmix_token_logprobs_t *p)
 {
     if (score_check(p) != KVMIX_OK) return 0;
-    const int64_t n = score_chunks(p->rows, p->vocab, p->top);
+    const int64_t n = score_plan(p->rows, p->vocab, p->dtype).chunks;
     return n > 1 ? p->rows * n * (p->top * 8 + (int64_t)sizeof(ScoreStats)) : 0;
 }
 
@@ -371,19 +425,24 @@ extern "C" int kvmix_token_logprobs(const kvmix_token_logprobs_t *p, void *works
     a.x = p->logits, a.row_stride = p->row_stride, a.targets = p->targets;
     a.logprob = p->logprob, a.entropy = p->entropy, a.top_logprob = p->top_logprob, a.top_id = p->top_id, a.stats = p->stats;
     a.rows = (int)p->rows, a.vocab = (int)p->vocab, a.top = (int)p->top;
-    a.chunks = (int)score_chunks(p->rows, p->vocab, p->top);
-    a.chunk = (int)chunk_of(p->vocab, a.chunks);
+    const ScorePlan plan = score_plan(p->rows, p->vocab, p->dtype);
+    a.chunks = (int)plan.chunks, a.chunk = (int)plan.chunk;
     a.part_keys = (uint64_t *)workspace;
     a.part = (ScoreStats *)((uint64_t *)workspace + p->rows * a.chunks * p->top);
     hipStream_t st = (hipStream_t)stream;
     with_type(p->dtype, [&](auto zero) {
         using T = decltype(zero);
         const unsigned grid = (unsigned)(p->rows * a.chunks);
-        if (p->top) score_rows<T, true><<<grid, kScoreThreads, 0, st>>>(a);
-        else score_rows<T, false><<<grid, kScoreThreads, 0, st>>>(a);
+        if (plan.threads == 256) {
+            if (p->top) score_rows<T, 256, true><<<grid, 256, 0, st>>>(a);
+            else score_rows<T, 256, false><<<grid, 256, 0, st>>>(a);
+        } else {
+            if (p->top) score_rows<T, 1024, true><<<grid, 1024, 0, st>>>(a);
+            else score_rows<T, 1024, false><<<grid, 1024, 0, st>>>(a);
+        }
         if (a.chunks > 1) {
-            if (p->top) score_join<T, true><<<(unsigned)p->rows, kScoreThreads, 0, st>>>(a);
-            else score_join<T, false><<<(unsigned)p->rows, kScoreThreads, 0, st>>>(a);
+            if (p->top) score_join<T, true><<<(unsigned)p->rows, 256, 0, st>>>(a);
+            else score_join<T, false><<<(unsigned)p->rows, 256, 0, st>>>(a);
         }
     });
     return launch_status();
@@ -403,6 +462,6 @@ extern "C" int kvmix_token_logprobs_grad(const kvmix_token_logprobs_t *p, const 
     a.chunks = (int)((p->vocab + kGradChunk - 1) / kGradChunk);
     a.chunk = (int)chunk_of(p->vocab, a.chunks);
     a.grad_logprob = grad_logprob, a.grad_entropy = grad_entropy, a.dx = grad_logits, a.dx_stride = grad_row_stride;
-    with_type(p->dtype, [&](auto zero) { score_grad<decltype(zero)><<<(unsigned)(p->rows * a.chunks), kScoreThreads, 0, (hipStream_t)stream>>>(a); });
+    with_type(p->dtype, [&](auto zero) { score_grad<decltype(zero)><<<(unsigned)(p->rows * a.chunks), 256, 0, (hipStream_t)stream>>>(a); });
     return launch_status();
 }
