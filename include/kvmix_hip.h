@@ -580,8 +580,8 @@ typedef struct kvmix_paged_plan {
     int64_t tokens;                              /* new tokens of all sequences */
     int64_t heads, kv_heads, head_dim, page_size, table_stride;
     int64_t row_pages, packed_pages;             /* pages that the pools must have at least */
-    int64_t slots_at, seqs_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
-    int64_t few, tiles, joins;                   /* items per kv head: of a few query rows, of many, rows to be joined */
+    int64_t slots_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
+    int64_t few, columns, tiles, joins;          /* per kv head: items of a few query rows, blocks that share them, items of many, rows to be joined */
     int64_t few_rows;                            /* query rows of an item of few: 16 or 32 */
     int64_t part_rows;                           /* rows of partial results per kv head */
 } kvmix_paged_plan_t;

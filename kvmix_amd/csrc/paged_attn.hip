@@ -17,10 +17,17 @@ namespace kvmix {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr int kItemWords = 6;  // sequence, first row, rows, first and last block (tile), part (-1: the whole sequence)
-constexpr int kSeqWords = 4;   // first new token, new tokens, tokens, packed tokens
+// sequence, first row, rows, first and last block (tile), part (-1: the whole sequence); of the sequence: first new token, new
+// tokens, tokens, packed tokens (here, so that what a block needs is one load away); in paged_few, with the first item of a block,
+// how many it has and where the others begin
+constexpr int kItemWords = 12;
+constexpr float kShrink = 0.015625f;  // of queries in paged_few: their products with keys' scales stay in fp16's range up to 4e6
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// The plan's words: nobody writes them while a kernel runs, so they are read through the scalar cache (as ordinary memory every
+// look at a page table waited for all loads in flight).
+typedef const __attribute__((address_space(4))) int32_t *PlanWords;
 
 struct PagedArgs {
     const _Float16 *q;
@@ -28,7 +35,7 @@ struct PagedArgs {
     int64_t q_ts, q_hs, o_ts, o_hs;
     const _Float16 *rows;
     const uint32_t *packed;
-    const int32_t *seqs, *table, *items;
+    PlanWords table, items;
     int table_stride, kv_heads, group, blocks_log2;  // blocks_log2: of 32 tokens to a page
     float scale;                                     // with log2(e)
     float *part;                                     // [kv heads][part_rows][D], relative to the maximum in part_ml
@@ -37,13 +44,13 @@ struct PagedArgs {
 };
 
 struct PagedItem {
-    int seq, row0, rows, begin, end, part;
+    int seq, row0, rows, begin, end, part, q_start, q_len, kv_len, packed, items, next;
 };
 
-__device__ __forceinline__ PagedItem item_of(const int32_t *items, int nth)
+__device__ __forceinline__ PagedItem item_of(PlanWords items, int nth)
 {
-    const int32_t *p = items + nth * kItemWords;
-    return {p[0], p[1], p[2], p[3], p[4], p[5]};
+    const PlanWords p = items + nth * kItemWords;
+    return {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11]};
 }
 
 // the larger of a lane's and those of the lanes with its place in the other rows of sixteen
@@ -78,14 +85,17 @@ __device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uin
     load_words<D / 32>(at + D * (KB + VB), lane, b.side);
 }
 
-// Few rows.  Every wave of a block takes every fourth block of 32 tokens of the item's span, sixteen (NR times) rows of queries
+// Few rows.  A block works through the items of its column (parts of sequences that add up to the same number of tokens for every
+// column).  Every wave takes every fourth block of 32 tokens of an item's span, sixteen (NR times) rows of queries
 // at once, with v_mfma_f32_16x16x32: the logits transposed (tokens as rows of the result), so that a lane holds those of one query
 // and its probabilities are the operand of out^T = v^T p^T as they are.  Codes go from memory to registers, a block ahead, become
 // fp16 there and are used once.
 template <int D, int KB, int VB, int NR>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_few(PagedArgs a)
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 3 : 2))) paged_few(PagedArgs a)
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
+    constexpr bool kScaleQueries = NR == 1;
+    constexpr int DEPTH = KB + VB > 6 ? 2 : KB + VB > 3 ? 3 : 4;  // blocks in flight
     constexpr int kPad = D + 4;
     __shared__ union {
         uint32_t side[4][2 * D];
@@ -95,195 +105,229 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         } join;
     } lds;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
-    const int head = blockIdx.x % a.kv_heads;
-    const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
-    const int32_t *seq = a.seqs + it.seq * kSeqWords;
-    const int q_start = seq[0], q_len = seq[1], kv_len = seq[2], packed = seq[3];
-    const int32_t *table = a.table + it.seq * a.table_stride;
+    const int head = blockIdx.x % a.kv_heads, column = blockIdx.x / a.kv_heads;
     const int per_page = 1 << a.blocks_log2;
+    const float scale = a.scale / kShrink;
+    const Exponents<KB> ke;
+    const Exponents<VB> ve;
 
-    half8v q[NR][KS];
-    int limit[NR];  // the row's own token
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        const int r = it.row0 + min(16 * n + m, it.rows - 1), token = r / a.group;
-        limit[n] = kv_len - q_len + token;
-        const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * g;
-#pragma unroll
-        for (int s = 0; s < KS; s++) q[n][s] = *(const half8v *)(at + 32 * s);
-    }
-    const int first_limit = kv_len - q_len + it.row0 / a.group;
+    PagedItem it = item_of(a.items, column);
+    const int items = it.items, next = it.next;
+    for (int nth = 0; nth < items; nth++) {
+        if (nth) it = item_of(a.items, next + nth - 1);
+        const int q_start = it.q_start, q_len = it.q_len, kv_len = it.kv_len, packed = it.packed;
+        const PlanWords table = a.table + it.seq * a.table_stride;
 
-    floatx4 acc[NR][DT];
-    float top[NR], sum[NR];
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        top[n] = -1e30f, sum[n] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DT; t++) acc[n][t] = floatx4{};
-    }
-
-    // a block's logits to probabilities; the maximum is moved when some row's has grown by more than 2^8 (they stay well inside
-    // fp16's range below that)
-    auto probabilities = [&](floatx4 (&x)[2][NR], half8v (&p)[NR], int block) {
-        if (block * kBlock + kBlock - 1 > first_limit) {
-#pragma unroll
-            for (int n = 0; n < NR; n++) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (block * kBlock + 8 * g + i > limit[n]) x[i / 4][n][i % 4] = -__builtin_inff();
-            }
-        }
+        half8v q[NR][KS];
+        int limit[NR];  // the row's own token
 #pragma unroll
         for (int n = 0; n < NR; n++) {
-            float most = x[0][n][0];
+            const int r = it.row0 + min(16 * n + m, it.rows - 1), token = r / a.group;
+            limit[n] = kv_len - q_len + token;
+            const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * g;
 #pragma unroll
-            for (int i = 1; i < 8; i++) most = fmaxf(most, x[i / 4][n][i % 4]);
-            most *= a.scale;
-            if (__any(most > top[n] + 8.0f)) {
-                const float grown = fmaxf(top[n], max_of_rows(most));
-                const float shrink = __builtin_amdgcn_exp2f(top[n] - grown);
-                top[n] = grown;
-                sum[n] *= shrink;
-#pragma unroll
-                for (int t = 0; t < DT; t++) acc[n][t] *= shrink;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[i / 4][n][i % 4], a.scale, -top[n]));
-                if (i % 2) sum[n] = __builtin_amdgcn_fdot2(half2v{p[n][i - 1], p[n][i]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum[n], false);
-            }
+            for (int s = 0; s < KS; s++) q[n][s] = *(const half8v *)(at + 32 * s) * (_Float16)kShrink;
         }
-    };
+        const int first_limit = kv_len - q_len + it.row0 / a.group;
 
-    auto take_packed = [&](const PackedBlock<D, KB, VB> &b, int block) {
-        uint32_t *side = lds.side[wave];
-        store_words<D / 32>(side, lane, b.side);
-        __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
-        const _Float16 *sides = (const _Float16 *)side + 8 * g;
-        floatx4 x[2][NR] = {};
+        floatx4 acc[NR][DT];
+        float top[NR], sum[NR];
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const half8v scale = *(const half8v *)(sides + 32 * s), zero = *(const half8v *)(sides + D + 32 * s);
+        for (int n = 0; n < NR; n++) {
+            top[n] = -1e30f, sum[n] = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const half8v k = piece_values<KB, NK>(b.k, u * KS + s, scale, zero);
-#pragma unroll
-                for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
-            }
+            for (int t = 0; t < DT; t++) acc[n][t] = floatx4{};
         }
-        half8v p[NR];
-        probabilities(x, p, block);
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const half8v scale = *(const half8v *)(sides + 2 * D + 32 * s), zero = *(const half8v *)(sides + 3 * D + 32 * s);
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const half8v v = piece_values<VB, NV>(b.v, 2 * s + u, scale, zero);
-#pragma unroll
-                for (int n = 0; n < NR; n++) acc[n][2 * s + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n], acc[n][2 * s + u], 0, 0, 0);
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-    };
 
-    const int packed_end = min(it.end, packed / kBlock);
-    auto packed_at = [&](int block) {
-        const int64_t page = table[block >> a.blocks_log2];
-        return a.packed + (((page * a.kv_heads + head) << a.blocks_log2) + (block & (per_page - 1))) * block_words(D, KB, VB);
-    };
-    int block = it.begin + wave;
-    if (block < packed_end) {
-        PackedBlock<D, KB, VB> one, two;
-        load_packed(one, packed_at(block), lane);
-        while (true) {
-            if (block + 4 < packed_end) load_packed(two, packed_at(block + 4), lane);
-            take_packed(one, block);
-            block += 4;
-            if (block >= packed_end) break;
-            if (block + 4 < packed_end) load_packed(one, packed_at(block + 4), lane);
-            take_packed(two, block);
-            block += 4;
-            if (block >= packed_end) break;
-        }
-    }
-    for (; block < it.end; block += 4) {
-        const int64_t page = table[block >> a.blocks_log2];
-        const int64_t P = kBlock << a.blocks_log2;
-        const _Float16 *keys = a.rows + (page * a.kv_heads + head) * 2 * P * D + (block & (per_page - 1)) * kBlock * D;
-        const _Float16 *values = keys + P * D;
-        floatx4 x[2][NR] = {};
-        half8v v[DT];
+        // a block's logits to probabilities; the maximum is moved when some row's has grown by more than 2^8 (they stay well inside
+        // fp16's range below that)
+        auto probabilities = [&](floatx4 (&x)[2][NR], half8v (&p)[NR], int block, auto packed_tokens) {
+            if (!packed_tokens.value && block * kBlock + kBlock - 1 > first_limit) {  // (every new token sees all packed ones)
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
+                for (int n = 0; n < NR; n++) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const half8v k = *(const half8v *)(keys + (8 * (m / 4) + 4 * u + m % 4) * D + 32 * s + 8 * g);
-                v[2 * s + u] = *(const half8v *)(values + (16 * (2 * s + u) + m) * kBlock + 8 * g);
+                    for (int i = 0; i < 8; i++)
+                        if (block * kBlock + 8 * g + i > limit[n]) x[i / 4][n][i % 4] = -__builtin_inff();
+                }
+            }
 #pragma unroll
-                for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+            for (int n = 0; n < NR; n++) {
+                float most = x[0][n][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) most = fmaxf(most, x[i / 4][n][i % 4]);
+                most *= scale;
+                if (__any(most > top[n] + 8.0f)) {
+                    const float grown = fmaxf(top[n], max_of_rows(most));
+                    const float shrink = __builtin_amdgcn_exp2f(top[n] - grown);
+                    top[n] = grown;
+                    sum[n] *= shrink;
+#pragma unroll
+                    for (int t = 0; t < DT; t++) acc[n][t] *= shrink;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[i / 4][n][i % 4], scale, -top[n]));
+                    if (i % 2) sum[n] = __builtin_amdgcn_fdot2(half2v{p[n][i - 1], p[n][i]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum[n], false);
+                }
+            }
+        };
+
+        auto take_packed = [&](const PackedBlock<D, KB, VB> &b) {
+            uint32_t *side = lds.side[wave];
+            store_words<D / 32>(side, lane, b.side);
+            __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+            const _Float16 *sides = (const _Float16 *)side + 8 * g;
+            floatx4 x[2][NR] = {};
+            if constexpr (kScaleQueries) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) x[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8v *)(sides + D + 32 * s), q[0][s], x[0][0], 0, 0, 0);
+                x[1][0] = x[0][0];
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const half8v scales = *(const half8v *)(sides + 32 * s);
+                if constexpr (kScaleQueries) {
+                    const half8v scaled = q[0][s] * scales;
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece_codes<KB, NK>(b.k, u * KS + s, ke), scaled, x[u][0], 0, 0, 0);
+                } else {
+                    const half8v zeros = *(const half8v *)(sides + D + 32 * s);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const half8v k = piece_values<KB, NK>(b.k, u * KS + s, scales, zeros, ke);
+#pragma unroll
+                        for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+                    }
+                }
+            }
+            half8v p[NR];
+            probabilities(x, p, 0, std::true_type());
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const half8v scales = *(const half8v *)(sides + 2 * D + 32 * s), zeros = *(const half8v *)(sides + 3 * D + 32 * s);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const half8v v = piece_values<VB, NV>(b.v, 2 * s + u, scales, zeros, ve);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) acc[n][2 * s + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n], acc[n][2 * s + u], 0, 0, 0);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        };
+
+        const int packed_end = min(it.end, packed / kBlock);
+        int block = it.begin + wave;
+        if (block < packed_end) {
+            // The coming blocks are on their way while one is worked on.  Every turn loads one, past the end the last one again:
+            // with the loads under a condition each use waited for all of them.
+            const int last_block = packed_end - 1;
+            auto page_of = [&](int block) { return table[min(block, last_block) >> a.blocks_log2]; };
+            auto fetch = [&](PackedBlock<D, KB, VB> &to, int block, int page) {
+                const int in_page = min(block, last_block) & (per_page - 1);
+                load_packed(to, a.packed + ((((int64_t)page * a.kv_heads + head) << a.blocks_log2) + in_page) * block_words(D, KB, VB), lane);
+            };
+            PackedBlock<D, KB, VB> held[DEPTH];
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) fetch(held[i], block + 4 * i, page_of(block + 4 * i));
+            int page = page_of(block + 4 * DEPTH);
+            const int count = (packed_end - block + 3) / 4;
+            for (int turn = 0; turn < count / DEPTH; turn++) {
+#pragma unroll
+                for (int i = 0; i < DEPTH; i++) {
+                    take_packed(held[i]);
+                    fetch(held[i], block + 4 * DEPTH, page);
+                    block += 4;
+                    page = page_of(block + 4 * DEPTH);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < DEPTH - 1; i++) {
+                if (i < count % DEPTH) {
+                    take_packed(held[i]);
+                    block += 4;
+                }
             }
         }
-        half8v p[NR];
-        probabilities(x, p, block);
-        if (block * kBlock + kBlock > kv_len) {  // (whatever lies behind the last token: zero times it may not be zero)
+        for (; block < it.end; block += 4) {
+            const int64_t page = table[block >> a.blocks_log2];
+            const int64_t P = kBlock << a.blocks_log2;
+            const _Float16 *keys = a.rows + (page * a.kv_heads + head) * 2 * P * D + (block & (per_page - 1)) * kBlock * D;
+            const _Float16 *values = keys + P * D;
+            floatx4 x[2][NR] = {};
+            half8v v[DT];
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const half8v k = *(const half8v *)(keys + (8 * (m / 4) + 4 * u + m % 4) * D + 32 * s + 8 * g);
+                    v[2 * s + u] = *(const half8v *)(values + (16 * (2 * s + u) + m) * kBlock + 8 * g);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+                }
+            }
+            half8v p[NR];
+            probabilities(x, p, block, std::false_type());
+            if (block * kBlock + kBlock > kv_len) {  // (whatever lies behind the last token: zero times it may not be zero)
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (block * kBlock + 8 * g + j >= kv_len) v[t][j] = (_Float16)0.0f;
+                }
+            }
 #pragma unroll
             for (int t = 0; t < DT; t++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (block * kBlock + 8 * g + j >= kv_len) v[t][j] = (_Float16)0.0f;
+                for (int n = 0; n < NR; n++) acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], p[n], acc[n][t], 0, 0, 0);
             }
         }
-#pragma unroll
-        for (int t = 0; t < DT; t++) {
-#pragma unroll
-            for (int n = 0; n < NR; n++) acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], p[n], acc[n][t], 0, 0, 0);
-        }
-    }
 
-    // the four waves' sums together
-    __syncthreads();
+        // the four waves' sums together
+        __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NR; n++) {
-        const float total = sum_of_rows(sum[n]);
-        if (g == 0) lds.join.ml[wave][16 * n + m] = make_float2(top[n], total);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        float most = top[n];
-#pragma unroll
-        for (int w = 0; w < 4; w++) most = fmaxf(most, lds.join.ml[w][16 * n + m].x);
-        const float shrink = __builtin_amdgcn_exp2f(top[n] - most);
-#pragma unroll
-        for (int t = 0; t < DT; t++) *(floatx4 *)&lds.join.out[wave][16 * n + m][16 * t + 4 * g] = acc[n][t] * shrink;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < it.rows * (D / 8); i += 256) {
-        const int r = i / (D / 8), c = i % (D / 8) * 8;
-        float most = lds.join.ml[0][r].x, total = 0.0f;
-#pragma unroll
-        for (int w = 1; w < 4; w++) most = fmaxf(most, lds.join.ml[w][r].x);
-        floatx4 o[2] = {};
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            total += lds.join.ml[w][r].y * __builtin_amdgcn_exp2f(lds.join.ml[w][r].x - most);
-            o[0] += *(const floatx4 *)&lds.join.out[w][r][c];
-            o[1] += *(const floatx4 *)&lds.join.out[w][r][c + 4];
+        for (int n = 0; n < NR; n++) {
+            const float total = sum_of_rows(sum[n]);
+            if (g == 0) lds.join.ml[wave][16 * n + m] = make_float2(top[n], total);
         }
-        if (it.part >= 0) {
-            const int64_t to = head * a.part_rows + it.part + r;
-            *(floatx4 *)(a.part + to * D + c) = o[0];
-            *(floatx4 *)(a.part + to * D + c + 4) = o[1];
-            if (c == 0) a.part_ml[to] = make_float2(most, total);
-        } else {
-            const float inv = 1.0f / total;
-            half8v w;
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = (_Float16)(o[j / 4][j % 4] * inv);
-            const int token = (it.row0 + r) / a.group, h = head * a.group + (it.row0 + r) % a.group;
-            *(half8v *)(a.out + (int64_t)(q_start + token) * a.o_ts + (int64_t)h * a.o_hs + c) = w;
+        for (int n = 0; n < NR; n++) {
+            float most = top[n];
+#pragma unroll
+            for (int w = 0; w < 4; w++) most = fmaxf(most, lds.join.ml[w][16 * n + m].x);
+            const float shrink = __builtin_amdgcn_exp2f(top[n] - most);
+#pragma unroll
+            for (int t = 0; t < DT; t++) *(floatx4 *)&lds.join.out[wave][16 * n + m][16 * t + 4 * g] = acc[n][t] * shrink;
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < it.rows * (D / 8); i += 256) {
+            const int r = i / (D / 8), c = i % (D / 8) * 8;
+            float most = lds.join.ml[0][r].x, total = 0.0f;
+#pragma unroll
+            for (int w = 1; w < 4; w++) most = fmaxf(most, lds.join.ml[w][r].x);
+            floatx4 o[2] = {};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                total += lds.join.ml[w][r].y * __builtin_amdgcn_exp2f(lds.join.ml[w][r].x - most);
+                o[0] += *(const floatx4 *)&lds.join.out[w][r][c];
+                o[1] += *(const floatx4 *)&lds.join.out[w][r][c + 4];
+            }
+            if (it.part >= 0) {
+                const int64_t to = head * a.part_rows + it.part + r;
+                *(floatx4 *)(a.part + to * D + c) = o[0];
+                *(floatx4 *)(a.part + to * D + c + 4) = o[1];
+                if (c == 0) a.part_ml[to] = make_float2(most, total);
+            } else {
+                const float inv = 1.0f / total;
+                half8v w;
+#pragma unroll
+                for (int j = 0; j < 8; j++) w[j] = (_Float16)(o[j / 4][j % 4] * inv);
+                const int token = (it.row0 + r) / a.group, h = head * a.group + (it.row0 + r) % a.group;
+                *(half8v *)(a.out + (int64_t)(q_start + token) * a.o_ts + (int64_t)h * a.o_hs + c) = w;
+            }
+        }
+        __syncthreads();  // (the next item's scales go where these sums are)
     }
 }
 
@@ -312,9 +356,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int m = lane % 16, g = lane / 16;
     const int head = blockIdx.x % a.kv_heads;
     const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
-    const int32_t *seq = a.seqs + it.seq * kSeqWords;
-    const int q_start = seq[0], q_len = seq[1], kv_len = seq[2], packed_blocks = seq[3] / kBlock, blocks = (kv_len + kBlock - 1) / kBlock;
-    const int32_t *table = a.table + it.seq * a.table_stride;
+    const int q_start = it.q_start, q_len = it.q_len, kv_len = it.kv_len, packed_blocks = it.packed / kBlock, blocks = (kv_len + kBlock - 1) / kBlock;
+    const PlanWords table = a.table + it.seq * a.table_stride;
     const int per_page = 1 << a.blocks_log2;
 
     const int own = 32 * wave + col, r = it.row0 + min(own, it.rows - 1), token = r / a.group, limit = kv_len - q_len + token;
@@ -350,6 +393,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             }
         }
     };
+    const Exponents<KB> ke;
+    const Exponents<VB> ve;
     auto place = [&](int tile, int buf) {
         const int block = 2 * tile + which;
         uint8_t *to = lds[buf][matrix];
@@ -362,16 +407,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             store_words<D / 64>(sides[wave], lane, side);
             __builtin_amdgcn_wave_barrier();
             const _Float16 *s = (const _Float16 *)sides[wave] + 8 * g;
-            auto turn = [&](auto bits) {
+            auto turn = [&](const auto &e, auto bits) {
                 constexpr int B = decltype(bits)::value;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     const int set = matrix ? p / 2 : p % (D / 32);
-                    put(p, piece_values<B, lane_words(D, B)>(held, p, *(const half8v *)(s + 32 * set), *(const half8v *)(s + D + 32 * set)));
+                    put(p, piece_values<B, lane_words(D, B)>(held, p, *(const half8v *)(s + 32 * set), *(const half8v *)(s + D + 32 * set), e));
                 }
             };
-            if (matrix) turn(std::integral_constant<int, VB>());
-            else turn(std::integral_constant<int, KB>());
+            if (matrix) turn(ve, std::integral_constant<int, VB>());
+            else turn(ke, std::integral_constant<int, KB>());
             __builtin_amdgcn_wave_barrier();
         } else if (block < blocks) {
 #pragma unroll
@@ -485,32 +530,58 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
 }
 
-// The spans of one sequence's rows together: a row per wave; the item's `begin` is the number of spans, `end` the rows between them.
+// The spans of one sequence's rows together: a row per wave, or per block where there are many spans; the item's `begin` is the
+// number of spans, `end` the rows between them.  Bound by latency: spans are read eight at a time.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join(PagedArgs a)
 {
-    constexpr int PER = D / kWave;
+    constexpr int PER = D / kWave, kAhead = 8, kShared = 8;
+    typedef float floats __attribute__((ext_vector_type(PER)));
+    __shared__ floats sums[4][kWave];
+    __shared__ float totals[4];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int head = blockIdx.x % a.kv_heads;
     const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
-    const int q_start = a.seqs[it.seq * kSeqWords];
-    for (int r = blockIdx.y * 4 + wave; r < it.rows; r += 4 * gridDim.y) {
+    const int spans = it.begin;
+    const bool shared = spans > kShared;
+    const int step = shared ? 4 : 1, mine = shared ? wave : 0;
+    for (int r = shared ? blockIdx.y : blockIdx.y * 4 + wave; r < it.rows; r += gridDim.y * (shared ? 1 : 4)) {
         const int64_t first = head * a.part_rows + it.part + r;
         float most = -1e30f;
-        for (int i = lane; i < it.begin; i += kWave) most = fmaxf(most, a.part_ml[first + (int64_t)i * it.end].x);
+        for (int i = lane; i < spans; i += kWave) most = fmaxf(most, a.part_ml[first + (int64_t)i * it.end].x);
         most = wave_reduce<true>(most);
-        float total = 0.0f, o[PER] = {};
-        for (int i = 0; i < it.begin; i++) {
-            const int64_t at = first + (int64_t)i * it.end;
-            const float2 ml = a.part_ml[at];
-            const float w = __builtin_amdgcn_exp2f(ml.x - most);
-            total = fmaf(ml.y, w, total);
+        float total = 0.0f;
+        floats o = {};
+        for (int i0 = mine; i0 < spans; i0 += step * kAhead) {
+            float2 ml[kAhead];
+            floats x[kAhead];
 #pragma unroll
-            for (int j = 0; j < PER; j++) o[j] = fmaf(a.part[at * D + PER * lane + j], w, o[j]);
+            for (int i = 0; i < kAhead; i++) {
+                const int64_t at = first + (int64_t)min(i0 + i * step, spans - 1) * it.end;
+                ml[i] = a.part_ml[at];
+                x[i] = *(const floats *)(a.part + at * D + PER * lane);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                if (i0 + i * step < spans) {
+                    const float w = __builtin_amdgcn_exp2f(ml[i].x - most);
+                    total = fmaf(ml[i].y, w, total);
+                    o += x[i] * w;
+                }
+            }
+        }
+        if (shared) {
+            sums[wave][lane] = o;
+            if (lane == 0) totals[wave] = total;
+            __syncthreads();
+            o = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+            total = totals[0] + totals[1] + totals[2] + totals[3];
+            __syncthreads();
+            if (wave) continue;
         }
         const float inv = 1.0f / total;
         const int row = it.row0 + r;
-        _Float16 *to = a.out + (int64_t)(q_start + row / a.group) * a.o_ts + (int64_t)(head * a.group + row % a.group) * a.o_hs + PER * lane;
+        _Float16 *to = a.out + (int64_t)(it.q_start + row / a.group) * a.o_ts + (int64_t)(head * a.group + row % a.group) * a.o_hs + PER * lane;
 #pragma unroll
         for (int j = 0; j < PER; j++) to[j] = (_Float16)(o[j] * inv);
     }
@@ -518,17 +589,21 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a)
 
 namespace {
 
-constexpr int64_t kFewMost = 32;      // rows of a sequence and kv head that go to paged_few
-constexpr int64_t kFewLaunch = 1024;  // blocks that its launch aims at ...
-constexpr int64_t kFewSpan = 8;       // ... of that many blocks of tokens at least
+constexpr int64_t kFewMost = 32;    // rows of a sequence and kv head that go to paged_few
+constexpr int64_t kFewUnit = 4;     // blocks of tokens, one to a wave: what its launch is cut by ...
+constexpr int64_t kFewLeast = 2;    // ... of which a column has that many at least
 constexpr int64_t kTileLaunch = 1024;
-constexpr int64_t kTileSpan = 8;      // tiles
+constexpr int64_t kTileSpan = 8;    // tiles
+
+// Blocks of paged_few that the chip holds at once: three to a CU by their registers (sixteen rows), or two (32).
+int64_t few_resident(int64_t rows) { return rows > 16 ? 512 : 768; }
 
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Span {
-    int32_t word[kItemWords];
+    int32_t word[6];
     int64_t cost;
+    int32_t items = 0, next = 0;
 };
 
 int batch_check(const kvmix_paged_batch_t *b)
@@ -549,7 +624,7 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
     *plan = kvmix_paged_plan_t{};
     plan->heads = b->heads, plan->kv_heads = b->kv_heads, plan->head_dim = b->head_dim, plan->page_size = P;
     plan->table_stride = b->table_stride;
-    int64_t few_cost = 0, tile_cost = 0;
+    int64_t few_units = 0, tile_cost = 0;
     plan->few_rows = 16;
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], pk = b->packed_lens[s], n = b->q_lens[s];
@@ -563,7 +638,7 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         }
         plan->tokens += n;
         if (n * G <= kFewMost) {
-            few_cost += n ? (kv + kBlock - 1) / kBlock : 0;
+            few_units += n ? (kv + kFewUnit * kBlock - 1) / (kFewUnit * kBlock) : 0;
             if (n * G > 16) plan->few_rows = kFewMost;
         } else {
             for (int64_t r = 0; r < n * G; r += kTileRows)
@@ -571,7 +646,10 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         }
     }
     if ((__int128)plan->row_pages * P > kMost32) return KVMIX_ERR_UNSUPPORTED;
-    const int64_t few_span = std::max(kFewSpan, up((few_cost * b->kv_heads + kFewLaunch - 1) / kFewLaunch, 4));
+    // One round of blocks: as many columns as the chip holds blocks, each of the same number of units, whatever sequences they
+    // are of.  (Spans of sequences as the items, the longest first, left a second round of a few: of 1048 blocks of which 1024
+    // fit 85 us instead of @@, of 1248 75 instead of @@.)
+    const int64_t few_columns = std::min(std::max<int64_t>(few_resident(plan->few_rows) / b->kv_heads, 1), (few_units + kFewLeast - 1) / kFewLeast);
     const int64_t tile_span = std::max(kTileSpan, (tile_cost * b->kv_heads + kTileLaunch - 1) / kTileLaunch);
 
     std::vector<Span> few, tiles, joins;
@@ -588,11 +666,31 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         }
         return part <= kMostTokens;
     };
+    std::vector<int32_t> columns;
+    int64_t column_end = 0, unit = 0;  // units up to and with the column that is being filled, units dealt
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], n = b->q_lens[s], rows = n * G;
         if (n == 0) continue;
         if (rows <= kFewMost) {
-            if (!cut(few, s, 0, rows, (kv + kBlock - 1) / kBlock, up(few_span, 4), rows)) return KVMIX_ERR_UNSUPPORTED;
+            const int64_t blocks = (kv + kBlock - 1) / kBlock, units = (blocks + kFewUnit - 1) / kFewUnit;
+            const size_t first = few.size();
+            for (int64_t at = 0; at < units;) {
+                if (unit == column_end) {
+                    columns.push_back((int32_t)few.size());
+                    column_end = few_units * (int64_t)columns.size() / few_columns;
+                    continue;
+                }
+                const int64_t here = std::min(units - at, column_end - unit);
+                few.push_back({{(int32_t)s, 0, (int32_t)rows, (int32_t)(at * kFewUnit), (int32_t)std::min((at + here) * kFewUnit, blocks), -1}, here});
+                at += here, unit += here;
+            }
+            const int64_t spans = (int64_t)(few.size() - first);
+            if (spans > 1) {
+                for (int64_t i = 0; i < spans; i++) few[first + i].word[5] = (int32_t)(part + i * rows);
+                joins.push_back({{(int32_t)s, 0, (int32_t)rows, (int32_t)spans, (int32_t)rows, (int32_t)part}, rows});
+                part += spans * rows;
+            }
+            if (part > kMostTokens) return KVMIX_ERR_UNSUPPORTED;
         } else {
             for (int64_t r = 0; r < rows; r += kTileRows) {
                 const int64_t here = std::min<int64_t>(kTileRows, rows - r);
@@ -600,9 +698,23 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
             }
         }
     }
+    plan->columns = (int64_t)columns.size();
+    {
+        // the first item of every column, then the others
+        columns.push_back((int32_t)few.size());
+        std::vector<Span> firsts, others;
+        for (size_t c = 0; c + 1 < columns.size(); c++) {
+            firsts.push_back(few[columns[c]]);
+            firsts.back().items = columns[c + 1] - columns[c];
+            firsts.back().next = (int32_t)(plan->columns + others.size());
+            others.insert(others.end(), few.begin() + columns[c] + 1, few.begin() + columns[c + 1]);
+        }
+        few = std::move(firsts);
+        few.insert(few.end(), others.begin(), others.end());
+    }
     if (std::max({few.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMost32) return KVMIX_ERR_UNSUPPORTED;
     // the longest first: what ends a launch is short then
-    for (auto *list : {&few, &tiles}) std::stable_sort(list->begin(), list->end(), [](const Span &x, const Span &y) { return x.cost > y.cost; });
+    std::stable_sort(tiles.begin(), tiles.end(), [](const Span &x, const Span &y) { return x.cost > y.cost; });
     plan->few = (int64_t)few.size(), plan->tiles = (int64_t)tiles.size(), plan->joins = (int64_t)joins.size(), plan->part_rows = part;
     int64_t at = 0;
     auto take = [&](int64_t n) {
@@ -611,7 +723,6 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         return was;
     };
     plan->slots_at = take(plan->tokens);
-    plan->seqs_at = take(b->sequences * kSeqWords);
     plan->table_at = take(b->sequences * b->table_stride);
     plan->few_at = take(plan->few * kItemWords);
     plan->tile_at = take(plan->tiles * kItemWords);
@@ -621,16 +732,22 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
     if (!words) return KVMIX_OK;
     if (capacity < at) return KVMIX_ERR_WORKSPACE;
     std::fill(words, words + at, 0);
+    std::vector<int32_t> starts(b->sequences);
     int64_t token = 0;
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], n = b->q_lens[s];
-        const int32_t record[kSeqWords] = {(int32_t)token, (int32_t)n, (int32_t)kv, (int32_t)b->packed_lens[s]};
-        std::copy(record, record + kSeqWords, words + plan->seqs_at + s * kSeqWords);
+        starts[s] = (int32_t)token;
         for (int64_t t = kv - n; t < kv; t++) words[plan->slots_at + token++] = (int32_t)(b->table[s * b->table_stride + t / P] * P + t % P);
     }
     if (b->sequences && b->table_stride) std::copy(b->table, b->table + b->sequences * b->table_stride, words + plan->table_at);
     auto write = [&](const std::vector<Span> &list, int64_t to) {
-        for (const Span &s : list) to = std::copy(s.word, s.word + kItemWords, words + to) - words;
+        for (const Span &s : list) {
+            const int32_t q = s.word[0];
+            const int32_t of_seq[6] = {starts[q], (int32_t)b->q_lens[q], (int32_t)b->kv_lens[q], (int32_t)b->packed_lens[q], s.items, s.next};
+            std::copy(s.word, s.word + 6, words + to);
+            std::copy(of_seq, of_seq + 6, words + to + 6);
+            to += kItemWords;
+        }
     };
     write(few, plan->few_at), write(tiles, plan->tile_at), write(joins, plan->join_at);
     return KVMIX_OK;
@@ -685,7 +802,8 @@ extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_pa
     a.q = (const _Float16 *)c->q, a.out = (_Float16 *)c->out;
     a.q_ts = c->q_token_stride, a.q_hs = c->q_head_stride, a.o_ts = c->out_token_stride, a.o_hs = c->out_head_stride;
     a.rows = (const _Float16 *)p->rows, a.packed = (const uint32_t *)p->packed;
-    a.seqs = c->list + plan->seqs_at, a.table = c->list + plan->table_at, a.items = nullptr;
+    const PlanWords list = (PlanWords)c->list;
+    a.table = list + plan->table_at, a.items = nullptr;
     a.table_stride = (int)plan->table_stride, a.kv_heads = (int)plan->kv_heads, a.group = (int)(plan->heads / plan->kv_heads);
     a.blocks_log2 = __builtin_ctzll((uint64_t)plan->page_size / kBlock);
     a.scale = c->scale * kLog2e;
@@ -696,20 +814,20 @@ extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_pa
         with_bits(p->k_bits, [&](auto KB) {
             with_bits(p->v_bits, [&](auto VB) {
                 if (plan->tiles) {
-                    a.items = c->list + plan->tile_at;
+                    a.items = list + plan->tile_at;
                     paged_tile<D.value, KB.value, VB.value><<<(unsigned)(plan->tiles * plan->kv_heads), 256, 0, st>>>(a);
                 }
                 if (plan->few) {
-                    a.items = c->list + plan->few_at;
-                    const unsigned grid = (unsigned)(plan->few * plan->kv_heads);
+                    a.items = list + plan->few_at;
+                    const unsigned grid = (unsigned)(plan->columns * plan->kv_heads);
                     if (plan->few_rows > 16) paged_few<D.value, KB.value, VB.value, 2><<<grid, 256, 0, st>>>(a);
                     else paged_few<D.value, KB.value, VB.value, 1><<<grid, 256, 0, st>>>(a);
                 }
             });
         });
         if (plan->joins) {
-            a.items = c->list + plan->join_at;
-            const unsigned rows = plan->tiles ? kTileRows / 4 : (unsigned)(plan->few_rows + 3) / 4;
+            a.items = list + plan->join_at;
+            const unsigned rows = plan->tiles ? kTileRows / 4 : (unsigned)plan->few_rows / 4;
             paged_join<D.value><<<dim3((unsigned)(plan->joins * plan->kv_heads), rows), 256, 0, st>>>(a);
         }
     });

@@ -70,27 +70,43 @@ __device__ __forceinline__ void store_words(uint32_t *at, int lane, const uint32
 template <int BITS, int N>
 struct Pairs {
     static constexpr int per = BITS == 3 ? 5 : 16 / BITS;
-    static constexpr bool whole(int t) { return t < N * per; }
 };
 
 // Pair `t` as two halves that hold the codes exactly.  A field at bit s of a half, under the exponent of 2^(10 - s), is the code
-// plus 2^(10 - s): the bits are masked in place and that is subtracted.
+// plus 2^(10 - s): the bits are masked in place, in one operation with the exponent (v_and_or_b32 takes one scalar and no
+// literal: the exponents are kept in registers, Exponents below), and that is subtracted.
+template <int BITS>
+struct Exponents {
+    // fields lie in the ten bits of a half's fraction, or are shifted there
+    static constexpr int shift = BITS == 4 ? 8 : BITS == 3 ? 9 : 10;
+    static constexpr int count = (10 - BITS) / BITS + 1;
+    uint32_t at[count];
+
+    __device__ __forceinline__ Exponents()
+    {
+#pragma unroll
+        for (int i = 0; i < count; i++) {
+            const uint32_t e = (0x6400u - 0x400u * (i * BITS)) * 0x00010001u;
+            asm volatile("v_mov_b32 %0, %1" : "=v"(at[i]) : "s"(e));
+        }
+    }
+};
+
 template <int BITS, int N>
-__device__ __forceinline__ half2v code_pair(const uint32_t *w, int t)
+__device__ __forceinline__ half2v code_pair(const uint32_t *w, int t, const Exponents<BITS> &e)
 {
     constexpr uint32_t ones = 0x00010001u;
     constexpr uint32_t mask = (1u << BITS) - 1;
     constexpr int per = Pairs<BITS, N>::per;
     if (t >= N * per) {  // (3 bits only)
         const int r = 3 * (t - N * per);
-        const uint32_t c = (w[r] >> 15 & ones) | (w[r + 1] >> 14 & 2 * ones) | (w[r + 2] >> 13 & 4 * ones) | 0x64006400u;
+        const uint32_t c = (w[r] >> 15 & ones) | (w[r + 1] >> 14 & 2 * ones) | (w[r + 2] >> 13 & 4 * ones) | e.at[0];
         return __builtin_bit_cast(half2v, c) - half2v{(_Float16)1024.0f, (_Float16)1024.0f};
     }
     int s = t % per * BITS;
-    uint32_t v = w[t / per];
-    constexpr int shift = BITS == 4 ? 8 : BITS == 3 ? 9 : 10;  // fields that do not lie in the ten bits of a half's fraction
-    if (s + BITS > 10) v >>= shift, s -= shift;
-    const uint32_t c = (v & (mask * ones << s)) | (0x6400u - 0x400u * s) * ones;
+    uint32_t v = w[t / per], c;
+    if (s + BITS > 10) v >>= Exponents<BITS>::shift, s -= Exponents<BITS>::shift;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(c) : "v"(v), "s"(mask * ones << s), "v"(e.at[s / BITS]));
     const _Float16 base = (_Float16)(float)(1 << (10 - s));
     return __builtin_bit_cast(half2v, c) - half2v{base, base};
 }
@@ -110,18 +126,23 @@ __device__ __forceinline__ void put_pair(uint32_t *w, int t, uint32_t first, uin
     }
 }
 
-// Piece `piece` of a lane's words as values: code * scale + zero, each rounded once, to fp16.
+// Piece `piece` of a lane's words: its codes, and its values code * scale + zero, each rounded once, to fp16.
 template <int BITS, int N>
-__device__ __forceinline__ half8v piece_values(const uint32_t *w, int piece, half8v scale, half8v zero)
+__device__ __forceinline__ half8v piece_codes(const uint32_t *w, int piece, const Exponents<BITS> &e)
 {
     half8v out;
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        const half2v c = code_pair<BITS, N>(w, 4 * piece + p);
-        const half2v v = __builtin_elementwise_fma(c, half2v{scale[2 * p], scale[2 * p + 1]}, half2v{zero[2 * p], zero[2 * p + 1]});
-        out[2 * p] = v[0], out[2 * p + 1] = v[1];
+        const half2v c = code_pair<BITS, N>(w, 4 * piece + p, e);
+        out[2 * p] = c[0], out[2 * p + 1] = c[1];
     }
     return out;
+}
+
+template <int BITS, int N>
+__device__ __forceinline__ half8v piece_values(const uint32_t *w, int piece, half8v scale, half8v zero, const Exponents<BITS> &e)
+{
+    return __builtin_elementwise_fma(piece_codes<BITS, N>(w, piece, e), scale, zero);
 }
 
 constexpr int64_t kMost32 = 0x7fffffff;

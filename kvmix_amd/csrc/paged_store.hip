@@ -192,10 +192,11 @@ __global__ void __launch_bounds__(256) paged_read(ReadArgs a, PagePairs ids)
             constexpr int N = lane_words(D, B.value);
             uint32_t w[N];
             load_words<N>(values ? from + D * a.k_bits : from, lane, w);
+            const Exponents<B.value> e;
 #pragma unroll
             for (int p = 0; p < NP; p++) {
                 const int s = values ? p / 2 : p % (D / 32);
-                x[p] = piece_values<B.value, N>(w, p, *(const half8v *)(side + 32 * s), *(const half8v *)(side + D + 32 * s));
+                x[p] = piece_values<B.value, N>(w, p, *(const half8v *)(side + 32 * s), *(const half8v *)(side + D + 32 * s), e);
             }
         });
     }

@@ -5,7 +5,7 @@ import pytest
 
 from kvmix_amd import _lib
 
-ITEM, SEQ = 6, 4
+ITEM = 12
 
 
 def make(lens, packed, new, heads=8, kv_heads=2, page=64, D=128, seed=0, width=None):
@@ -21,7 +21,7 @@ def make(lens, packed, new, heads=8, kv_heads=2, page=64, D=128, seed=0, width=N
 
 
 def items(words, at, n):
-    return [tuple(words[at + ITEM * i:at + ITEM * i + ITEM]) for i in range(n)]
+    return [tuple(words[at + ITEM * i:at + ITEM * i + 6]) for i in range(n)]
 
 
 CASES = [
@@ -45,8 +45,10 @@ def test_every_pair_of_row_and_token_is_covered_once(lens, packed, new, how):
     # sequences, tables and slots
     token = 0
     for s, (n, p, k) in enumerate(zip(lens, packed, new)):
-        at = plan["seqs_at"] + SEQ * s
-        assert words[at:at + SEQ] == [token, k, n, p]
+        for at, count in ((plan["few_at"], plan["few"]), (plan["tile_at"], plan["tiles"]), (plan["join_at"], plan["joins"])):
+            for i in range(count):
+                if words[at + ITEM * i] == s:
+                    assert words[at + ITEM * i + 6:at + ITEM * i + 10] == [token, k, n, p]
         at = plan["table_at"] + plan["table_stride"] * s
         assert words[at:at + plan["table_stride"]] == table[s]
         for i in range(k):
@@ -76,6 +78,15 @@ def test_every_pair_of_row_and_token_is_covered_once(lens, packed, new, how):
     for s, k in enumerate(new):
         spans = sorted(rows_seen.get(s, []))
         assert sum(n for _, n in spans) == k * G and all(a + n == b for (a, n), (b, _) in zip(spans, spans[1:]))
+    # columns share the items of few rows out, to within a unit of four blocks
+    dealt, seen = [], []
+    for c in range(plan["columns"]):
+        count, after = words[plan["few_at"] + ITEM * c + 10:plan["few_at"] + ITEM * c + 12]
+        mine = [c] + list(range(after, after + count - 1))
+        seen += mine
+        dealt.append(sum(-(-(few[i][4] - few[i][3]) // 4) for i in mine))
+    assert sorted(seen) == list(range(len(few)))
+    assert not dealt or max(dealt) - min(dealt) <= 1
     # joined rows are those in parts, and parts do not overlap
     assert {(j[0], j[1]) for j in joins} == set(parts)
     used = set()
