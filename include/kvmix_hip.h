@@ -542,11 +542,6 @@ typedef struct kvmix_paged_pool {
     int k_bits, v_bits;         /* not read where only fp16 pages are meant */
 } kvmix_paged_pool_t;
 
-/* New tokens into fp16 pages: k, v [tokens, kv_heads, head_dim] fp16 (strides in elements, multiples of 8; 16-byte aligned),
- * slots [tokens] device memory: page * page_size + place; a token whose slot is negative or outside the pool is not stored. */
-int kvmix_paged_append(const kvmix_paged_pool_t *pool, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
-                       int64_t v_token_stride, int64_t v_head_stride, const int32_t *slots, int64_t tokens, kvmix_stream_t stream);
-
 /* fp16 pages to packed pages: pairs [count][2] = (fp16 page, packed page); a packed page is named once at most
  * (KVMIX_ERR_PAGE_ORDER). */
 int kvmix_paged_quantize(const kvmix_paged_pool_t *pool, const int32_t *pairs, int64_t count, kvmix_stream_t stream);
@@ -580,12 +575,18 @@ typedef struct kvmix_paged_plan {
     int64_t tokens;                              /* new tokens of all sequences */
     int64_t heads, kv_heads, head_dim, page_size, table_stride;
     int64_t row_pages, packed_pages;             /* pages that the pools must have at least */
-    int64_t slots_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
+    int64_t slots_at, store_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
+    int64_t stores;                              /* blocks of pages that get new tokens */
     int64_t few, columns, tiles, joins;          /* per kv head: items of a few query rows, blocks that share them, items of many, rows to be joined */
     int64_t few_rows;                            /* query rows of an item of few: 16 or 32 */
     int64_t part_rows;                           /* rows of partial results per kv head */
 } kvmix_paged_plan_t;
 int kvmix_paged_plan(const kvmix_paged_batch_t *batch, int32_t *words, int64_t capacity, kvmix_paged_plan_t *plan);
+
+/* The new tokens of a step into their fp16 pages: k, v [plan.tokens, kv_heads, head_dim] fp16 (strides in elements, multiples of 8;
+ * 16-byte aligned), sequence after sequence; list: the plan's words in device memory. */
+int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t *plan, const int32_t *list, const void *k, int64_t k_token_stride,
+                       int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride, kvmix_stream_t stream);
 
 /*
  * Attention of a batch's new tokens over its pages:  out[i, h] = sum_{j <= pos(i)} softmax_j(scale q[i, h] . k[j, h']) v[j, h'],

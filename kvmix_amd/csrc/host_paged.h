@@ -78,8 +78,8 @@ void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &rows, co
     if (plan.c.row_pages > p.row_pages) check(KVMIX_ERR_PAGE);
     const Tensor k = pieces3(k_in), v = pieces3(v_in);
     const c10::DeviceGuard guard(rows.device());
-    check(api.paged_append(&p, k.data_ptr(), stride_of(k, 0), stride_of(k, 1), v.data_ptr(), stride_of(v, 0), stride_of(v, 1),
-                           plan.list.data_ptr<int32_t>() + plan.c.slots_at, plan.c.tokens, stream_of(rows)));
+    check(api.paged_append(&p, &plan.c, plan.list.data_ptr<int32_t>(), k.data_ptr(), stride_of(k, 0), stride_of(k, 1), v.data_ptr(), stride_of(v, 0),
+                           stride_of(v, 1), stream_of(rows)));
 }
 
 void paged_quantize(const Tensor &rows, const Tensor &packed, const Tensor &pairs_in, int64_t k_bits, int64_t v_bits)

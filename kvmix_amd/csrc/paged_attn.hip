@@ -25,10 +25,6 @@ constexpr float kShrink = 0.015625f;  // of queries in paged_few: their products
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// The plan's words: nobody writes them while a kernel runs, so they are read through the scalar cache (as ordinary memory every
-// look at a page table waited for all loads in flight).
-typedef const __attribute__((address_space(4))) int32_t *PlanWords;
-
 struct PagedArgs {
     const _Float16 *q;
     _Float16 *out;
@@ -723,6 +719,11 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         return was;
     };
     plan->slots_at = take(plan->tokens);
+    for (int64_t s = 0; s < b->sequences; s++) {
+        const int64_t kv = b->kv_lens[s], n = b->q_lens[s];
+        plan->stores += n ? (kv - 1) / kBlock - (kv - n) / kBlock + 1 : 0;
+    }
+    plan->store_at = take(plan->stores * kStoreWords);
     plan->table_at = take(b->sequences * b->table_stride);
     plan->few_at = take(plan->few * kItemWords);
     plan->tile_at = take(plan->tiles * kItemWords);
@@ -733,11 +734,17 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
     if (capacity < at) return KVMIX_ERR_WORKSPACE;
     std::fill(words, words + at, 0);
     std::vector<int32_t> starts(b->sequences);
-    int64_t token = 0;
+    int64_t token = 0, store = plan->store_at;
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], n = b->q_lens[s];
         starts[s] = (int32_t)token;
-        for (int64_t t = kv - n; t < kv; t++) words[plan->slots_at + token++] = (int32_t)(b->table[s * b->table_stride + t / P] * P + t % P);
+        const int32_t *pages = b->table + s * b->table_stride;
+        for (int64_t t = kv - n; t < kv;) {  // block by block
+            const int64_t end = std::min(kv, t / kBlock * kBlock + kBlock);
+            const int32_t record[kStoreWords] = {(int32_t)token, (int32_t)(pages[t / P] * P + t % P), (int32_t)(end - t), 0};
+            store = std::copy(record, record + kStoreWords, words + store) - words;
+            for (; t < end; t++) words[plan->slots_at + token++] = (int32_t)(pages[t / P] * P + t % P);
+        }
     }
     if (b->sequences && b->table_stride) std::copy(b->table, b->table + b->sequences * b->table_stride, words + plan->table_at);
     auto write = [&](const std::vector<Span> &list, int64_t to) {

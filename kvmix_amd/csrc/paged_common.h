@@ -25,7 +25,12 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
-constexpr int kBlock = 32;  // tokens
+constexpr int kBlock = 32;      // tokens
+constexpr int kStoreWords = 4;  // new tokens of one block of a page: the first one's number, its page * page_size + place, how many; one of no use
+
+// The plan's words: nobody writes them while a kernel runs, so they are read through the scalar cache (as ordinary memory every
+// look at a page table waited for all loads in flight).
+typedef const __attribute__((address_space(4))) int32_t *PlanWords;
 
 __host__ __device__ constexpr int lane_words(int D, int bits) { return D * bits / 64; }
 __host__ __device__ constexpr int run_words(int words) { return words % 4 == 0 ? 4 : words % 2 == 0 ? 2 : 1; }

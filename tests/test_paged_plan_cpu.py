@@ -55,6 +55,14 @@ def test_every_pair_of_row_and_token_is_covered_once(lens, packed, new, how):
             t = n - k + i
             assert words[plan["slots_at"] + token + i] == table[s][t // page] * page + t % page
         token += k
+    # blocks of pages that get new tokens: all slots, in order
+    slots = words[plan["slots_at"]:plan["slots_at"] + token]
+    stored = []
+    for i in range(plan["stores"]):
+        first, slot, count, _ = words[plan["store_at"] + 4 * i:plan["store_at"] + 4 * i + 4]
+        assert first == len(stored) and count > 0 and slot % 32 + count <= 32
+        stored += range(slot, slot + count)
+    assert stored == slots
     # rows by keys
     few, tiles = items(words, plan["few_at"], plan["few"]), items(words, plan["tile_at"], plan["tiles"])
     joins = items(words, plan["join_at"], plan["joins"])
