@@ -438,12 +438,138 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     for (int t = 0; t < DT; t++) o[t] = floatx16{};
     float top = -1e30f, sum = 0.0f;
 
-    fetch(it.begin);
-    place(it.begin, 0);
-    if (it.begin + 1 < it.end) fetch(it.begin + 1);
-    __syncthreads();
-    int buf = 0;
-    for (int tile = it.begin; tile < it.end; tile++) {
+    auto key_piece = [&](int buf, int t, int s) { return *(const half8v *)(lds[buf][0] + tile_key<D>(32 * t + k_row, 2 * s + h2)); };
+    auto value_piece = [&](int buf, int t, int kk) { return *(const half8v *)(lds[buf][1] + tile_value(32 * t + col, 2 * kk + h2)); };
+
+    // A tile's logits to probabilities and their product with its values: x[t][8 kk + j] is the logit of token 32 t + 16 kk + 8 h2 + j.
+    auto weigh = [&](floatx16 (&x)[2], int buf) {
+        float most = x[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; i++) most = fmaxf(most, x[i / 16][i % 16]);
+        {
+            const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+            most = fmaxf(__uint_as_float(e[0]), __uint_as_float(e[1])) * a.scale;
+        }
+        if (__any(most > top + 8.0f)) {
+            const float grown = fmaxf(top, most), shrink = __builtin_amdgcn_exp2f(top - grown);
+            top = grown;
+            sum *= shrink;
+#pragma unroll
+            for (int t = 0; t < DT; t++) o[t] *= shrink;
+        }
+        half8v p[2];
+        auto probabilities = [&](int kk) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p[kk % 2][j] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[kk / 2][8 * (kk % 2) + j], a.scale, -top));
+                if (j % 2) sum = __builtin_amdgcn_fdot2(half2v{p[kk % 2][j - 1], p[kk % 2][j]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+            }
+        };
+        half8v v[DT], ahead[DT];
+#pragma unroll
+        for (int t = 0; t < DT; t++) v[t] = value_piece(buf, t, 0);
+        probabilities(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {  // (a step's reads and probabilities between the products of the one before)
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                if (kk < 3) ahead[t] = value_piece(buf, t, kk + 1);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[t], p[kk % 2], o[t], 0, 0, 0);
+            }
+            if (kk < 3) probabilities(kk + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < DT; t++) v[t] = ahead[t];
+        }
+    };
+
+    int tile = it.begin, buf = 0;
+    const int packed_tiles = min(it.end, packed_blocks / 2);  // up to there both blocks of a tile are packed
+    if (tile < packed_tiles) {
+        // Tiles of codes whose successor is one of codes too: no masks, nothing under a condition, and the codes of the next tile
+        // become values between the products of this one's keys.  One loop for the waves that turn keys and one for those that
+        // turn values.
+        auto run = [&](auto is_value) {
+            constexpr bool V = is_value.value;
+            constexpr int B = V ? VB : KB, N = lane_words(D, B);
+            const Exponents<B> e;
+            uint32_t w[N], sd[D / 64];
+            auto page_of = [&](int tile) { return table[(2 * min(tile, packed_tiles - 1) + which) >> a.blocks_log2]; };
+            auto load = [&](int tile, int page) {
+                const int in_page = (2 * min(tile, packed_tiles - 1) + which) & (per_page - 1);
+                const uint32_t *at = a.packed + ((((int64_t)page * a.kv_heads + head) << a.blocks_log2) + in_page) * block_words(D, KB, VB);
+                load_words<N>(at + (V ? D * KB : 0), lane, w);
+                load_words<D / 64>(at + D * (KB + VB) + (V ? D : 0), lane, sd);
+            };
+            const _Float16 *side_at = (const _Float16 *)sides[wave] + 8 * g;
+            auto start = [&]() {
+                store_words<D / 64>(sides[wave], lane, sd);
+                __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+            };
+            struct Side {
+                half8v scale, zero;
+            };
+            auto side_of = [&](int p) {
+                const int set = V ? p / 2 : p % (D / 32);
+                return Side{*(const half8v *)(side_at + 32 * set), *(const half8v *)(side_at + D + 32 * set)};
+            };
+            auto turn = [&](int p, int buf, const Side &side) {
+                const half8v x = piece_values<B, N>(w, p, side.scale, side.zero, e);
+                const int at = V ? tile_value(16 * p + m, 4 * which + g)
+                                 : tile_key<D>(kBlock * which + 8 * (m / 4) + 4 * (p / (D / 32)) + m % 4, 4 * (p % (D / 32)) + g);
+                *(half8v *)(lds[buf][V] + at) = x;
+            };
+            load(tile, page_of(tile));
+            int page = page_of(tile + 1);
+            start();
+#pragma unroll
+            for (int p = 0; p < NP; p++) turn(p, 0, side_of(p));
+            load(tile + 1, page);
+            page = page_of(tile + 2);
+            __syncthreads();
+            for (; tile < packed_tiles - 1; tile++) {
+                start();
+                if (wave_last >= 0) {
+                    floatx16 x[2] = {floatx16{}, floatx16{}};
+                    half8v k[2] = {key_piece(buf, 0, 0), key_piece(buf, 1, 0)};
+                    Side side = side_of(0);
+#pragma unroll
+                    for (int s = 0; s < KS; s++) {  // (the LDS is read a step ahead)
+                        half8v k_ahead[2];
+                        Side side_ahead;
+                        if (s + 1 < KS) {
+                            side_ahead = side_of(s + 1);
+                            k_ahead[0] = key_piece(buf, 0, s + 1), k_ahead[1] = key_piece(buf, 1, s + 1);
+                        }
+#pragma unroll
+                        for (int t = 0; t < 2; t++) x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[s], x[t], 0, 0, 0);
+                        turn(s, buf ^ 1, side);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (s + 1 < KS) k[0] = k_ahead[0], k[1] = k_ahead[1], side = side_ahead;
+                    }
+                    load(tile + 2, page);
+                    page = page_of(tile + 3);
+                    weigh(x, buf);
+                } else {
+#pragma unroll
+                    for (int p = 0; p < NP; p++) turn(p, buf ^ 1, side_of(p));
+                    load(tile + 2, page);
+                    page = page_of(tile + 3);
+                }
+                buf ^= 1;
+                __syncthreads();
+            }
+        };
+        if (matrix) run(std::true_type());
+        else run(std::false_type());
+    } else {
+        fetch(tile);
+        place(tile, 0);
+        __syncthreads();
+    }
+    // the last of them, and those with tokens in fp16
+    if (tile + 1 < it.end) fetch(tile + 1);
+    for (; tile < it.end; tile++) {
         if (tile + 1 < it.end) place(tile + 1, buf ^ 1);  // (that buffer was last read before the barrier that ended the turn before)
         if (tile + 2 < it.end) fetch(tile + 2);
         const int k0 = tile * kTileKeys;
@@ -452,45 +578,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
             for (int s = 0; s < KS; s++) {
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const half8v k = *(const half8v *)(lds[buf][0] + tile_key<D>(32 * t + k_row, 2 * s + h2));
-                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], x[t], 0, 0, 0);
-                }
+                for (int t = 0; t < 2; t++) x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key_piece(buf, t, s), q[s], x[t], 0, 0, 0);
+                if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (all reads of a tile ahead of its products would spill)
             }
-            // x[t][8 kk + j] is the logit of token 32 t + 16 kk + 8 h2 + j
             if (k0 + kTileKeys - 1 > wave_first) {
 #pragma unroll
                 for (int i = 0; i < 32; i++)
                     if (k0 + 32 * (i / 16) + 16 * (i % 16 / 8) + 8 * h2 + i % 8 > limit) x[i / 16][i % 16] = -__builtin_inff();
             }
-            float most = x[0][0];
-#pragma unroll
-            for (int i = 1; i < 32; i++) most = fmaxf(most, x[i / 16][i % 16]);
-            {
-                const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
-                most = fmaxf(__uint_as_float(e[0]), __uint_as_float(e[1])) * a.scale;
-            }
-            if (__any(most > top + 8.0f)) {
-                const float grown = fmaxf(top, most), shrink = __builtin_amdgcn_exp2f(top - grown);
-                top = grown;
-                sum *= shrink;
-#pragma unroll
-                for (int t = 0; t < DT; t++) o[t] *= shrink;
-            }
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                half8v p;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    p[j] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[kk / 2][8 * (kk % 2) + j], a.scale, -top));
-                    if (j % 2) sum = __builtin_amdgcn_fdot2(half2v{p[j - 1], p[j]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
-                }
-#pragma unroll
-                for (int t = 0; t < DT; t++) {
-                    const half8v v = *(const half8v *)(lds[buf][1] + tile_value(32 * t + col, 2 * kk + h2));
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[t], 0, 0, 0);
-                }
-            }
+            weigh(x, buf);
         }
         buf ^= 1;
         __syncthreads();
