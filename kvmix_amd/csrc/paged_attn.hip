@@ -476,7 +476,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
                 if (kk < 3) ahead[t] = value_piece(buf, t, kk + 1);
                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[t], p[kk % 2], o[t], 0, 0, 0);
             }
-            if (kk < 3) probabilities(kk + 1);
+            if (kk < 3) {
+                probabilities(kk + 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, DT, 0);
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 24 / DT, 0);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < DT; t++) v[t] = ahead[t];
@@ -544,6 +552,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                         for (int t = 0; t < 2; t++) x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[t], q[s], x[t], 0, 0, 0);
                         turn(s, buf ^ 1, side);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
                         __builtin_amdgcn_sched_barrier(0);
                         if (s + 1 < KS) k[0] = k_ahead[0], k[1] = k_ahead[1], side = side_ahead;
                     }
