@@ -577,7 +577,7 @@ typedef struct kvmix_paged_plan {
     int64_t row_pages, packed_pages;             /* pages that the pools must have at least */
     int64_t slots_at, store_at, table_at, few_at, tile_at, join_at; /* where the parts of the list begin */
     int64_t stores;                              /* blocks of pages that get new tokens */
-    int64_t few, columns, tiles, joins;          /* per kv head: items of a few query rows, blocks that share them, items of many, rows to be joined */
+    int64_t few, few_columns, tiles, joins;      /* per kv head: items of a few query rows, blocks that share them, items of many, rows to be joined */
     int64_t few_rows;                            /* query rows of an item of few: 16 or 32 */
     int64_t part_rows;                           /* rows of partial results per kv head */
 } kvmix_paged_plan_t;

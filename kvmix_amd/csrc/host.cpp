@@ -806,7 +806,7 @@ PYBIND11_MODULE(_host, m)
         .def_property_readonly("tokens", [](const PagedPlan &p) { return p.c.tokens; })
         .def_property_readonly("slots", [](const PagedPlan &p) { return p.slots(); })
         .def_property_readonly("device", [](const PagedPlan &p) { return p.list.device(); })
-        .def_property_readonly("launches", [](const PagedPlan &p) { return std::make_tuple(p.c.columns, p.c.tiles, p.c.joins); });
+        .def_property_readonly("launches", [](const PagedPlan &p) { return std::make_tuple(p.c.few_columns, p.c.tiles, p.c.joins); });
     m.def("paged_plan", &paged_plan, NoGil());
     m.def("paged_append", &paged_append, NoGil());
     m.def("paged_quantize", &paged_quantize, NoGil());

@@ -389,8 +389,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             }
         }
     };
-    const Exponents<KB> ke;
-    const Exponents<VB> ve;
     auto place = [&](int tile, int buf) {
         const int block = 2 * tile + which;
         uint8_t *to = lds[buf][matrix];
@@ -403,16 +401,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             store_words<D / 64>(sides[wave], lane, side);
             __builtin_amdgcn_wave_barrier();
             const _Float16 *s = (const _Float16 *)sides[wave] + 8 * g;
-            auto turn = [&](const auto &e, auto bits) {
+            auto turn = [&](auto bits) {
                 constexpr int B = decltype(bits)::value;
+                const Exponents<B> e;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     const int set = matrix ? p / 2 : p % (D / 32);
                     put(p, piece_values<B, lane_words(D, B)>(held, p, *(const half8v *)(s + 32 * set), *(const half8v *)(s + D + 32 * set), e));
                 }
             };
-            if (matrix) turn(ve, std::integral_constant<int, VB>());
-            else turn(ke, std::integral_constant<int, KB>());
+            if (matrix) turn(std::integral_constant<int, VB>());
+            else turn(std::integral_constant<int, KB>());
             __builtin_amdgcn_wave_barrier();
         } else if (block < blocks) {
 #pragma unroll
@@ -697,11 +696,11 @@ namespace {
 constexpr int64_t kFewMost = 32;    // rows of a sequence and kv head that go to paged_few
 constexpr int64_t kFewUnit = 4;     // blocks of tokens, one to a wave: what its launch is cut by ...
 constexpr int64_t kFewLeast = 2;    // ... of which a column has that many at least
-constexpr int64_t kTileLaunch = 1024;
-constexpr int64_t kTileSpan = 8;    // tiles
-
 // Blocks of paged_few that the chip holds at once: three to a CU by their registers (sixteen rows), or two (32).
 int64_t few_resident(int64_t rows) { return rows > 16 ? 512 : 768; }
+
+// The same of paged_tile, and the tiles' worth of time that a block of it takes beside its tiles.
+constexpr int64_t kTileResident = 512, kTileStart = 3;
 
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
@@ -710,6 +709,75 @@ struct Span {
     int64_t cost;
     int32_t items = 0, next = 0;
 };
+
+// Items dealt to columns of equal cost, cut where a column ends.
+struct Deal {
+    int64_t units = 0, columns = 0;  // of all items together; columns to deal to
+    std::vector<Span> list;
+    std::vector<int32_t> starts;     // the first item of each column
+    int64_t dealt = 0, column_end = 0;
+
+    // `length` blocks, of which kFewUnit make a unit
+    void add(int64_t seq, int64_t rows, int64_t length)
+    {
+        const int64_t count = (length + kFewUnit - 1) / kFewUnit;
+        for (int64_t at = 0; at < count;) {
+            if (dealt == column_end) {
+                starts.push_back((int32_t)list.size());
+                column_end = units * (int64_t)starts.size() / columns;
+                continue;
+            }
+            const int64_t here = std::min(count - at, column_end - dealt);
+            list.push_back({{(int32_t)seq, 0, (int32_t)rows, (int32_t)(at * kFewUnit), (int32_t)std::min((at + here) * kFewUnit, length), -1}, here});
+            at += here, dealt += here;
+        }
+    }
+
+    // The first item of every column, then the others.
+    void close()
+    {
+        std::vector<Span> firsts, others;
+        for (size_t c = 0; c < starts.size(); c++) {
+            const size_t from = starts[c], to = c + 1 < starts.size() ? starts[c + 1] : list.size();
+            firsts.push_back(list[from]);
+            firsts.back().items = (int32_t)(to - from);
+            firsts.back().next = (int32_t)(starts.size() + others.size());
+            others.insert(others.end(), list.begin() + from + 1, list.begin() + to);
+        }
+        list = std::move(firsts);
+        list.insert(list.end(), others.begin(), others.end());
+    }
+};
+
+// Tiles that a block of paged_tile takes at most, from the lengths of the 128-row problems of one kv head.  Spans such that all
+// blocks are resident in one round (two, three, four), or problems left whole and dealt as blocks end; whichever is estimated to
+// end first.
+int64_t tile_span(const std::vector<int64_t> &lengths, int64_t kv_heads)
+{
+    int64_t total = 0, longest = 0;
+    for (int64_t n : lengths) total += n, longest = std::max(longest, n);
+    const auto blocks = [&](int64_t span) {
+        int64_t n = 0;
+        for (int64_t l : lengths) n += (l + span - 1) / span;
+        return n * kv_heads;
+    };
+    const int64_t whole = blocks(longest);
+    int64_t best = longest;
+    double least = (double)total * kv_heads / kTileResident + longest / 2.0 + kTileStart * (double)((whole + kTileResident - 1) / kTileResident);
+    if (whole <= kTileResident) least = longest + kTileStart;
+    for (int64_t rounds = 1; rounds <= 4; rounds++) {
+        int64_t low = 1, high = longest;  // the shortest spans whose blocks fit
+        while (low < high) {
+            const int64_t mid = (low + high) / 2;
+            if (blocks(mid) <= rounds * kTileResident) high = mid;
+            else low = mid + 1;
+        }
+        if (blocks(low) > rounds * kTileResident) continue;
+        const double time = (double)rounds * (low + kTileStart);
+        if (time < least) least = time, best = low;
+    }
+    return best;
+}
 
 int batch_check(const kvmix_paged_batch_t *b)
 {
@@ -729,7 +797,8 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
     *plan = kvmix_paged_plan_t{};
     plan->heads = b->heads, plan->kv_heads = b->kv_heads, plan->head_dim = b->head_dim, plan->page_size = P;
     plan->table_stride = b->table_stride;
-    int64_t few_units = 0, tile_cost = 0;
+    Deal few;
+    std::vector<int64_t> lengths;  // of the problems of 128 rows, in tiles
     plan->few_rows = 16;
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], pk = b->packed_lens[s], n = b->q_lens[s];
@@ -743,84 +812,57 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         }
         plan->tokens += n;
         if (n * G <= kFewMost) {
-            few_units += n ? (kv + kFewUnit * kBlock - 1) / (kFewUnit * kBlock) : 0;
+            few.units += n ? (kv + kFewUnit * kBlock - 1) / (kFewUnit * kBlock) : 0;
             if (n * G > 16) plan->few_rows = kFewMost;
         } else {
             for (int64_t r = 0; r < n * G; r += kTileRows)
-                tile_cost += (kv - n + std::min(n * G - 1, r + kTileRows - 1) / G) / kTileKeys + 1;
+                lengths.push_back((kv - n + std::min(n * G - 1, r + kTileRows - 1) / G) / kTileKeys + 1);
         }
     }
     if ((__int128)plan->row_pages * P > kMost32) return KVMIX_ERR_UNSUPPORTED;
     // One round of blocks: as many columns as the chip holds blocks, each of the same number of units, whatever sequences they
     // are of.  (Spans of sequences as the items, the longest first, left a second round of a few: of 1048 blocks of which 1024
-    // fit 85 us instead of @@, of 1248 75 instead of @@.)
-    const int64_t few_columns = std::min(std::max<int64_t>(few_resident(plan->few_rows) / b->kv_heads, 1), (few_units + kFewLeast - 1) / kFewLeast);
-    const int64_t tile_span = std::max(kTileSpan, (tile_cost * b->kv_heads + kTileLaunch - 1) / kTileLaunch);
+    // fit 85 us instead of 77.)
+    few.columns = std::min(std::max<int64_t>(few_resident(plan->few_rows) / b->kv_heads, 1), (few.units + kFewLeast - 1) / kFewLeast);
+    const int64_t span = lengths.empty() ? 1 : tile_span(lengths, b->kv_heads);
 
-    std::vector<Span> few, tiles, joins;
+    std::vector<Span> tiles, joins;
     int64_t part = 0;
-    auto cut = [&](std::vector<Span> &to, int64_t s, int64_t row0, int64_t rows, int64_t length, int64_t span, int64_t stride) {
-        const int64_t spans = (length + span - 1) / span, even = (length + spans - 1) / spans;
-        for (int64_t i = 0; i < spans; i++) {
-            const int64_t from = std::min(i * even, length), to_ = std::min(from + even, length);
-            to.push_back({{(int32_t)s, (int32_t)row0, (int32_t)rows, (int32_t)from, (int32_t)to_, spans > 1 ? (int32_t)(part + i * stride) : -1}, to_ - from});
-        }
-        if (spans > 1) {
-            joins.push_back({{(int32_t)s, (int32_t)row0, (int32_t)rows, (int32_t)spans, (int32_t)stride, (int32_t)part}, rows});
-            part += spans * stride;
-        }
-        return part <= kMostTokens;
+    // the spans list[first ..) of one problem
+    auto joined = [&](std::vector<Span> &list, size_t first) {
+        const int64_t spans = (int64_t)(list.size() - first);
+        if (spans < 2) return;
+        const Span &one = list[first];
+        joins.push_back({{one.word[0], one.word[1], one.word[2], (int32_t)spans, one.word[2], (int32_t)part}, 0});
+        for (int64_t i = 0; i < spans; i++, part += one.word[2]) list[first + i].word[5] = (int32_t)part;
     };
-    std::vector<int32_t> columns;
-    int64_t column_end = 0, unit = 0;  // units up to and with the column that is being filled, units dealt
+    size_t problem = 0;
     for (int64_t s = 0; s < b->sequences; s++) {
         const int64_t kv = b->kv_lens[s], n = b->q_lens[s], rows = n * G;
         if (n == 0) continue;
         if (rows <= kFewMost) {
-            const int64_t blocks = (kv + kBlock - 1) / kBlock, units = (blocks + kFewUnit - 1) / kFewUnit;
-            const size_t first = few.size();
-            for (int64_t at = 0; at < units;) {
-                if (unit == column_end) {
-                    columns.push_back((int32_t)few.size());
-                    column_end = few_units * (int64_t)columns.size() / few_columns;
-                    continue;
-                }
-                const int64_t here = std::min(units - at, column_end - unit);
-                few.push_back({{(int32_t)s, 0, (int32_t)rows, (int32_t)(at * kFewUnit), (int32_t)std::min((at + here) * kFewUnit, blocks), -1}, here});
-                at += here, unit += here;
-            }
-            const int64_t spans = (int64_t)(few.size() - first);
-            if (spans > 1) {
-                for (int64_t i = 0; i < spans; i++) few[first + i].word[5] = (int32_t)(part + i * rows);
-                joins.push_back({{(int32_t)s, 0, (int32_t)rows, (int32_t)spans, (int32_t)rows, (int32_t)part}, rows});
-                part += spans * rows;
-            }
-            if (part > kMostTokens) return KVMIX_ERR_UNSUPPORTED;
+            const size_t first = few.list.size();
+            few.add(s, rows, (kv + kBlock - 1) / kBlock);
+            joined(few.list, first);
         } else {
             for (int64_t r = 0; r < rows; r += kTileRows) {
-                const int64_t here = std::min<int64_t>(kTileRows, rows - r);
-                if (!cut(tiles, s, r, here, (kv - n + (r + here - 1) / G) / kTileKeys + 1, tile_span, here)) return KVMIX_ERR_UNSUPPORTED;
+                const int64_t length = lengths[problem++], spans = (length + span - 1) / span, even = (length + spans - 1) / spans;
+                const size_t first = tiles.size();
+                for (int64_t from = 0; from < length; from += even) {
+                    const int64_t to = std::min(from + even, length);
+                    tiles.push_back({{(int32_t)s, (int32_t)r, (int32_t)std::min<int64_t>(kTileRows, rows - r), (int32_t)from, (int32_t)to, -1}, to - from});
+                }
+                joined(tiles, first);
             }
         }
+        if (part > kMostTokens) return KVMIX_ERR_UNSUPPORTED;
     }
-    plan->columns = (int64_t)columns.size();
-    {
-        // the first item of every column, then the others
-        columns.push_back((int32_t)few.size());
-        std::vector<Span> firsts, others;
-        for (size_t c = 0; c + 1 < columns.size(); c++) {
-            firsts.push_back(few[columns[c]]);
-            firsts.back().items = columns[c + 1] - columns[c];
-            firsts.back().next = (int32_t)(plan->columns + others.size());
-            others.insert(others.end(), few.begin() + columns[c] + 1, few.begin() + columns[c + 1]);
-        }
-        few = std::move(firsts);
-        few.insert(few.end(), others.begin(), others.end());
-    }
-    if (std::max({few.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMost32) return KVMIX_ERR_UNSUPPORTED;
-    // the longest first: what ends a launch is short then
+    few.close();
+    // (what ends a launch is short then)
     std::stable_sort(tiles.begin(), tiles.end(), [](const Span &x, const Span &y) { return x.cost > y.cost; });
-    plan->few = (int64_t)few.size(), plan->tiles = (int64_t)tiles.size(), plan->joins = (int64_t)joins.size(), plan->part_rows = part;
+    if (std::max({few.list.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    plan->few = (int64_t)few.list.size(), plan->tiles = (int64_t)tiles.size(), plan->joins = (int64_t)joins.size(), plan->part_rows = part;
+    plan->few_columns = (int64_t)few.starts.size();
     int64_t at = 0;
     auto take = [&](int64_t n) {
         const int64_t was = at;
@@ -865,7 +907,7 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
             to += kItemWords;
         }
     };
-    write(few, plan->few_at), write(tiles, plan->tile_at), write(joins, plan->join_at);
+    write(few.list, plan->few_at), write(tiles, plan->tile_at), write(joins, plan->join_at);
     return KVMIX_OK;
 }
 
@@ -935,7 +977,7 @@ extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_pa
                 }
                 if (plan->few) {
                     a.items = list + plan->few_at;
-                    const unsigned grid = (unsigned)(plan->columns * plan->kv_heads);
+                    const unsigned grid = (unsigned)(plan->few_columns * plan->kv_heads);
                     if (plan->few_rows > 16) paged_few<D.value, KB.value, VB.value, 2><<<grid, 256, 0, st>>>(a);
                     else paged_few<D.value, KB.value, VB.value, 1><<<grid, 256, 0, st>>>(a);
                 }

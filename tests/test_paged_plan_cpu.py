@@ -88,13 +88,16 @@ def test_every_pair_of_row_and_token_is_covered_once(lens, packed, new, how):
         assert sum(n for _, n in spans) == k * G and all(a + n == b for (a, n), (b, _) in zip(spans, spans[1:]))
     # columns share the items of few rows out, to within a unit of four blocks
     dealt, seen = [], []
-    for c in range(plan["columns"]):
+    for c in range(plan["few_columns"]):
         count, after = words[plan["few_at"] + ITEM * c + 10:plan["few_at"] + ITEM * c + 12]
         mine = [c] + list(range(after, after + count - 1))
         seen += mine
         dealt.append(sum(-(-(few[i][4] - few[i][3]) // 4) for i in mine))
     assert sorted(seen) == list(range(len(few)))
     assert not dealt or max(dealt) - min(dealt) <= 1
+    # items of many rows: the longest first
+    spans = [i[4] - i[3] for i in tiles]
+    assert spans == sorted(spans, reverse=True)
     # joined rows are those in parts, and parts do not overlap
     assert {(j[0], j[1]) for j in joins} == set(parts)
     used = set()
