@@ -100,7 +100,7 @@ __device__ __forceinline__ half8v row_piece(const _Float16 *page_head, int page,
 struct QuantizeArgs {
     const _Float16 *rows;
     uint32_t *packed;
-    int heads, page, units;  // units: waves of work, pair by head by block by matrix
+    int heads, page, units;  // units: waves of work per pair, head by block by matrix
     int k_bits, v_bits;
 };
 
@@ -119,62 +119,112 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b)
     return o;
 }
 
-template <int N>
-__device__ __forceinline__ uint32_t pair_ror(uint32_t v)
+// One halving step over the lanes of a row of sixteen whose numbers differ in the bits of MASK (15, 7, 3, 1: mirrors of the row,
+// of its halves, of quarters and of pairs): the lane with MASK's highest bit clear gets the lower half of v over the pair.
+template <int MASK, bool MAX, int N>
+__device__ __forceinline__ void halve_pairs(uint32_t *v, int lane)
 {
-    return __float_as_uint(row_ror<N>(__uint_as_float(v)));
+    constexpr int control = MASK == 15 ? 0x140 : MASK == 7 ? 0x141 : MASK == 3 ? 0x1b : 0xb1;
+    const bool up = (lane & (MASK + 1) / 2) != 0;
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        const uint32_t keep = up ? v[N / 2 + i] : v[i], send = up ? v[i] : v[N / 2 + i];
+        const uint32_t other = __builtin_amdgcn_update_dpp(0, send, control, 0xf, 0xf, true);
+        v[i] = MAX ? pair_max(keep, other) : pair_min(keep, other);
+    }
 }
 
+// What the lanes of a row need to know of its groups, two to an entry: minimum and reciprocal of the scale, and the scale where
+// the reciprocal will not do.
+template <int D>
+struct GroupTable {
+    float fast[4][D / 8][4];   // [row of lanes][pair of groups][minimum, reciprocal, minimum, reciprocal]
+    float scale[4][D / 8][2];
+};
+
 // One matrix of one block per wave.  A group's 32 values are two of a lane's (the keys' two tokens, the values' two channels)
-// and those of the sixteen lanes of a row: extremes by packed halves and exchanges within the row.  The codes are those of
-// kvmix_quant_pack_last_dim with KVMIX_SCALE_RECIPROCAL, bit for bit.
+// and those of the sixteen lanes of a row.  Its extremes are found by halving, so that each lane ends with two groups (one at
+// D = 64) whose scales it works out for the row; with every lane working out all 32 of them, and a branch for every two codes,
+// 120 pages of 32 heads took 54 instead of @@ us.  The codes are those of kvmix_quant_pack_last_dim with
+// KVMIX_SCALE_RECIPROCAL, bit for bit.
 template <int D, int BITS, bool KEYS>
-__device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, int block, uint32_t *to, _Float16 *side, int lane)
+__device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, int block, uint32_t *to, _Float16 *side, int lane, GroupTable<D> &table)
 {
-    constexpr int NP = D / 16, S = D / 32, N = lane_words(D, BITS);
+    constexpr int NP = D / 16, S = D / 32, N = lane_words(D, BITS), PAIRS = D / 8;
     constexpr int QMAX = (1 << BITS) - 1;
+    const int g = lane / 16;
     half8v x[NP];  // [set of eight groups][two of the group]
 #pragma unroll
     for (int s = 0; s < S; s++) {
 #pragma unroll
         for (int w = 0; w < 2; w++) x[2 * s + w] = row_piece<D, KEYS>(from, page, block, lane, KEYS ? w * S + s : 2 * s + w);
     }
+    uint32_t lo[PAIRS], hi[PAIRS];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const uint4v a = __builtin_bit_cast(uint4v, x[2 * s]), b = __builtin_bit_cast(uint4v, x[2 * s + 1]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) lo[4 * s + j] = pair_min(a[j], b[j]), hi[4 * s + j] = pair_max(a[j], b[j]);
+    }
+    halve_pairs<15, false, PAIRS>(lo, lane), halve_pairs<15, true, PAIRS>(hi, lane);
+    halve_pairs<7, false, PAIRS / 2>(lo, lane), halve_pairs<7, true, PAIRS / 2>(hi, lane);
+    halve_pairs<3, false, PAIRS / 4>(lo, lane), halve_pairs<3, true, PAIRS / 4>(hi, lane);
+    if constexpr (PAIRS == 16) {
+        halve_pairs<1, false, 2>(lo, lane), halve_pairs<1, true, 2>(hi, lane);
+    } else {  // (one left: both lanes of a pair get it)
+        lo[0] = pair_min(lo[0], __builtin_amdgcn_update_dpp(0, lo[0], 0xb1, 0xf, 0xf, true));
+        hi[0] = pair_max(hi[0], __builtin_amdgcn_update_dpp(0, hi[0], 0xb1, 0xf, 0xf, true));
+    }
+    const int mine = lane % 16 * PAIRS / 16;
+    {
+        const half2v l = __builtin_bit_cast(half2v, lo[0]), h = __builtin_bit_cast(half2v, hi[0]);
+        half2v scales;
+        float fast[4], exact[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float mn = (float)l[i], range = (float)h[i] - mn, scale = range / (float)QMAX;
+            fast[2 * i] = mn, fast[2 * i + 1] = quantize_rcp(scale), exact[i] = scale;
+            scales[i] = (_Float16)scale_for_output(range, scale, 1.0f / (float)QMAX, KVMIX_SCALE_RECIPROCAL);
+        }
+        *(floatx4 *)table.fast[g][mine] = floatx4{fast[0], fast[1], fast[2], fast[3]};
+        table.scale[g][mine][0] = exact[0], table.scale[g][mine][1] = exact[1];
+        _Float16 *at = side + 32 * (mine / 4) + 8 * g + 2 * (mine % 4);
+        *(half2v *)at = scales;
+        *(uint32_t *)(at + D) = lo[0];
+    }
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
     uint32_t words[N] = {};
 #pragma unroll
     for (int s = 0; s < S; s++) {
-        half2v lo[4], hi[4];
-        const uint4v a = __builtin_bit_cast(uint4v, x[2 * s]), b = __builtin_bit_cast(uint4v, x[2 * s + 1]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t l = pair_min(a[j], b[j]), h = pair_max(a[j], b[j]);
-            l = pair_min(l, pair_ror<8>(l)), h = pair_max(h, pair_ror<8>(h));
-            l = pair_min(l, pair_ror<4>(l)), h = pair_max(h, pair_ror<4>(h));
-            l = pair_min(l, pair_ror<2>(l)), h = pair_max(h, pair_ror<2>(h));
-            l = pair_min(l, pair_ror<1>(l)), h = pair_max(h, pair_ror<1>(h));
-            lo[j] = __builtin_bit_cast(half2v, l), hi[j] = __builtin_bit_cast(half2v, h);
-        }
-        half8v scales, zeros;
         uint32_t q[2][8];
+        bool near = false;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float mn = (float)lo[j / 2][j % 2], range = (float)hi[j / 2][j % 2] - mn;
-            const float scale = range / (float)QMAX;
-            const float v[2] = {(float)x[2 * s][j], (float)x[2 * s + 1][j]};
-            uint32_t c[2];
-            quantize_codes<2>(v, mn, scale, quantize_rcp(scale), [](int) { return QMAX; }, c);
-            q[0][j] = c[0], q[1][j] = c[1];
-            scales[j] = (_Float16)scale_for_output(range, scale, 1.0f / (float)QMAX, KVMIX_SCALE_RECIPROCAL);
-            zeros[j] = (_Float16)mn;
+        for (int p = 0; p < 4; p++) {
+            const floatx4 f = *(const floatx4 *)table.fast[g][4 * s + p];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    // (as quantize_code_fast, but for the limit: a quotient above it is near)
+                    const float u = fmaf((float)x[2 * s + w][2 * p + i] - f[2 * i], f[2 * i + 1], 0.5f);
+                    near |= !(fabsf(__builtin_amdgcn_fractf(u) - 0.5f) <= 0.5f - 0.000030517578125f);
+                    q[w][2 * p + i] = (uint32_t)u;
+                }
+            }
+        }
+        if (__builtin_expect(near, 0)) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+#pragma unroll
+                for (int w = 0; w < 2; w++)
+                    q[w][j] = quantize_code((float)x[2 * s + w][j], table.fast[g][4 * s + j / 2][j % 2 * 2], table.scale[g][4 * s + j / 2][j % 2], QMAX);
+            }
         }
 #pragma unroll
         for (int w = 0; w < 2; w++) {
             const int piece = KEYS ? w * S + s : 2 * s + w;
 #pragma unroll
             for (int p = 0; p < 4; p++) put_pair<BITS, N>(words, 4 * piece + p, q[w][2 * p], q[w][2 * p + 1]);
-        }
-        if (lane % 16 == s) {
-            *(half8v *)(side + 32 * s + 8 * (lane / 16)) = scales;
-            *(half8v *)(side + D + 32 * s + 8 * (lane / 16)) = zeros;
         }
     }
     store_words<N>(to, lane, words);
@@ -183,16 +233,17 @@ __device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, 
 template <int D>
 __global__ void __launch_bounds__(256) paged_quantize(QuantizeArgs a, PagePairs pairs)
 {
-    const int lane = threadIdx.x % kWave;
-    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
-    if (unit >= a.units) return;
-    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks % a.heads;
-    const int2 pair = pairs.at[unit / 2 / blocks / a.heads];
+    __shared__ GroupTable<D> tables[4];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int unit = blockIdx.x * 4 + wave;
+    if (unit >= a.units) return;  // (waves share nothing but the array, of which each has its own part)
+    const int2 pair = pairs.at[blockIdx.y];  // (at once with the other arguments, which come from far)
+    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks;
     const _Float16 *from = a.rows + ((int64_t)pair.x * a.heads + head) * 2 * a.page * D;
     uint32_t *to = a.packed + (((int64_t)pair.y * a.heads + head) * blocks + block) * block_words(D, a.k_bits, a.v_bits);
     _Float16 *side = (_Float16 *)(to + D * (a.k_bits + a.v_bits));
-    if (values) with_bits(a.v_bits, [&](auto B) { quantize_matrix<D, B.value, false>(from, a.page, block, to + D * a.k_bits, side + 2 * D, lane); });
-    else with_bits(a.k_bits, [&](auto B) { quantize_matrix<D, B.value, true>(from, a.page, block, to, side, lane); });
+    if (values) with_bits(a.v_bits, [&](auto B) { quantize_matrix<D, B.value, false>(from, a.page, block, to + D * a.k_bits, side + 2 * D, lane, tables[wave]); });
+    else with_bits(a.k_bits, [&](auto B) { quantize_matrix<D, B.value, true>(from, a.page, block, to, side, lane, tables[wave]); });
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -213,8 +264,10 @@ __global__ void __launch_bounds__(256) paged_read(ReadArgs a, PagePairs ids)
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, m = lane % 16, g = lane / 16;
     const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);
     if (unit >= a.units) return;  // (waves share nothing but the array, of which each has its own part)
-    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks % a.heads, nth = unit / 2 / blocks / a.heads;
-    const int64_t id = nth % 2 ? ids.at[nth / 2].y : ids.at[nth / 2].x;
+    const int nth = blockIdx.y;
+    const int2 two = ids.at[nth / 2];
+    const int64_t id = nth % 2 ? two.y : two.x;
+    const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks;
     half8v x[NP];
     if constexpr (ROWS) {
         const _Float16 *from = (const _Float16 *)a.pool + (id * a.heads + head) * 2 * a.page * D;
@@ -268,17 +321,17 @@ constexpr uint32_t kCopyBytes = 256 * 16 * kCopyPieces;
 struct CopyArgs {
     uint8_t *pool[kCopyPools];
     uint32_t bytes[kCopyPools];      // of a page
-    uint32_t blocks[kCopyPools];     // up to and with this pool, per pair
-    int pools, pairs;
+    uint32_t blocks[kCopyPools];     // up to and with this pool
+    int pools;
 };
 
 __global__ void __launch_bounds__(256) paged_copy(CopyArgs a, PagePairs pairs)
 {
-    const uint32_t per = a.blocks[a.pools - 1], nth = blockIdx.x / per, at = blockIdx.x % per;
+    const uint32_t at = blockIdx.x;
+    const int2 pair = pairs.at[blockIdx.y];
     int p = 0;
     while (at >= a.blocks[p]) p++;
     const uint32_t piece = at - (p ? a.blocks[p - 1] : 0);
-    const int2 pair = pairs.at[nth];
     const uint32_t bytes = a.bytes[p];
     const uint8_t *src = a.pool[p] + (int64_t)pair.x * bytes;
     uint8_t *dst = a.pool[p] + (int64_t)pair.y * bytes;
@@ -363,9 +416,9 @@ extern "C" int kvmix_paged_quantize(const kvmix_paged_pool_t *p, const int32_t *
         const int n = (int)(count - first < kStorePairs ? count - first : kStorePairs);
         PagePairs list{};
         for (int i = 0; i < n; i++) list.at[i] = make_int2(pairs[2 * (first + i)], pairs[2 * (first + i) + 1]);
-        const QuantizeArgs a = {(const _Float16 *)p->rows, (uint32_t *)p->packed, (int)p->kv_heads, (int)p->page_size, (int)(n * per),
-                                p->k_bits, p->v_bits};
-        const unsigned grid = (unsigned)((n * per + 3) / 4);
+        const QuantizeArgs a = {(const _Float16 *)p->rows, (uint32_t *)p->packed, (int)p->kv_heads, (int)p->page_size, (int)per, p->k_bits,
+                                p->v_bits};
+        const dim3 grid((unsigned)((per + 3) / 4), (unsigned)n);
         with_dim(p->head_dim, [&](auto D) { paged_quantize<D.value><<<grid, 256, 0, (hipStream_t)stream>>>(a, list); });
         if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
     }
@@ -389,8 +442,8 @@ extern "C" int kvmix_paged_read(const kvmix_paged_pool_t *p, int packed, const i
         PagePairs list{};
         for (int i = 0; i < n; i++) (i % 2 ? list.at[i / 2].y : list.at[i / 2].x) = pages[first + i];
         const ReadArgs a = {packed ? p->packed : p->rows, (_Float16 *)k + first * size, (_Float16 *)v + first * size, (int)p->kv_heads,
-                            (int)p->page_size, (int)(n * per), p->k_bits, p->v_bits};
-        const unsigned grid = (unsigned)((n * per + 3) / 4);
+                            (int)p->page_size, (int)per, p->k_bits, p->v_bits};
+        const dim3 grid((unsigned)((per + 3) / 4), (unsigned)n);
         with_dim(p->head_dim, [&](auto D) {
             if (packed) paged_read<D.value, false><<<grid, 256, 0, (hipStream_t)stream>>>(a, list);
             else paged_read<D.value, true><<<grid, 256, 0, (hipStream_t)stream>>>(a, list);
@@ -432,8 +485,7 @@ extern "C" int kvmix_paged_copy(void *const *pools, const int64_t *page_bytes, i
             const int64_t n = count - first < kStorePairs ? count - first : kStorePairs;
             PagePairs list{};
             for (int64_t i = 0; i < n; i++) list.at[i] = make_int2(pairs[2 * (first + i)], pairs[2 * (first + i) + 1]);
-            a.pairs = (int)n;
-            paged_copy<<<(unsigned)(n * blocks), 256, 0, (hipStream_t)stream>>>(a, list);
+            paged_copy<<<dim3(blocks, (unsigned)n), 256, 0, (hipStream_t)stream>>>(a, list);
             if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
         }
     }
