@@ -100,7 +100,7 @@ __device__ __forceinline__ half8v row_piece(const _Float16 *page_head, int page,
 struct QuantizeArgs {
     const _Float16 *rows;
     uint32_t *packed;
-    int heads, page, units;  // units: waves of work per pair, head by block by matrix
+    int heads, page;
     int k_bits, v_bits;
 };
 
@@ -134,48 +134,38 @@ __device__ __forceinline__ void halve_pairs(uint32_t *v, int lane)
     }
 }
 
-// What the lanes of a row need to know of its groups, two to an entry: minimum and reciprocal of the scale, and the scale where
-// the reciprocal will not do.
-template <int D>
+// A wave's groups, 32 tokens' or channels': minimum, reciprocal of the scale, scale; and a matrix's words as they are put together.
 struct GroupTable {
-    float fast[4][D / 8][4];   // [row of lanes][pair of groups][minimum, reciprocal, minimum, reciprocal]
-    float scale[4][D / 8][2];
+    float at[4][4][8];  // [row of lanes][pair of groups][minimum, reciprocal, minimum, reciprocal, scale, scale]
 };
 
-// One matrix of one block per wave.  A group's 32 values are two of a lane's (the keys' two tokens, the values' two channels)
-// and those of the sixteen lanes of a row.  Its extremes are found by halving, so that each lane ends with two groups (one at
-// D = 64) whose scales it works out for the row; with every lane working out all 32 of them, and a branch for every two codes,
-// 120 pages of 32 heads took 54 instead of @@ us.  The codes are those of kvmix_quant_pack_last_dim with
-// KVMIX_SCALE_RECIPROCAL, bit for bit.
+// A quarter of one matrix of one block per wave (half at D = 64): the groups of 32 channels (keys) or tokens (values), of each of
+// which a lane has two values and the sixteen lanes of a row the rest.  Extremes are found by halving, so that each lane ends with
+// the two groups whose scales it works out for the row.  With a matrix to a wave, every lane working out all its groups and a
+// branch for every two codes, 120 pages of 32 heads took 54 instead of 51 us; without the last two 42, but four pages of 8 heads 10.7
+// instead of 6.3: that much code in a line takes longer to arrive than to run.  The codes are those of kvmix_quant_pack_last_dim
+// with KVMIX_SCALE_RECIPROCAL, bit for bit.
 template <int D, int BITS, bool KEYS>
-__device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, int block, uint32_t *to, _Float16 *side, int lane, GroupTable<D> &table)
+__device__ __forceinline__ void quantize_set(const _Float16 *from, int page, int block, int set, uint32_t *words, _Float16 *side, int lane, GroupTable &table)
 {
-    constexpr int NP = D / 16, S = D / 32, N = lane_words(D, BITS), PAIRS = D / 8;
+    constexpr int S = D / 32, N = lane_words(D, BITS), R = run_words(N);
     constexpr int QMAX = (1 << BITS) - 1;
     const int g = lane / 16;
-    half8v x[NP];  // [set of eight groups][two of the group]
+    half8v x[2];
 #pragma unroll
-    for (int s = 0; s < S; s++) {
+    for (int w = 0; w < 2; w++) x[w] = row_piece<D, KEYS>(from, page, block, lane, KEYS ? w * S + set : 2 * set + w);
+    uint32_t lo[4], hi[4];
+    const uint4v a = __builtin_bit_cast(uint4v, x[0]), b = __builtin_bit_cast(uint4v, x[1]);
 #pragma unroll
-        for (int w = 0; w < 2; w++) x[2 * s + w] = row_piece<D, KEYS>(from, page, block, lane, KEYS ? w * S + s : 2 * s + w);
-    }
-    uint32_t lo[PAIRS], hi[PAIRS];
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-        const uint4v a = __builtin_bit_cast(uint4v, x[2 * s]), b = __builtin_bit_cast(uint4v, x[2 * s + 1]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) lo[4 * s + j] = pair_min(a[j], b[j]), hi[4 * s + j] = pair_max(a[j], b[j]);
-    }
-    halve_pairs<15, false, PAIRS>(lo, lane), halve_pairs<15, true, PAIRS>(hi, lane);
-    halve_pairs<7, false, PAIRS / 2>(lo, lane), halve_pairs<7, true, PAIRS / 2>(hi, lane);
-    halve_pairs<3, false, PAIRS / 4>(lo, lane), halve_pairs<3, true, PAIRS / 4>(hi, lane);
-    if constexpr (PAIRS == 16) {
-        halve_pairs<1, false, 2>(lo, lane), halve_pairs<1, true, 2>(hi, lane);
-    } else {  // (one left: both lanes of a pair get it)
-        lo[0] = pair_min(lo[0], __builtin_amdgcn_update_dpp(0, lo[0], 0xb1, 0xf, 0xf, true));
-        hi[0] = pair_max(hi[0], __builtin_amdgcn_update_dpp(0, hi[0], 0xb1, 0xf, 0xf, true));
-    }
-    const int mine = lane % 16 * PAIRS / 16;
+    for (int j = 0; j < 4; j++) lo[j] = pair_min(a[j], b[j]), hi[j] = pair_max(a[j], b[j]);
+    halve_pairs<15, false, 4>(lo, lane), halve_pairs<15, true, 4>(hi, lane);
+    halve_pairs<7, false, 2>(lo, lane), halve_pairs<7, true, 2>(hi, lane);
+    // (one left: the lanes of a quarter all get it)
+    lo[0] = pair_min(lo[0], __builtin_amdgcn_update_dpp(0, lo[0], 0x1b, 0xf, 0xf, true));
+    hi[0] = pair_max(hi[0], __builtin_amdgcn_update_dpp(0, hi[0], 0x1b, 0xf, 0xf, true));
+    lo[0] = pair_min(lo[0], __builtin_amdgcn_update_dpp(0, lo[0], 0xb1, 0xf, 0xf, true));
+    hi[0] = pair_max(hi[0], __builtin_amdgcn_update_dpp(0, hi[0], 0xb1, 0xf, 0xf, true));
+    const int mine = lane % 16 / 4;
     {
         const half2v l = __builtin_bit_cast(half2v, lo[0]), h = __builtin_bit_cast(half2v, hi[0]);
         half2v scales;
@@ -186,64 +176,94 @@ __device__ __forceinline__ void quantize_matrix(const _Float16 *from, int page, 
             fast[2 * i] = mn, fast[2 * i + 1] = quantize_rcp(scale), exact[i] = scale;
             scales[i] = (_Float16)scale_for_output(range, scale, 1.0f / (float)QMAX, KVMIX_SCALE_RECIPROCAL);
         }
-        *(floatx4 *)table.fast[g][mine] = floatx4{fast[0], fast[1], fast[2], fast[3]};
-        table.scale[g][mine][0] = exact[0], table.scale[g][mine][1] = exact[1];
-        _Float16 *at = side + 32 * (mine / 4) + 8 * g + 2 * (mine % 4);
-        *(half2v *)at = scales;
-        *(uint32_t *)(at + D) = lo[0];
+        if (lane % 4 == 0) {
+            *(floatx4 *)table.at[g][mine] = floatx4{fast[0], fast[1], fast[2], fast[3]};
+            table.at[g][mine][4] = exact[0], table.at[g][mine][5] = exact[1];
+            _Float16 *at = side + 32 * set + 8 * g + 2 * mine;
+            *(half2v *)at = scales;
+            *(uint32_t *)(at + D) = lo[0];
+        }
     }
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
-    uint32_t words[N] = {};
+    uint32_t q[2][8];
+    bool near = false;
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-        uint32_t q[2][8];
-        bool near = false;
+    for (int p = 0; p < 4; p++) {
+        const floatx4 f = *(const floatx4 *)table.at[g][p];
 #pragma unroll
-        for (int p = 0; p < 4; p++) {
-            const floatx4 f = *(const floatx4 *)table.fast[g][4 * s + p];
+        for (int i = 0; i < 2; i++) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                // (as quantize_code_fast, but for the limit: a quotient above it is near)
+                const float u = fmaf((float)x[w][2 * p + i] - f[2 * i], f[2 * i + 1], 0.5f);
+                near |= !(fabsf(__builtin_amdgcn_fractf(u) - 0.5f) <= 0.5f - 0.000030517578125f);
+                q[w][2 * p + i] = (uint32_t)u;
+            }
+        }
+    }
+    if (__builtin_expect(near, 0)) {
+#pragma unroll 1
+        for (int p = 0; p < 4; p++) {  // (values and codes by selection: a loop over registers)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    // (as quantize_code_fast, but for the limit: a quotient above it is near)
-                    const float u = fmaf((float)x[2 * s + w][2 * p + i] - f[2 * i], f[2 * i + 1], 0.5f);
-                    near |= !(fabsf(__builtin_amdgcn_fractf(u) - 0.5f) <= 0.5f - 0.000030517578125f);
-                    q[w][2 * p + i] = (uint32_t)u;
+                    const half8v y = x[w];
+                    const float v = (float)(p == 0 ? y[i] : p == 1 ? y[2 + i] : p == 2 ? y[4 + i] : y[6 + i]);
+                    const uint32_t c = quantize_code(v, table.at[g][p][2 * i], table.at[g][p][4 + i], QMAX);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) q[w][2 * k + i] = k == p ? c : q[w][2 * k + i];
                 }
             }
         }
-        if (__builtin_expect(near, 0)) {
+    }
+    auto put = [&](int word, uint32_t bits) { atomicOr(&words[word / R * kWave * R + lane * R + word % R], bits); };
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+    for (int w = 0; w < 2; w++) {
+        const int piece = KEYS ? w * S + set : 2 * set + w;
+        if constexpr (BITS != 3) {  // a piece is a part of one word
+            uint32_t part = 0;
 #pragma unroll
-                for (int w = 0; w < 2; w++)
-                    q[w][j] = quantize_code((float)x[2 * s + w][j], table.fast[g][4 * s + j / 2][j % 2 * 2], table.scale[g][4 * s + j / 2][j % 2], QMAX);
+            for (int p = 0; p < 4; p++) part |= (q[w][2 * p] | q[w][2 * p + 1] << 16) << (BITS * p);
+            put(piece * BITS / 4, part << (piece * BITS % 4 * 4));
+        } else {
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                const uint32_t c = q[w][2 * p] | q[w][2 * p + 1] << 16;
+                const int t = 4 * piece + p;
+                if (t < 5 * N) {
+                    put(t / 5, c << (t % 5 * 3));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 3; i++) put(3 * (t - 5 * N) + i, (c >> i & 0x00010001u) << 15);
+                }
             }
         }
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-            const int piece = KEYS ? w * S + s : 2 * s + w;
-#pragma unroll
-            for (int p = 0; p < 4; p++) put_pair<BITS, N>(words, 4 * piece + p, q[w][2 * p], q[w][2 * p + 1]);
-        }
     }
-    store_words<N>(to, lane, words);
 }
 
 template <int D>
 __global__ void __launch_bounds__(256) paged_quantize(QuantizeArgs a, PagePairs pairs)
 {
-    __shared__ GroupTable<D> tables[4];
+    constexpr int S = D / 32, M = 4 / S;  // waves to a matrix, matrices to a block
+    __shared__ GroupTable tables[4];
+    __shared__ __attribute__((aligned(16))) uint32_t words[M][kWave * lane_words(D, 4)];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int unit = blockIdx.x * 4 + wave;
-    if (unit >= a.units) return;  // (waves share nothing but the array, of which each has its own part)
     const int2 pair = pairs.at[blockIdx.y];  // (at once with the other arguments, which come from far)
+    const int unit = blockIdx.x * M + wave / S, set = wave % S;
     const int blocks = a.page / kBlock, values = unit % 2, block = unit / 2 % blocks, head = unit / 2 / blocks;
     const _Float16 *from = a.rows + ((int64_t)pair.x * a.heads + head) * 2 * a.page * D;
     uint32_t *to = a.packed + (((int64_t)pair.y * a.heads + head) * blocks + block) * block_words(D, a.k_bits, a.v_bits);
     _Float16 *side = (_Float16 *)(to + D * (a.k_bits + a.v_bits));
-    if (values) with_bits(a.v_bits, [&](auto B) { quantize_matrix<D, B.value, false>(from, a.page, block, to + D * a.k_bits, side + 2 * D, lane, tables[wave]); });
-    else with_bits(a.k_bits, [&](auto B) { quantize_matrix<D, B.value, true>(from, a.page, block, to, side, lane, tables[wave]); });
+    uint32_t *mine = words[wave / S];
+    for (int i = set * kWave + lane; i < kWave * lane_words(D, 4) / 4; i += S * kWave) ((uint4v *)mine)[i] = uint4v{0, 0, 0, 0};
+    __syncthreads();
+    if (values) with_bits(a.v_bits, [&](auto B) { quantize_set<D, B.value, false>(from, a.page, block, set, mine, side + 2 * D, lane, tables[wave]); });
+    else with_bits(a.k_bits, [&](auto B) { quantize_set<D, B.value, true>(from, a.page, block, set, mine, side, lane, tables[wave]); });
+    __syncthreads();
+    const int bits = values ? a.v_bits : a.k_bits;
+    to += values ? D * a.k_bits : 0;
+    for (int i = set * kWave + lane; i < D * bits / 4; i += S * kWave) ((uint4v *)to)[i] = ((const uint4v *)mine)[i];
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -416,9 +436,8 @@ extern "C" int kvmix_paged_quantize(const kvmix_paged_pool_t *p, const int32_t *
         const int n = (int)(count - first < kStorePairs ? count - first : kStorePairs);
         PagePairs list{};
         for (int i = 0; i < n; i++) list.at[i] = make_int2(pairs[2 * (first + i)], pairs[2 * (first + i) + 1]);
-        const QuantizeArgs a = {(const _Float16 *)p->rows, (uint32_t *)p->packed, (int)p->kv_heads, (int)p->page_size, (int)per, p->k_bits,
-                                p->v_bits};
-        const dim3 grid((unsigned)((per + 3) / 4), (unsigned)n);
+        const QuantizeArgs a = {(const _Float16 *)p->rows, (uint32_t *)p->packed, (int)p->kv_heads, (int)p->page_size, p->k_bits, p->v_bits};
+        const dim3 grid((unsigned)(per / (128 / p->head_dim)), (unsigned)n);
         with_dim(p->head_dim, [&](auto D) { paged_quantize<D.value><<<grid, 256, 0, (hipStream_t)stream>>>(a, list); });
         if (launch_status() != KVMIX_OK) return KVMIX_ERR_LAUNCH;
     }
