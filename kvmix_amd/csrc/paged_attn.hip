@@ -92,6 +92,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
     constexpr bool kScaleQueries = NR == 1;
     constexpr int DEPTH = KB + VB > 6 ? 2 : KB + VB > 3 ? 3 : 4;  // blocks in flight
+    // whether keys' channels, and values' tokens, are taken in the order in which two-bit codes come cheapest (a lane then has
+    // whole pieces of scales and minima, D = 128)
+    constexpr bool kTurnK = KB == 2 && D == 128, kTurnV = VB == 2 && D == 128;
     constexpr int kPad = D + 4;
     __shared__ union {
         uint32_t side[4][2 * D];
@@ -122,7 +125,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             limit[n] = kv_len - q_len + token;
             const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * g;
 #pragma unroll
-            for (int s = 0; s < KS; s++) q[n][s] = *(const half8v *)(at + 32 * s) * (_Float16)kShrink;
+            for (int s = 0; s < KS; s++) {
+                q[n][s] = *(const half8v *)(at + 32 * s) * (_Float16)kShrink;
+                if constexpr (kTurnK) q[n][s] = turned(q[n][s]);
+            }
         }
         const int first_limit = kv_len - q_len + it.row0 / a.group;
 
@@ -162,15 +168,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[i / 4][n][i % 4], scale, -top[n]));
+                    const int t = kTurnV && packed_tokens.value ? i / 2 + i % 2 * 4 : i;  // (the order of the values' tokens)
+                    p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[t / 4][n][t % 4], scale, -top[n]));
                     if (i % 2) sum[n] = __builtin_amdgcn_fdot2(half2v{p[n][i - 1], p[n][i]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum[n], false);
                 }
             }
         };
 
+        auto key_codes = [&](const PackedBlock<D, KB, VB> &b, int piece) {
+            if constexpr (kTurnK) return piece_codes_turned(b.k, piece);
+            else return piece_codes<KB, NK>(b.k, piece, ke);
+        };
+        auto value_codes = [&](const PackedBlock<D, KB, VB> &b, int piece) {
+            if constexpr (kTurnV) return piece_codes_turned(b.v, piece);
+            else return piece_codes<VB, NV>(b.v, piece, ve);
+        };
         auto take_packed = [&](const PackedBlock<D, KB, VB> &b) {
             uint32_t *side = lds.side[wave];
-            store_words<D / 32>(side, lane, b.side);
+            if constexpr (kTurnK || kTurnV) {  // (lanes 0 .. 31 have the keys', the others the values')
+                const half8v natural = __builtin_bit_cast(half8v, uint4v{b.side[0], b.side[1], b.side[2], b.side[3]}), other = turned(natural);
+                const bool turn = kTurnK && kTurnV ? true : kTurnV == (lane >= 32);
+                *(uint4v *)(side + 4 * lane) = turn ? __builtin_bit_cast(uint4v, other) : __builtin_bit_cast(uint4v, natural);
+            } else {
+                store_words<D / 32>(side, lane, b.side);
+            }
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
             const _Float16 *sides = (const _Float16 *)side + 8 * g;
             floatx4 x[2][NR] = {};
@@ -186,12 +207,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     const half8v scaled = q[0][s] * scales;
 #pragma unroll
                     for (int u = 0; u < 2; u++)
-                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece_codes<KB, NK>(b.k, u * KS + s, ke), scaled, x[u][0], 0, 0, 0);
+                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes(b, u * KS + s), scaled, x[u][0], 0, 0, 0);
                 } else {
                     const half8v zeros = *(const half8v *)(sides + D + 32 * s);
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        const half8v k = piece_values<KB, NK>(b.k, u * KS + s, scales, zeros, ke);
+                        const half8v k = __builtin_elementwise_fma(key_codes(b, u * KS + s), scales, zeros);
 #pragma unroll
                         for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
                     }
@@ -204,7 +225,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 const half8v scales = *(const half8v *)(sides + 2 * D + 32 * s), zeros = *(const half8v *)(sides + 3 * D + 32 * s);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const half8v v = piece_values<VB, NV>(b.v, 2 * s + u, scales, zeros, ve);
+                    const half8v v = __builtin_elementwise_fma(value_codes(b, 2 * s + u), scales, zeros);
 #pragma unroll
                     for (int n = 0; n < NR; n++) acc[n][2 * s + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n], acc[n][2 * s + u], 0, 0, 0);
                 }
@@ -243,6 +264,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     take_packed(held[i]);
                     block += 4;
                 }
+            }
+        }
+        if constexpr (kTurnK) {
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) q[n][s] = turned_back(q[n][s]);
             }
         }
         for (; block < it.end; block += 4) {
