@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
     constexpr bool kScaleQueries = NR == 1;
-    constexpr int DEPTH = KB + VB > 6 ? 2 : KB + VB > 3 ? 3 : 4;  // blocks in flight
+    constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB > 3 ? 3 : 4;  // blocks in flight
     // whether keys' channels, and values' tokens, are taken in the order in which two-bit codes come cheapest (a lane then has
     // whole pieces of scales and minima, D = 128)
     constexpr bool kTurnK = KB == 2 && D == 128, kTurnV = VB == 2 && D == 128;
@@ -194,20 +194,24 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             }
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
             const _Float16 *sides = (const _Float16 *)side + 8 * g;
-            floatx4 x[2][NR] = {};
+            floatx4 x[2][NR] = {}, low[2] = {};  // (sums of their own: half as long a chain of products)
             if constexpr (kScaleQueries) {
 #pragma unroll
-                for (int s = 0; s < KS; s++) x[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8v *)(sides + D + 32 * s), q[0][s], x[0][0], 0, 0, 0);
-                x[1][0] = x[0][0];
+                for (int s = 0; s < KS; s++) low[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8v *)(sides + D + 32 * s), q[0][s], low[0], 0, 0, 0);
+                low[1] = low[0];
             }
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 const half8v scales = *(const half8v *)(sides + 32 * s);
                 if constexpr (kScaleQueries) {
-                    const half8v scaled = q[0][s] * scales;
+                    // in two halves, the product and what it rounds off: the logits are then exact but for the sums
+                    const half8v scaled = q[0][s] * scales, rest = __builtin_elementwise_fma(q[0][s], scales, -scaled);
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_codes(b, u * KS + s), scaled, x[u][0], 0, 0, 0);
+                    for (int u = 0; u < 2; u++) {
+                        const half8v codes = key_codes(b, u * KS + s);
+                        low[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, rest, low[u], 0, 0, 0);
+                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, scaled, x[u][0], 0, 0, 0);
+                    }
                 } else {
                     const half8v zeros = *(const half8v *)(sides + D + 32 * s);
 #pragma unroll
@@ -217,6 +221,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                         for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
                     }
                 }
+            }
+            if constexpr (kScaleQueries) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) x[u][0] += low[u];
             }
             half8v p[NR];
             probabilities(x, p, 0, std::true_type());
