@@ -973,7 +973,7 @@ extern "C" int kvmix_paged_plan(const kvmix_paged_batch_t *batch, int32_t *words
     if (!plan) return KVMIX_ERR_NULL;
     try {
         return make_plan(batch, words, capacity, plan);
-    } catch (const std::bad_alloc &) {
+    } catch (...) {  // (lists that do not fit in memory; no exception leaves a C entry)
         return KVMIX_ERR_MEMORY;
     }
 }

@@ -2,6 +2,7 @@
 // memory, or by the launch where there is little of it.
 #include <stdlib.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_common.h"
@@ -381,17 +382,15 @@ using namespace kvmix;
 
 namespace {
 
-// Whether no page of [0, pages) is written twice by these pairs, nor (`read_too`) written and read.
-int pairs_apart(const int32_t *pairs, int64_t count, int64_t pages, bool read_too)
+// Whether no page is written twice by these pairs, nor (`read_too`) written and read.
+int pairs_apart(const int32_t *pairs, int64_t count, bool read_too)
 {
-    uint8_t *written = (uint8_t *)calloc((size_t)pages, 1);
+    int32_t *written = (int32_t *)malloc((size_t)count * sizeof(int32_t));
     if (!written) return KVMIX_ERR_MEMORY;
-    bool apart = true;
-    for (int64_t i = 0; i < count; i++) {
-        apart = apart && !written[pairs[2 * i + 1]];
-        written[pairs[2 * i + 1]] = 1;
-    }
-    for (int64_t i = 0; read_too && i < count; i++) apart = apart && !written[pairs[2 * i]];
+    for (int64_t i = 0; i < count; i++) written[i] = pairs[2 * i + 1];
+    std::sort(written, written + count);
+    bool apart = std::adjacent_find(written, written + count) == written + count;
+    for (int64_t i = 0; read_too && apart && i < count; i++) apart = !std::binary_search(written, written + count, pairs[2 * i]);
     free(written);
     return apart ? KVMIX_OK : KVMIX_ERR_PAGE_ORDER;
 }
@@ -429,7 +428,7 @@ extern "C" int kvmix_paged_quantize(const kvmix_paged_pool_t *p, const int32_t *
     if (!pairs || !p->rows || !p->packed) return KVMIX_ERR_NULL;
     for (int64_t i = 0; i < count; i++)
         if (pairs[2 * i] < 0 || pairs[2 * i] >= p->row_pages || pairs[2 * i + 1] < 0 || pairs[2 * i + 1] >= p->packed_pages) return KVMIX_ERR_PAGE;
-    rc = pairs_apart(pairs, count, p->packed_pages, false);
+    rc = pairs_apart(pairs, count, false);
     if (rc != KVMIX_OK) return rc;
     const int64_t per = p->kv_heads * (p->page_size / kBlock) * 2;
     for (int64_t first = 0; first < count; first += kStorePairs) {
@@ -487,7 +486,7 @@ extern "C" int kvmix_paged_copy(void *const *pools, const int64_t *page_bytes, i
     if (pages > kMost32) return KVMIX_ERR_UNSUPPORTED;
     for (int64_t i = 0; i < 2 * count; i++)
         if (pairs[i] < 0 || pairs[i] >= pages) return KVMIX_ERR_PAGE;
-    const int rc = pairs_apart(pairs, count, pages, true);
+    const int rc = pairs_apart(pairs, count, true);
     if (rc != KVMIX_OK) return rc;
     for (int64_t p0 = 0; p0 < n_pools; p0 += kCopyPools) {
         CopyArgs a{};

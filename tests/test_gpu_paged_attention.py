@@ -108,6 +108,42 @@ def test_new_tokens_see_their_own_past_only(dev):
     del k, v
 
 
+def test_pages_beyond_32_bit_offsets(dev):
+    """Pools whose last pages lie behind 2^31 elements (4.3 GB of fp16 pages, 10.7 GB of packed ones)."""
+    from kvmix_amd import ops
+
+    b = Batch(dev, [300, 150], [128, 64], [1, 40], 4, 4, 128, 64, 4, 4, seed=13)
+    want = attend(b)
+    far = 1 << 15                                     # 65536 halves to a page of 4 heads
+    rows = torch.empty(far + b.rows.shape[0], *b.rows.shape[1:], dtype=torch.float16, device=dev)
+    rows[far:] = b.rows
+    words = b.packed.shape[1] * b.packed.shape[2]     # 10240 to a page
+    behind = -(-(1 << 31) // words) + 5
+    packed = torch.empty(behind + b.packed.shape[0], *b.packed.shape[1:], dtype=torch.int32, device=dev)
+    ids = torch.arange(b.packed.shape[0])
+    k, v = ops.paged_read(b.packed, ids, 4, 4, 128)
+    packed[behind:] = b.packed
+    table = b.table.clone()
+    for s, p in enumerate((2, 1)):
+        table[s, :p] += behind
+        table[s, p:] += far
+    plan = ops.paged_plan(table, b.lens, b.packed_lens, b.new, 4, 4, 128, 64, dev)
+    assert torch.equal(ops.paged_attention(b.q, rows, packed, plan, 4, 4), want)
+    again = ops.paged_read(packed, ids + behind, 4, 4, 128)
+    for got, ref in zip(again, (k, v)):               # by their bits: unused pages hold NaN
+        assert torch.equal(got.view(torch.int16), ref.view(torch.int16))
+    ops.paged_quantize(rows, packed, torch.tensor([[far, behind - 1]]), 4, 4)
+    one = torch.zeros_like(b.packed)
+    ops.paged_quantize(b.rows, one, torch.tensor([[0, 1]]), 4, 4)
+    assert torch.equal(packed[behind - 1], one[1])
+    ops.paged_copy([packed], torch.tensor([[behind + 1, 0]]))
+    assert torch.equal(packed[0], b.packed[1])
+    kv = torch.randn(41, 4, 128, dtype=torch.float16, device=dev)
+    ops.paged_append(kv, kv, rows, plan)
+    ops.paged_append(kv, kv, b.rows, b.plan)
+    assert torch.equal(rows[far:].nan_to_num(9.0), b.rows.nan_to_num(9.0))
+
+
 def test_strides_and_alignment_of_queries(dev):
     b = Batch(dev, [333, 64], [128, 0], [40, 1], 8, 4, 128, 64, 2, 4, seed=9)
     want = attend(b)
