@@ -108,4 +108,65 @@ class PagedDecoder:
         return torch.cat(lp), torch.cat(entropy)
 
 
+def main() -> None:
+    """A server in small, on random weights: prompts that arrive in chunks beside sequences that are being answered, several
+    answers from one prompt, and what the quantized cache makes of a text's likelihoods."""
+    import argparse
+    import time
+
+    from .decoder import init_weights
+
+    ap = argparse.ArgumentParser(description=main.__doc__)
+    ap.add_argument("--layers", type=int, default=8)
+    ap.add_argument("--kv-heads", type=int, default=8)
+    ap.add_argument("--prompts", type=int, default=8)
+    ap.add_argument("--prompt", type=int, default=2000, help="tokens of the longest prompt")
+    ap.add_argument("--chunk", type=int, default=512)
+    ap.add_argument("--answers", type=int, default=4, help="sequences forked from each prompt")
+    ap.add_argument("--new", type=int, default=32, help="tokens of each answer")
+    ap.add_argument("--bits", type=int, default=4)
+    args = ap.parse_args()
+    cfg = DecoderConfig(num_layers=args.layers, num_kv_heads=args.kv_heads)
+    weights = init_weights(cfg, "cuda")
+    bits = [args.bits] * args.layers
+    pages = args.prompts * args.answers * 8
+    model = PagedDecoder(cfg, weights, bits, bits, row_pages=pages + args.prompts * (args.prompt // 64 + 2),
+                         packed_pages=args.prompts * (args.prompt // 64 + args.answers * (args.new // 64 + 4)))
+    lens = [max(1, args.prompt - i * args.prompt // (2 * args.prompts)) for i in range(args.prompts)]
+    texts = {model.add(): torch.randint(0, cfg.vocab_size, (n,), device="cuda") for n in lens}
+
+    def timed(what, count, f):
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        r = f()
+        torch.cuda.synchronize()
+        print(f"{what}: {count} tokens, {count / (time.perf_counter() - t):.0f} tokens/s", flush=True)
+        return r
+
+    def read_prompts():
+        last, at = {}, 0
+        while any(at < t.numel() for t in texts.values()):
+            last.update(model.forward({s: t[at:at + args.chunk] for s, t in texts.items()}))
+            at += args.chunk
+        return last
+
+    last = timed("prompts in chunks", sum(lens), read_prompts)
+    answers, first = [], []
+    for s in texts:
+        twins = [s] + [model.fork(s) for _ in range(args.answers - 1)]
+        answers += twins
+        _, _, _, top = ops.token_logprobs(last[s], last[s].argmax(), top=args.answers)  # each answer begins with another token
+        first += list(top)
+    ids = timed("answers", len(answers) * (args.new - 1), lambda: model.generate(answers, torch.stack(first), args.new))
+    print("pages free (fp16, packed):", model.cache.free_pages())
+    for s in answers:
+        model.free(s)
+    text = torch.cat([next(iter(texts.values())), ids[0]])
+    lp, entropy = timed("likelihoods", text.numel() - 1, lambda: model.score(text, args.chunk))
+    print(f"mean log probability {lp.mean():.4f}, mean entropy {entropy.mean():.4f}")
+
+
 __all__ = ["PagedDecoder"]
+
+if __name__ == "__main__":
+    main()
