@@ -594,7 +594,7 @@ int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t 
  * pages already).  Packed values are taken as fp16 (code * scale + minimum, rounded once), logits, softmax and sums in fp32,
  * probabilities rounded to fp16 for the product with the values and for its sum alike.
  *   q, out [plan.tokens, heads, head_dim] fp16, unit stride along head_dim, strides in elements, multiples of 8; 16-byte aligned
- *   list: the plan's words in device memory;  scale > 0
+ *   list: the plan's words in device memory;  0 < scale <= 2^40
  * What pages hold behind a sequence's last token is not used, whatever it is.  The values of a sequence's own tokens are expected to
  * be finite: the products are made for blocks of 32 or 64 tokens, and zero times an infinite value of a later new token of the
  * same block is NaN in that channel of the new tokens before it.  (Keys may be anything: a logit that is not to be seen is replaced.)

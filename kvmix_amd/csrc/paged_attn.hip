@@ -21,7 +21,6 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // tokens, tokens, packed tokens (here, so that what a block needs is one load away); in paged_few, with the first item of a block,
 // how many it has and where the others begin
 constexpr int kItemWords = 12;
-constexpr float kShrink = 0.015625f;  // of queries in paged_few: their products with keys' scales stay in fp16's range up to 4e6
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -91,7 +90,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
     constexpr bool kScaleQueries = NR == 1;
-    constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB > 3 ? 3 : 4;  // blocks in flight
+    constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB + NR > 4 ? 3 : 4;  // blocks in flight: what the registers hold
     // whether keys' channels, and values' tokens, are taken in the order in which two-bit codes come cheapest (a lane then has
     // whole pieces of scales and minima, D = 128)
     constexpr bool kTurnK = KB == 2 && D == 128, kTurnV = VB == 2 && D == 128;
@@ -106,7 +105,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const int head = blockIdx.x % a.kv_heads, column = blockIdx.x / a.kv_heads;
     const int per_page = 1 << a.blocks_log2;
-    const float scale = a.scale / kShrink;
     const Exponents<KB> ke;
     const Exponents<VB> ve;
 
@@ -119,6 +117,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 
         half8v q[NR][KS];
         int limit[NR];  // the row's own token
+        float scale = a.scale;
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const int r = it.row0 + min(16 * n + m, it.rows - 1), token = r / a.group;
@@ -126,9 +125,24 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             const _Float16 *at = a.q + (int64_t)(q_start + token) * a.q_ts + (int64_t)(head * a.group + r % a.group) * a.q_hs + 8 * g;
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                q[n][s] = *(const half8v *)(at + 32 * s) * (_Float16)kShrink;
+                q[n][s] = *(const half8v *)(at + 32 * s);
                 if constexpr (kTurnK) q[n][s] = turned(q[n][s]);
             }
+        }
+        if constexpr (kScaleQueries) {
+            // A row's queries times the power of two that puts the largest into [0.5, 1): their products with the keys' scales are
+            // then finite whatever both are, and small queries keep their bits.
+            half8v most = q[0][0] < (_Float16)0.0f ? -q[0][0] : q[0][0];
+#pragma unroll
+            for (int s = 1; s < KS; s++) most = __builtin_elementwise_max(most, q[0][s] < (_Float16)0.0f ? -q[0][s] : q[0][s]);
+            float largest = (float)most[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) largest = fmaxf(largest, (float)most[j]);
+            const int e = min(max((int)(__float_as_uint(max_of_rows(largest)) >> 23) - 126, -24), 16);
+            const _Float16 once = (_Float16)__builtin_ldexpf(1.0f, -e / 2), twice = (_Float16)__builtin_ldexpf(1.0f, -e - -e / 2);
+#pragma unroll
+            for (int s = 0; s < KS; s++) q[0][s] = q[0][s] * once * twice;
+            scale = __builtin_ldexpf(scale, e);
         }
         const int first_limit = kv_len - q_len + it.row0 / a.group;
 
@@ -954,7 +968,8 @@ int attention_check(const kvmix_paged_pool_t *p, const kvmix_paged_plan_t *plan,
     if (rc != KVMIX_OK) return rc;
     if (plan->kv_heads != p->kv_heads || plan->head_dim != p->head_dim || plan->page_size != p->page_size) return KVMIX_ERR_SHAPE;
     if (plan->row_pages > p->row_pages || plan->packed_pages > p->packed_pages) return KVMIX_ERR_PAGE;
-    if (!(c->scale > 0.0f) || c->scale > 1e30f) return KVMIX_ERR_UNSUPPORTED;
+    if (!(c->scale > 0.0f) || c->scale > 0x1p40f)  // (no logit of fp16 numbers is beyond 1e25 then)
+        return KVMIX_ERR_UNSUPPORTED;
     for (int64_t s : {c->q_token_stride, c->q_head_stride, c->out_token_stride, c->out_head_stride})
         if (s % 8 != 0) return KVMIX_ERR_UNSUPPORTED;
     if (((uintptr_t)c->q | (uintptr_t)c->out) % 16 != 0 || (uintptr_t)c->list % 4 != 0) return KVMIX_ERR_UNSUPPORTED;

@@ -76,6 +76,17 @@ def test_small_and_large_values(dev, size):
     assert ((got.cpu().double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("bits", [(4, 4), (2, 2), (1, 3)])
+@pytest.mark.parametrize("q_size, k_size, scale", [(1e-3, 300.0, None), (1e-6, 1000.0, 20.0), (6000.0, 1e-3, 1e-2), (6000.0, 1000.0, 1e-9)])
+def test_queries_of_other_sizes(dev, bits, q_size, k_size, scale):
+    b = Batch(dev, [700, 450, 300], [512, 256, 128], [1, 50, 5], 4, 2, 128, 64, *bits, seed=17, scale=k_size)
+    b.q[0, 1] = 0.0
+    b.q *= q_size
+    got = attend(b, scale=scale)
+    want, tol = b.want(scale)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
 def test_one_token_takes_all(dev):
     """A key that is far above all others: exactly its value comes back, and nothing overflows."""
     b = Batch(dev, [300, 300], [128, 128], [1, 64], 2, 2, 128, 64, 4, 4, seed=7)
