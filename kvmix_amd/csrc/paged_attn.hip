@@ -83,8 +83,16 @@ __device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uin
 // Few rows.  A block works through the items of its column (parts of sequences that add up to the same number of tokens for every
 // column).  Every wave takes every fourth block of 32 tokens of an item's span, sixteen (NR times) rows of queries
 // at once, with v_mfma_f32_16x16x32: the logits transposed (tokens as rows of the result), so that a lane holds those of one query
-// and its probabilities are the operand of out^T = v^T p^T as they are.  Codes go from memory to registers, a block ahead, become
+// and its probabilities are the operand of out^T = v^T p^T as they are.  Codes go from memory to registers, DEPTH blocks ahead, become
 // fp16 there and are used once.
+//
+// q.k = sum_d (q_d s_d) c_d + q_d z_d with a channel's scale s and minimum z: for sixteen rows the scales go to the queries (a
+// product per block and channel, not per code), in two halves, so that the logits of packed keys are exact but for the sums (with
+// one half the error of the whole against 64 bits was 1.2 to 1.5e-3, with two 2.7 to 3.2e-4; a result's own rounding is 2.1e-4.
+// It costs 5 us of 70).  For 32 rows that would be two products each, so there keys become fp16 first.
+//
+// Bound by vector instructions and memory together: 16 x 8192 tokens of 32 heads, 2/2 bits, 66 us (314 MB, 4.8 TB/s; one byte of
+// codes is eight values to convert), 4/4 bits 92 us (490 MB, 5.3 TB/s), 3/2 bits of 8 heads over 32768 tokens 73 us (4.5 TB/s).
 template <int D, int KB, int VB, int NR>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 3 : 2))) paged_few(PagedArgs a)
 {
@@ -390,7 +398,11 @@ __device__ __forceinline__ int tile_value(int channel, int c) { return channel *
 // Many rows: 128 of them to a block, 32 to a wave, over tiles of 64 tokens.  A tile is four matrices of 32 tokens, keys and values
 // of two blocks; each wave turns one of them from codes to fp16, for all four.  Products with v_mfma_f32_32x32x16: logits
 // transposed, keys as rows in an order in which a lane's logits are those of eight tokens that follow one another, as the
-// values' pieces are.
+// values' pieces are.  Packed keys and values are rounded to fp16 once (code * scale + minimum): the matrix cores take no others at this rate.
+//
+// Bound by the matrix cores and, in turns with them, the vector ALU (exponentials 9 cycles each, conversions of codes): 4 chunks of 2048 tokens over
+// 8192, 32 heads, 4/4 bits: 800 us, 860 TFLOP/s of the 1490 that a fp16 product of 16384 reaches (855 with the codes converted between
+// tiles, on a box on which the others took 786).  Two blocks to a CU is what the LDS (66 KB each) and the registers (256) hold.
 template <int D, int KB, int VB>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) paged_tile(PagedArgs a)
 {
@@ -685,7 +697,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 }
 
 // The spans of one sequence's rows together: a row per wave, or per block where there are many spans; the item's `begin` is the
-// number of spans, `end` the rows between them.  Bound by latency: spans are read eight at a time.
+// number of spans, `end` the rows between them.  Bound by latency, 3 to 5 us: spans are read eight at a time.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join(PagedArgs a)
 {

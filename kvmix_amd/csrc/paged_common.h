@@ -70,12 +70,8 @@ __device__ __forceinline__ void store_words(uint32_t *at, int lane, const uint32
     }
 }
 
-// Where pair `t` of a lane's N words lies: word and bit (the second code 16 bits higher).  Three-bit pairs past 5 N take the top
-// bits of three words' halves, one bit from each.
-template <int BITS, int N>
-struct Pairs {
-    static constexpr int per = BITS == 3 ? 5 : 16 / BITS;
-};
+// Pairs of codes to a word.  Three-bit pairs past 5 N of a lane's N words take the top bits of three words' halves, one bit from each.
+__host__ __device__ constexpr int word_pairs(int bits) { return bits == 3 ? 5 : 16 / bits; }
 
 // Pair `t` as two halves that hold the codes exactly.  A field at bit s of a half, under the exponent of 2^(10 - s), is the code
 // plus 2^(10 - s): the bits are masked in place, in one operation with the exponent (v_and_or_b32 takes one scalar and no
@@ -102,7 +98,7 @@ __device__ __forceinline__ half2v code_pair(const uint32_t *w, int t, const Expo
 {
     constexpr uint32_t ones = 0x00010001u;
     constexpr uint32_t mask = (1u << BITS) - 1;
-    constexpr int per = Pairs<BITS, N>::per;
+    constexpr int per = word_pairs(BITS);
     if (t >= N * per) {  // (3 bits only)
         const int r = 3 * (t - N * per);
         const uint32_t c = (w[r] >> 15 & ones) | (w[r + 1] >> 14 & 2 * ones) | (w[r + 2] >> 13 & 4 * ones) | e.at[0];
@@ -114,21 +110,6 @@ __device__ __forceinline__ half2v code_pair(const uint32_t *w, int t, const Expo
     asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(c) : "v"(v), "s"(mask * ones << s), "v"(e.at[s / BITS]));
     const _Float16 base = (_Float16)(float)(1 << (10 - s));
     return __builtin_bit_cast(half2v, c) - half2v{base, base};
-}
-
-// Codes (0 .. 2^BITS - 1) of pair t into the words (which start at zero).
-template <int BITS, int N>
-__device__ __forceinline__ void put_pair(uint32_t *w, int t, uint32_t first, uint32_t second)
-{
-    constexpr int per = Pairs<BITS, N>::per;
-    const uint32_t c = first | second << 16;
-    if (t >= N * per) {
-        const int r = 3 * (t - N * per);
-#pragma unroll
-        for (int i = 0; i < 3; i++) w[r + i] |= (c >> i & 0x00010001u) << 15;
-    } else {
-        w[t / per] |= c << (t % per * BITS);
-    }
 }
 
 // Piece `piece` of a lane's words: its codes, and its values code * scale + zero, each rounded once, to fp16.

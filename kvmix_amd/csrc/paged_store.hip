@@ -20,7 +20,8 @@ struct PagePairs {
 // append: the new tokens of one block of a page and one head per wave (the plan lists such blocks).  Keys are copied as they
 // come; values go through the LDS, turned round: eight tokens that follow one another in a page are one piece of sixteen bytes
 // (token by token, two bytes at a time, 83 instead of 62 us for 8 x 1021 tokens of 32 heads).  A single token's values touch D
-// rows of 64 bytes: sixteen times the lines that it has to, for a store that is read at every step after it.
+// rows of 64 bytes: sixteen times the lines that it has to, for a store that is read at every step after it.  8 x 1021 tokens:
+// 62 us for 268 MB moved, 4.3 TB/s (a large copy 4.75); 64 x 1 of 8 heads 4.8 us, a launch.
 
 struct AppendArgs {
     const _Float16 *k, *v;
@@ -268,7 +269,8 @@ __global__ void __launch_bounds__(256) paged_quantize(QuantizeArgs a, PagePairs 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// read: the values of pages, token by token: [pages, P, heads, D].  A block of one head per wave pair, keys and values.
+// read: the values of pages, token by token: [pages, P, heads, D].  A block of one head per wave pair, keys and values.  Bound by its
+// writes: 120 pages of 32 heads, 3/2 bits, 25 us (126 MB written, 28 read: 6.1 TB/s); four pages of 8 heads 3.8, a launch.
 
 struct ReadArgs {
     const void *pool;
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(256) paged_read(ReadArgs a, PagePairs ids)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// copy: pages of up to kCopyPools pools, the same pairs in all of them, 16 KiB to a block.
+// copy: pages of up to kCopyPools pools, the same pairs in all of them, 16 KiB to a block: four loads of sixteen bytes in flight per
+// thread, then their stores.  2.9 GB moved in 701 pages of 32 pools 579 us, 5.1 TB/s; 134 MB in 32 us with its launch.
 
 constexpr int kCopyPieces = 4;  // of 16 bytes per thread
 constexpr uint32_t kCopyBytes = 256 * 16 * kCopyPieces;

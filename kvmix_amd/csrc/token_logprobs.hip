@@ -13,6 +13,9 @@
 // a lower bound of the row's k-th largest value that few others reach (25 values for k = 20).  It is found by bisection over
 // the lanes, by its upper sixteen bits; what reaches it is collected and put in order by counting.  Equal logits come in the
 // order of their indexes.  Rows in which too many reach it (constant ones), or with NaN, are searched value by value.
+//
+// 8192 rows of 32000 halves with the top 20: 104 us, 5.0 TB/s (a pure read 6.2); one row with the top 5: 6.5 us, a launch of one
+// chain of latencies; 4099 rows with both gradients 161 us (787 MB, 4.9 TB/s; a large copy 4.75).
 #include <type_traits>
 
 #include "kvmix_common.h"
