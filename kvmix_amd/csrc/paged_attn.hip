@@ -696,39 +696,46 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
 }
 
-// The spans of one sequence's rows together: a row per wave, or per block where there are many spans; the item's `begin` is the
-// number of spans, `end` the rows between them.  Bound by latency, 3 to 5 us: spans are read eight at a time.
+// The spans of one sequence's rows together; the item's `begin` is the number of spans, `end` the rows between them.  A row's D sums
+// are four to a lane; a row is a group of lanes, or where there are many spans all groups of the block, each for every GROUPS-th of
+// them.  Eight spans' sums and maxima are asked for at once, the maximum runs along: one wait on memory, which is what bounds it
+// (3 us for a few rows; the spans of 19392 rows, 55 MB, JOIN_US us).
+constexpr int kJoinAhead = 8;
+
 template <int D>
 __global__ void __launch_bounds__(256) paged_join(PagedArgs a)
 {
-    constexpr int PER = D / kWave, kAhead = 8, kShared = 8;
-    typedef float floats __attribute__((ext_vector_type(PER)));
-    __shared__ floats sums[4][kWave];
-    __shared__ float totals[4];
-    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+    __shared__ floatx4 sums[GROUPS][LANES];
+    __shared__ float2 stats[GROUPS];
+    const int group = threadIdx.x / LANES, c = threadIdx.x % LANES;
     const int head = blockIdx.x % a.kv_heads;
     const PagedItem it = item_of(a.items, blockIdx.x / a.kv_heads);
     const int spans = it.begin;
-    const bool shared = spans > kShared;
-    const int step = shared ? 4 : 1, mine = shared ? wave : 0;
-    for (int r = shared ? blockIdx.y : blockIdx.y * 4 + wave; r < it.rows; r += gridDim.y * (shared ? 1 : 4)) {
+    const bool shared = spans > kJoinAhead;
+    const int step = shared ? GROUPS : 1, first_span = shared ? group : 0, rows = shared ? 1 : GROUPS;
+    for (int r0 = blockIdx.y * rows; r0 < it.rows; r0 += gridDim.y * rows) {
+        const int r = shared ? r0 : min(r0 + group, it.rows - 1);
         const int64_t first = head * a.part_rows + it.part + r;
-        float most = -1e30f;
-        for (int i = lane; i < spans; i += kWave) most = fmaxf(most, a.part_ml[first + (int64_t)i * it.end].x);
-        most = wave_reduce<true>(most);
-        float total = 0.0f;
-        floats o = {};
-        for (int i0 = mine; i0 < spans; i0 += step * kAhead) {
-            float2 ml[kAhead];
-            floats x[kAhead];
+        float top = -1e30f, total = 0.0f;
+        floatx4 o = {};
+        for (int i0 = first_span; i0 < spans; i0 += step * kJoinAhead) {
+            float2 ml[kJoinAhead];
+            floatx4 x[kJoinAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) {
+            for (int i = 0; i < kJoinAhead; i++) {
                 const int64_t at = first + (int64_t)min(i0 + i * step, spans - 1) * it.end;
                 ml[i] = a.part_ml[at];
-                x[i] = *(const floats *)(a.part + at * D + PER * lane);
+                x[i] = *(const floatx4 *)(a.part + at * D + 4 * c);
             }
+            float most = top;
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) {
+            for (int i = 0; i < kJoinAhead; i++) most = fmaxf(most, ml[i].x);  // (past the end: the last one's again)
+            const float shrink = __builtin_amdgcn_exp2f(top - most);
+            top = most, total *= shrink, o *= shrink;
+#pragma unroll
+            for (int i = 0; i < kJoinAhead; i++) {
                 if (i0 + i * step < spans) {
                     const float w = __builtin_amdgcn_exp2f(ml[i].x - most);
                     total = fmaf(ml[i].y, w, total);
@@ -737,19 +744,28 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a)
             }
         }
         if (shared) {
-            sums[wave][lane] = o;
-            if (lane == 0) totals[wave] = total;
+            sums[group][c] = o;
+            if (c == 0) stats[group] = make_float2(top, total);
             __syncthreads();
-            o = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
-            total = totals[0] + totals[1] + totals[2] + totals[3];
+            float most = -1e30f;
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++) most = fmaxf(most, stats[i].x);
+            o = floatx4{}, total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++) {
+                const float w = __builtin_amdgcn_exp2f(stats[i].x - most);
+                total = fmaf(stats[i].y, w, total);
+                o += sums[i][c] * w;
+            }
             __syncthreads();
-            if (wave) continue;
         }
+        if (shared ? group != 0 : r0 + group >= it.rows) continue;
         const float inv = 1.0f / total;
         const int row = it.row0 + r;
-        _Float16 *to = a.out + (int64_t)(it.q_start + row / a.group) * a.o_ts + (int64_t)(head * a.group + row % a.group) * a.o_hs + PER * lane;
+        half4v w;
 #pragma unroll
-        for (int j = 0; j < PER; j++) to[j] = (_Float16)(o[j] * inv);
+        for (int j = 0; j < 4; j++) w[j] = (_Float16)(o[j] * inv);
+        *(half4v *)(a.out + (int64_t)(it.q_start + row / a.group) * a.o_ts + (int64_t)(head * a.group + row % a.group) * a.o_hs + 4 * c) = w;
     }
 }
 
@@ -895,6 +911,8 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         const int64_t spans = (int64_t)(list.size() - first);
         if (spans < 2) return;
         const Span &one = list[first];
+        const int64_t at_once = spans > kJoinAhead ? 1 : 1024 / b->head_dim;  // rows of a block of paged_join
+        plan->join_blocks = std::max<int64_t>(plan->join_blocks, (one.word[2] + at_once - 1) / at_once);
         joins.push_back({{one.word[0], one.word[1], one.word[2], (int32_t)spans, one.word[2], (int32_t)part}, 0});
         for (int64_t i = 0; i < spans; i++, part += one.word[2]) list[first + i].word[5] = (int32_t)part;
     };
@@ -1048,8 +1066,7 @@ extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_pa
         });
         if (plan->joins) {
             a.items = list + plan->join_at;
-            const unsigned rows = plan->tiles ? kTileRows / 4 : (unsigned)plan->few_rows / 4;
-            paged_join<D.value><<<dim3((unsigned)(plan->joins * plan->kv_heads), rows), 256, 0, st>>>(a);
+            paged_join<D.value><<<dim3((unsigned)(plan->joins * plan->kv_heads), (unsigned)plan->join_blocks), 256, 0, st>>>(a);
         }
     });
     return launch_status();
