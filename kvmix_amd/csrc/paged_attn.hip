@@ -8,6 +8,7 @@
 // and paged_join puts the spans together.  Who takes what is decided on the host, once for all layers of a step
 // (kvmix_paged_plan): lengths that differ within a batch then cost no idle blocks.
 #include <algorithm>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // The spans of one sequence's rows together; the item's `begin` is the number of spans, `end` the rows between them.  A row's D sums
 // are four to a lane; a row is a group of lanes, or where there are many spans all groups of the block, each for every GROUPS-th of
 // them.  Eight spans' sums and maxima are asked for at once, the maximum runs along: one wait on memory, which is what bounds it
-// (3 us for a few rows; the spans of 19392 rows, 55 MB, JOIN_US us).
+// (3 us for a few rows; the spans of 19392 rows, 55 MB, 9 us).
 constexpr int kJoinAhead = 8;
 
 template <int D>
@@ -829,20 +830,34 @@ struct Deal {
 
 // Tiles that a block of paged_tile takes at most, from the lengths of the 128-row problems of one kv head.  Spans such that all
 // blocks are resident in one round (two, three, four), or problems left whole and dealt as blocks end; whichever is estimated to
-// end first.
-int64_t tile_span(const std::vector<int64_t> &lengths, int64_t kv_heads)
+// end first, in units of a tile's time in a block that shares its CU with another (1.8 us; alone 1.35).  What is cut costs the
+// spans' sums, written and read again.  (Without that, and with one speed, two chunks of 1000 tokens over 16000 and 10667, 32 heads over 8:
+// 256 spans and 546 us instead of 64 and 500.)
+constexpr double kTileAlone = 0.75, kJoinTiles = 1.5, kSpanTiles = 0.006;
+
+int64_t tile_span(std::vector<int64_t> lengths, int64_t kv_heads)
 {
-    int64_t total = 0, longest = 0;
-    for (int64_t n : lengths) total += n, longest = std::max(longest, n);
+    std::sort(lengths.begin(), lengths.end(), std::greater<int64_t>());
+    int64_t total = 0;
+    const int64_t longest = lengths[0], cus = kTileResident / 2;
+    for (int64_t n : lengths) total += n;
     const auto blocks = [&](int64_t span) {
         int64_t n = 0;
         for (int64_t l : lengths) n += (l + span - 1) / span;
         return n * kv_heads;
     };
+    const auto joins = [&](int64_t span) {
+        int64_t n = 0;
+        for (int64_t l : lengths) n += l > span ? (l + span - 1) / span : 0;
+        return n ? kJoinTiles + kSpanTiles * (double)(n * kv_heads) : 0.0;
+    };
     const int64_t whole = blocks(longest);
     int64_t best = longest;
     double least = (double)total * kv_heads / kTileResident + longest / 2.0 + kTileStart * (double)((whole + kTileResident - 1) / kTileResident);
-    if (whole <= kTileResident) least = longest + kTileStart;
+    if (whole <= kTileResident) {  // (the longest with the longest of those that are dealt in the second turn, then alone)
+        const int64_t beside = whole > cus ? lengths[cus / kv_heads] : 0;
+        least = longest * kTileAlone + beside * (1.0 - kTileAlone) + kTileStart;
+    }
     for (int64_t rounds = 1; rounds <= 4; rounds++) {
         int64_t low = 1, high = longest;  // the shortest spans whose blocks fit
         while (low < high) {
@@ -851,7 +866,7 @@ int64_t tile_span(const std::vector<int64_t> &lengths, int64_t kv_heads)
             else low = mid + 1;
         }
         if (blocks(low) > rounds * kTileResident) continue;
-        const double time = (double)rounds * (low + kTileStart);
+        const double time = (double)rounds * (low + kTileStart) + joins(low);
         if (time < least) least = time, best = low;
     }
     return best;
