@@ -100,9 +100,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
     constexpr bool kScaleQueries = NR == 1;
     constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB + NR > 4 ? 3 : 4;  // blocks in flight: what the registers hold
-    // whether keys' channels, and values' tokens, are taken in the order in which two-bit codes come cheapest (a lane then has
-    // whole pieces of scales and minima, D = 128)
-    constexpr bool kTurnK = KB == 2 && D == 128, kTurnV = VB == 2 && D == 128;
+    // whether keys' channels, and values' tokens, are taken in the order in which two- and four-bit codes come cheapest (a lane then
+    // has whole pieces of scales and minima, D = 128)
+    constexpr bool kTurnK = KB % 2 == 0 && D == 128, kTurnV = VB % 2 == 0 && D == 128;
     constexpr int kPad = D + 4;
     __shared__ union {
         uint32_t side[4][2 * D];
@@ -199,11 +199,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         };
 
         auto key_codes = [&](const PackedBlock<D, KB, VB> &b, int piece) {
-            if constexpr (kTurnK) return piece_codes_turned(b.k, piece);
+            if constexpr (kTurnK) return piece_codes_turned<KB>(b.k, piece);
             else return piece_codes<KB, NK>(b.k, piece, ke);
         };
         auto value_codes = [&](const PackedBlock<D, KB, VB> &b, int piece) {
-            if constexpr (kTurnV) return piece_codes_turned(b.v, piece);
+            if constexpr (kTurnV) return piece_codes_turned<VB>(b.v, piece);
             else return piece_codes<VB, NV>(b.v, piece, ve);
         };
         auto take_packed = [&](const PackedBlock<D, KB, VB> &b) {
