@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
     constexpr bool kScaleQueries = NR == 1;
-    constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB + NR > 4 ? 3 : 4;  // blocks in flight: what the registers hold
+    constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB + NR > 4 ? 3 : 4;  // blocks in flight: what the registers hold (4/4 bits, 16 x 8192 tokens: 96 us, with three 99)
     // whether keys' channels, and values' tokens, are taken in the order in which two- and four-bit codes come cheapest (a lane then
     // has whole pieces of scales and minima, D = 128)
     constexpr bool kTurnK = KB % 2 == 0 && D == 128, kTurnV = VB % 2 == 0 && D == 128;
