@@ -87,10 +87,10 @@ __device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uin
 // and its probabilities are the operand of out^T = v^T p^T as they are.  Codes go from memory to registers, DEPTH blocks ahead, become
 // fp16 there and are used once.
 //
-// q.k = sum_d (q_d s_d) c_d + q_d z_d with a channel's scale s and minimum z: for sixteen rows the scales go to the queries (a
-// product per block and channel, not per code), in two halves, so that the logits of packed keys are exact but for the sums (with
-// one half the error of the whole against 64 bits was 1.2 to 1.5e-3, with two 2.7 to 3.2e-4; a result's own rounding is 2.1e-4.
-// It costs 5 us of 70).  For 32 rows that would be two products each, so there keys become fp16 first.
+// q.k = sum_d (q_d s_d) c_d + q_d z_d with a channel's scale s and minimum z: the scales go to the queries (a product per block,
+// row and channel, not per code), in two halves, so that the logits of packed keys are exact but for the sums (with
+// one half the error of the whole against 64 bits was 1.2 to 1.5e-3, with keys rounded to fp16 4e-4, with two 2.7 to 3.2e-4; a result's
+// own rounding is 2.1e-4.  For sixteen rows it costs 5 us of 70, for 32 rows, 16 x 16384 tokens of 8 heads, 12 of 67).
 //
 // Bound by vector instructions and memory together: 16 x 8192 tokens of 32 heads, 2/2 bits, 66 us (314 MB, 4.8 TB/s; one byte of
 // codes is eight values to convert), 4/4 bits 92 us (490 MB, 5.3 TB/s), 3/2 bits of 8 heads over 32768 tokens 73 us (4.5 TB/s).
@@ -98,7 +98,6 @@ template <int D, int KB, int VB, int NR>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 3 : 2))) paged_few(PagedArgs a)
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
-    constexpr bool kScaleQueries = NR == 1;
     constexpr int DEPTH = KB + VB > 5 ? 2 : KB + VB + NR > 4 ? 3 : 4;  // blocks in flight: what the registers hold (4/4 bits, 16 x 8192 tokens: 96 us, with three 99)
     // whether keys' channels, and values' tokens, are taken in the order in which two- and four-bit codes come cheapest (a lane then
     // has whole pieces of scales and minima, D = 128)
@@ -126,7 +125,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 
         half8v q[NR][KS];
         int limit[NR];  // the row's own token
-        float scale = a.scale;
+        float scale[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const int r = it.row0 + min(16 * n + m, it.rows - 1), token = r / a.group;
@@ -138,20 +137,21 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 if constexpr (kTurnK) q[n][s] = turned(q[n][s]);
             }
         }
-        if constexpr (kScaleQueries) {
-            // A row's queries times the power of two that puts the largest into [0.5, 1): their products with the keys' scales are
-            // then finite whatever both are, and small queries keep their bits.
-            half8v most = q[0][0] < (_Float16)0.0f ? -q[0][0] : q[0][0];
+        // A row's queries times the power of two that puts the largest into [0.5, 1): their products with the keys' scales are then
+        // finite whatever both are, and small queries keep their bits.
 #pragma unroll
-            for (int s = 1; s < KS; s++) most = __builtin_elementwise_max(most, q[0][s] < (_Float16)0.0f ? -q[0][s] : q[0][s]);
+        for (int n = 0; n < NR; n++) {
+            half8v most = q[n][0] < (_Float16)0.0f ? -q[n][0] : q[n][0];
+#pragma unroll
+            for (int s = 1; s < KS; s++) most = __builtin_elementwise_max(most, q[n][s] < (_Float16)0.0f ? -q[n][s] : q[n][s]);
             float largest = (float)most[0];
 #pragma unroll
             for (int j = 1; j < 8; j++) largest = fmaxf(largest, (float)most[j]);
             const int e = min(max((int)(__float_as_uint(max_of_rows(largest)) >> 23) - 126, -24), 16);
             const _Float16 once = (_Float16)__builtin_ldexpf(1.0f, -e / 2), twice = (_Float16)__builtin_ldexpf(1.0f, -e - -e / 2);
 #pragma unroll
-            for (int s = 0; s < KS; s++) q[0][s] = q[0][s] * once * twice;
-            scale = __builtin_ldexpf(scale, e);
+            for (int s = 0; s < KS; s++) q[n][s] = q[n][s] * once * twice;
+            scale[n] = __builtin_ldexpf(a.scale, e);
         }
         const int first_limit = kv_len - q_len + it.row0 / a.group;
 
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 float most = x[0][n][0];
 #pragma unroll
                 for (int i = 1; i < 8; i++) most = fmaxf(most, x[i / 4][n][i % 4]);
-                most *= scale;
+                most *= scale[n];
                 if (__any(most > top[n] + 8.0f)) {
                     const float grown = fmaxf(top[n], max_of_rows(most));
                     const float shrink = __builtin_amdgcn_exp2f(top[n] - grown);
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int t = kTurnV && packed_tokens.value ? i / 2 + i % 2 * 4 : i;  // (the order of the values' tokens)
-                    p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[t / 4][n][t % 4], scale, -top[n]));
+                    p[n][i] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[t / 4][n][t % 4], scale[n], -top[n]));
                     if (i % 2) sum[n] = __builtin_amdgcn_fdot2(half2v{p[n][i - 1], p[n][i]}, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum[n], false);
                 }
             }
@@ -217,37 +217,36 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             }
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
             const _Float16 *sides = (const _Float16 *)side + 8 * g;
-            floatx4 x[2][NR] = {}, low[2] = {};  // (sums of their own: half as long a chain of products)
-            if constexpr (kScaleQueries) {
+            floatx4 x[2][NR] = {}, low[2][NR] = {};  // (sums of their own: half as long a chain of products)
 #pragma unroll
-                for (int s = 0; s < KS; s++) low[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8v *)(sides + D + 32 * s), q[0][s], low[0], 0, 0, 0);
-                low[1] = low[0];
+            for (int s = 0; s < KS; s++) {
+                const half8v zeros = *(const half8v *)(sides + D + 32 * s);
+#pragma unroll
+                for (int n = 0; n < NR; n++) low[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zeros, q[n][s], low[0][n], 0, 0, 0);
             }
+#pragma unroll
+            for (int n = 0; n < NR; n++) low[1][n] = low[0][n];
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 const half8v scales = *(const half8v *)(sides + 32 * s);
-                if constexpr (kScaleQueries) {
-                    // in two halves, the product and what it rounds off: the logits are then exact but for the sums
-                    const half8v scaled = q[0][s] * scales, rest = __builtin_elementwise_fma(q[0][s], scales, -scaled);
+                // in two halves, the product and what it rounds off: the logits are then exact but for the sums
+                half8v scaled[NR], rest[NR];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const half8v codes = key_codes(b, u * KS + s);
-                        low[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, rest, low[u], 0, 0, 0);
-                        x[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, scaled, x[u][0], 0, 0, 0);
-                    }
-                } else {
-                    const half8v zeros = *(const half8v *)(sides + D + 32 * s);
+                for (int n = 0; n < NR; n++) scaled[n] = q[n][s] * scales, rest[n] = __builtin_elementwise_fma(q[n][s], scales, -scaled[n]);
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const half8v k = __builtin_elementwise_fma(key_codes(b, u * KS + s), scales, zeros);
+                for (int u = 0; u < 2; u++) {
+                    const half8v codes = key_codes(b, u * KS + s);
 #pragma unroll
-                        for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
+                    for (int n = 0; n < NR; n++) {
+                        low[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, rest[n], low[u][n], 0, 0, 0);
+                        x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, scaled[n], x[u][n], 0, 0, 0);
                     }
                 }
             }
-            if constexpr (kScaleQueries) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) x[u][0] += low[u];
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int n = 0; n < NR; n++) x[u][n] += low[u][n];
             }
             half8v p[NR];
             probabilities(x, p, 0, std::true_type());
