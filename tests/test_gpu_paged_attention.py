@@ -235,7 +235,7 @@ def test_refusals(dev):
 
 
 def test_layout_helpers_agree_with_the_rows(dev):
-    """The checker's own reading of a packed page is the fp16 page that it was made of, to within half a step."""
+    """The plain reading of a packed page is the fp16 page that it was made of, to within half a step."""
     from kvmix_amd import ops
 
     g = torch.Generator().manual_seed(1)
