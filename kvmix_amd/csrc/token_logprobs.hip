@@ -19,12 +19,12 @@
 #include <type_traits>
 
 #include "kvmix_common.h"
+#include "score_plan.h"
 
 namespace kvmix {
 
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-constexpr int kPieces = 16;        // of sixteen bytes that a thread holds
 constexpr float kStale = 20.0f;    // how far a value may exceed what sums are relative to: 2^d stays below 2^29
 constexpr int kTopMost = 64, kCandidates = 1024;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -404,28 +404,6 @@ __global__ void __launch_bounds__(256) score_grad(ScoreArgs a)
 }
 
 namespace {
-
-constexpr int64_t kGradChunk = 8192;
-
-// Threads to a row, and chunks of it.  Blocks of 256 threads, of which several share a CU, where there are rows enough for all CUs
-// and they fit; else of 1024: a row's latency is what counts, or its length.
-struct ScorePlan {
-    int threads;
-    int64_t chunks, chunk;
-};
-
-constexpr int64_t kManyRows = 512;
-
-ScorePlan score_plan(int64_t rows, int64_t vocab, int dtype)
-{
-    const int64_t per = dtype == KVMIX_F32 ? 4 : 8;
-    const int threads = rows >= kManyRows && vocab <= (256 * kPieces - 1) * per ? 256 : 1024;
-    const int64_t most = (threads * kPieces - 1) * per;  // (a piece for a row that is not aligned)
-    const int64_t chunks = (vocab + most - 1) / most;
-    return {threads, chunks, chunks > 1 ? ((vocab + chunks - 1) / chunks + 7) / 8 * 8 : vocab};
-}
-
-int64_t chunk_of(int64_t vocab, int64_t chunks) { return ((vocab + chunks - 1) / chunks + 7) / 8 * 8; }
 
 int score_check(const kvmix_token_logprobs_t *p)
 {
