@@ -2,9 +2,25 @@
 import pytest
 import torch
 
-from test_gpu_token_logprobs import logits
+from test_gpu_token_logprobs import KINDS, check, logits
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab", [65528, 65529, 65532, 65533, 131053, 131057, 131061, 131063, 131064, 131065, 196585, 196595, 262113])
+def test_ends_of_chunks(dev, kind, vocab):
+    """Vocabularies of nearly as many values as whole blocks hold: the largest logit and the target among the last values that
+    a block takes, in rows of every alignment."""
+    x, t = logits(dev, 5, vocab, kind, seed=vocab)
+    for at in (65533, 65534, 65535, 131071, vocab - 1):
+        if at < vocab:
+            y = x.clone()
+            y[:, at] = 30.0
+            check(y, torch.full_like(t, at), 3)
+    wide = torch.zeros(3, vocab + 4, dtype=kind, device=dev)
+    wide[:, 1:1 + vocab] = x[:3]
+    check(wide[:, 1:1 + vocab], t[:3], 20)
 
 
 @pytest.mark.parametrize("vocab", [131061, 196595])
@@ -21,3 +37,16 @@ def test_gradient_at_ends_of_chunks(dev, vocab):
     want.scatter_add_(1, t[:, None], torch.ones(3, 1, device=dev, dtype=torch.float64))
     # (a probability is good to 2^-17, one minus it to that of one)
     assert ((x.grad.double() - want).abs() <= 2.0 ** -15).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(5, 3001), (600, 3001), (5, 40007), (5, 196585), (5, 262144)])
+def test_one_token_takes_nearly_all(dev, kind, rows, vocab):
+    """Entropies near zero, with the largest logit anywhere in the row."""
+    x, t = logits(dev, rows, vocab, kind, seed=vocab)
+    for at in (0, 1500, 65533, 65534, 131071, vocab - 1):
+        if at < vocab:
+            for size in (17.0, 30.0):
+                y = x.clone()
+                y[:, at] = size
+                check(y, torch.full_like(t, at), 3)
