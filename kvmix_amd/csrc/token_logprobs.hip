@@ -26,6 +26,7 @@ namespace kvmix {
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr float kStale = 20.0f;    // how far a value may exceed what sums are relative to: 2^d stays below 2^29
+constexpr float kFar = 16777216.0f;  // up to there the rounding of m log2(e) is 1 at most (at 1e10 it is 512 and more, and 2^512 no number)
 constexpr int kTopMost = 64, kCandidates = 1024;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
 
     // The sums as the pieces arrive, relative to a value of the wave's that is moved when another exceeds it by kStale.  One
     // operation for x log2(e) - m log2(e); the rounding of the latter, the same in every term, leaves the sums at the end.  Two
-    // where that product would overflow.
+    // beyond kFar.
     float largest = -__builtin_inff(), m2 = 0.0f;
     ScoreStats t = {-__builtin_inff(), 0.0f, 0.0f};
     bool far = false;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
             if (__any(most > t.m + kStale)) {  // (also what leaves -inf)
                 const float m = wave_reduce<true>(largest);
                 const bool was = far;
-                far = !std::is_same<T, _Float16>::value && __builtin_amdgcn_readfirstlane(!(fabsf(m) < 1e37f));
+                far = !std::is_same<T, _Float16>::value && __builtin_amdgcn_readfirstlane(!(fabsf(m) < kFar));
                 const float d = fmaxf(far || was || t.m == -__builtin_inff() ? (t.m - m) * kLog2e : m2 - m * kLog2e, -1e30f);
                 const float f = __builtin_amdgcn_exp2f(d);
                 t.u = fmaf(t.s, d, t.u) * f, t.s *= f, t.m = m, m2 = m * kLog2e;

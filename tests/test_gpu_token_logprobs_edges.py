@@ -50,3 +50,15 @@ def test_one_token_takes_nearly_all(dev, kind, rows, vocab):
                 y = x.clone()
                 y[:, at] = size
                 check(y, torch.full_like(t, at), 3)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [4, 600])
+@pytest.mark.parametrize("size", [1e4, 1e7, 3e8, 1e10, 1e20, 1e36])
+def test_logits_of_any_size(dev, kind, rows, size):
+    x, t = logits(dev, rows, 5001, kind, seed=50)
+    check((x.float() * size).to(kind), t, 4)
+    x = torch.full((rows, 3000), size, dtype=kind, device=dev)  # all alike but for a few
+    x[:, ::7] = 0.0
+    x[:, 1::7] = -size
+    check(x, t % 3000, 4)
