@@ -27,6 +27,7 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr float kStale = 20.0f;    // how far a value may exceed what sums are relative to: 2^d stays below 2^29
 constexpr float kFar = 16777216.0f;  // up to there the rounding of m log2(e) is 1 at most (at 1e10 it is 512 and more, and 2^512 no number)
+constexpr float kNothing = -1024.0f;  // 2^d is zero from here on, and its products with sums and gradients of any size are finite
 constexpr int kTopMost = 64, kCandidates = 1024;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -127,7 +128,7 @@ __device__ __forceinline__ ScoreStats merged(ScoreStats a, ScoreStats b)
 {
     // (references of -inf: nothing summed yet; the difference is kept finite, so that nothing times it is nothing)
     const float m = fmaxf(a.m, b.m);
-    const float da = fmaxf((a.m - m) * kLog2e, -1e30f), db = fmaxf((b.m - m) * kLog2e, -1e30f);
+    const float da = fmaxf((a.m - m) * kLog2e, kNothing), db = fmaxf((b.m - m) * kLog2e, kNothing);
     const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
     return {m, a.s * fa + b.s * fb, (a.u + a.s * da) * fa + (b.u + b.s * db) * fb};
 }
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
         for (int j = 0; j < PER; j++) {
             const float d = difference(to_float(w.t[j])), e = __builtin_amdgcn_exp2f(d);
             t.s += e;
-            t.u = fmaf(e, fmaxf(d, -1e30f), t.u);  // (zero times -inf is to be zero)
+            t.u = fmaf(e, fmaxf(d, kNothing), t.u);  // (zero times -inf is to be zero)
         }
     };
 #pragma unroll
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
                 const float m = wave_reduce<true>(largest);
                 const bool was = far;
                 far = !std::is_same<T, _Float16>::value && __builtin_amdgcn_readfirstlane(!(fabsf(m) < kFar));
-                const float d = fmaxf(far || was || t.m == -__builtin_inff() ? (t.m - m) * kLog2e : m2 - m * kLog2e, -1e30f);
+                const float d = fmaxf(far || was || t.m == -__builtin_inff() ? (t.m - m) * kLog2e : m2 - m * kLog2e, kNothing);
                 const float f = __builtin_amdgcn_exp2f(d);
                 t.u = fmaf(t.s, d, t.u) * f, t.s *= f, t.m = m, m2 = m * kLog2e;
             }
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(NT) score_rows(ScoreArgs a)
     // which one takes nearly all came out as 1.06e-5 for 2.6e-6.)
     const float m = wave_reduce<true>(largest);
     if (m != -__builtin_inff()) {
-        const float d = far ? fmaxf((t.m - m) * kLog2e, -1e30f) : fmaf(-m, kLog2e, m2), f = __builtin_amdgcn_exp2f(d);
+        const float d = far ? fmaxf((t.m - m) * kLog2e, kNothing) : fmaf(-m, kLog2e, m2), f = __builtin_amdgcn_exp2f(d);
         t.u = fmaf(t.s, d, t.u) * f, t.s *= f, t.m = m;
     }
     t.s = wave_reduce<false>(t.s), t.u = wave_reduce<false>(t.u);
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(256) score_grad(ScoreArgs a)
         float g[PER];
 #pragma unroll
         for (int j = 0; j < PER; j++) {
-            const float q = fmaxf(fmaf(to_float(w.t[j]) - m, kLog2e, -sum2), -1e30f);
+            const float q = fmaxf(fmaf(to_float(w.t[j]) - m, kLog2e, -sum2), kNothing);
             g[j] = -__builtin_amdgcn_exp2f(q) * (ga + gb * (q * kLn2 + entropy));
         }
         if (hit >= i && hit < i + PER) {

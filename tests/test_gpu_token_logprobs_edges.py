@@ -62,3 +62,32 @@ def test_logits_of_any_size(dev, kind, rows, size):
     x[:, ::7] = 0.0
     x[:, 1::7] = -size
     check(x, t % 3000, 4)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,most", [(2, 15000, 15.0), (600, 15000, 15.0), (2, 60000, 19.5)])
+def test_a_huge_logit_behind_many_ordinary_ones(dev, kind, rows, vocab, most):
+    """Ordinary logits that sum up to much, and then one beside which they are nothing."""
+    x = torch.zeros(rows, vocab, dtype=kind, device=dev)
+    x[:, 4096:] = most
+    for at in (vocab - 1, vocab - 1000, 5000):
+        for size in (1e30, 1e37, 3e38):
+            y = x.clone()
+            y[:, at] = size
+            check(y, torch.full((rows,), at, device=dev), 2)
+            check(y, torch.full((rows,), 7, device=dev), 0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_large_gradients_of_masked_tokens(dev, kind):
+    """Gradients of the entropy that are large: a token without probability gets exactly zero."""
+    from kvmix_amd import ops
+
+    x, t = logits(dev, 3, 5000, kind, seed=40)
+    dead = torch.rand(3, 5000, device=dev) < 0.5
+    dead.scatter_(1, t[:, None], False)
+    x = x.masked_fill(dead, float("-inf")).requires_grad_()
+    lp, H = ops.token_logprobs(x, t)
+    for size in (1.0, 1e9, 1e30):
+        (got,) = torch.autograd.grad((lp, H), x, (torch.full_like(lp, size), torch.full_like(H, size)), retain_graph=True)
+        assert (got[dead] == 0).all() and not got.isnan().any()
