@@ -16,6 +16,7 @@
 //
 // 8192 rows of 32000 halves with the top 20: 104 us, 5.0 TB/s (a pure read 6.2); one row with the top 5: 6.5 us, a launch of one
 // chain of latencies; 4099 rows with both gradients 161 us (787 MB, 4.9 TB/s; a large copy 4.75).
+#include <algorithm>
 #include <type_traits>
 
 #include "kvmix_common.h"
@@ -421,6 +422,30 @@ int score_check(const kvmix_token_logprobs_t *p)
     return KVMIX_OK;
 }
 
+// f(first, rows) for launches of fewer than 2^32 threads together
+template <typename F>
+void launches_of(int64_t rows, int64_t threads_per_row, F f)
+{
+    const int64_t most = 0xffffffffll / threads_per_row;
+    for (int64_t first = 0; first < rows; first += most) f(first, (unsigned)std::min(most, rows - first));
+}
+
+// The rows from `first` on.
+template <typename T>
+ScoreArgs rows_from(ScoreArgs a, int64_t first)
+{
+    a.x = (const T *)a.x + first * a.row_stride;
+    a.targets += first;
+    if (a.logprob) a.logprob += first, a.entropy += first;
+    if (a.top) a.top_logprob += first * a.top, a.top_id += first * a.top;
+    if (a.stats) a.stats += 4 * first;
+    if (a.chunks > 1) a.part += first * a.chunks, a.part_keys += first * a.chunks * a.top;
+    if (a.grad_logprob) a.grad_logprob += first;
+    if (a.grad_entropy) a.grad_entropy += first;
+    if (a.dx) a.dx = (T *)a.dx + first * a.dx_stride;
+    return a;
+}
+
 template <typename F>
 void with_type(int dtype, F f)
 {
@@ -460,18 +485,21 @@ extern "C" int kvmix_token_logprobs(const kvmix_token_logprobs_t *p, void *works
     hipStream_t st = (hipStream_t)stream;
     with_type(p->dtype, [&](auto zero) {
         using T = decltype(zero);
-        const unsigned grid = (unsigned)(p->rows * a.chunks);
-        if (plan.threads == 256) {
-            if (p->top) score_rows<T, 256, true><<<grid, 256, 0, st>>>(a);
-            else score_rows<T, 256, false><<<grid, 256, 0, st>>>(a);
-        } else {
-            if (p->top) score_rows<T, 1024, true><<<grid, 1024, 0, st>>>(a);
-            else score_rows<T, 1024, false><<<grid, 1024, 0, st>>>(a);
-        }
-        if (a.chunks > 1) {
-            if (p->top) score_join<T, true><<<(unsigned)p->rows, 256, 0, st>>>(a);
-            else score_join<T, false><<<(unsigned)p->rows, 256, 0, st>>>(a);
-        }
+        launches_of(p->rows, plan.threads * a.chunks, [&](int64_t first, unsigned rows) {
+            const ScoreArgs part = rows_from<T>(a, first);
+            const unsigned grid = rows * (unsigned)a.chunks;
+            if (plan.threads == 256) {
+                if (p->top) score_rows<T, 256, true><<<grid, 256, 0, st>>>(part);
+                else score_rows<T, 256, false><<<grid, 256, 0, st>>>(part);
+            } else {
+                if (p->top) score_rows<T, 1024, true><<<grid, 1024, 0, st>>>(part);
+                else score_rows<T, 1024, false><<<grid, 1024, 0, st>>>(part);
+            }
+            if (a.chunks > 1) {
+                if (p->top) score_join<T, true><<<rows, 256, 0, st>>>(part);
+                else score_join<T, false><<<rows, 256, 0, st>>>(part);
+            }
+        });
     });
     return launch_status();
 }
@@ -490,6 +518,11 @@ extern "C" int kvmix_token_logprobs_grad(const kvmix_token_logprobs_t *p, const 
     a.chunks = (int)((p->vocab + kGradChunk - 1) / kGradChunk);
     a.chunk = (int)chunk_of(p->vocab, a.chunks);
     a.grad_logprob = grad_logprob, a.grad_entropy = grad_entropy, a.dx = grad_logits, a.dx_stride = grad_row_stride;
-    with_type(p->dtype, [&](auto zero) { score_grad<decltype(zero)><<<(unsigned)(p->rows * a.chunks), 256, 0, (hipStream_t)stream>>>(a); });
+    with_type(p->dtype, [&](auto zero) {
+        using T = decltype(zero);
+        launches_of(p->rows, 256 * a.chunks, [&](int64_t first, unsigned rows) {
+            score_grad<T><<<rows * (unsigned)a.chunks, 256, 0, (hipStream_t)stream>>>(rows_from<T>(a, first));
+        });
+    });
     return launch_status();
 }

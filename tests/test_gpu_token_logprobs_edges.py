@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_token_logprobs import KINDS, check, logits
+from test_gpu_token_logprobs import KINDS, best_of, check, close, logits, wanted
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,28 @@ def test_large_gradients_of_masked_tokens(dev, kind):
     for size in (1.0, 1e9, 1e30):
         (got,) = torch.autograd.grad((lp, H), x, (torch.full_like(lp, size), torch.full_like(H, size)), retain_graph=True)
         assert (got[dead] == 0).all() and not got.isnan().any()
+
+
+def test_more_rows_than_a_launch_has_blocks(dev):
+    """2^24 rows and a few: with 256 threads to a row more than a launch's 2^32."""
+    from kvmix_amd import ops
+
+    rows = (1 << 24) + 5
+    x = (torch.arange(rows, device=dev)[:, None] % 11 * torch.tensor([0.5, 1.0, -0.25, 0.125], device=dev)).half().requires_grad_()
+    t = torch.arange(rows, device=dev) % 4
+    lp, H, top_lp, top_id = ops.token_logprobs(x, t, top=2)
+    (got,) = torch.autograd.grad(lp.sum() + H.sum(), x)
+    for part in (slice(0, 44), slice(rows // 2, rows // 2 + 44), slice(rows - 44, rows)):
+        y = x.detach()[part]
+        want, entropy, every = wanted(y, t[part])
+        close(lp[part], want, 0)
+        close(H[part], entropy, entropy.cpu().abs())
+        best = best_of(y, 2)
+        assert torch.equal(top_id[part], best)
+        close(top_lp[part], every.gather(-1, best), 0)
+        p = every.exp()
+        hit = (torch.arange(4, device=dev) == t[part][:, None]).double()
+        grad = hit - p - p * (every + entropy[:, None])
+        # (as test_gradient_against_the_formula)
+        size = p * (2 + every.abs() + entropy.abs()[:, None]) + hit
+        assert ((got[part].double() - grad).abs() <= 2.0 ** -15 * size + 2.0 ** -11 * grad.abs() + 2.0 ** -25).all()
