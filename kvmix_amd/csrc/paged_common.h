@@ -158,6 +158,7 @@ __device__ __forceinline__ half8v piece_values(const uint32_t *w, int piece, hal
 }
 
 constexpr int64_t kMost32 = 0x7fffffff;
+constexpr int64_t kMostBlocks = (1 << 24) - 1;  // of 256 threads: a launch of 2^32 threads or more runs modulo 2^32, without an error
 constexpr int64_t kMostHeads = 4096;
 
 inline bool page_size_ok(int64_t n) { return n >= kBlock && n <= 1024 && (n & (n - 1)) == 0; }

@@ -412,7 +412,7 @@ extern "C" int kvmix_paged_append(const kvmix_paged_pool_t *p, const kvmix_paged
     if (k_token_stride % 8 || k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8 || ((uintptr_t)k | (uintptr_t)v) % 16) return KVMIX_ERR_UNSUPPORTED;
     if (plan->stores == 0) return KVMIX_OK;
     if (!k || !v || !list || !p->rows) return KVMIX_ERR_NULL;
-    if ((__int128)plan->stores * p->kv_heads > kMost32) return KVMIX_ERR_UNSUPPORTED;
+    if ((__int128)plan->stores * p->kv_heads > 4 * kMostBlocks) return KVMIX_ERR_UNSUPPORTED;  // (four units to a block)
     const AppendArgs a = {(const _Float16 *)k, (const _Float16 *)v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, (_Float16 *)p->rows,
                           (PlanWords)list + plan->store_at, (int)p->kv_heads, (int)(plan->stores * p->kv_heads),
                           __builtin_ctzll((uint64_t)p->page_size)};

@@ -1,0 +1,33 @@
+"""Sizes that a launch over pages cannot have: refused when the plan is made.  No GPU."""
+import ctypes
+
+import pytest
+
+from kvmix_amd import _lib
+
+
+def plan_of(sequences, new, heads, page=64):
+    """kvmix_paged_plan of equal sequences of `new` tokens in the same page: (code, plan)"""
+    n = (ctypes.c_int64 * sequences)
+    batch, plan = _lib.PagedBatch(), _lib.PagedPlan()
+    pages, lens, packed = (ctypes.c_int32 * sequences)(), n(*[new] * sequences), n()
+    batch.table, batch.table_stride = ctypes.addressof(pages), 1
+    batch.kv_lens = batch.q_lens = ctypes.addressof(lens)
+    batch.packed_lens = ctypes.addressof(packed)
+    batch.sequences, batch.heads, batch.kv_heads, batch.head_dim, batch.page_size = sequences, heads, heads, 64, page
+    return _lib.load().kvmix_paged_plan(ctypes.byref(batch), None, 0, ctypes.byref(plan)), plan
+
+
+@pytest.mark.parametrize("sequences,ok", [(4095, True), (4096, False), (5000, False)])
+def test_blocks_of_the_attention(sequences, ok):
+    """33 tokens of 4096 heads are 4096 blocks of 256 threads: 2^32 threads or more are more than a launch counts."""
+    code, plan = plan_of(sequences, 33, 4096)
+    assert code == (0 if ok else -9)
+    assert not ok or plan.tiles * plan.kv_heads * 256 < 1 << 32
+
+
+@pytest.mark.parametrize("sequences,ok", [(16380, True), (16384, False), (20000, False)])
+def test_blocks_of_the_store(sequences, ok):
+    """One token of 4096 heads each: four heads to a block of 256 threads."""
+    code, _ = plan_of(sequences, 1, 4096)
+    assert code == (0 if ok else -9)
