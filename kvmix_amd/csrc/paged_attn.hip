@@ -954,7 +954,7 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
     few.close();
     // (what ends a launch is short then)
     std::stable_sort(tiles.begin(), tiles.end(), [](const Span &x, const Span &y) { return x.cost > y.cost; });
-    if (std::max({few.list.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
+    if (few.list.size() > (size_t)kMost32 || std::max({few.starts.size(), tiles.size(), joins.size()}) * (__int128)b->kv_heads > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
     plan->few = (int64_t)few.list.size(), plan->tiles = (int64_t)tiles.size(), plan->joins = (int64_t)joins.size(), plan->part_rows = part;
     plan->few_columns = (int64_t)few.starts.size();
     int64_t at = 0;
