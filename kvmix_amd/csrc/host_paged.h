@@ -7,6 +7,16 @@ struct PagedPlan {
     Tensor slots() const { return list.narrow(0, c.slots_at, c.tokens); }
 };
 
+// Nothing here has a derivative (the likelihoods have one, backwards, which the caller records): a call that should record one, or
+// whose result a trace would keep as a constant, is refused.
+void need_no_record(const char *name, std::initializer_list<const Tensor *> ts)
+{
+    if (torch::jit::tracer::isTracing()) fail(std::string(name) + " cannot be part of a trace");
+    for (const Tensor *t : ts)
+        if ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())
+            fail(std::string(name) + " has no derivative for this tensor: call it under torch.no_grad() or with detached tensors");
+}
+
 // int32 numbers in host memory, [n] or [n, 2]
 Tensor host_list(const Tensor &t, int64_t dim, const char *what)
 {
@@ -67,6 +77,7 @@ PagedPlan paged_plan(const Tensor &table_in, const std::vector<int64_t> &kv_lens
 
 void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &rows, const PagedPlan &plan)
 {
+    need_no_record("paged_append", {&k_in, &v_in, &rows});
     kvmix_paged_pool_t p{};
     use_rows(p, rows);
     need_half({&k_in, &v_in});
@@ -84,6 +95,7 @@ void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &rows, co
 
 void paged_quantize(const Tensor &rows, const Tensor &packed, const Tensor &pairs_in, int64_t k_bits, int64_t v_bits)
 {
+    need_no_record("paged_quantize", {&rows});
     kvmix_paged_pool_t p{};
     use_rows(p, rows);
     use_packed(p, packed, p.kv_heads, p.page_size, p.head_dim, k_bits, v_bits);
@@ -96,6 +108,7 @@ void paged_quantize(const Tensor &rows, const Tensor &packed, const Tensor &pair
 std::tuple<Tensor, Tensor> paged_read(const Tensor &pool, const Tensor &pages_in, const std::optional<int64_t> &k_bits, const std::optional<int64_t> &v_bits,
                                       const std::optional<int64_t> &head_dim)
 {
+    need_no_record("paged_read", {&pool});
     kvmix_paged_pool_t p{};
     const bool packed = k_bits || v_bits;
     if (packed) {
@@ -125,6 +138,7 @@ void paged_copy(const std::vector<Tensor> &pools, const Tensor &pairs_in)
     const int64_t pages = pools[0].dim() ? pools[0].size(0) : 0;
     for (size_t i = 0; i < pools.size(); i++) {
         const Tensor &t = pools[i];
+        need_no_record("paged_copy", {&t});
         need_gpu({&t});
         need_with(pools[0], {&t});
         if (t.dim() < 2 || t.size(0) != pages || !t.is_contiguous()) fail("paged_copy: pools must be contiguous, with the same number of pages");
@@ -137,6 +151,7 @@ void paged_copy(const std::vector<Tensor> &pools, const Tensor &pairs_in)
 Tensor paged_attention(const Tensor &q_in, const Tensor &rows, const Tensor &packed, const PagedPlan &plan, int64_t k_bits, int64_t v_bits,
                        const std::optional<double> &scale)
 {
+    need_no_record("paged_attention", {&q_in, &rows});
     kvmix_paged_pool_t p{};
     use_rows(p, rows);
     use_packed(p, packed, p.kv_heads, p.page_size, p.head_dim, k_bits, v_bits);
@@ -178,6 +193,7 @@ Tensor score_rows2(const Tensor &logits)
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &targets_in, int64_t top, bool want_stats)
 {
+    need_no_record("token_logprobs", {&logits});
     need_gpu({&logits});
     need_with(logits, {&targets_in});
     if (logits.scalar_type() != at::kHalf && logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)

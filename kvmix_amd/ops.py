@@ -541,7 +541,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0):
     """Log probabilities of given tokens: logits [..., vocabulary] fp16, bf16 or fp32, targets [...] int64 -> (log probability
     of each target, entropy of each row) in fp32, and with top > 0 (at most 64) also (the log probabilities of the `top` most
     likely tokens, their indexes) [..., top], equal logits in the order of their indexes.  A negative target is none (log
-    probability 0).  The first two are differentiable in the logits; their gradient is computed in the logits' type."""
+    probability 0).  The first two are differentiable in the logits, backwards and once; their gradient is computed in the logits'
+    type."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLogprobs.apply(logits, targets, top)
     lp, entropy, top_lp, top_id, _ = _host().token_logprobs(logits, targets, top, False)
