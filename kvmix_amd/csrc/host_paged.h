@@ -17,12 +17,23 @@ void need_no_record(const char *name, std::initializer_list<const Tensor *> ts)
             fail(std::string(name) + " has no derivative for this tensor: call it under torch.no_grad() or with detached tensors");
 }
 
-// int32 numbers in host memory, [n] or [n, 2]
+// Page numbers as the library takes them, in 32 bits.  What is beyond them is no page: -1.
+Tensor page_numbers(const Tensor &t)
+{
+    if (c10::elementSize(t.scalar_type()) < 4 || t.scalar_type() == at::kInt) return t.to(at::kInt).contiguous();
+    const Tensor from = t.to(at::kLong).contiguous(), to = at::empty(t.sizes(), at::kInt);
+    const int64_t *x = from.data_ptr<int64_t>();
+    int32_t *y = to.data_ptr<int32_t>();
+    for (int64_t i = 0; i < from.numel(); i++) y[i] = x[i] < 0 || x[i] > 0x7fffffff ? -1 : (int32_t)x[i];
+    return to;
+}
+
+// page numbers in host memory, [n] or [n, 2]
 Tensor host_list(const Tensor &t, int64_t dim, const char *what)
 {
     if (t.is_cuda() || !at::isIntegralType(t.scalar_type(), false) || t.dim() != dim || (dim == 2 && t.size(1) != 2))
         fail(std::string(what) + " must be a tensor of whole numbers in host memory, " + (dim == 2 ? "[n, 2]" : "[n]"));
-    return t.to(at::kInt).contiguous();
+    return page_numbers(t);
 }
 
 void use_rows(kvmix_paged_pool_t &p, const Tensor &rows)
@@ -61,7 +72,7 @@ PagedPlan paged_plan(const Tensor &table_in, const std::vector<int64_t> &kv_lens
     if (table_in.is_cuda() || !at::isIntegralType(table_in.scalar_type(), false) || table_in.dim() != 2)
         fail("paged_plan: the table must be whole numbers in host memory, [sequences, pages]");
     if (!device.is_cuda()) fail("KVmix operators run on the GPU only: got " + device.str());
-    const Tensor table = table_in.to(at::kInt).contiguous();
+    const Tensor table = page_numbers(table_in);
     const int64_t n = table.size(0);
     for (const auto *lens : {&kv_lens, &packed_lens, &q_lens})
         if ((int64_t)lens->size() != n) fail("paged_plan: as many lengths as the table has sequences");

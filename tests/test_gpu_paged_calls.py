@@ -62,3 +62,22 @@ def test_a_function_mode_is_no_derivative(dev):
     with torch.device(dev), torch.autocast("cuda"):
         for a, b in zip(ops.token_logprobs(x, t), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 1, -(1 << 32), 1 << 31, (1 << 63) - 1, -(1 << 63) + 1])
+def test_page_numbers_that_are_none(dev, far):
+    """64-bit numbers beyond 32 bits are no pages, whatever their low bits are."""
+    from kvmix_amd import ops
+
+    rows = torch.zeros(4, 2, 2, 64, 128, dtype=torch.float16, device=dev)
+    packed = torch.zeros(4, 2, 2 * 128 * 10, dtype=torch.int32, device=dev)
+    for pair in ([far, 1], [1, far]):
+        with pytest.raises(RuntimeError, match="page number"):
+            ops.paged_quantize(rows, packed, torch.tensor([[0, 0], pair]), 4, 4)
+        with pytest.raises(RuntimeError, match="page number"):
+            ops.paged_copy([rows], torch.tensor([pair]))
+    with pytest.raises(RuntimeError, match="page number"):
+        ops.paged_read(rows, torch.tensor([0, far]))
+    with pytest.raises(RuntimeError, match="page number"):
+        ops.paged_plan(torch.tensor([[0, far]]), [100], [0], [1], 4, 2, 128, 64, dev)
+    assert ops.paged_plan(torch.tensor([[0, far]]), [64], [0], [1], 4, 2, 128, 64, dev).tokens == 1  # (a cell that no token needs)
