@@ -7,10 +7,14 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/Event.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <memory>
 #include <stdexcept>
 #include <string>
 #include <tuple>

@@ -1,10 +1,33 @@
 // The host side of the paged cache's operators and of the token likelihoods: part of host.cpp, whose helpers it uses.
 
+c10::Stream torch_stream(const at::Device &device) { return c10::impl::VirtualGuardImpl(device.type()).getStream(device); }
+
+bool captures(const at::Device &device)
+{
+    const c10::DeviceGuard guard(device);
+    return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
 struct PagedPlan {
     kvmix_paged_plan_t c{};
     Tensor list;  // the plan's words on the device
+    std::optional<c10::Stream> made_on;
+    std::shared_ptr<c10::Event> made;  // when they are there
 
     Tensor slots() const { return list.narrow(0, c.slots_at, c.tokens); }
+
+    // The words for a call on the current stream.  On another stream than the plan was made on they are waited for, and their memory is
+    // given to nobody else before the call has read it (they are hidden from the caller, who could not see to it).  A
+    // capture begins with the device idle and cannot wait for what lies outside it.
+    const int32_t *words() const
+    {
+        const c10::Stream now = torch_stream(list.device());
+        if (now != *made_on) {
+            if (!captures(list.device())) made->block(now);
+            list.record_stream(now);
+        }
+        return list.data_ptr<int32_t>();
+    }
 };
 
 // Nothing here has a derivative (the likelihoods have one, backwards, which the caller records): a call that should record one, or
@@ -72,6 +95,8 @@ PagedPlan paged_plan(const Tensor &table_in, const std::vector<int64_t> &kv_lens
     if (table_in.is_cuda() || !at::isIntegralType(table_in.scalar_type(), false) || table_in.dim() != 2)
         fail("paged_plan: the table must be whole numbers in host memory, [sequences, pages]");
     if (!device.is_cuda()) fail("KVmix operators run on the GPU only: got " + device.str());
+    // (a replay would copy the list again, from memory that is no longer its own)
+    if (captures(device)) fail("paged_plan: a plan cannot be made while a graph is captured");
     const Tensor table = page_numbers(table_in);
     const int64_t n = table.size(0);
     for (const auto *lens : {&kv_lens, &packed_lens, &q_lens})
@@ -83,6 +108,9 @@ PagedPlan paged_plan(const Tensor &table_in, const std::vector<int64_t> &kv_lens
     check(api.paged_plan(&b, host.data_ptr<int32_t>(), plan.c.words, &plan.c));
     plan.list = at::empty({plan.c.words}, at::TensorOptions(at::kInt).device(device));
     plan.list.copy_(host, true);
+    plan.made_on = torch_stream(device);
+    plan.made = std::make_shared<c10::Event>(device.type());
+    plan.made->record(*plan.made_on);
     return plan;
 }
 
@@ -100,7 +128,7 @@ void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &rows, co
     if (plan.c.row_pages > p.row_pages) check(KVMIX_ERR_PAGE);
     const Tensor k = pieces3(k_in), v = pieces3(v_in);
     const c10::DeviceGuard guard(rows.device());
-    check(api.paged_append(&p, &plan.c, plan.list.data_ptr<int32_t>(), k.data_ptr(), stride_of(k, 0), stride_of(k, 1), v.data_ptr(), stride_of(v, 0),
+    check(api.paged_append(&p, &plan.c, plan.words(), k.data_ptr(), stride_of(k, 0), stride_of(k, 1), v.data_ptr(), stride_of(v, 0),
                            stride_of(v, 1), stream_of(rows)));
 }
 
@@ -179,7 +207,7 @@ Tensor paged_attention(const Tensor &q_in, const Tensor &rows, const Tensor &pac
     kvmix_paged_attn_t c{};
     c.q = q.data_ptr(), c.q_token_stride = stride_of(q, 0), c.q_head_stride = stride_of(q, 1);
     c.out = out.data_ptr(), c.out_token_stride = out.stride(0), c.out_head_stride = out.stride(1);
-    c.list = plan.list.data_ptr<int32_t>();
+    c.list = plan.words();
     c.scale = scale ? (float)*scale : 1.0f / std::sqrt((float)p.head_dim);
     const c10::DeviceGuard guard(rows.device());
     check(api.paged_attention(&p, &plan.c, &c, need ? ws.data_ptr() : nullptr, need, stream_of(rows)));

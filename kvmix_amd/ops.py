@@ -476,7 +476,9 @@ def paged_plan(table: torch.Tensor, kv_lens, packed_lens, q_lens, heads: int, kv
 
     table: the sequences' pages, whole numbers in host memory [sequences, pages]: token t of a sequence lies in page
     table[t // page_size], a packed page for t < packed_lens (whole pages), an fp16 page from there on.  kv_lens: tokens of each
-    sequence, the q_lens newest of them new (none of them packed).  The plan is made on torch's current stream of `device`."""
+    sequence, the q_lens newest of them new (none of them packed).  The plan is copied to `device` on torch's current stream and can be
+    used on any stream: calls on another one wait for it.  It cannot be made while a graph is captured; a graph in which it is used
+    needs it as long as the graph is replayed."""
     return _host().paged_plan(table, list(kv_lens), list(packed_lens), list(q_lens), heads, kv_heads, head_dim, page_size, _cuda(device))
 
 

@@ -81,3 +81,49 @@ def test_page_numbers_that_are_none(dev, far):
     with pytest.raises(RuntimeError, match="page number"):
         ops.paged_plan(torch.tensor([[0, far]]), [100], [0], [1], 4, 2, 128, 64, dev)
     assert ops.paged_plan(torch.tensor([[0, far]]), [64], [0], [1], 4, 2, 128, 64, dev).tokens == 1  # (a cell that no token needs)
+
+
+def test_a_plan_made_on_another_stream(dev):
+    """A plan can be used on any stream: its list is waited for, and not given to others while it is read."""
+    from kvmix_amd import ops
+
+    b = Batch(dev, [700, 60, 300], [512, 0, 128], [1, 40, 3], 8, 2, 128, 64, 4, 4, seed=3)
+    kv = torch.randn(44, 2, 128, dtype=torch.float16, device=dev)
+    want_rows = b.rows.clone()
+    ops.paged_append(kv, kv, want_rows, b.plan)
+    want = ops.paged_attention(b.q, want_rows, b.packed, b.plan, 4, 4)
+    rows, other_rows = b.rows.clone(), b.rows.clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    # made behind other work, used at once
+    torch.cuda._sleep(200_000_000)
+    plan = ops.paged_plan(b.table, b.lens, b.packed_lens, b.new, 8, 2, 128, 64, dev)
+    with torch.cuda.stream(side):
+        ops.paged_append(kv, kv, rows, plan)
+        got = ops.paged_attention(b.q, rows, b.packed, plan, 4, 4)
+    side.synchronize()
+    assert torch.equal(got, want)
+    # dropped while it is still to be read
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        ops.paged_append(kv, kv, other_rows, plan)
+        got = ops.paged_attention(b.q, other_rows, b.packed, plan, 4, 4)
+    words = plan.slots.untyped_storage().nbytes() // 4
+    del plan
+    others = [torch.zeros(words, dtype=torch.int32, device=dev) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and not any(t.any() for t in others)
+
+
+def test_plans_are_made_outside_of_captures(dev):
+    from kvmix_amd import ops
+
+    table = torch.tensor([[0, 1]])
+    x = torch.zeros(4, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="captured"):
+            ops.paged_plan(table, [100], [0], [1], 4, 2, 128, 64, dev)
+    graph.replay()
+    assert ops.paged_plan(table, [100], [0], [1], 4, 2, 128, 64, dev).tokens == 1 and float(x[0]) == 1.0
