@@ -24,6 +24,10 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kItemWords = 12;
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
+// Probabilities are halves relative to 2^-kAbove of the largest, so that one of 2^-31 of it still is a number (from 1 on, those
+// below 2^-25 were none: 100000 tokens just below that, 2.6e-3 of the mass together, went missing).  The reference may lag behind
+// a larger one by kLag in all: 2^15 is well inside fp16's range.
+constexpr float kAbove = 7.0f, kLag = 15.0f;
 
 struct PagedArgs {
     const _Float16 *q;
@@ -34,8 +38,8 @@ struct PagedArgs {
     PlanWords table, items;
     int table_stride, kv_heads, group, blocks_log2;  // blocks_log2: of 32 tokens to a page
     float scale;                                     // with log2(e)
-    float *part;                                     // [kv heads][part_rows][D], relative to the maximum in part_ml
-    float2 *part_ml;                                 // [kv heads][part_rows] maximum (of log2) and sum
+    float *part;                                     // [kv heads][part_rows][D], relative to the reference in part_ml
+    float2 *part_ml;                                 // [kv heads][part_rows] reference (of log2) and sum
     int64_t part_rows;
 };
 
@@ -164,8 +168,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             for (int t = 0; t < DT; t++) acc[n][t] = floatx4{};
         }
 
-        // a block's logits to probabilities; the maximum is moved when some row's has grown by more than 2^8 (they stay well inside
-        // fp16's range below that)
+        // a block's logits to probabilities, relative to a reference that is moved when some row's largest is kLag above it
         auto probabilities = [&](floatx4 (&x)[2][NR], half8v (&p)[NR], int block, auto packed_tokens) {
             if (!packed_tokens.value && block * kBlock + kBlock - 1 > first_limit) {  // (every new token sees all packed ones)
 #pragma unroll
@@ -181,8 +184,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
 #pragma unroll
                 for (int i = 1; i < 8; i++) most = fmaxf(most, x[i / 4][n][i % 4]);
                 most *= scale[n];
-                if (__any(most > top[n] + 8.0f)) {
-                    const float grown = fmaxf(top[n], max_of_rows(most));
+                if (__any(most > top[n] + kLag)) {
+                    const float grown = fmaxf(top[n], max_of_rows(most) - kAbove);
                     const float shrink = __builtin_amdgcn_exp2f(top[n] - grown);
                     top[n] = grown;
                     sum[n] *= shrink;
@@ -511,8 +514,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
             most = fmaxf(__uint_as_float(e[0]), __uint_as_float(e[1])) * a.scale;
         }
-        if (__any(most > top + 8.0f)) {
-            const float grown = fmaxf(top, most), shrink = __builtin_amdgcn_exp2f(top - grown);
+        if (__any(most > top + kLag)) {
+            const float grown = fmaxf(top, most - kAbove), shrink = __builtin_amdgcn_exp2f(top - grown);
             top = grown;
             sum *= shrink;
 #pragma unroll
