@@ -6,7 +6,7 @@ concatenation.  Here the tokens of all sequences lie in pages of pools that are 
 (codes of 1 to 4 bits per layer, fp16 scales and minima, the reference's quantizer in groups of 32), its newest in fp16, at
 least `window` tokens of them.  A page is packed as a whole once it has left the window.  All layers use the same page numbers, so
 that one table per sequence serves all of them; a packed page never changes and is shared by the sequences forked from one
-another, as is every full fp16 page.
+another, as is every full fp16 page: the first of them that packs such a page does it for all.
 
     cache = PagedKVCache(k_bits, v_bits, heads=32, kv_heads=8, head_dim=128, row_pages=256, packed_pages=4096)
     a = cache.new()
@@ -111,6 +111,8 @@ class PagedKVCache:
         self.packed = [torch.zeros(packed_pages, kv_heads, page_size // 32 * head_dim * (kb + vb + 2), dtype=torch.int32, device=self.device)
                        for kb, vb in zip(k_bits, v_bits)]
         self._row_pages, self._packed_pages = _Pages(row_pages), _Pages(packed_pages)
+        self._packed_as: Dict[int, int] = {}  # fp16 pages still in use -> the packed page made of them, in use too
+        self._made_of: Dict[int, int] = {}    # the other way round
         self._sequences: Dict[int, _Sequence] = {}
         self._next = 0
 
@@ -164,9 +166,19 @@ class PagedKVCache:
         old = self._sequence(s)
         del self._sequences[s]
         for p in old.packed:
-            self._packed_pages.drop(p)
+            self._drop_packed(p)
         for p in old.rows:
-            self._row_pages.drop(p)
+            self._drop_row(p)
+
+    def _drop_row(self, page: int) -> None:
+        self._row_pages.drop(page)
+        if not self._row_pages.users[page] and page in self._packed_as:
+            del self._made_of[self._packed_as.pop(page)]
+
+    def _drop_packed(self, page: int) -> None:
+        self._packed_pages.drop(page)
+        if not self._packed_pages.users[page] and page in self._made_of:
+            del self._packed_as[self._made_of.pop(page)]
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the pools, all layers with one call per kind of page (what lies behind them
@@ -179,6 +191,11 @@ class PagedKVCache:
             ops.paged_copy(pools, torch.tensor(list(moves.items()), dtype=torch.int32))
             for seq in self._sequences.values():
                 setattr(seq, of, [moves.get(p, p) for p in getattr(seq, of)])
+            if of == "rows":
+                self._packed_as = {moves.get(r, r): p for r, p in self._packed_as.items()}
+            else:
+                self._packed_as = {r: moves.get(p, p) for r, p in self._packed_as.items()}
+            self._made_of = {p: r for r, p in self._packed_as.items()}
             moved += len(moves)
         return moved
 
@@ -195,7 +212,7 @@ class PagedKVCache:
         if any(n < 0 for _, _, n in seqs):
             raise RuntimeError("step: a negative number of new tokens")
         flush = [(seq, self._leaves_window(seq)) for _, seq, _ in seqs]
-        need_packed = sum(n for _, n in flush)
+        need_packed = len({page for seq, n in flush for page in seq.rows[:n]} - self._packed_as.keys())
         need_rows = sum(-(-(seq.length + n) // P) - len(seq.packed) - len(seq.rows) for _, seq, n in seqs)
         gained = self._freed(flush)
         if need_packed > len(self._packed_pages.free) or need_rows > len(self._row_pages.free) + gained:
@@ -204,8 +221,13 @@ class PagedKVCache:
         pairs = []
         for seq, n in flush:
             for page in seq.rows[:n]:
-                to = self._packed_pages.take()
-                pairs.append((page, to))
+                to = self._packed_as.get(page)
+                if to is None:
+                    to = self._packed_pages.take()
+                    pairs.append((page, to))
+                    self._packed_as[page], self._made_of[to] = to, page
+                else:  # (by a fork before, or in this step)
+                    self._packed_pages.share(to)
                 seq.packed.append(to)
         if pairs:
             listed = torch.tensor(pairs, dtype=torch.int32)
@@ -213,7 +235,7 @@ class PagedKVCache:
                 ops.paged_quantize(self.rows[layer], self.packed[layer], listed, kb, vb)
         for seq, n in flush:
             for page in seq.rows[:n]:
-                self._row_pages.drop(page)
+                self._drop_row(page)
             del seq.rows[:n]
         for _, seq, n in seqs:
             seq.length += n
