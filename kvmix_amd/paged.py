@@ -22,6 +22,7 @@ The numbers of pages are kept on the host; nothing here waits for the GPU.
 """
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass, field
 from typing import Dict, List, Sequence
 
@@ -72,13 +73,15 @@ class _Sequence:
     rows: List[int] = field(default_factory=list)    # the fp16 pages after them
 
 
-@dataclass
+@dataclass(eq=False)
 class Step:
     """What PagedKVCache.step returns: the plan that append and attend of every layer use, and where each sequence's new tokens
-    lie among those of the step."""
+    lie among those of the step.  It serves until one of its sequences takes another step or ends, or pages move."""
     plan: object
     sequences: List[int]
     counts: List[int]
+    cache: object = field(default=None, repr=False)
+    over: bool = False
 
     def tokens(self) -> Dict[int, slice]:
         out, at = {}, 0
@@ -115,6 +118,7 @@ class PagedKVCache:
         self._made_of: Dict[int, int] = {}    # the other way round
         self._sequences: Dict[int, _Sequence] = {}
         self._next = 0
+        self._steps: Dict[int, weakref.ref] = {}  # the latest step of each sequence
 
     # -- sequences ---------------------------------------------------------------------------
     def new(self) -> int:
@@ -164,11 +168,19 @@ class PagedKVCache:
     def free(self, s: int) -> None:
         """Ends a sequence: pages that no other one uses can be taken again."""
         old = self._sequence(s)
+        self._end_steps([s])
         del self._sequences[s]
         for p in old.packed:
             self._drop_packed(p)
         for p in old.rows:
             self._drop_row(p)
+
+    def _end_steps(self, sequences) -> None:
+        """The plans of these sequences' steps name pages that are written, given away or moved from now on."""
+        for s in sequences:
+            step = self._steps.pop(s, lambda: None)()
+            if step is not None:
+                step.over = True
 
     def _drop_row(self, page: int) -> None:
         self._row_pages.drop(page)
@@ -197,6 +209,8 @@ class PagedKVCache:
                 self._packed_as = {r: moves.get(p, p) for r, p in self._packed_as.items()}
             self._made_of = {p: r for r, p in self._packed_as.items()}
             moved += len(moves)
+        if moved:
+            self._end_steps(list(self._steps))
         return moved
 
     # -- steps -------------------------------------------------------------------------------
@@ -218,6 +232,7 @@ class PagedKVCache:
         if need_packed > len(self._packed_pages.free) or need_rows > len(self._row_pages.free) + gained:
             raise OutOfPages(f"step needs {need_packed} packed and {need_rows} fp16 pages; {len(self._packed_pages.free)} and "
                              f"{len(self._row_pages.free) + gained} can be had")
+        self._end_steps([s for s, _, _ in seqs])
         pairs = []
         for seq, n in flush:
             for page in seq.rows[:n]:
@@ -260,16 +275,25 @@ class PagedKVCache:
             table[i, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
         plan = ops.paged_plan(table, [seq.length for _, seq, _ in seqs], [len(seq.packed) * P for _, seq, _ in seqs], [n for _, _, n in seqs],
                               self.heads, self.kv_heads, self.head_dim, P, self.device)
-        return Step(plan, [s for s, _, _ in seqs], [n for _, _, n in seqs])
+        step = Step(plan, [s for s, _, _ in seqs], [n for _, _, n in seqs], self)
+        self._steps.update((s, weakref.ref(step)) for s, _, _ in seqs)
+        return step
 
     # -- what a layer does in a step ---------------------------------------------------------
+    def _plan(self, step: Step):
+        if step.cache is not self:
+            raise RuntimeError("this step is of another cache")
+        if step.over:
+            raise RuntimeError("this step is over: a sequence of it has taken another one or ended, or its pages have moved")
+        return step.plan
+
     def append(self, layer: int, step: Step, k: torch.Tensor, v: torch.Tensor) -> None:
         """The new tokens' keys and values [tokens, kv_heads, head_dim], sequence after sequence."""
-        ops.paged_append(k, v, self.rows[layer], step.plan)
+        ops.paged_append(k, v, self.rows[layer], self._plan(step))
 
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float = None) -> torch.Tensor:
         """Attention of the new tokens' queries [tokens, heads, head_dim] over their sequences, themselves included."""
-        return ops.paged_attention(q, self.rows[layer], self.packed[layer], step.plan, self.k_bits[layer], self.v_bits[layer], scale)
+        return ops.paged_attention(q, self.rows[layer], self.packed[layer], self._plan(step), self.k_bits[layer], self.v_bits[layer], scale)
 
     def read(self, layer: int, s: int):
         """Keys and values [length, kv_heads, head_dim] of a sequence as the cache holds them, in fp16."""
