@@ -74,23 +74,30 @@ class PagedDecoder:
     def generate(self, sequences: Sequence[int], first: torch.Tensor, new_tokens: int, alternatives: int = 0):
         """Greedy decoding of several sequences at once, from their next tokens `first` [n]: the ids [n, new_tokens], `first`
         among them; with alternatives > 0 also the log probabilities and the ids of the most likely tokens at each step after it,
-        [n, new_tokens - 1, alternatives]."""
+        [n, new_tokens - 1, alternatives] (none where there is no step after it)."""
         out: List[torch.Tensor] = [first.reshape(-1)]
+        if new_tokens < 0 or len(set(sequences)) != len(sequences) or out[0].numel() != len(sequences):
+            raise RuntimeError("generate: a number of tokens that is not negative, sequences that are different, and one first token for each")
         best = []
-        for _ in range(new_tokens - 1):
+        for _ in range(new_tokens - 1 if len(sequences) else 0):
             logits = self.forward({s: out[-1][i:i + 1] for i, s in enumerate(sequences)})
             stacked = torch.stack([logits[s] for s in sequences])
             _, _, top_logprob, top_id = ops.token_logprobs(stacked, out[-1], top=max(alternatives, 1))
             out.append(top_id[:, 0])
             best.append((top_logprob, top_id))
-        ids = torch.stack(out, 1)
+        ids = torch.stack(out, 1)[:, :new_tokens] if len(sequences) else out[0].new_empty(0, new_tokens)
         if not alternatives:
             return ids
+        if not best:
+            empty = ids.new_empty(len(sequences), max(new_tokens - 1, 0), alternatives)
+            return ids, empty.float(), empty
         return ids, *(torch.stack([b[i] for b in best], 1) for i in range(2))
 
     def score(self, ids: torch.Tensor, chunk: int = 512):
         """(log probabilities, entropies) [len(ids) - 1] of the tokens of a text after its first, each given those before it, read
         through the quantized cache in chunks."""
+        if chunk <= 0:
+            raise RuntimeError("score: a chunk has at least one token")
         ids = ids.reshape(-1).to(self.w["embed"].device)
         s = self.add()
         lp, entropy = [], []
