@@ -151,7 +151,8 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor &pool, const Tensor &pages_in
     kvmix_paged_pool_t p{};
     const bool packed = k_bits || v_bits;
     if (packed) {
-        if (!k_bits || !v_bits || !head_dim || *head_dim <= 0) fail("paged_read: packed pages need both widths and the head dimension");
+        if (!k_bits || !v_bits || !head_dim) fail("paged_read: packed pages need both widths and the head dimension");
+        if (*head_dim != 64 && *head_dim != 128) fail("paged_read: the head dimension is 64 or 128");
         check_bits(*k_bits);
         check_bits(*v_bits);
         if (pool.dim() != 3) fail("packed pages must be contiguous int32 [pages, kv_heads, page_size / 32 * head_dim * (k_bits + v_bits + 2)]");

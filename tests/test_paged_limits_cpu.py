@@ -31,3 +31,22 @@ def test_blocks_of_the_store(sequences, ok):
     """One token of 4096 heads each: four heads to a block of 256 threads."""
     code, _ = plan_of(sequences, 1, 4096)
     assert code == (0 if ok else -9)
+
+
+@pytest.mark.parametrize("head_dim", [1 << 61, 1 << 62, -(1 << 61), 0, -64, 96, (1 << 63) - 1])
+def test_head_dimensions_of_packed_pages(head_dim):
+    """Refused, whatever their product with the widths is (2^61 times 8 is 0 in 64 bits, and was divided by).  In a process of its own,
+    as a division by zero ends it."""
+    import subprocess
+    import sys
+
+    code = f"""
+import torch
+from kvmix_amd import ops
+try:
+    ops.paged_read(torch.zeros(1, 1, 1024, dtype=torch.int32), torch.tensor([0]), 4, 2, {head_dim})
+except RuntimeError as e:
+    print("refused:", e)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "head dimension" in done.stdout, (done.returncode, done.stdout, done.stderr[-500:])
