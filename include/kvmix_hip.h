@@ -597,9 +597,8 @@ int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t 
  * product with the values and for its sum alike.
  *   q, out [plan.tokens, heads, head_dim] fp16, unit stride along head_dim, strides in elements, multiples of 8; 16-byte aligned
  *   list: the plan's words in device memory;  0 < scale <= 2^40
- * What pages hold behind a sequence's last token is not used, whatever it is.  The values of a sequence's own tokens are expected to
- * be finite: the products are made for blocks of 32 or 64 tokens, and zero times an infinite value of a later new token of the
- * same block is NaN in that channel of the new tokens before it.  (Keys may be anything: a logit that is not to be seen is replaced.)
+ * What pages hold behind a sequence's last token is not used, whatever it is, and a token's key and value reach the tokens that see
+ * it and no others, also where they are infinite or NaN (the result is infinite or NaN then, where such a value's weight is not zero).
  */
 typedef struct kvmix_paged_attn {
     const void *q;

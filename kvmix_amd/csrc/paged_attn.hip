@@ -70,6 +70,45 @@ __device__ __forceinline__ float sum_of_rows(float v)
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// Values that are no numbers.  The products are made for whole blocks of tokens, and zero times an infinite value of a token that
+// a row does not see is not zero.  So the values of blocks that not every new token sees wholly are looked through; where one is
+// infinite or NaN, a finite one goes into the products instead, and which token first brings such a value to a channel is kept
+// here, to be added to the results of the rows that see it.
+template <int D>
+struct Beyond {
+    int first[3][D];  // +inf, -inf, NaN
+    int any;
+
+    // by `count` threads
+    __device__ __forceinline__ void clear(int thread, int count)
+    {
+#pragma unroll
+        for (int i = thread; i < 3 * D; i += count) first[0][i] = 0x7fffffff;
+        if (thread == 0) any = 0;
+    }
+
+    // value `bits` of a token and channel
+    __device__ __forceinline__ void note(uint32_t bits, int token, int channel)
+    {
+        if ((bits & 0x7c00u) != 0x7c00u) return;
+        atomicMin(&first[bits & 0x3ffu ? 2 : bits >> 15][channel], token);
+        any = 1;
+    }
+
+    // what to add to channel c of a row that sees the tokens up to `limit`
+    __device__ __forceinline__ float of(int c, int limit) const
+    {
+        const bool up = first[0][c] <= limit, down = first[1][c] <= limit;
+        return first[2][c] <= limit || (up && down) ? __builtin_nanf("") : up ? __builtin_inff() : down ? -__builtin_inff() : 0.0f;
+    }
+};
+
+// NaN from the first infinite value or NaN on
+__device__ __forceinline__ float beyond_sum(uint32_t pair, float sum)
+{
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), half2v{(_Float16)0.0f, (_Float16)0.0f}, sum, false);
+}
+
 // A packed block as a lane holds it: its codes, and its share of the scales and minima, which go through the LDS to the lanes
 // that need them (each is wanted by sixteen).
 template <int D, int KB, int VB>
@@ -114,6 +153,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             float2 ml[4][16 * NR];
         } join;
     } lds;
+    __shared__ Beyond<D> beyond[4];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const int head = blockIdx.x % a.kv_heads, column = blockIdx.x / a.kv_heads;
     const int per_page = 1 << a.blocks_log2;
@@ -126,6 +166,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         if (nth) it = item_of(a.items, next + nth - 1);
         const int q_start = it.q_start, q_len = it.q_len, kv_len = it.kv_len, packed = it.packed;
         const PlanWords table = a.table + it.seq * a.table_stride;
+        beyond[wave].clear(lane, kWave);
 
         half8v q[NR][KS];
         int limit[NR];  // the row's own token
@@ -323,6 +364,26 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
                 }
             }
+            if (block * kBlock + kBlock - 1 > first_limit) {
+                float found = 0.0f;
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) found = beyond_sum(__builtin_bit_cast(uint4v, v[t])[j], found);
+                }
+                if (__builtin_expect(__any(found != found), 0)) {
+                    int from = lane;
+                    asm volatile("" : "+v"(from));  // (nothing of this is worked out before)
+#pragma unroll 1
+                    for (int i = from; i < D * kBlock; i += kWave) {
+                        const int token = block * kBlock + i % kBlock;
+                        if (token < kv_len) beyond[wave].note(((const uint16_t *)values)[i], token, i / kBlock);
+                    }
+                    const half8v largest = (half8v)(_Float16)65504.0f;
+#pragma unroll
+                    for (int t = 0; t < DT; t++) v[t] = __builtin_elementwise_max(__builtin_elementwise_min(v[t], largest), -largest);
+                }
+            }
             half8v p[NR];
             probabilities(x, p, block, std::false_type());
             if (block * kBlock + kBlock > kv_len) {  // (whatever lies behind the last token: zero times it may not be zero)
@@ -370,6 +431,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 o[0] += *(const floatx4 *)&lds.join.out[w][r][c];
                 o[1] += *(const floatx4 *)&lds.join.out[w][r][c + 4];
             }
+            if (__builtin_expect(beyond[0].any | beyond[1].any | beyond[2].any | beyond[3].any, 0)) {
+                const int sees = kv_len - q_len + (it.row0 + r) / a.group;
+#pragma unroll 1
+                for (int w = 0; w < 4; w++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[j / 4][j % 4] += beyond[w].of(c + j, sees);
+                }
+            }
             if (it.part >= 0) {
                 const int64_t to = head * a.part_rows + it.part + r;
                 *(floatx4 *)(a.part + to * D + c) = o[0];
@@ -413,6 +482,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     constexpr int kBytes = kTileKeys * D * 2;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kBytes];
     __shared__ uint32_t sides[4][D];
+    __shared__ Beyond<D> beyond;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane & 31, h2 = lane >> 5;
     const int m = lane % 16, g = lane / 16;
     const int head = blockIdx.x % a.kv_heads;
@@ -420,6 +490,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int q_start = it.q_start, q_len = it.q_len, kv_len = it.kv_len, packed_blocks = it.packed / kBlock, blocks = (kv_len + kBlock - 1) / kBlock;
     const PlanWords table = a.table + it.seq * a.table_stride;
     const int per_page = 1 << a.blocks_log2;
+    beyond.clear(threadIdx.x, 256);  // (a barrier follows before fp16 pages are placed)
 
     const int own = 32 * wave + col, r = it.row0 + min(own, it.rows - 1), token = r / a.group, limit = kv_len - q_len + token;
     const int wave_first = kv_len - q_len + (it.row0 + min(32 * wave, it.rows - 1)) / a.group;
@@ -479,6 +550,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
             else turn(std::integral_constant<int, KB>());
             __builtin_amdgcn_wave_barrier();
         } else if (block < blocks) {
+            float found = 0.0f;
+            if (matrix && block * kBlock + kBlock - 1 > kv_len - q_len) {
+#pragma unroll
+                for (int i = 0; i < 4 * NP; i++) found = beyond_sum(held[i], found);
+            }
 #pragma unroll
             for (int p = 0; p < NP; p++) {
                 half8v x = __builtin_bit_cast(half8v, *(const uint4v *)&held[4 * p]);
@@ -488,6 +564,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
                         if (block * kBlock + 8 * g + j >= kv_len) x[j] = (_Float16)0.0f;
                 }
                 put(p, x);
+            }
+            if (__builtin_expect(__any(found != found), 0)) {  // (in the LDS: a wave's operations there are done in order)
+                int row = m;
+                asm volatile("" : "+v"(row));  // (nothing of this is worked out before)
+#pragma unroll 1
+                for (int p = 0; p < NP; p++, row += 16) {
+                    _Float16 *at = (_Float16 *)(to + tile_value(row, 4 * which + g));
+#pragma unroll 1
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t bits = __builtin_bit_cast(uint16_t, at[j]);
+                        beyond.note(bits, block * kBlock + 8 * g + j, row);
+                        if ((bits & 0x7c00u) == 0x7c00u) at[j] = (_Float16)0.0f;
+                    }
+                }
             }
         } else {
 #pragma unroll
@@ -641,6 +731,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         else run(std::false_type());
     } else {
         fetch(tile);
+        __syncthreads();
         place(tile, 0);
         __syncthreads();
     }
@@ -667,6 +758,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
         buf ^= 1;
         __syncthreads();
+    }
+    if (__builtin_expect(beyond.any, 0)) {
+#pragma unroll
+        for (int t = 0; t < DT; t++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] += beyond.of(32 * t + 8 * (i / 4) + 4 * h2 + i % 4, limit);
+        }
     }
     if (own >= it.rows) return;
     {
