@@ -593,8 +593,8 @@ int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t 
  * Attention of a batch's new tokens over its pages:  out[i, h] = sum_{j <= pos(i)} softmax_j(scale q[i, h] . k[j, h']) v[j, h'],
  * h' = h / (heads / kv_heads), over the tokens of i's own sequence up to itself (the new tokens' keys and values are in their
  * pages already).  Packed values are taken as fp16 (code * scale + minimum, rounded once); packed keys as well where a sequence's new
- * tokens times heads / kv_heads are more than 32, as they are below.  Logits, softmax and sums in fp32, probabilities rounded to fp16 for the
- * product with the values and for its sum alike.
+ * tokens times heads / kv_heads are more than 32, exactly where they are not.  Logits, softmax and sums in fp32, probabilities rounded to fp16
+ * (to 2^-31 of the largest) for the product with the values and for its sum alike.
  *   q, out [plan.tokens, heads, head_dim] fp16, unit stride along head_dim, strides in elements, multiples of 8; 16-byte aligned
  *   list: the plan's words in device memory;  0 < scale <= 2^40
  * What pages hold behind a sequence's last token is not used, whatever it is, and a token's key and value reach the tokens that see

@@ -135,8 +135,9 @@ __device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uin
 // one half the error of the whole against 64 bits was 1.2 to 1.5e-3, with keys rounded to fp16 4e-4, with two 2.7 to 3.2e-4; a result's
 // own rounding is 2.1e-4.  For sixteen rows it costs 5 us of 70, for 32 rows, 16 x 16384 tokens of 8 heads, 12 of 67).
 //
-// Bound by vector instructions and memory together: 16 x 8192 tokens of 32 heads, 2/2 bits, 66 us (314 MB, 4.8 TB/s; one byte of
-// codes is eight values to convert), 4/4 bits 92 us (490 MB, 5.3 TB/s), 3/2 bits of 8 heads over 32768 tokens 73 us (4.5 TB/s).
+// Bound by vector instructions and memory together: 16 x 8192 tokens of 32 heads, 2/2 bits, 64 us (314 MB, 4.9 TB/s; a byte of
+// codes is four values to convert; the vector ALU is at work for 65 % of the time, the matrix cores for 28), 4/4 bits 94 us (490 MB,
+// 5.2 TB/s), 3/2 bits of 8 heads over 32768 tokens 73 us (4.6 TB/s; 69 and 27 %).
 template <int D, int KB, int VB, int NR>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 3 : 2))) paged_few(PagedArgs a)
 {
@@ -473,8 +474,8 @@ __device__ __forceinline__ int tile_value(int channel, int c) { return channel *
 // values' pieces are.  Packed keys and values are rounded to fp16 once (code * scale + minimum): the matrix cores take no others at this rate.
 //
 // Bound by the matrix cores and, in turns with them, the vector ALU (exponentials 9 cycles each, conversions of codes): 4 chunks of 2048 tokens over
-// 8192, 32 heads, 4/4 bits: 800 us, 860 TFLOP/s of the 1490 that a fp16 product of 16384 reaches (855 with the codes converted between
-// tiles, on a box on which the others took 786).  Two blocks to a CU is what the LDS (66 KB each) and the registers (256) hold.
+// 8192, 32 heads, 4/4 bits: 826 us, 831 TFLOP/s of the 1490 that a fp16 product of 16384 reaches; matrix cores at work for 41 % of the time,
+// vector ALU for 52 (with the codes converted between tiles 855 us, on a box on which the others took 786).  Two blocks to a CU is what the LDS (66 KB each) and the registers (256) hold.
 template <int D, int KB, int VB>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) paged_tile(PagedArgs a)
 {
@@ -800,7 +801,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // The spans of one sequence's rows together; the item's `begin` is the number of spans, `end` the rows between them.  A row's D sums
 // are four to a lane; a row is a group of lanes, or where there are many spans all groups of the block, each for every GROUPS-th of
 // them.  Eight spans' sums and maxima are asked for at once, the maximum runs along: one wait on memory, which is what bounds it
-// (3 us for a few rows; the spans of 19392 rows, 55 MB, 9 us).
+// (3 us for a few rows; 19392 rows in two or three spans, 25 MB, 9 us).
 constexpr int kJoinAhead = 8;
 
 template <int D>

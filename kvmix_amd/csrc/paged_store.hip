@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(256) paged_quantize(QuantizeArgs a, PagePairs 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // read: the values of pages, token by token: [pages, P, heads, D].  A block of one head per wave pair, keys and values.  Bound by its
-// writes: 120 pages of 32 heads, 3/2 bits, 25 us (126 MB written, 28 read: 6.1 TB/s); four pages of 8 heads 3.8, a launch.
+// writes: 120 pages of 32 heads, 3/2 bits, 25 us (126 MB written, 28 read: 6.1 TB/s); four pages of 8 heads 3.8, a launch; 120 fp16 pages 42 us
+// (252 MB, 6.0 TB/s).
 
 struct ReadArgs {
     const void *pool;

@@ -14,8 +14,9 @@
 // the lanes, by its upper sixteen bits; what reaches it is collected and put in order by counting.  Equal logits come in the
 // order of their indexes.  Rows in which too many reach it (constant ones), or with NaN, are searched value by value.
 //
-// 8192 rows of 32000 halves with the top 20: 104 us, 5.0 TB/s (a pure read 6.2); one row with the top 5: 6.5 us, a launch of one
-// chain of latencies; 4099 rows with both gradients 161 us (787 MB, 4.9 TB/s; a large copy 4.75).
+// 8192 rows of 32000 halves with the top 20: 100 us, 5.2 TB/s (a pure read 6.2); one row with the top 5: 6.8 us, a launch of one
+// chain of latencies; 4099 rows with both gradients 161 us (787 MB, 4.9 TB/s; a large copy 4.75); 4096 rows with the top 20 in bf16
+// 74 us, in fp32 140 (3.5 and 3.7 TB/s).
 #include <algorithm>
 #include <type_traits>
 

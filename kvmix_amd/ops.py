@@ -478,7 +478,8 @@ def paged_plan(table: torch.Tensor, kv_lens, packed_lens, q_lens, heads: int, kv
     table[t // page_size], a packed page for t < packed_lens (whole pages), an fp16 page from there on.  kv_lens: tokens of each
     sequence, the q_lens newest of them new (none of them packed).  The plan is copied to `device` on torch's current stream and can be
     used on any stream: calls on another one wait for it.  It cannot be made while a graph is captured; a graph in which it is used
-    needs it as long as the graph is replayed."""
+    needs it as long as the graph is replayed.  Its `slots` [tokens] say where each new token goes (fp16 page * page_size + place), for
+    a caller's own kernels."""
     return _host().paged_plan(table, list(kv_lens), list(packed_lens), list(q_lens), heads, kv_heads, head_dim, page_size, _cuda(device))
 
 
@@ -516,7 +517,8 @@ def paged_copy(pools, pairs: torch.Tensor) -> None:
 def paged_attention(q: torch.Tensor, rows: torch.Tensor, packed: torch.Tensor, plan, k_bits: int, v_bits: int, scale: float = None) -> torch.Tensor:
     """Attention of a step's new tokens, one or many of each sequence, over the sequences' pages (kvmix_paged_attention): q
     [plan.tokens, heads, head_dim] fp16 -> the same shape.  A token sees its own sequence up to itself; keys and values of the
-    new tokens are in their pages already (paged_append).  scale: head_dim ** -0.5 unless given."""
+    new tokens are in their pages already (paged_append).  scale: head_dim ** -0.5 unless given.  Packed keys enter exactly where a
+    sequence has at most 32 new tokens times heads / kv_heads, rounded to fp16 where it has more."""
     return _host().paged_attention(q, rows, packed, plan, k_bits, v_bits, scale)
 
 
