@@ -581,6 +581,7 @@ typedef struct kvmix_paged_plan {
     int64_t few_rows;                            /* query rows of an item of few: 16 or 32 */
     int64_t part_rows;                           /* rows of partial results per kv head */
     int64_t join_blocks;                         /* blocks that put the parts of one join together */
+    int64_t few_tokens;                          /* new tokens of a sequence of few rows: the most */
 } kvmix_paged_plan_t;
 int kvmix_paged_plan(const kvmix_paged_batch_t *batch, int32_t *words, int64_t capacity, kvmix_paged_plan_t *plan);
 

@@ -151,7 +151,7 @@ class PagedPlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int64) for name in (
         "words", "tokens", "heads", "kv_heads", "head_dim", "page_size", "table_stride", "row_pages", "packed_pages", "slots_at",
         "store_at", "table_at", "few_at", "tile_at", "join_at", "stores", "few", "few_columns", "tiles", "joins", "few_rows", "part_rows",
-        "join_blocks")]
+        "join_blocks", "few_tokens")]
 
 
 LINEAR_PLAIN, LINEAR_FLOAT, LINEAR_RESIDUAL, LINEAR_SWIGLU, LINEAR_ROPE_APPEND = range(5)

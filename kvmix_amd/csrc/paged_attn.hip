@@ -138,7 +138,11 @@ __device__ __forceinline__ void load_packed(PackedBlock<D, KB, VB> &b, const uin
 // Bound by vector instructions and memory together: 16 x 8192 tokens of 32 heads, 2/2 bits, 64 us (314 MB, 4.9 TB/s; a byte of
 // codes is four values to convert; the vector ALU is at work for 65 % of the time, the matrix cores for 28), 4/4 bits 94 us (490 MB,
 // 5.2 TB/s), 3/2 bits of 8 heads over 32768 tokens 73 us (4.6 TB/s; 69 and 27 %).
-template <int D, int KB, int VB, int NR>
+//
+// LATER: whether values may be infinite in tokens that some row does not see, which takes a sequence of several new tokens.  Where
+// there is none the kernel is made without looking for them: at 168 registers it costs 0 to 8 % (16 x 8192 tokens, 3/1 bits, 86.4
+// instead of 93.3 us; 2/2 bits 79 both).
+template <int D, int KB, int VB, int NR, bool LATER>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 3 : 2))) paged_few(PagedArgs a)
 {
     constexpr int KS = D / 32, DT = D / 16, NK = lane_words(D, KB), NV = lane_words(D, VB);
@@ -154,7 +158,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
             float2 ml[4][16 * NR];
         } join;
     } lds;
-    __shared__ Beyond<D> beyond[4];
+    __shared__ typename std::conditional<LATER, Beyond<D>, int>::type beyond[4];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const int head = blockIdx.x % a.kv_heads, column = blockIdx.x / a.kv_heads;
     const int per_page = 1 << a.blocks_log2;
@@ -167,7 +171,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
         if (nth) it = item_of(a.items, next + nth - 1);
         const int q_start = it.q_start, q_len = it.q_len, kv_len = it.kv_len, packed = it.packed;
         const PlanWords table = a.table + it.seq * a.table_stride;
-        beyond[wave].clear(lane, kWave);
+        if constexpr (LATER) beyond[wave].clear(lane, kWave);
 
         half8v q[NR][KS];
         int limit[NR];  // the row's own token
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                     for (int n = 0; n < NR; n++) x[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][s], x[u][n], 0, 0, 0);
                 }
             }
-            if (block * kBlock + kBlock - 1 > first_limit) {
+            if constexpr (LATER) if (block * kBlock + kBlock - 1 > first_limit) {
                 float found = 0.0f;
 #pragma unroll
                 for (int t = 0; t < DT; t++) {
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 
                 o[0] += *(const floatx4 *)&lds.join.out[w][r][c];
                 o[1] += *(const floatx4 *)&lds.join.out[w][r][c + 4];
             }
-            if (__builtin_expect(beyond[0].any | beyond[1].any | beyond[2].any | beyond[3].any, 0)) {
+            if constexpr (LATER) if (__builtin_expect(beyond[0].any | beyond[1].any | beyond[2].any | beyond[3].any, 0)) {
                 const int sees = kv_len - q_len + (it.row0 + r) / a.group;
 #pragma unroll 1
                 for (int w = 0; w < 4; w++) {
@@ -1008,6 +1012,7 @@ int make_plan(const kvmix_paged_batch_t *b, int32_t *words, int64_t capacity, kv
         if (n * G <= kFewMost) {
             few.units += n ? (kv + kFewUnit * kBlock - 1) / (kFewUnit * kBlock) : 0;
             if (n * G > 16) plan->few_rows = kFewMost;
+            plan->few_tokens = std::max(plan->few_tokens, n);
         } else {
             for (int64_t r = 0; r < n * G; r += kTileRows)
                 lengths.push_back((kv - n + std::min(n * G - 1, r + kTileRows - 1) / G) / kTileKeys + 1);
@@ -1176,8 +1181,9 @@ extern "C" int kvmix_paged_attention(const kvmix_paged_pool_t *p, const kvmix_pa
                 if (plan->few) {
                     a.items = list + plan->few_at;
                     const unsigned grid = (unsigned)(plan->few_columns * plan->kv_heads);
-                    if (plan->few_rows > 16) paged_few<D.value, KB.value, VB.value, 2><<<grid, 256, 0, st>>>(a);
-                    else paged_few<D.value, KB.value, VB.value, 1><<<grid, 256, 0, st>>>(a);
+                    if (plan->few_rows > 16) paged_few<D.value, KB.value, VB.value, 2, true><<<grid, 256, 0, st>>>(a);
+                    else if (plan->few_tokens > 1) paged_few<D.value, KB.value, VB.value, 1, true><<<grid, 256, 0, st>>>(a);
+                    else paged_few<D.value, KB.value, VB.value, 1, false><<<grid, 256, 0, st>>>(a);
                 }
             });
         });

@@ -50,3 +50,11 @@ except RuntimeError as e:
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "head dimension" in done.stdout, (done.returncode, done.stdout, done.stderr[-500:])
+
+
+def test_the_most_new_tokens_of_few_rows():
+    """What the attention's kernel of few rows is chosen by: sequences of many rows and idle ones do not count."""
+    table = [[i] for i in range(4)]
+    for new, most in (([1, 1, 0, 1], 1), ([1, 3, 0, 1], 3), ([1, 60, 0, 1], 1), ([0, 60, 0, 0], 0), ([4, 60, 5, 0], 5)):
+        plan, _ = _lib.paged_plan(table, [64] * 4, [0] * 4, new, 8, 2, 128, 64)
+        assert plan["few_tokens"] == most
