@@ -103,7 +103,7 @@ class PagedKVCache:
             raise RuntimeError("page_size must be 32, 64, 128, 256, 512 or 1024")
         if head_dim not in (64, 128):
             raise RuntimeError("head_dim must be 64 or 128")
-        if kv_heads <= 0 or heads % kv_heads:
+        if kv_heads <= 0 or heads <= 0 or heads % kv_heads:
             raise RuntimeError("Total heads must be divisible by KV heads")
         if window < 0 or row_pages <= 0 or packed_pages < 0:
             raise RuntimeError("window and the numbers of pages must not be negative")

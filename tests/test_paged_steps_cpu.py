@@ -72,3 +72,9 @@ def test_a_step_of_another_cache(pools, monkeypatch):
     other = Pools(monkeypatch, 32)
     with pytest.raises(RuntimeError, match="another cache"):
         other.cache.attend(0, step, torch.zeros(1))
+
+
+@pytest.mark.parametrize("heads", [0, -4])
+def test_numbers_of_heads_that_are_none(heads):
+    with pytest.raises(RuntimeError, match="heads"):
+        paged.PagedKVCache([4], [4], heads, 2, 64, row_pages=4, packed_pages=4, device="cpu")
