@@ -140,7 +140,8 @@ class PagedKVCache:
 
     def fork(self, s: int, count: int = 1):
         """`count` new sequences with the tokens of `s` (the one sequence's number for a count of 1, else a list).  Pages are
-        shared; the one that is not full yet is copied, in all layers with one call."""
+        shared; the one that is not full yet is copied, in all layers with one call (so the tokens of the latest step are appended
+        before)."""
         old, P = self._sequence(s), self.page_size
         partial = old.length % P != 0
         if count < 1:
@@ -225,6 +226,8 @@ class PagedKVCache:
         seqs = [(s, self._sequence(s), int(n)) for s, n in new_tokens.items()]
         if any(n < 0 for _, _, n in seqs):
             raise RuntimeError("step: a negative number of new tokens")
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("step: pages are not taken while a graph is captured")
         flush = [(seq, self._leaves_window(seq)) for _, seq, _ in seqs]
         need_packed = len({page for seq, n in flush for page in seq.rows[:n]} - self._packed_as.keys())
         need_rows = sum(-(-(seq.length + n) // P) - len(seq.packed) - len(seq.rows) for _, seq, n in seqs)

@@ -127,3 +127,23 @@ def test_plans_are_made_outside_of_captures(dev):
             ops.paged_plan(table, [100], [0], [1], 4, 2, 128, 64, dev)
     graph.replay()
     assert ops.paged_plan(table, [100], [0], [1], 4, 2, 128, 64, dev).tokens == 1 and float(x[0]) == 1.0
+
+
+def test_steps_are_taken_outside_of_captures(dev):
+    """A step that is refused leaves the cache as it was."""
+    from kvmix_amd.paged import PagedKVCache
+
+    c = PagedKVCache([4], [4], 4, 2, 64, row_pages=16, packed_pages=16, page_size=32, window=32)
+    a = c.new()
+    step = c.step({a: 200})
+    kv = torch.randn(200, 2, 64, dtype=torch.float16, device=dev)
+    c.append(0, step, kv, kv)
+    q = torch.randn(200, 4, 64, dtype=torch.float16, device=dev)
+    want, state = c.attend(0, step, q), (c.length(a), c.free_pages())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q += 0
+        with pytest.raises(RuntimeError, match="captured"):
+            c.step({a: 3})
+    assert (c.length(a), c.free_pages()) == state
+    assert torch.equal(c.attend(0, step, q), want)
