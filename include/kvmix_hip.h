@@ -591,6 +591,27 @@ int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t 
                        int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride, kvmix_stream_t stream);
 
 /*
+ * The same from the projection of a step's new tokens, with the rotary embedding on the way: qkv [plan.tokens, heads + 2 kv_heads,
+ * head_dim] fp16, queries first, then keys, then values.  Queries and keys are rotated,
+ *   y[d] = x[d] cos[d] - x[d + head_dim / 2] sin[d]  (d < head_dim / 2),   y[d] = x[d] cos[d] + x[d - head_dim / 2] sin[d]  (d beyond),
+ * queries go to q [plan.tokens, heads, head_dim], keys and values into their pages.
+ *   cos, sin [plan.tokens, head_dim]: fp16 (each product and the sum rounded to fp16, as kvmix_rope_append does) or fp32 (one
+ *   rounding at the end).  Strides in elements, tokens' ones of the tables may be 0; all in whole pieces of 16 bytes, which the
+ *   pointers are aligned to, and unit stride along head_dim.
+ */
+typedef struct kvmix_paged_rope {
+    const void *qkv;
+    int64_t qkv_token_stride, qkv_head_stride;
+    const void *cos, *sin;
+    int64_t cos_token_stride, sin_token_stride;
+    int table_dtype;  /* KVMIX_F16 or KVMIX_F32 */
+    void *q;
+    int64_t q_token_stride, q_head_stride;
+} kvmix_paged_rope_t;
+int kvmix_paged_rope_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t *plan, const int32_t *list, const kvmix_paged_rope_t *call,
+                            kvmix_stream_t stream);
+
+/*
  * Attention of a batch's new tokens over its pages:  out[i, h] = sum_{j <= pos(i)} softmax_j(scale q[i, h] . k[j, h']) v[j, h'],
  * h' = h / (heads / kv_heads), over the tokens of i's own sequence up to itself (the new tokens' keys and values are in their
  * pages already).  Packed values are taken as fp16 (code * scale + minimum, rounded once); packed keys as well where a sequence's new

@@ -48,6 +48,7 @@ EXPORTS = (
     "kvmix_grow",
     "kvmix_probe_stream_read",
     "kvmix_paged_append",
+    "kvmix_paged_rope_append",
     "kvmix_paged_quantize",
     "kvmix_paged_read",
     "kvmix_paged_copy",

@@ -49,6 +49,7 @@ struct Api {
     decltype(&kvmix_grow) grow;
     decltype(&kvmix_linear_rows) linear_rows;
     decltype(&kvmix_paged_append) paged_append;
+    decltype(&kvmix_paged_rope_append) paged_rope_append;
     decltype(&kvmix_paged_quantize) paged_quantize;
     decltype(&kvmix_paged_read) paged_read;
     decltype(&kvmix_paged_copy) paged_copy;
@@ -81,6 +82,7 @@ void bind(const std::unordered_map<std::string, uintptr_t> &at)
     KVMIX_BIND(grow);
     KVMIX_BIND(linear_rows);
     KVMIX_BIND(paged_append);
+    KVMIX_BIND(paged_rope_append);
     KVMIX_BIND(paged_quantize);
     KVMIX_BIND(paged_read);
     KVMIX_BIND(paged_copy);
@@ -813,6 +815,7 @@ PYBIND11_MODULE(_host, m)
         .def_property_readonly("launches", [](const PagedPlan &p) { return std::make_tuple(p.c.few_columns, p.c.tiles, p.c.joins); });
     m.def("paged_plan", &paged_plan, NoGil());
     m.def("paged_append", &paged_append, NoGil());
+    m.def("paged_rope_append", &paged_rope_append, NoGil());
     m.def("paged_quantize", &paged_quantize, NoGil());
     m.def("paged_read", &paged_read, NoGil());
     m.def("paged_copy", &paged_copy, NoGil());

@@ -132,6 +132,43 @@ void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &rows, co
                            stride_of(v, 1), stream_of(rows)));
 }
 
+// [tokens, head_dim], or one row [head_dim] for all: as 16-byte pieces can be read from it
+Tensor table_pieces(const Tensor &t_in, int64_t tokens, int64_t head_dim)
+{
+    if (t_in.scalar_type() != at::kHalf && t_in.scalar_type() != at::kFloat)
+        fail("paged_rope_append: cos and sin must be float16 or float32, got " + dtype_name(t_in));
+    if (t_in.dim() < 1 || t_in.dim() > 2 || t_in.size(-1) != head_dim || (t_in.dim() == 2 && t_in.size(0) != 1 && t_in.size(0) != tokens))
+        fail("paged_rope_append: cos and sin must be [the plan's new tokens, head_dim], or one row for all of them");
+    const Tensor t = t_in.dim() == 1 ? t_in.unsqueeze(0) : t_in;
+    const bool ok = t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) * t.element_size() % 16 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor paged_rope_append(const Tensor &qkv_in, const Tensor &cos_in, const Tensor &sin_in, const Tensor &rows, const PagedPlan &plan)
+{
+    need_no_record("paged_rope_append", {&qkv_in, &cos_in, &sin_in, &rows});
+    kvmix_paged_pool_t p{};
+    use_rows(p, rows);
+    need_half({&qkv_in});
+    need_with(rows, {&qkv_in, &cos_in, &sin_in, &plan.list});
+    if (qkv_in.dim() != 3 || qkv_in.size(0) != plan.c.tokens || qkv_in.size(1) != plan.c.heads + 2 * plan.c.kv_heads || qkv_in.size(2) != plan.c.head_dim)
+        fail("paged_rope_append: the projection must be [the plan's new tokens, heads + 2 kv_heads, head_dim]");
+    if (plan.c.kv_heads != p.kv_heads || plan.c.page_size != p.page_size || plan.c.head_dim != p.head_dim)
+        fail("paged_rope_append: the plan is for pages of another shape");
+    if (cos_in.scalar_type() != sin_in.scalar_type()) fail("paged_rope_append: cos and sin must be of one type");
+    if (plan.c.row_pages > p.row_pages) check(KVMIX_ERR_PAGE);
+    const Tensor qkv = pieces3(qkv_in), cos = table_pieces(cos_in, plan.c.tokens, p.head_dim), sin = table_pieces(sin_in, plan.c.tokens, p.head_dim);
+    Tensor q = at::empty({plan.c.tokens, plan.c.heads, p.head_dim}, qkv.options());
+    kvmix_paged_rope_t c{};
+    c.qkv = qkv.data_ptr(), c.qkv_token_stride = stride_of(qkv, 0), c.qkv_head_stride = stride_of(qkv, 1);
+    c.cos = cos.data_ptr(), c.cos_token_stride = stride_of(cos, 0), c.sin = sin.data_ptr(), c.sin_token_stride = stride_of(sin, 0);
+    c.table_dtype = dtype_tag(cos);
+    c.q = q.data_ptr(), c.q_token_stride = q.stride(0), c.q_head_stride = q.stride(1);
+    const c10::DeviceGuard guard(rows.device());
+    check(api.paged_rope_append(&p, &plan.c, plan.words(), &c, stream_of(rows)));
+    return q;
+}
+
 void paged_quantize(const Tensor &rows, const Tensor &packed, const Tensor &pairs_in, int64_t k_bits, int64_t v_bits)
 {
     need_no_record("paged_quantize", {&rows});

@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "paged_common.h"
+#include "rope.h"
 
 namespace kvmix {
 
@@ -30,6 +31,29 @@ struct AppendArgs {
     PlanWords blocks;
     int heads, units, page_log2;  // units: blocks of tokens by heads
 };
+
+// A wave's values of one block of a page from the LDS, where it has put them token by token: eight tokens of a channel as one piece, or
+// the new ones of them.
+template <int D>
+__device__ __forceinline__ void write_turned(const _Float16 (*turned)[D + 2], _Float16 *values, int place, int n, int lane)
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int first = place / 8, last = (place + n - 1) / 8;
+    for (int i = lane; i < D * 4; i += kWave) {
+        const int d = i / 4, g = i % 4;
+        if (g < first || g > last) continue;
+        if (8 * g >= place && 8 * g + 8 <= place + n) {
+            half8v w;
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = turned[8 * g + j][d];
+            *(half8v *)(values + d * kBlock + 8 * g) = w;
+        } else {
+            for (int t = max(8 * g, place); t < min(8 * g + 8, place + n); t++) values[d * kBlock + t] = turned[t][d];
+        }
+    }
+}
 
 template <int D>
 __global__ void __launch_bounds__(256) paged_append(AppendArgs a)
@@ -65,23 +89,136 @@ __global__ void __launch_bounds__(256) paged_append(AppendArgs a)
             for (int j = 0; j < 4; j++) *(half2v *)&turned[wave][place + t][8 * c + 2 * j] = half2v{value[i][2 * j], value[i][2 * j + 1]};
         }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    // eight tokens of one channel: as one piece, or the new ones of them
-    const int first = place / 8, last = (place + n - 1) / 8;
-    for (int i = lane; i < D * 4; i += kWave) {
-        const int d = i / 4, g = i % 4;
-        if (g < first || g > last) continue;
-        if (8 * g >= place && 8 * g + 8 <= place + n) {
-            half8v w;
+    write_turned<D>(turned[wave], values, place, n, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// rotated append: the fused projection of the new tokens, [tokens][heads + 2 kv_heads][D].  The first blocks of the launch rotate
+// queries (to a tensor of their own) and keys (to their pages), the last ones turn the values round as in paged_append.
+// With u = x[d], w = x[d + D / 2]:  u cos_d - w sin_d  and  w cos_d' + u sin_d', d' = d + D / 2.
+// Bound by memory.  A wave takes one token: its lanes are the pairs of pieces of several heads (eight of 128 channels), a turn of the
+// loop as many heads again, so that a lane reads its four pieces of the tables once for all turns, and a turn's reads are 2 KB that follow
+// one another.  Where there are few tokens a wave takes one turn only: latency is what counts, and the chip is not full.
+
+template <typename T>
+struct TablePieces {  // eight channels of the first half, eight of the second
+    float c1[8], c2[8], s1[8], s2[8];
+};
+
+template <>
+struct TablePieces<_Float16> {
+    half8v c1, c2, s1, s2;
+};
+
+__device__ __forceinline__ void load_table(half8v &to, const _Float16 *at) { to = *(const half8v *)at; }
+
+__device__ __forceinline__ void load_table(float (&to)[8], const float *at)
+{
+    const floatx4 a = *(const floatx4 *)at, b = *(const floatx4 *)(at + 4);
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = turned[wave][8 * g + j][d];
-            *(half8v *)(values + d * kBlock + 8 * g) = w;
-        } else {
-            for (int t = max(8 * g, place); t < min(8 * g + 8, place + n); t++) values[d * kBlock + t] = turned[wave][t][d];
+    for (int j = 0; j < 4; j++) to[j] = a[j], to[4 + j] = b[j];
+}
+
+// fp16 tables: as the fp16 tensor expression rounds, each product and the sum (kvmix_rope_append does the same).  fp32 tables: one
+// rounding at the end.
+__device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TablePieces<_Float16> &t)
+{
+    typedef uint16_t bits8 __attribute__((ext_vector_type(8)));
+    const bits8 x = __builtin_bit_cast(bits8, u), y = __builtin_bit_cast(bits8, w);
+    const bits8 c1 = __builtin_bit_cast(bits8, t.c1), c2 = __builtin_bit_cast(bits8, t.c2), s1 = __builtin_bit_cast(bits8, t.s1), s2 = __builtin_bit_cast(bits8, t.s2);
+    bits8 a, b;
+#pragma unroll
+    for (int j = 0; j < 8; j++) a[j] = rope_one(x[j], y[j], c1[j], s1[j], true), b[j] = rope_one(y[j], x[j], c2[j], s2[j], false);
+    u = __builtin_bit_cast(half8v, a), w = __builtin_bit_cast(half8v, b);
+}
+
+__device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TablePieces<float> &t)
+{
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float x = (float)u[j], y = (float)w[j];
+        u[j] = (_Float16)fmaf(x, t.c1[j], -(y * t.s1[j]));
+        w[j] = (_Float16)fmaf(y, t.c2[j], x * t.s2[j]);
+    }
+}
+
+struct RopeStoreArgs {
+    const _Float16 *qkv;
+    int64_t x_ts, x_hs;
+    const void *cos, *sin;
+    int64_t cos_ts, sin_ts;
+    _Float16 *q;
+    int64_t q_ts, q_hs;
+    _Float16 *rows;
+    PlanWords slots, blocks;
+    int tokens, heads, kv_heads, units, page_log2;  // units: blocks of tokens by kv heads
+    int parts, rotating;                            // waves to a token; blocks of the launch that rotate
+};
+
+// TURNS: turns of a wave at most.
+template <int D, typename T, int TURNS>
+__global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
+{
+    constexpr int C = D / 8, HALF = C / 2;
+    constexpr int kTurns = kBlock * C / kWave;
+    __shared__ _Float16 turned[4][kBlock][D + 2];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if ((int)blockIdx.x < a.rotating) {
+        const int nth = blockIdx.x * 4 + wave, token = nth / a.parts, part = nth % a.parts;
+        if (token >= a.tokens) return;
+        const int slot = a.slots[token], at = 8 * (lane % HALF), total = a.heads + a.kv_heads;
+        const T *cos = (const T *)a.cos + token * a.cos_ts + at, *sin = (const T *)a.sin + token * a.sin_ts + at;
+        const _Float16 *x = a.qkv + token * a.x_ts + at;
+        const int first = part * TURNS * (kWave / HALF) + lane / HALF;
+        half8v u[TURNS], w[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+            const int head = first + i * (kWave / HALF);
+            if (head < total) {
+                u[i] = *(const half8v *)(x + head * a.x_hs);
+                w[i] = *(const half8v *)(x + head * a.x_hs + D / 2);
+            }
+        }
+        TablePieces<T> t;
+        load_table(t.c1, cos), load_table(t.c2, cos + D / 2), load_table(t.s1, sin), load_table(t.s2, sin + D / 2);
+        _Float16 *q = a.q + token * a.q_ts + at;
+        const int page = slot >> a.page_log2, place = slot & ((1 << a.page_log2) - 1);
+        _Float16 *keys = a.rows + ((((int64_t)page * a.kv_heads) * 2) << a.page_log2) * D + (int64_t)place * D + at;
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+            const int head = first + i * (kWave / HALF);
+            if (head < total) {
+                rotate_pieces(u[i], w[i], t);
+                _Float16 *to = head < a.heads ? q + head * a.q_hs : keys + (((int64_t)(head - a.heads) * 2) << a.page_log2) * D;
+                *(half8v *)to = u[i];
+                *(half8v *)(to + D / 2) = w[i];
+            }
+        }
+        return;
+    }
+    const int unit = (blockIdx.x - a.rotating) * 4 + wave;
+    if (unit >= a.units) return;
+    const int head = unit % a.kv_heads;
+    const PlanWords p = a.blocks + unit / a.kv_heads * kStoreWords;
+    const int64_t token = p[0];
+    const int slot = p[1], n = p[2], place = slot & (kBlock - 1), page = slot >> a.page_log2, in_page = (slot & ((1 << a.page_log2) - 1)) - place;
+    _Float16 *values = a.rows + (((((int64_t)page * a.kv_heads + head) * 2) + 1) << a.page_log2) * D + (int64_t)in_page * D;
+    const _Float16 *v = a.qkv + token * a.x_ts + (a.heads + a.kv_heads + head) * a.x_hs;
+    half8v value[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; i++) {
+        const int t = (i * kWave + lane) / C, c = (i * kWave + lane) % C;
+        if (t < n) value[i] = *(const half8v *)(v + t * a.x_ts + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < kTurns; i++) {
+        const int t = (i * kWave + lane) / C, c = (i * kWave + lane) % C;
+        if (t < n) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) *(half2v *)&turned[wave][place + t][8 * c + 2 * j] = half2v{value[i][2 * j], value[i][2 * j + 1]};
         }
     }
+    write_turned<D>(turned[wave], values, place, n, lane);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -419,6 +556,44 @@ extern "C" int kvmix_paged_append(const kvmix_paged_pool_t *p, const kvmix_paged
                           __builtin_ctzll((uint64_t)p->page_size)};
     const unsigned grid = (unsigned)((plan->stores * p->kv_heads + 3) / 4);
     with_dim(p->head_dim, [&](auto D) { paged_append<D.value><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    return launch_status();
+}
+
+extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_paged_plan_t *plan, const int32_t *list, const kvmix_paged_rope_t *c,
+                                       kvmix_stream_t stream)
+{
+    const int rc = pool_check(p);
+    if (rc != KVMIX_OK) return rc;
+    if (!plan || !c) return KVMIX_ERR_NULL;
+    if (plan->page_size != p->page_size || plan->kv_heads != p->kv_heads || plan->head_dim != p->head_dim) return KVMIX_ERR_SHAPE;
+    if (plan->row_pages > p->row_pages) return KVMIX_ERR_PAGE;
+    if (c->table_dtype != KVMIX_F16 && c->table_dtype != KVMIX_F32) return KVMIX_ERR_DTYPE;
+    const int64_t per = c->table_dtype == KVMIX_F16 ? 8 : 4;
+    if (c->qkv_token_stride % 8 || c->qkv_head_stride % 8 || c->q_token_stride % 8 || c->q_head_stride % 8 || c->cos_token_stride % per ||
+        c->sin_token_stride % per || ((uintptr_t)c->qkv | (uintptr_t)c->cos | (uintptr_t)c->sin | (uintptr_t)c->q) % 16)
+        return KVMIX_ERR_UNSUPPORTED;
+    if (plan->tokens == 0) return KVMIX_OK;
+    if (!c->qkv || !c->cos || !c->sin || !c->q || !list || !p->rows) return KVMIX_ERR_NULL;
+    // Four turns to a wave once that leaves every CU two waves for each of its SIMDs.
+    const int64_t turns = ((plan->heads + p->kv_heads) * (p->head_dim / 16) + kWave - 1) / kWave;
+    const bool many = plan->tokens * ((turns + 3) / 4) >= 2048;
+    const int64_t parts = many ? (turns + 3) / 4 : turns;
+    const __int128 rotating = ((__int128)plan->tokens * parts + 3) / 4, turning = ((__int128)plan->stores * p->kv_heads + 3) / 4;
+    if (rotating + turning > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
+    const RopeStoreArgs a = {(const _Float16 *)c->qkv, c->qkv_token_stride, c->qkv_head_stride, c->cos, c->sin, c->cos_token_stride, c->sin_token_stride,
+                             (_Float16 *)c->q, c->q_token_stride, c->q_head_stride, (_Float16 *)p->rows, (PlanWords)list + plan->slots_at,
+                             (PlanWords)list + plan->store_at, (int)plan->tokens, (int)plan->heads, (int)p->kv_heads, (int)(plan->stores * p->kv_heads),
+                             __builtin_ctzll((uint64_t)p->page_size), (int)parts, (int)rotating};
+    const unsigned grid = (unsigned)(rotating + turning);
+    with_dim(p->head_dim, [&](auto D) {
+        if (c->table_dtype == KVMIX_F16) {
+            if (many) paged_rope_append<D.value, _Float16, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+            else paged_rope_append<D.value, _Float16, 1><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        } else {
+            if (many) paged_rope_append<D.value, float, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+            else paged_rope_append<D.value, float, 1><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        }
+    });
     return launch_status();
 }
 

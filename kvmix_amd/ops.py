@@ -495,6 +495,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, plan) -> 
     _host().paged_append(k, v, rows, plan)
 
 
+def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rows: torch.Tensor, plan) -> torch.Tensor:
+    """The projection qkv [plan.tokens, heads + 2 kv_heads, head_dim] fp16 of a step's new tokens: its queries and keys rotated
+    (x * cos + rotate_half(x) * sin), keys and values into the fp16 pages as paged_append does, in one launch; returns the rotated
+    queries [plan.tokens, heads, head_dim].  cos, sin [plan.tokens, head_dim], or one row for all: fp16 tables give what the fp16
+    tensor expression gives, bit for bit; fp32 ones are rounded once, at the end."""
+    return _host().paged_rope_append(qkv, cos, sin, rows, plan)
+
+
 def paged_quantize(rows: torch.Tensor, packed: torch.Tensor, pairs: torch.Tensor, k_bits: int, v_bits: int) -> None:
     """fp16 pages to packed pages: pairs [n, 2] in host memory = (page of `rows`, page of `packed`); packed int32 [pages,
     kv_heads, page_size / 32 * head_dim * (k_bits + v_bits + 2)].  Keys in groups of 32 tokens per channel, values in groups of 32

@@ -12,7 +12,7 @@ another, as is every full fp16 page: the first of them that packs such a page do
     a = cache.new()
     step = cache.step({a: 700})                       # room for 700 new tokens of `a`; pages that left the window are packed
     for layer in range(layers):
-        cache.append(layer, step, k, v)               # k, v [700, kv_heads, head_dim]
+        cache.append(layer, step, k, v)               # k, v [700, kv_heads, head_dim] (or append_rotated, from the projection)
         out = cache.attend(layer, step, q)            # q [700, heads, head_dim]
     b = cache.fork(a)                                 # shares a's pages, but for the one that is being written
     cache.free(a)
@@ -293,6 +293,11 @@ class PagedKVCache:
     def append(self, layer: int, step: Step, k: torch.Tensor, v: torch.Tensor) -> None:
         """The new tokens' keys and values [tokens, kv_heads, head_dim], sequence after sequence."""
         ops.paged_append(k, v, self.rows[layer], self._plan(step))
+
+    def append_rotated(self, layer: int, step: Step, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        """The same from the new tokens' projection [tokens, heads + 2 kv_heads, head_dim], queries and keys rotated on the way with the
+        tables [tokens, head_dim]; returns the queries (ops.paged_rope_append)."""
+        return ops.paged_rope_append(qkv, cos, sin, self.rows[layer], self._plan(step))
 
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float = None) -> torch.Tensor:
         """Attention of the new tokens' queries [tokens, heads, head_dim] over their sequences, themselves included."""

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from .decoder import DecoderConfig, add_mlp, add_projection, apply_rope, head_logits, rms_norm, rope_tables
+from .decoder import DecoderConfig, add_mlp, add_projection, head_logits, rms_norm, rope_tables
 from .paged import PagedKVCache
 
 
@@ -54,13 +54,12 @@ class PagedDecoder:
         ids = torch.cat([ids.to(device) for ids in new_ids.values()])
         pos = torch.cat([torch.arange(before[s], before[s] + i.numel(), device=device) for s, i in new_ids.items()])
         x = self.w["embed"][ids][:, None]                       # [tokens, 1, hidden]: rows, as the projections' kernels take them
-        cos, sin = (t[0, 0][:, None] for t in rope_tables(cfg, pos, x.dtype))
+        cos, sin = (t[0, 0] for t in rope_tables(cfg, pos, x.dtype))
         nh, nkv = cfg.num_heads, cfg.num_kv_heads
         for layer, lw in enumerate(self.w["layers"]):
             qkv = F.linear(rms_norm(x, lw["input_norm"], cfg.rms_norm_eps), lw["wqkv"]).view(-1, nh + 2 * nkv, cfg.head_dim)
-            qk = apply_rope(qkv[:, :nh + nkv], cos, sin)
-            cache.append(layer, step, qk[:, nh:], qkv[:, nh + nkv:])
-            out = cache.attend(layer, step, qk[:, :nh])
+            q = cache.append_rotated(layer, step, qkv, cos, sin)
+            out = cache.attend(layer, step, q)
             x = add_projection(x, out.reshape(-1, 1, cfg.hidden_size), lw["wo"])
             x = add_mlp(x, lw, cfg.rms_norm_eps)
         spans = step.tokens()
