@@ -51,10 +51,11 @@ extern "C" {
 #define KVMIX_ERR_PAGE_ORDER (-16) /* kvmix_paged_copy: a page written twice, or written and read */
 #define KVMIX_ERR_LENGTHS (-17)    /* kvmix_paged_plan: lengths that do not fit one another or the table */
 #define KVMIX_ERR_MEMORY (-18)     /* host memory could not be had */
+#define KVMIX_ERR_ADAPTER (-19)    /* an adapter's number outside its pool */
 
 #define KVMIX_F16 0
 #define KVMIX_F32 1
-#define KVMIX_BF16 2 /* kvmix_token_logprobs only */
+#define KVMIX_BF16 2 /* where a call says so */
 
 #define KVMIX_FMT_REF 0
 #define KVMIX_FMT_DENSE3 1
@@ -659,6 +660,42 @@ int64_t kvmix_token_logprobs_workspace_bytes(const kvmix_token_logprobs_t *p);
 int kvmix_token_logprobs(const kvmix_token_logprobs_t *p, void *workspace, int64_t workspace_bytes, kvmix_stream_t stream);
 int kvmix_token_logprobs_grad(const kvmix_token_logprobs_t *p, const float *grad_logprob, const float *grad_entropy, void *grad_logits,
                               int64_t grad_row_stride, kvmix_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a projection that they share (no counterpart in the reference):
+ *   out[t] = base[t] + scales[i] B_i (A_i x[t])   for token t of a sequence with adapter i,   out[t] = base[t] where it has none.
+ * The plan of a step, made on the host and used by every projection of the step: adapters [sequences], each below n_adapters, negative
+ * for none; counts [sequences]: tokens of each, sequence after sequence.  Made in two calls, as kvmix_paged_plan.
+ */
+typedef struct kvmix_adapter_plan {
+    int64_t words;        /* 32-bit words of the list */
+    int64_t tokens;       /* of all sequences */
+    int64_t adapters;     /* that the pool must have at least */
+    int64_t rows;         /* tokens with an adapter */
+    int64_t tiles, bare;  /* pieces of work: tokens of one adapter, tokens without one */
+    int64_t most;         /* tokens of a piece at most */
+    int64_t rows_at;      /* where the list of tokens begins */
+} kvmix_adapter_plan_t;
+int kvmix_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t sequences, int64_t n_adapters, int32_t *words, int64_t capacity,
+                       kvmix_adapter_plan_t *plan);
+
+/*
+ * x [tokens, k], a [adapters, rank, k], b [adapters, n, rank], base, out [tokens, n]: fp16 or bf16 (KVMIX_BF16), unit stride along
+ * the last dimension, sizes and strides in whole eights, 16-byte aligned; k and n up to 2^24, rank up to 128.  scales [adapters] fp32,
+ * or NULL for 1.  out may be base (the tokens without an adapter are left alone then), but not overlap it otherwise.  Sums in fp32; u = A x
+ * is held to 2^-22 (bf16: 2^-16) of the token's largest for the second product; out is rounded once.
+ */
+typedef struct kvmix_adapters {
+    const void *x, *a, *b, *base;
+    void *out;
+    int64_t x_token_stride, a_adapter_stride, a_rank_stride, b_adapter_stride, b_row_stride, base_token_stride, out_token_stride;
+    const float *scales;
+    int64_t adapters, rank, k, n;
+    int dtype;
+} kvmix_adapters_t;
+int64_t kvmix_add_adapters_workspace_bytes(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *call);
+int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_t *list, const kvmix_adapters_t *call, void *workspace, int64_t workspace_bytes,
+                       kvmix_stream_t stream);
 
 /*
  * Measurement support, no counterpart in the reference and not called by any operator: a kernel

@@ -55,6 +55,9 @@ EXPORTS = (
     "kvmix_paged_plan",
     "kvmix_paged_attention_workspace_bytes",
     "kvmix_paged_attention",
+    "kvmix_adapter_plan",
+    "kvmix_add_adapters_workspace_bytes",
+    "kvmix_add_adapters",
     "kvmix_token_logprobs_workspace_bytes",
     "kvmix_token_logprobs",
     "kvmix_token_logprobs_grad",
@@ -155,6 +158,20 @@ class PagedPlan(ctypes.Structure):
         "join_blocks", "few_tokens")]
 
 
+class AdapterPlan(ctypes.Structure):
+    """kvmix_adapter_plan_t"""
+    _fields_ = [(name, ctypes.c_int64) for name in ("words", "tokens", "adapters", "rows", "tiles", "bare", "most", "rows_at")]
+
+
+class Adapters(ctypes.Structure):
+    """kvmix_adapters_t"""
+    _i64, _vp = ctypes.c_int64, ctypes.c_void_p
+    _fields_ = [("x", _vp), ("a", _vp), ("b", _vp), ("base", _vp), ("out", _vp),
+                ("x_token_stride", _i64), ("a_adapter_stride", _i64), ("a_rank_stride", _i64), ("b_adapter_stride", _i64),
+                ("b_row_stride", _i64), ("base_token_stride", _i64), ("out_token_stride", _i64), ("scales", _vp),
+                ("adapters", _i64), ("rank", _i64), ("k", _i64), ("n", _i64), ("dtype", ctypes.c_int)]
+
+
 LINEAR_PLAIN, LINEAR_FLOAT, LINEAR_RESIDUAL, LINEAR_SWIGLU, LINEAR_ROPE_APPEND = range(5)
 
 
@@ -247,6 +264,12 @@ def load() -> ctypes.CDLL:
     L.kvmix_grow.argtypes = [vp, i32, ctypes.POINTER(KeyFlush), ctypes.POINTER(ValueFlush), vp]
     L.kvmix_paged_plan.restype = i32
     L.kvmix_paged_plan.argtypes = [ctypes.POINTER(PagedBatch), vp, i64, ctypes.POINTER(PagedPlan)]
+    L.kvmix_adapter_plan.restype = i32
+    L.kvmix_adapter_plan.argtypes = [vp, vp, i64, i64, vp, i64, ctypes.POINTER(AdapterPlan)]
+    L.kvmix_add_adapters_workspace_bytes.restype = i64
+    L.kvmix_add_adapters_workspace_bytes.argtypes = [ctypes.POINTER(AdapterPlan), ctypes.POINTER(Adapters)]
+    L.kvmix_add_adapters.restype = i32
+    L.kvmix_add_adapters.argtypes = [ctypes.POINTER(AdapterPlan), vp, ctypes.POINTER(Adapters), vp, i64, vp]
     L.kvmix_probe_stream_read.restype = i32
     L.kvmix_probe_stream_read.argtypes = [vp, i32, i64, i64, i32, i32, i32, i32, i32, vp, vp]
     _lib = L
@@ -334,6 +357,17 @@ def paged_plan(table, kv_lens, packed_lens, q_lens, heads: int, kv_heads: int, h
     words = (ctypes.c_int32 * max(plan.words, 1))()
     check(load().kvmix_paged_plan(ctypes.byref(batch), words, plan.words, ctypes.byref(plan)))
     return {name: getattr(plan, name) for name, _ in PagedPlan._fields_}, list(words)
+
+
+def adapter_plan(adapters, counts, n_adapters: int):
+    """kvmix_adapter_plan: (the plan's fields as a dict, its words as a list of int).  Needs no GPU."""
+    n = len(adapters)
+    ids, many = ((ctypes.c_int64 * max(n, 1))(*x) for x in (adapters, counts))
+    plan = AdapterPlan()
+    check(load().kvmix_adapter_plan(ids, many, n, n_adapters, None, 0, ctypes.byref(plan)))
+    words = (ctypes.c_int32 * max(plan.words, 1))()
+    check(load().kvmix_adapter_plan(ids, many, n, n_adapters, words, plan.words, ctypes.byref(plan)))
+    return {name: getattr(plan, name) for name, _ in AdapterPlan._fields_}, list(words)[:plan.words]
 
 
 def flush_batch(keys, values, stream) -> int:

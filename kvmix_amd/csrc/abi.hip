@@ -34,6 +34,7 @@ extern "C" const char *kvmix_strerror(int code)
         return "lengths of a sequence do not fit: 0 <= new tokens <= tokens, 0 <= packed tokens <= tokens in whole pages, new tokens "
                "not packed, pages for all tokens in the table";
     case KVMIX_ERR_MEMORY: return "host memory could not be had";
+    case KVMIX_ERR_ADAPTER: return "an adapter's number lies outside the pool of adapters";
     default: return "unknown kvmix error";
     }
 }

@@ -1,0 +1,364 @@
+// Low-rank adapters of many requests beside a projection that they share:  y_t = base_t + s_i B_i (A_i x_t), i the adapter of token t.
+//
+// Bound by memory: the weights of the adapters in use and the activations are read once, two operations for a value of them and rank.
+// Two launches, because every value of y wants all of x:
+//   shrink   u = A x.  A tile is up to 64 tokens of one adapter (kvmix_adapter_plan deals them out, whichever sequences they are of), a
+//            block a tile and a stretch of k, its four waves a quarter of that each.  Ranks are the rows of v_mfma_f32_16x16x32, tokens
+//            its columns, so that a lane has eight k of one row of A and of one token: sixteen bytes, as both lie in memory.  The
+//            waves' sums come together in the LDS, those of the stretches (there are several where there are few tiles) in
+//   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then its waves take 32 columns of y at a time.  u is
+//            kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest to
+//            2^13: next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be off by
+//            2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
+//            columns of one token that follow one another.
+// Sums in fp32; y is rounded once.
+#include <algorithm>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "kvmix_common.h"
+
+namespace kvmix {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) int32_t *PlanWords;
+
+constexpr int kTile = 64, kSub = 16;       // tokens of a tile, of a column of a matrix product
+constexpr int kTileWords = 4;              // adapter or -1, first of the list, how many, one of no use
+constexpr int kWaves = 4;
+constexpr int64_t kMostRank = 128;
+
+template <typename T>
+struct Vec8 {
+    typedef T type __attribute__((ext_vector_type(8)));
+};
+
+__device__ __forceinline__ floatx4 product(Vec8<_Float16>::type a, Vec8<_Float16>::type b, floatx4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ floatx4 product(Vec8<__bf16>::type a, Vec8<__bf16>::type b, floatx4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+struct AdapterArgs {
+    const void *x, *a, *b, *base;
+    void *out;
+    int64_t x_ts, a_as, a_rs, b_as, b_ns, base_ts, out_ts;
+    const float *scales;    // may be NULL: 1
+    float *part;            // [splits][adapted tokens][padded rank]
+    PlanWords tiles, rows;  // tiles; their tokens
+    int64_t part_rows;
+    int rank, padded, k, n, splits, rank_chunks, n_blocks, units;  // units: of 32 columns, of a wave of expand
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+// Ranks [first, first + 16 RT) of a tile of up to 16 ST tokens, over the 32-wide units [from, to) of k.
+template <typename T, int RT, int ST>
+__device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *const (&x)[ST], int from, int to, int k, int g, floatx4 (&acc)[RT][ST])
+{
+    typedef typename Vec8<T>::type V;
+    constexpr int UN = RT * ST >= 8 ? 2 : 4;  // units whose reads are in flight together
+    const int whole = min(to, k / 32);
+    int u = from;
+    for (; u + UN <= whole; u += UN) {
+        V av[UN][RT], xv[UN][ST];
+#pragma unroll
+        for (int i = 0; i < UN; i++) {
+#pragma unroll
+            for (int r = 0; r < RT; r++) av[i][r] = *(const V *)(a[r] + 32 * (u + i));
+#pragma unroll
+            for (int s = 0; s < ST; s++) xv[i][s] = *(const V *)(x[s] + 32 * (u + i));
+        }
+#pragma unroll
+        for (int i = 0; i < UN; i++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int s = 0; s < ST; s++) acc[r][s] = product(av[i][r], xv[i][s], acc[r][s]);
+    }
+    for (; u < to; u++) {
+        V av[RT], xv[ST];
+        const bool in = 32 * u + 8 * g < k;  // (k in whole eights)
+#pragma unroll
+        for (int r = 0; r < RT; r++) av[r] = in ? *(const V *)(a[r] + 32 * u) : V{};
+#pragma unroll
+        for (int s = 0; s < ST; s++) xv[s] = in ? *(const V *)(x[s] + 32 * u) : V{};
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int s = 0; s < ST; s++) acc[r][s] = product(av[r], xv[s], acc[r][s]);
+    }
+}
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
+{
+    constexpr int LD = RT * 16, Q = RT * 4;
+    extern __shared__ float sums[];  // [waves][tokens][ranks]; the fours of ranks of token t in an order of its own, so that lanes meet in no bank
+    auto place = [](int row, int t, int four) { return row * LD + 4 * (four ^ t % Q); };
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
+    const int split = blockIdx.x % p.splits, nth = blockIdx.x / p.splits, chunk = nth % p.rank_chunks;
+    const PlanWords tile = p.tiles + nth / p.rank_chunks * kTileWords;
+    const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
+    const int units = (p.k + 31) / 32, begin = (int)((int64_t)units * split / p.splits), length = (int)((int64_t)units * (split + 1) / p.splits) - begin;
+    const int from = begin + length * wave / kWaves, to = begin + length * (wave + 1) / kWaves;
+    const T *a[RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) a[r] = (const T *)p.a + adapter * p.a_as + min((chunk * RT + r) * 16 + m, p.rank - 1) * p.a_rs + 8 * g;  // (what lies beyond is not kept)
+    auto run = [&](auto st) {
+        constexpr int ST = decltype(st)::value;
+        const T *x[ST];
+#pragma unroll
+        for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + (int64_t)p.rows[first + min(kSub * s + m, count - 1)] * p.x_ts + 8 * g;
+        floatx4 acc[RT][ST] = {};
+        shrink_tile<T, RT, ST>(a, x, from, to, p.k, g, acc);
+#pragma unroll
+        for (int s = 0; s < ST; s++)
+            if (s < subs)
+#pragma unroll
+                for (int r = 0; r < RT; r++) *(floatx4 *)(sums + place((wave * subs + s) * kSub + m, m, 4 * r + g)) = acc[r][s];
+    };
+    if (subs == 1) run(std::integral_constant<int, 1>());
+    else if (subs == 2) run(std::integral_constant<int, 2>());
+    else run(std::integral_constant<int, 4>());
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * Q; i += 256) {
+        const int t = i / Q, c = i % Q, rank = (chunk * Q + c) * 4;
+        floatx4 s = *(const floatx4 *)(sums + place(t, t % kSub, c));
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) s += *(const floatx4 *)(sums + place(w * subs * kSub + t, t % kSub, c));
+        if (rank < p.padded) *(floatx4 *)(p.part + (split * p.part_rows + first + t) * p.padded + rank) = s;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+// RX: the rank, rounded up to 16, 32, 64 or 128.
+template <typename T, int RX>
+__global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
+{
+    typedef typename Vec8<T>::type V;
+    constexpr int NF = RX >= 32 ? RX / 32 : 1, LD = 2 * RX + 8, L = RX / 4;  // pieces of a row of B; of u: its two parts; lanes to a token
+    __shared__ alignas(16) T u[kTile][LD];
+    __shared__ float power[kTile];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
+    const PlanWords tile = p.tiles + blockIdx.x / p.n_blocks * kTileWords;
+    const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
+    const int begin = (blockIdx.x % p.n_blocks * kWaves + wave) * p.units, end = min(begin + p.units, (p.n + 31) / 32);
+    if (adapter < 0) {  // (tokens without one: to be copied)
+        for (int i = begin; i < end; i++) {
+            const int column = 32 * i + 8 * g;
+            for (int t = m; t < count && column < p.n; t += 16) {
+                const int64_t row = p.rows[first + t];
+                *(V *)((T *)p.out + row * p.out_ts + column) = *(const V *)((const T *)p.base + row * p.base_ts + column);
+            }
+        }
+        return;
+    }
+    const int c = threadIdx.x % L;
+    for (int t = threadIdx.x / L; t < subs * kSub; t += 256 / L) {
+        floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (t < count && 4 * c < p.rank) {
+            const float *at = p.part + (int64_t)(first + t) * p.padded + 4 * c;
+            for (int i = 0; i < p.splits; i++) s += *(const floatx4 *)(at + i * p.part_rows * p.padded);
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(s[j]) < __builtin_inff() ? fabsf(s[j]) : 0.0f);
+#pragma unroll
+        for (int o = L / 2; o; o /= 2) most = fmaxf(most, __shfl_xor(most, o));
+        // (the power of numbers below 2^-100 is that of 2^-100; infinities go through as they are, and their second part is nothing)
+        const int e = (most > 0.0f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0) - 14;
+        typedef T four __attribute__((ext_vector_type(4)));
+        four high, low;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float v = ldexpf(s[j], -e);
+            const T h = (T)v;
+            high[j] = h, low[j] = fabsf(v) < __builtin_inff() ? (T)(v - (float)h) : (T)0.0f;
+        }
+        *(four *)&u[t][4 * c] = high;
+        *(four *)&u[t][RX + 4 * c] = low;
+        if (c == 0) power[t] = ldexpf(1.0f, e);
+    }
+    __syncthreads();
+    const float scale = p.scales ? p.scales[adapter] : 1.0f;
+    const T *b = (const T *)p.b + adapter * p.b_as;
+    for (int i = begin; i < end; i++) {
+        const int n0 = 32 * i, column = n0 + 8 * g;
+        V w[2][NF];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const int row = min(n0 + 8 * (m / 4) + 4 * h + m % 4, p.n - 1), r = (32 * f + 8 * g) % RX;
+                w[h][f] = r < p.rank ? *(const V *)(b + row * p.b_ns + r) : V{};
+            }
+        for (int s = 0; s < subs; s++) {
+            const int t = kSub * s + m;
+            const bool in = t < count && column < p.n;
+            int64_t row = 0;
+            V y{};
+            if (in) row = p.rows[first + t], y = *(const V *)((const T *)p.base + row * p.base_ts + column);
+            floatx4 acc[2] = {};
+#pragma unroll
+            for (int f = 0; f < RX / 16; f++) {
+                const V v = *(const V *)&u[t][32 * f + 8 * g];
+                acc[0] = product(w[0][f % NF], v, acc[0]);
+                acc[1] = product(w[1][f % NF], v, acc[1]);
+            }
+            if (!in) continue;
+            const float two = power[t];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = (T)fmaf(acc[j / 4][j % 4] * two, scale, (float)y[j]);
+            *(V *)((T *)p.out + row * p.out_ts + column) = y;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+namespace {
+
+constexpr int64_t kMostTokens = int64_t(1) << 30;
+constexpr int64_t kMostBlocks = (1 << 24) - 1;  // of 256 threads: a launch of 2^32 threads or more runs modulo 2^32, without an error
+
+int make_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t sequences, int64_t n_adapters, int32_t *words, int64_t capacity,
+                      kvmix_adapter_plan_t *plan)
+{
+    *plan = kvmix_adapter_plan_t{};
+    std::vector<int64_t> of(n_adapters + 1);  // tokens of each adapter, of none last
+    for (int64_t s = 0; s < sequences; s++) {
+        if (counts[s] < 0) return KVMIX_ERR_SHAPE;
+        if (adapters[s] >= n_adapters) return KVMIX_ERR_ADAPTER;
+        if (counts[s] > kMostTokens - plan->tokens) return KVMIX_ERR_UNSUPPORTED;
+        plan->tokens += counts[s];
+        of[adapters[s] < 0 ? n_adapters : adapters[s]] += counts[s];
+        if (counts[s]) plan->adapters = std::max(plan->adapters, adapters[s] + 1);
+    }
+    for (int64_t i = 0; i <= n_adapters; i++) {
+        (i < n_adapters ? plan->tiles : plan->bare) += (of[i] + kTile - 1) / kTile;
+        if (i < n_adapters) plan->rows += of[i], plan->most = std::max(plan->most, std::min<int64_t>(of[i], kTile));
+    }
+    plan->rows_at = (plan->tiles + plan->bare) * kTileWords;
+    plan->words = plan->rows_at + plan->tokens;
+    if (!words) return KVMIX_OK;
+    if (capacity < plan->words) return KVMIX_ERR_WORKSPACE;
+    std::vector<int64_t> next(n_adapters + 1);  // where each adapter's tokens go
+    int32_t *tile = words;
+    int64_t first = 0;
+    for (int64_t i = 0; i <= n_adapters; i++) {
+        next[i] = plan->rows_at + first;
+        const int64_t tiles = (of[i] + kTile - 1) / kTile, even = tiles ? ((of[i] + tiles - 1) / tiles + kSub - 1) / kSub * kSub : 0;
+        for (int64_t t = 0; t < tiles; t++, tile += kTileWords) {
+            tile[0] = i < n_adapters ? (int32_t)i : -1, tile[1] = (int32_t)(first + t * even), tile[3] = 0;
+            tile[2] = (int32_t)std::min(even, of[i] - t * even);
+        }
+        first += of[i];
+    }
+    int32_t token = 0;
+    for (int64_t s = 0; s < sequences; s++)
+        for (int64_t t = 0; t < counts[s]; t++) words[next[adapters[s] < 0 ? n_adapters : adapters[s]]++] = token++;
+    return KVMIX_OK;
+}
+
+int64_t padded_rank(int64_t rank) { return (rank + 15) / 16 * 16; }
+
+int64_t rank_chunks(int64_t rank) { return (rank + 63) / 64; }
+
+// Stretches of k: blocks enough for all CUs, but no less than four units to a wave.
+int64_t splits_of(const kvmix_adapter_plan_t *plan, int64_t rank, int64_t k)
+{
+    const int64_t blocks = std::max<int64_t>(plan->tiles * rank_chunks(rank), 1);
+    return std::max<int64_t>(1, std::min<int64_t>({(512 + blocks - 1) / blocks, k / 512, 16}));
+}
+
+bool whole(int64_t v) { return v % 8 == 0; }
+
+int adapters_check(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
+{
+    if (!plan || !c) return KVMIX_ERR_NULL;
+    if (c->dtype != KVMIX_F16 && c->dtype != KVMIX_BF16) return KVMIX_ERR_DTYPE;
+    if (c->adapters < 0 || c->rank <= 0 || c->k <= 0 || c->n <= 0) return KVMIX_ERR_SHAPE;
+    if (plan->adapters > c->adapters) return KVMIX_ERR_ADAPTER;
+    if (c->rank > kMostRank || c->k > (1 << 24) || c->n > (1 << 24) || !whole(c->rank) || !whole(c->k) || !whole(c->n) || !whole(c->x_token_stride) ||
+        !whole(c->a_adapter_stride) || !whole(c->a_rank_stride) || !whole(c->b_adapter_stride) || !whole(c->b_row_stride) || !whole(c->base_token_stride) ||
+        !whole(c->out_token_stride) || ((uintptr_t)c->x | (uintptr_t)c->a | (uintptr_t)c->b | (uintptr_t)c->base | (uintptr_t)c->out) % 16)
+        return KVMIX_ERR_UNSUPPORTED;
+    return KVMIX_OK;
+}
+
+template <typename F>
+void with_rank(int64_t rank, F f)
+{
+    if (rank <= 16) f(std::integral_constant<int, 16>());
+    else if (rank <= 32) f(std::integral_constant<int, 32>());
+    else if (rank <= 64) f(std::integral_constant<int, 64>());
+    else f(std::integral_constant<int, 128>());
+}
+
+}  // namespace
+}  // namespace kvmix
+
+using namespace kvmix;
+
+extern "C" int kvmix_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t sequences, int64_t n_adapters, int32_t *words, int64_t capacity,
+                                  kvmix_adapter_plan_t *plan)
+{
+    if (!plan || (sequences > 0 && (!adapters || !counts))) return KVMIX_ERR_NULL;
+    if (sequences < 0 || n_adapters < 0) return KVMIX_ERR_SHAPE;
+    if (n_adapters > (1 << 20) || sequences > kMostTokens) return KVMIX_ERR_UNSUPPORTED;
+    try {
+        return make_adapter_plan(adapters, counts, sequences, n_adapters, words, capacity, plan);
+    } catch (const std::bad_alloc &) {
+        return KVMIX_ERR_MEMORY;
+    }
+}
+
+extern "C" int64_t kvmix_add_adapters_workspace_bytes(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
+{
+    if (adapters_check(plan, c) != KVMIX_OK) return 0;
+    return splits_of(plan, c->rank, c->k) * plan->rows * padded_rank(c->rank) * (int64_t)sizeof(float);
+}
+
+extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_t *list, const kvmix_adapters_t *c, void *workspace, int64_t workspace_bytes,
+                                  kvmix_stream_t stream)
+{
+    const int rc = adapters_check(plan, c);
+    if (rc != KVMIX_OK) return rc;
+    if (plan->tokens == 0) return KVMIX_OK;
+    if (!c->x || !c->base || !c->out || !list || (plan->rows && (!c->a || !c->b))) return KVMIX_ERR_NULL;
+    const bool in_place = c->out == c->base;
+    if (in_place && c->out_token_stride != c->base_token_stride) return KVMIX_ERR_SHAPE;
+    const int64_t need = kvmix_add_adapters_workspace_bytes(plan, c);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return KVMIX_ERR_WORKSPACE;
+    AdapterArgs p{};
+    p.x = c->x, p.a = c->a, p.b = c->b, p.base = c->base, p.out = c->out;
+    p.x_ts = c->x_token_stride, p.a_as = c->a_adapter_stride, p.a_rs = c->a_rank_stride, p.b_as = c->b_adapter_stride, p.b_ns = c->b_row_stride;
+    p.base_ts = c->base_token_stride, p.out_ts = c->out_token_stride, p.scales = c->scales, p.part = (float *)workspace;
+    p.tiles = (PlanWords)list, p.rows = (PlanWords)list + plan->rows_at, p.part_rows = plan->rows;
+    p.rank = (int)c->rank, p.padded = (int)padded_rank(c->rank), p.k = (int)c->k, p.n = (int)c->n;
+    p.splits = (int)splits_of(plan, c->rank, c->k), p.rank_chunks = (int)rank_chunks(c->rank);
+    const int64_t shrink = plan->tiles * p.rank_chunks * p.splits, tiles = plan->tiles + (in_place ? 0 : plan->bare), columns = (c->n + 31) / 32;
+    p.units = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * columns / (kWaves * 512)));
+    p.n_blocks = (int)((columns + kWaves * p.units - 1) / (kWaves * p.units));
+    if (shrink > kMostBlocks || tiles * p.n_blocks > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
+    hipStream_t st = (hipStream_t)stream;
+    auto run = [&](auto zero) {
+        using T = decltype(zero);
+        with_rank(c->rank, [&](auto RX) {
+            constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
+            const size_t lds = (size_t)kWaves * ((plan->most + kSub - 1) / kSub) * kSub * (RT * 16) * sizeof(float);
+            if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
+            if (tiles) adapter_expand<T, RX.value><<<(unsigned)(tiles * p.n_blocks), 256, 0, st>>>(p);
+        });
+    };
+    if (c->dtype == KVMIX_F16) run((_Float16)0);
+    else run((__bf16)0.0f);
+    return launch_status();
+}

@@ -56,6 +56,9 @@ struct Api {
     decltype(&kvmix_paged_plan) paged_plan;
     decltype(&kvmix_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
     decltype(&kvmix_paged_attention) paged_attention;
+    decltype(&kvmix_adapter_plan) adapter_plan;
+    decltype(&kvmix_add_adapters_workspace_bytes) add_adapters_workspace_bytes;
+    decltype(&kvmix_add_adapters) add_adapters;
     decltype(&kvmix_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
     decltype(&kvmix_token_logprobs) token_logprobs;
     decltype(&kvmix_token_logprobs_grad) token_logprobs_grad;
@@ -89,6 +92,9 @@ void bind(const std::unordered_map<std::string, uintptr_t> &at)
     KVMIX_BIND(paged_plan);
     KVMIX_BIND(paged_attention_workspace_bytes);
     KVMIX_BIND(paged_attention);
+    KVMIX_BIND(adapter_plan);
+    KVMIX_BIND(add_adapters_workspace_bytes);
+    KVMIX_BIND(add_adapters);
     KVMIX_BIND(token_logprobs_workspace_bytes);
     KVMIX_BIND(token_logprobs);
     KVMIX_BIND(token_logprobs_grad);
@@ -787,6 +793,7 @@ Tensor qkv_rope_append(const Tensor &x_in, const std::vector<Tensor> &ws, int64_
 }
 
 #include "host_paged.h"
+#include "host_batch.h"
 
 }  // namespace
 
@@ -813,6 +820,12 @@ PYBIND11_MODULE(_host, m)
         .def_property_readonly("slots", [](const PagedPlan &p) { return p.slots(); })
         .def_property_readonly("device", [](const PagedPlan &p) { return p.list.device(); })
         .def_property_readonly("launches", [](const PagedPlan &p) { return std::make_tuple(p.c.few_columns, p.c.tiles, p.c.joins); });
+    py::class_<AdapterPlan>(m, "AdapterPlan", "Which token of a batch has which adapter (ops.adapter_plan).")
+        .def_property_readonly("tokens", [](const AdapterPlan &p) { return p.c.tokens; })
+        .def_property_readonly("rows", [](const AdapterPlan &p) { return p.c.rows; })
+        .def_property_readonly("device", [](const AdapterPlan &p) { return p.list.device(); });
+    m.def("adapter_plan", &adapter_plan, NoGil());
+    m.def("add_adapters", &add_adapters, NoGil());
     m.def("paged_plan", &paged_plan, NoGil());
     m.def("paged_append", &paged_append, NoGil());
     m.def("paged_rope_append", &paged_rope_append, NoGil());

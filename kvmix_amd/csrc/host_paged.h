@@ -8,15 +8,26 @@ bool captures(const at::Device &device)
     return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
-struct PagedPlan {
-    kvmix_paged_plan_t c{};
-    Tensor list;  // the plan's words on the device
+// The words of a plan on the device.
+struct PlanList {
+    Tensor list;
     std::optional<c10::Stream> made_on;
     std::shared_ptr<c10::Event> made;  // when they are there
 
-    Tensor slots() const { return list.narrow(0, c.slots_at, c.tokens); }
+    // `write` fills them in host memory; they are copied on the current stream.
+    template <typename F>
+    void make(int64_t words, const at::Device &device, F write)
+    {
+        Tensor host = at::empty({words}, at::TensorOptions(at::kInt).pinned_memory(true));
+        write(host.data_ptr<int32_t>());
+        list = at::empty({words}, at::TensorOptions(at::kInt).device(device));
+        list.copy_(host, true);
+        made_on = torch_stream(device);
+        made = std::make_shared<c10::Event>(device.type());
+        made->record(*made_on);
+    }
 
-    // The words for a call on the current stream.  On another stream than the plan was made on they are waited for, and their memory is
+    // For a call on the current stream.  On another stream than the plan was made on they are waited for, and their memory is
     // given to nobody else before the call has read it (they are hidden from the caller, who could not see to it).  A
     // capture begins with the device idle and cannot wait for what lies outside it.
     const int32_t *words() const
@@ -28,6 +39,12 @@ struct PagedPlan {
         }
         return list.data_ptr<int32_t>();
     }
+};
+
+struct PagedPlan : PlanList {
+    kvmix_paged_plan_t c{};
+
+    Tensor slots() const { return list.narrow(0, c.slots_at, c.tokens); }
 };
 
 // Nothing here has a derivative (the likelihoods have one, backwards, which the caller records): a call that should record one, or
@@ -104,13 +121,7 @@ PagedPlan paged_plan(const Tensor &table_in, const std::vector<int64_t> &kv_lens
     const kvmix_paged_batch_t b = {table.data_ptr<int32_t>(), table.size(1), kv_lens.data(), packed_lens.data(), q_lens.data(), n, heads, kv_heads, head_dim, page_size};
     PagedPlan plan;
     check(api.paged_plan(&b, nullptr, 0, &plan.c));
-    Tensor host = at::empty({plan.c.words}, at::TensorOptions(at::kInt).pinned_memory(true));
-    check(api.paged_plan(&b, host.data_ptr<int32_t>(), plan.c.words, &plan.c));
-    plan.list = at::empty({plan.c.words}, at::TensorOptions(at::kInt).device(device));
-    plan.list.copy_(host, true);
-    plan.made_on = torch_stream(device);
-    plan.made = std::make_shared<c10::Event>(device.type());
-    plan.made->record(*plan.made_on);
+    plan.make(plan.c.words, device, [&](int32_t *words) { check(api.paged_plan(&b, words, plan.c.words, &plan.c)); });
     return plan;
 }
 

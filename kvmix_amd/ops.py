@@ -530,6 +530,21 @@ def paged_attention(q: torch.Tensor, rows: torch.Tensor, packed: torch.Tensor, p
     return _host().paged_attention(q, rows, packed, plan, k_bits, v_bits, scale)
 
 
+def adapter_plan(adapters, counts, n_adapters: int, device="cuda"):
+    """Which token of a batch has which adapter, for every projection of a step (kvmix_adapter_plan): adapters [sequences], each a
+    number below n_adapters, or negative for none; counts [sequences]: the new tokens of each, sequence after sequence.  As paged_plan's it is
+    copied to `device` on the current stream, can be used on any, and cannot be made while a graph is captured."""
+    return _host().adapter_plan(list(adapters), list(counts), n_adapters, _cuda(device))
+
+
+def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan, scales: torch.Tensor = None, out: torch.Tensor = None):
+    """base + scales[i] * (x @ a[i].T) @ b[i].T for the tokens of the sequences with adapter i, base for those without one: base
+    [..., n] and x [..., k] of the plan's tokens, a [adapters, rank, k], b [adapters, n, rank], fp16 or bf16 alike; scales [adapters] fp32
+    or None for 1.  rank (at most 128), k and n in multiples of 8; smaller adapters are filled up with zeros.  Into `out` where it is
+    given, which may be base itself, else into a new tensor, which is returned."""
+    return _host().add_adapters(base, x, a, b, plan, scales, out)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top):
