@@ -698,6 +698,43 @@ int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_t *list, co
                        kvmix_stream_t stream);
 
 /*
+ * The best continuations of the beams of some requests (no counterpart in the reference): of each request the `count` largest of
+ *   scores[w] + x[w, v] - log sum_u exp x[w, u]   over its beams w and the tokens v,
+ * equal ones in the order of (w, v), with their beams and tokens, the best first.  A beam that has ended (done) has one continuation,
+ * `end` at its own score.  Where nothing can be computed (a score that is not finite; a row with NaN or +inf, or of -inf only), a beam's
+ * continuations count as -inf.  With `stay` (count = beams) a request's results are put in the places of beams: the best
+ * child of a beam where that beam was, the others where beams have none, best first.  Sums in fp32 over parts of a row, the rest in 64 bits.
+ *   logits [requests * beams, vocab] fp16, bf16 or fp32, rows row_stride elements apart; vocab up to 2^20, beams times
+ *   vocab up to 2^25;  scores [requests * beams];  done NULL or [requests * beams], 0 or 1;  beams and count up to 64, count up to vocab
+ *   out_scores, parents (0 .. beams - 1), tokens [requests, count]
+ */
+typedef struct kvmix_beam_select {
+    const void *logits;
+    int64_t row_stride;
+    int dtype;
+    const float *scores;
+    const uint8_t *done;
+    int64_t end;
+    int64_t requests, beams, vocab, count;
+    int stay;
+    float *out_scores;
+    int64_t *parents, *tokens;
+} kvmix_beam_select_t;
+int64_t kvmix_beam_select_workspace_bytes(const kvmix_beam_select_t *p);
+int kvmix_beam_select(const kvmix_beam_select_t *p, void *workspace, int64_t workspace_bytes, kvmix_stream_t stream);
+
+/*
+ * Tensors reordered along their first dimension in place, t[i] = old t[index[i]], all with the same index [rows] in device memory (rows up
+ * to 1024; an index outside of [0, rows) leaves its row as it is).  Entry i of a tensor lies batch_stride further on than entry
+ * i - 1 and is `outer` times `inner` rows of row_bytes; strides in bytes.  Entries must not overlap, and no two tensors may.
+ */
+typedef struct kvmix_reorder {
+    void *base;
+    int64_t batch_stride, outer, outer_stride, inner, inner_stride, row_bytes;
+} kvmix_reorder_t;
+int kvmix_reorder_rows(const kvmix_reorder_t *items, int64_t count, const int64_t *index, int64_t rows, kvmix_stream_t stream);
+
+/*
  * Measurement support, no counterpart in the reference and not called by any operator: a kernel
  * that only reads, in the access patterns of the GEMV kernels, to establish what streaming rate
  * the GPU reaches without arithmetic (the ceiling the GEMV figures are compared with), and how

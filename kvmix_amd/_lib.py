@@ -55,6 +55,9 @@ EXPORTS = (
     "kvmix_paged_plan",
     "kvmix_paged_attention_workspace_bytes",
     "kvmix_paged_attention",
+    "kvmix_beam_select_workspace_bytes",
+    "kvmix_beam_select",
+    "kvmix_reorder_rows",
     "kvmix_adapter_plan",
     "kvmix_add_adapters_workspace_bytes",
     "kvmix_add_adapters",
@@ -172,6 +175,21 @@ class Adapters(ctypes.Structure):
                 ("adapters", _i64), ("rank", _i64), ("k", _i64), ("n", _i64), ("dtype", ctypes.c_int)]
 
 
+class BeamSelect(ctypes.Structure):
+    """kvmix_beam_select_t"""
+    _i64, _vp = ctypes.c_int64, ctypes.c_void_p
+    _fields_ = [("logits", _vp), ("row_stride", _i64), ("dtype", ctypes.c_int), ("scores", _vp), ("done", _vp), ("end", _i64),
+                ("requests", _i64), ("beams", _i64), ("vocab", _i64), ("count", _i64), ("stay", ctypes.c_int),
+                ("out_scores", _vp), ("parents", _vp), ("tokens", _vp)]
+
+
+class Reorder(ctypes.Structure):
+    """kvmix_reorder_t"""
+    _i64 = ctypes.c_int64
+    _fields_ = [("base", ctypes.c_void_p), ("batch_stride", _i64), ("outer", _i64), ("outer_stride", _i64), ("inner", _i64),
+                ("inner_stride", _i64), ("row_bytes", _i64)]
+
+
 LINEAR_PLAIN, LINEAR_FLOAT, LINEAR_RESIDUAL, LINEAR_SWIGLU, LINEAR_ROPE_APPEND = range(5)
 
 
@@ -270,6 +288,12 @@ def load() -> ctypes.CDLL:
     L.kvmix_add_adapters_workspace_bytes.argtypes = [ctypes.POINTER(AdapterPlan), ctypes.POINTER(Adapters)]
     L.kvmix_add_adapters.restype = i32
     L.kvmix_add_adapters.argtypes = [ctypes.POINTER(AdapterPlan), vp, ctypes.POINTER(Adapters), vp, i64, vp]
+    L.kvmix_beam_select_workspace_bytes.restype = i64
+    L.kvmix_beam_select_workspace_bytes.argtypes = [ctypes.POINTER(BeamSelect)]
+    L.kvmix_beam_select.restype = i32
+    L.kvmix_beam_select.argtypes = [ctypes.POINTER(BeamSelect), vp, i64, vp]
+    L.kvmix_reorder_rows.restype = i32
+    L.kvmix_reorder_rows.argtypes = [vp, i64, vp, i64, vp]
     L.kvmix_probe_stream_read.restype = i32
     L.kvmix_probe_stream_read.argtypes = [vp, i32, i64, i64, i32, i32, i32, i32, i32, vp, vp]
     _lib = L

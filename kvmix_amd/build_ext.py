@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkvmix_hip.so")
 SOURCES = ["abi.hip", "quant_pack.hip", "dequant_gemv.hip", "decode_attn.hip", "fused_attn.hip", "linear_rows.hip", "prefill_attn.hip", "copy_rows.hip", "rope_append.hip", "stream_probe.hip",
-           "paged_attn.hip", "paged_store.hip", "token_logprobs.hip", "adapters.hip"]
+           "paged_attn.hip", "paged_store.hip", "token_logprobs.hip", "adapters.hip", "beam_select.hip", "reorder.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -289,6 +289,11 @@ class PackedKVCache:
         self._packed_views = (None,) * 6
         self._flushed_ahead = False
 
+    def reorder(self, index: torch.Tensor) -> None:
+        """The batch's sequences reordered in place, sequence i from what sequence index[i] was (reorder_caches below, which takes
+        the caches of all layers at once)."""
+        reorder_caches([self], index)
+
     # -- views -----------------------------------------------------------------------------
     def as_tuple(self) -> Tuple:
         """The reference's 9-tuple (models/modeling_llama_KVmix.py:270-273) as views of the
@@ -327,3 +332,14 @@ def flush_ahead(caches) -> int:
             c._flush_done(nk, nv, direct=False)
             c._flushed_ahead = True
     return len(todo)
+
+
+def reorder_caches(caches, index: torch.Tensor, *others: torch.Tensor) -> None:
+    """The batch of every cache (PackedKVCache, or the reference's 9-tuple; None holds nothing) reordered in place, and that of `others`:
+    entry i becomes what entry index[i] was, index int64 on the device.  What beam search does between two steps; all layers
+    together (ops.reorder_rows)."""
+    tensors = list(others)
+    for c in caches:
+        entries = () if c is None else c.as_tuple() if isinstance(c, PackedKVCache) else c
+        tensors += [t for t in entries if torch.is_tensor(t)]
+    ops.reorder_rows(tensors, index)

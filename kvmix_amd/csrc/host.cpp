@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -56,6 +57,9 @@ struct Api {
     decltype(&kvmix_paged_plan) paged_plan;
     decltype(&kvmix_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
     decltype(&kvmix_paged_attention) paged_attention;
+    decltype(&kvmix_beam_select_workspace_bytes) beam_select_workspace_bytes;
+    decltype(&kvmix_beam_select) beam_select;
+    decltype(&kvmix_reorder_rows) reorder_rows;
     decltype(&kvmix_adapter_plan) adapter_plan;
     decltype(&kvmix_add_adapters_workspace_bytes) add_adapters_workspace_bytes;
     decltype(&kvmix_add_adapters) add_adapters;
@@ -92,6 +96,9 @@ void bind(const std::unordered_map<std::string, uintptr_t> &at)
     KVMIX_BIND(paged_plan);
     KVMIX_BIND(paged_attention_workspace_bytes);
     KVMIX_BIND(paged_attention);
+    KVMIX_BIND(beam_select_workspace_bytes);
+    KVMIX_BIND(beam_select);
+    KVMIX_BIND(reorder_rows);
     KVMIX_BIND(adapter_plan);
     KVMIX_BIND(add_adapters_workspace_bytes);
     KVMIX_BIND(add_adapters);
@@ -825,6 +832,8 @@ PYBIND11_MODULE(_host, m)
         .def_property_readonly("rows", [](const AdapterPlan &p) { return p.c.rows; })
         .def_property_readonly("device", [](const AdapterPlan &p) { return p.list.device(); });
     m.def("adapter_plan", &adapter_plan, NoGil());
+    m.def("beam_select", &beam_select, NoGil());
+    m.def("reorder_rows", &reorder_rows, NoGil());
     m.def("add_adapters", &add_adapters, NoGil());
     m.def("paged_plan", &paged_plan, NoGil());
     m.def("paged_append", &paged_append, NoGil());

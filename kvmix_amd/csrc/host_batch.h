@@ -1,4 +1,4 @@
-// The host side of the operators on batches of requests (adapters): part of host.cpp, whose helpers it uses.
+// The host side of the operators on batches of requests (adapters, beams): part of host.cpp, whose helpers it uses.
 
 struct AdapterPlan : PlanList {
     kvmix_adapter_plan_t c{};
@@ -102,4 +102,100 @@ Tensor add_adapters(const Tensor &base_in, const Tensor &x_in, const Tensor &a_i
     const c10::DeviceGuard guard(base.device());
     check(api.add_adapters(&plan.c, plan.words(), &c, need ? ws.data_ptr() : nullptr, need, stream_of(base)));
     return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor &logits, const Tensor &scores_in, const std::optional<int64_t> &count_in, const OptTensor &done_in,
+                                               const std::optional<int64_t> &end, bool stay)
+{
+    need_no_record("beam_select", {&logits, &scores_in});
+    need_gpu({&logits});
+    need_with(logits, {&scores_in});
+    if (logits.scalar_type() != at::kHalf && logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)
+        fail("beam_select: logits must be float16, bfloat16 or float32, got " + dtype_name(logits));
+    if (logits.dim() != 3 || logits.size(1) == 0 || logits.size(2) == 0) fail("beam_select: logits must be [requests, beams, vocabulary], with a beam and a token at least");
+    const int64_t requests = logits.size(0), beams = logits.size(1), vocab = logits.size(2), count = count_in.value_or(beams);
+    if (scores_in.scalar_type() != at::kFloat || scores_in.dim() != 2 || scores_in.size(0) != requests || scores_in.size(1) != beams)
+        fail("beam_select: scores must be float32 [requests, beams]");
+    if (beams > 64 || count < 1 || count > 64 || count > vocab) fail("beam_select: at most 64 beams, a count between 1 and 64 that is not more than there are tokens");
+    if (vocab > (1 << 20) || beams * vocab > (1 << 25)) fail("beam_select: a vocabulary of at most 2^20 tokens, 2^25 with all beams of a request");
+    if (stay && count != beams) fail("beam_select: results stay in their beams' places only where there are as many as beams");
+    if (done_in) {
+        need_with(logits, {&*done_in});
+        if (done_in->scalar_type() != at::kBool || done_in->sizes() != scores_in.sizes()) fail("beam_select: done must be bool [requests, beams]");
+        if (!end || *end < 0 || *end >= vocab) fail("beam_select: beams that have ended need the token that ends them, one of the vocabulary");
+    }
+    const Tensor x = score_rows2(logits), scores = scores_in.contiguous(), done = done_in ? done_in->contiguous() : Tensor();
+    Tensor out = at::empty({requests, count}, scores.options()), parents = at::empty({requests, count}, scores.options().dtype(at::kLong));
+    Tensor tokens = at::empty_like(parents), ws;
+    kvmix_beam_select_t c{};
+    c.logits = x.data_ptr(), c.row_stride = x.size(0) > 1 ? x.stride(0) : vocab;
+    c.dtype = x.scalar_type() == at::kHalf ? KVMIX_F16 : x.scalar_type() == at::kFloat ? KVMIX_F32 : KVMIX_BF16;
+    c.scores = scores.data_ptr<float>(), c.done = done_in ? (const uint8_t *)done.data_ptr() : nullptr, c.end = end.value_or(0);
+    c.requests = requests, c.beams = beams, c.vocab = vocab, c.count = count, c.stay = stay;
+    c.out_scores = out.data_ptr<float>(), c.parents = parents.data_ptr<int64_t>(), c.tokens = tokens.data_ptr<int64_t>();
+    const int64_t need = api.beam_select_workspace_bytes(&c);
+    if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
+    const c10::DeviceGuard guard(x.device());
+    check(api.beam_select(&c, need ? ws.data_ptr() : nullptr, need, stream_of(x)));
+    return {out, parents, tokens};
+}
+
+// A tensor's first dimension and what belongs to one entry of it.
+kvmix_reorder_t reorder_item(const Tensor &t)
+{
+    const int64_t size = (int64_t)t.element_size();
+    struct Dim {
+        int64_t size, stride;
+    };
+    std::vector<Dim> dims;
+    for (int64_t d = 1; d < t.dim(); d++)
+        if (t.size(d) > 1) dims.push_back({t.size(d), t.stride(d) * size});
+    std::sort(dims.begin(), dims.end(), [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+    std::vector<Dim> all = dims;
+    if (t.size(0) > 1) all.push_back({t.size(0), t.stride(0) * size});
+    std::sort(all.begin(), all.end(), [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+    int64_t extent = size;  // of what the dimensions so far span
+    for (const Dim &d : all) {
+        if (d.stride < extent) fail("reorder_rows: entries of a tensor must not overlap");
+        extent += (d.size - 1) * d.stride;
+    }
+    kvmix_reorder_t item{};
+    item.base = t.data_ptr(), item.batch_stride = t.size(0) > 1 ? t.stride(0) * size : extent;
+    int64_t run = size;
+    std::vector<Dim> outer;
+    for (const Dim &d : dims) {
+        if (outer.empty() && d.stride == run) run *= d.size;
+        else if (!outer.empty() && d.stride == outer.back().stride * outer.back().size) outer.back().size *= d.size;
+        else outer.push_back(d);
+    }
+    if (outer.size() > 2) fail("reorder_rows: an entry of a tensor must be rows of memory in at most two dimensions");
+    item.row_bytes = run;
+    item.inner = outer.size() > 0 ? outer[0].size : 1, item.inner_stride = outer.size() > 0 ? outer[0].stride : 0;
+    item.outer = outer.size() > 1 ? outer[1].size : 1, item.outer_stride = outer.size() > 1 ? outer[1].stride : 0;
+    return item;
+}
+
+void reorder_rows(const std::vector<Tensor> &tensors, const Tensor &index_in)
+{
+    if (torch::jit::tracer::isTracing()) fail("reorder_rows cannot be part of a trace");
+    need_gpu({&index_in});
+    if (index_in.scalar_type() != at::kLong || index_in.dim() != 1) fail("reorder_rows: the index must be int64 [rows]");
+    const int64_t rows = index_in.size(0);
+    if (rows > 1024) fail("reorder_rows: at most 1024 rows");
+    std::vector<kvmix_reorder_t> items;
+    for (const Tensor &t : tensors) {
+        need_no_record("reorder_rows", {&t});
+        need_gpu({&t});
+        need_with(index_in, {&t});
+        if (t.dim() < 1 || t.size(0) != rows) fail("reorder_rows: every tensor must have as many entries as the index");
+        if (t.numel() == 0) continue;
+        items.push_back(reorder_item(t));
+    }
+    std::vector<const void *> bases;
+    for (const auto &item : items) bases.push_back(item.base);
+    std::sort(bases.begin(), bases.end());
+    if (std::adjacent_find(bases.begin(), bases.end()) != bases.end()) fail("reorder_rows: no two tensors may overlap");
+    const Tensor index = index_in.contiguous();
+    const c10::DeviceGuard guard(index.device());
+    check(api.reorder_rows(items.data(), (int64_t)items.size(), index.data_ptr<int64_t>(), rows, stream_of(index)));
 }

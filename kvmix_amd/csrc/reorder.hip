@@ -1,0 +1,171 @@
+// The first dimension of many tensors reordered in place:  t[i] = old t[index[i]], the same index for all of them (the states of beams
+// that go on).
+//
+// Bound by memory: rows that stay are neither read nor written, and a row that several others become is read by the same thread
+// for all of them, from HBM once.  A thread takes one piece of sixteen bytes of a row, at the same place of all rows, so that no other
+// thread reads what it writes and nothing has to be waited for.  Old values that are still wanted when their place is written
+// (of rows that change and are the source of others) are put in the LDS first, each by the thread that will want it; where they
+// are too many for all threads of a block, fewer take a turn.  With beams placed so that the first child stays where its
+// parent was there are none.
+#include "copy_rows.h"
+
+namespace kvmix {
+
+constexpr int kReorderItems = 40, kReorderThreads = 256, kReorderTiles = 4, kReorderAhead = 8;
+constexpr int kReorderRows = 1024, kReorderStage = 2048;  // rows at most; pieces in the LDS
+
+struct ReorderItem {
+    uint8_t *base;
+    int64_t batch, outer, inner;  // bytes from one to the next
+    int64_t row_bytes;
+    uint32_t pieces;              // of one i of the first dimension
+    CopyDiv per_row, rows;        // pieces of a row, rows of an outer one
+};
+
+struct ReorderArgs {
+    ReorderItem item[kReorderItems];
+    uint32_t first[kReorderItems + 1];
+    const int64_t *index;
+    int count, rows;
+};
+
+typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t word2 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t word1 __attribute__((aligned(1)));
+typedef uint16_t half1 __attribute__((aligned(1)));
+
+typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
+
+// Sixteen bytes, or the first n of them, piece by piece: the last of a row is followed by what another thread writes.
+__device__ __forceinline__ Bytes16 load_bytes(const uint8_t *p, int n)
+{
+    if (n == 16) return *(const word4 *)p;
+    uint32_t first[2] = {0, 0}, four = 0, tail = 0;
+    if (n & 8) {
+        const word2 x = *(const word2 *)p;
+        first[0] = x[0], first[1] = x[1];
+    }
+    if (n & 4) four = *(const word1 *)(p + (n & 8));
+    if (n & 2) tail = *(const half1 *)(p + (n & 12));
+    if (n & 1) tail |= (uint32_t)p[n & 14] << (n & 2) * 8;
+    return Bytes16{first[0], first[1], four, tail};
+}
+
+__device__ __forceinline__ void store_bytes(uint8_t *p, Bytes16 v, int n)
+{
+    if (n == 16) {
+        *(word4 *)p = v;
+        return;
+    }
+    if (n & 8) *(word2 *)p = word2{v[0], v[1]};
+    if (n & 4) *(word1 *)(p + (n & 8)) = v[2];
+    if (n & 2) *(half1 *)(p + (n & 12)) = (uint16_t)v[3];
+    if (n & 1) p[n & 14] = (uint8_t)(v[3] >> (n & 2) * 8);
+}
+
+__global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
+{
+    __shared__ Bytes16 stage[kReorderStage];
+    __shared__ int source[kReorderRows], change[kReorderRows], early[kReorderRows];
+    __shared__ int16_t slot[kReorderRows];  // of an old value in the LDS, or -1
+    __shared__ uint8_t wanted[kReorderRows];
+    __shared__ int changes, earlies;
+    const int t = threadIdx.x;
+    if (t == 0) changes = earlies = 0;
+    for (int i = t; i < a.rows; i += kReorderThreads) {
+        const int64_t from = a.index[i];
+        source[i] = from >= 0 && from < a.rows ? (int)from : i;  // (an index that is none changes nothing)
+        wanted[i] = 0;
+    }
+    __syncthreads();
+    for (int i = t; i < a.rows; i += kReorderThreads)
+        if (source[i] != i) wanted[source[i]] = 1;
+    __syncthreads();
+    for (int i = t; i < a.rows; i += kReorderThreads) {
+        slot[i] = -1;
+        if (source[i] == i) continue;
+        change[atomicAdd(&changes, 1)] = i;
+        if (wanted[i]) {
+            const int s = atomicAdd(&earlies, 1);
+            early[s] = i, slot[i] = (int16_t)s;
+        }
+    }
+    __syncthreads();
+    const int n = __builtin_amdgcn_readfirstlane(changes), staged = __builtin_amdgcn_readfirstlane(earlies);
+    if (n == 0) return;
+    int nth = 0;
+    while (nth + 1 < a.count && blockIdx.x >= a.first[nth + 1]) nth++;
+    const ReorderItem it = a.item[nth];
+    const int at_once = staged * kReorderThreads > kReorderStage ? kReorderStage / staged : kReorderThreads;
+    if (t >= at_once) return;
+    const uint32_t begin = (blockIdx.x - a.first[nth]) * (kReorderThreads * kReorderTiles);
+    const uint32_t end = begin + kReorderThreads * kReorderTiles < it.pieces ? begin + kReorderThreads * kReorderTiles : it.pieces;
+    for (uint32_t p = begin + t; p < end; p += at_once) {
+        const uint32_t row = copy_div(p, it.per_row), o = copy_div(row, it.rows);
+        const int64_t in = (int64_t)(p - row * it.per_row.d) * 16;
+        uint8_t *at = it.base + o * it.outer + (row - o * it.rows.d) * it.inner + in;
+        const int bytes = (int)(it.row_bytes - in < 16 ? it.row_bytes - in : 16);
+        for (int i = 0; i < staged; i++) stage[i * at_once + t] = load_bytes(at + __builtin_amdgcn_readfirstlane(early[i]) * it.batch, bytes);
+        for (int i = 0; i < n; i += kReorderAhead) {
+            Bytes16 v[kReorderAhead];
+#pragma unroll
+            for (int j = 0; j < kReorderAhead; j++) {
+                if (i + j < n) {
+                    const int from = __builtin_amdgcn_readfirstlane(source[__builtin_amdgcn_readfirstlane(change[i + j])]);
+                    const int s = __builtin_amdgcn_readfirstlane((int)slot[from]);
+                    v[j] = s >= 0 ? stage[s * at_once + t] : load_bytes(at + from * it.batch, bytes);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kReorderAhead; j++) {
+                if (i + j < n) store_bytes(at + __builtin_amdgcn_readfirstlane(change[i + j]) * it.batch, v[j], bytes);
+            }
+        }
+    }
+}
+
+}  // namespace kvmix
+
+using namespace kvmix;
+
+extern "C" int kvmix_reorder_rows(const kvmix_reorder_t *items, int64_t count, const int64_t *index, int64_t rows, kvmix_stream_t stream)
+{
+    if (count < 0 || rows < 0) return KVMIX_ERR_SHAPE;
+    if (count && !items) return KVMIX_ERR_NULL;
+    if (rows > kReorderRows) return KVMIX_ERR_UNSUPPORTED;
+    auto empty = [](const kvmix_reorder_t &p) { return p.outer == 0 || p.inner == 0 || p.row_bytes == 0; };
+    for (int64_t i = 0; i < count; i++) {
+        const kvmix_reorder_t &p = items[i];
+        if (p.outer < 0 || p.inner < 0 || p.row_bytes < 0) return KVMIX_ERR_SHAPE;
+        if (empty(p) || rows <= 1) continue;
+        if (!p.base) return KVMIX_ERR_NULL;
+        if ((p.inner > 1 && p.inner_stride < p.row_bytes) || (p.outer > 1 && p.outer_stride < p.row_bytes) || p.batch_stride < p.row_bytes) return KVMIX_ERR_SHAPE;
+        if (p.outer > (1ll << 31) || p.inner > (1ll << 31) || p.row_bytes > (1ll << 40) ||
+            (__int128)p.outer * p.inner * ((p.row_bytes + 15) / 16) > 0x7fffffff - kReorderThreads * kReorderTiles)
+            return KVMIX_ERR_UNSUPPORTED;
+    }
+    if (rows <= 1 || count == 0) return KVMIX_OK;  // (one row is itself)
+    if (!index) return KVMIX_ERR_NULL;
+    int rc = KVMIX_OK;
+    for (int64_t i = 0; i < count;) {
+        ReorderArgs a{};
+        a.index = index, a.rows = (int)rows;
+        for (; i < count && a.count < kReorderItems; i++) {
+            const kvmix_reorder_t &p = items[i];
+            if (empty(p)) continue;
+            ReorderItem &it = a.item[a.count];
+            it.base = (uint8_t *)p.base, it.batch = p.batch_stride, it.outer = p.outer_stride, it.inner = p.inner_stride, it.row_bytes = p.row_bytes;
+            it.per_row = copy_divisor((uint32_t)((p.row_bytes + 15) / 16)), it.rows = copy_divisor((uint32_t)p.inner);
+            it.pieces = (uint32_t)(p.outer * p.inner) * it.per_row.d;
+            const uint32_t blocks = (it.pieces + kReorderThreads * kReorderTiles - 1) / (kReorderThreads * kReorderTiles);
+            if (a.first[a.count] + (uint64_t)blocks >= 1u << 24) break;  // (a launch of 2^32 threads or more runs modulo 2^32)
+            a.first[a.count + 1] = a.first[a.count] + blocks;
+            a.count++;
+        }
+        if (!a.count) continue;
+        reorder_rows<<<a.first[a.count], kReorderThreads, 0, (hipStream_t)stream>>>(a);
+        rc = launch_status();
+        if (rc != KVMIX_OK) break;
+    }
+    return rc;
+}

@@ -20,18 +20,14 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "kvmix_common.h"
+#include "score_common.h"
 #include "score_plan.h"
 
 namespace kvmix {
 
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-
 constexpr float kStale = 20.0f;    // how far a value may exceed what sums are relative to: 2^d stays below 2^29
 constexpr float kFar = 16777216.0f;  // up to there the rounding of m log2(e) is 1 at most (at 1e10 it is 512 and more, and 2^512 no number)
 constexpr float kNothing = -1024.0f;  // 2^d is zero from here on, and its products with sums and gradients of any size are finite
-constexpr int kTopMost = 64, kCandidates = 1024;
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 struct ScoreStats {
     float m, s, u;  // reference (as a logit), sum of 2^d, sum of 2^d d
@@ -53,12 +49,6 @@ struct ScoreArgs {
     int64_t dx_stride;
 };
 
-template <typename T>
-__device__ __forceinline__ float to_float(T v)
-{
-    return (float)v;
-}
-
 // A row's values from `begin` on as sixteen-byte pieces of memory: the first and the last may hold others, of no concern, beside
 // it (they lie in the same sixteen aligned bytes as values of the row do).
 template <typename T>
@@ -74,32 +64,6 @@ struct Span {
         first = -skew, length = max(end - begin, 0), pieces = length ? (length + skew + PER - 1) / PER : 0;
     }
 };
-
-template <typename T>
-union Piece {
-    uint4v raw;
-    T t[16 / sizeof(T)];
-};
-
-// The largest of a piece's values (not NaN), two at a time where the type allows it.
-__device__ __forceinline__ float piece_max(const Piece<_Float16> &w)
-{
-    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-    uint32_t word = w.raw[0];
-#pragma unroll
-    for (int j = 1; j < 4; j++) asm("v_pk_max_f16 %0, %0, %1" : "+v"(word) : "v"(w.raw[j]));  // (without the builtin's quieting of both)
-    const half2v most = __builtin_bit_cast(half2v, word);
-    return fmaxf((float)most[0], (float)most[1]);
-}
-
-template <typename T>
-__device__ __forceinline__ float piece_max(const Piece<T> &w)
-{
-    float most = to_float(w.t[0]);
-#pragma unroll
-    for (int j = 1; j < Span<T>::PER; j++) most = fmaxf(most, to_float(w.t[j]));
-    return most;
-}
 
 // A piece of a span, with -inf for what is none of it.
 template <typename T>
@@ -135,17 +99,6 @@ __device__ __forceinline__ ScoreStats merged(ScoreStats a, ScoreStats b)
     return {m, a.s * fa + b.s * fb, (a.u + a.s * da) * fa + (b.u + b.s * db) * fb};
 }
 
-// order of the most likely: larger value first, then lower index; NaN is larger than anything
-__device__ __forceinline__ uint32_t value_key(float v)
-{
-    const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 is 0)
-    return v != v ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-
-__device__ __forceinline__ uint64_t full_key(float v, int index) { return (uint64_t)value_key(v) << 32 | (uint32_t)~index; }
-
 template <int NT>
 struct TopShared {
     uint32_t most[NT];
@@ -153,19 +106,6 @@ struct TopShared {
     uint64_t best[NT / kWave];
     int count;
 };
-
-// Calls f(rank, key) for the `top` first of `count` different keys, by the threads of a block.
-template <int NT, typename F>
-__device__ __forceinline__ void rank_keys(const uint64_t *key, int count, int top, F f)
-{
-    for (int i = threadIdx.x; i < count; i += NT) {
-        const uint64_t mine = key[i];
-        int rank = 0;
-#pragma unroll 8
-        for (int j = 0; j < count; j++) rank += key[j] > mine;
-        if (rank < top) f(rank, mine);
-    }
-}
 
 // The `top` first keys of a span, one by one: for rows in which too many values are alike.
 template <typename T, int NT, typename F>
@@ -445,14 +385,6 @@ ScoreArgs rows_from(ScoreArgs a, int64_t first)
     if (a.grad_entropy) a.grad_entropy += first;
     if (a.dx) a.dx = (T *)a.dx + first * a.dx_stride;
     return a;
-}
-
-template <typename F>
-void with_type(int dtype, F f)
-{
-    if (dtype == KVMIX_F16) f((_Float16)0);
-    else if (dtype == KVMIX_F32) f(0.0f);
-    else f((__bf16)0.0f);
 }
 
 }  // namespace

@@ -251,6 +251,32 @@ class Decoder:
                 on_step(step, logits)
         return torch.cat(out, dim=1)
 
+    def beam_search(self, prompt_ids: torch.Tensor, beams: int, new_tokens: int, end: Optional[int] = None):
+        """Beam search from prompts [B,Q], nothing cached before: (token ids [B, beams, new_tokens], sums of their log probabilities
+        [B, beams]), the best first.  A beam ends with the token `end`, which then fills it up.  The beams' caches are reordered
+        in place between the steps; nothing waits for the GPU."""
+        from . import ops
+        from .cache import reorder_caches
+
+        if beams < 1 or new_tokens < 1 or self.position:
+            raise RuntimeError("beam_search: a beam and a new token at least, from a prompt that nothing is cached of")
+        B = prompt_ids.shape[0]
+        logits = self.forward(prompt_ids.repeat_interleave(beams, 0))
+        ids = prompt_ids.new_zeros(B * beams, new_tokens)
+        scores = torch.full((B, beams), float("-inf"), device=ids.device)
+        scores[:, 0] = 0.0  # (the beams of a request are alike still)
+        first, done = beams * torch.arange(B, device=ids.device)[:, None], None
+        for step in range(new_tokens):
+            scores, parents, tokens = ops.beam_select(logits.view(B, beams, -1), scores, beams, done, end, stay=True)
+            last = step + 1 == new_tokens
+            reorder_caches([] if last else self.caches, (first + parents).reshape(-1), ids)
+            ids[:, step] = tokens.reshape(-1)
+            done = None if end is None else tokens == end
+            if not last:
+                logits = self.forward(tokens.reshape(-1, 1))
+        scores, order = scores.sort(dim=-1, descending=True, stable=True)
+        return ids.view(B, beams, -1).gather(1, order[:, :, None].expand(-1, -1, new_tokens)), scores
+
 
 class GraphDecoder(Decoder):
     """Decoder whose single-token steps are replayed from a captured HIP graph.

@@ -545,6 +545,22 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     return _host().add_adapters(base, x, a, b, plan, scales, out)
 
 
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int = None, done: torch.Tensor = None, end: int = None, stay: bool = False):
+    """The best continuations of the beams of every request: logits [requests, beams, vocabulary] fp16, bf16 or fp32, scores
+    [requests, beams] fp32 -> (scores, parents, tokens) [requests, count] of the `count` (as many as beams unless given) largest
+    scores + log_softmax(logits), the best first, equal ones in the order of (beam, token).  A beam that has ended (done, bool) goes on as
+    it is: its one continuation is the token `end` at its own score.  stay=True puts the best child of a beam in that beam's place and
+    the others, best first, where beams have no children: then the states of few beams have to be moved (reorder_rows).  Beams whose
+    score is not finite, or whose logits have NaN, +inf or nothing but -inf, go on at -inf, after all others."""
+    return _host().beam_select(logits, scores, count, done, end, stay)
+
+
+def reorder_rows(tensors, index: torch.Tensor) -> None:
+    """t[:] = t[index] for each of the tensors, in place: index int64 [rows] on the device, any types and strides of tensors [rows,
+    ...] that do not overlap (kvmix_reorder_rows).  Rows that stay are not touched; an index outside of the rows leaves its row as it is."""
+    _host().reorder_rows(list(tensors), index)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top):

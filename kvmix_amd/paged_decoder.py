@@ -6,39 +6,65 @@ beside single tokens, forks of a sequence, and the likelihoods of texts.
     logits = model.forward({a: prompt_ids})[a]               # of the last new token (every=True: of every one)
     answers = [a] + model.fork(a, 3)
     tokens = model.generate(answers, first_tokens, 64)        # greedy, all in one batch
+    best, scores = model.beam_search([a], logits[None], 4, 64)  # four beams, the best first
     logprobs, entropy = model.score(text_ids, chunk=512)      # of every token of a text given those before it
+
+With a pool of low-rank adapters (kvmix_amd.adapters.AdapterPool) every sequence may have one of its own, model.add(adapter=2).
 
 It stands where the reference's evaluation scripts drive its models (pred_long_benchprofile.py:95-133, Inference-comparision.py:126-153).
 """
 from __future__ import annotations
 
-from typing import Dict, List, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
 from . import ops
+from .adapters import AdapterPool
 from .decoder import DecoderConfig, add_mlp, add_projection, head_logits, rms_norm, rope_tables
 from .paged import PagedKVCache
 
 
 class PagedDecoder:
-    """weights: the dict of decoder.init_weights.  k_bits, v_bits: widths per layer.  row_pages, packed_pages: see PagedKVCache."""
+    """weights: the dict of decoder.init_weights.  k_bits, v_bits: widths per layer.  row_pages, packed_pages: see PagedKVCache.
+    adapters: a pool of which every sequence may have one."""
 
     def __init__(self, cfg: DecoderConfig, weights: dict, k_bits: Sequence[int], v_bits: Sequence[int], row_pages: int = 256,
-                 packed_pages: int = 1024, page_size: int = 64, window: int = 128):
-        self.cfg, self.w = cfg, weights
+                 packed_pages: int = 1024, page_size: int = 64, window: int = 128, adapters: Optional[AdapterPool] = None):
+        self.cfg, self.w, self.adapters = cfg, weights, adapters
+        self._adapter_of: Dict[int, int] = {}  # of the sequences that have one
         self.cache = PagedKVCache(k_bits, v_bits, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, row_pages, packed_pages, page_size, window,
                                   weights["embed"].device)
 
-    def add(self) -> int:
-        return self.cache.new()
+    def add(self, adapter: Optional[int] = None) -> int:
+        if adapter is not None and (self.adapters is None or not 0 <= adapter < self.adapters.count):
+            raise RuntimeError(f"no adapter {adapter} in this model's pool")
+        s = self.cache.new()
+        if adapter is not None:
+            self._adapter_of[s] = adapter
+        return s
 
     def fork(self, s: int, count: int = 1):
-        return self.cache.fork(s, count)
+        made = self.cache.fork(s, count)
+        if s in self._adapter_of:
+            self._adapter_of.update((t, self._adapter_of[s]) for t in ([made] if count == 1 else made))
+        return made
 
     def free(self, s: int) -> None:
         self.cache.free(s)
+        self._adapter_of.pop(s, None)
+
+    def _adapted_layer(self, layer: int, x: torch.Tensor, plan, attend):
+        """A layer of a step in which sequences have adapters: the projections, each with what the adapters add to it."""
+        lw, cfg, pool = self.w["layers"][layer], self.cfg, self.adapters
+        h = rms_norm(x, lw["input_norm"], cfg.rms_norm_eps)
+        out = attend(pool.add(F.linear(h, lw["wqkv"]), h, layer, "wqkv", plan))
+        x = pool.add(add_projection(x, out, lw["wo"]), out, layer, "wo", plan)
+        h = rms_norm(x, lw["post_norm"], cfg.rms_norm_eps)
+        gate, up = pool.add(F.linear(h, lw["w_gate_up"]), h, layer, "w_gate_up", plan).chunk(2, -1)
+        h = F.silu(gate) * up
+        return pool.add(add_projection(x, h, lw["w_down"]), h, layer, "w_down", plan)
 
     @torch.no_grad()
     def forward(self, new_ids: Dict[int, torch.Tensor], every: bool = False) -> Dict[int, torch.Tensor]:
@@ -56,11 +82,18 @@ class PagedDecoder:
         x = self.w["embed"][ids][:, None]                       # [tokens, 1, hidden]: rows, as the projections' kernels take them
         cos, sin = (t[0, 0] for t in rope_tables(cfg, pos, x.dtype))
         nh, nkv = cfg.num_heads, cfg.num_kv_heads
+        of = [self._adapter_of.get(s, -1) for s in new_ids]
+        plan = ops.adapter_plan(of, [i.numel() for i in new_ids.values()], self.adapters.count, device) if max(of) >= 0 else None
         for layer, lw in enumerate(self.w["layers"]):
-            qkv = F.linear(rms_norm(x, lw["input_norm"], cfg.rms_norm_eps), lw["wqkv"]).view(-1, nh + 2 * nkv, cfg.head_dim)
-            q = cache.append_rotated(layer, step, qkv, cos, sin)
-            out = cache.attend(layer, step, q)
-            x = add_projection(x, out.reshape(-1, 1, cfg.hidden_size), lw["wo"])
+            def attend(qkv):
+                q = cache.append_rotated(layer, step, qkv.view(-1, nh + 2 * nkv, cfg.head_dim), cos, sin)
+                return cache.attend(layer, step, q).reshape(-1, 1, cfg.hidden_size)
+
+            if plan is not None:
+                x = self._adapted_layer(layer, x, plan, attend)
+                continue
+            out = attend(F.linear(rms_norm(x, lw["input_norm"], cfg.rms_norm_eps), lw["wqkv"]))
+            x = add_projection(x, out, lw["wo"])
             x = add_mlp(x, lw, cfg.rms_norm_eps)
         spans = step.tokens()
         if not every:
@@ -91,6 +124,56 @@ class PagedDecoder:
             empty = ids.new_empty(len(sequences), max(new_tokens - 1, 0), alternatives)
             return ids, empty.float(), empty
         return ids, *(torch.stack([b[i] for b in best], 1) for i in range(2))
+
+    def beam_search(self, sequences: Sequence[int], logits: torch.Tensor, beams: int, new_tokens: int, end: Optional[int] = None):
+        """Beam search from sequences and the logits [n, vocab] of their last tokens: (token ids [n, beams, new_tokens], sums of
+        their log probabilities [n, beams]), the best first.  A beam ends with the token `end`, which then fills it up.  The
+        sequences stay as they are; the beams are forks of them, which share pages for as long as they agree, and end with the call."""
+        if beams < 1 or new_tokens < 1 or len(set(sequences)) != len(sequences) or logits.shape[:-1] != (len(sequences),):
+            raise RuntimeError("beam_search: a beam and a new token at least, sequences that are different, and a row of logits for each")
+        n, groups = len(sequences), []
+        if not n:
+            return logits.new_empty(0, beams, new_tokens, dtype=torch.int64), logits.new_empty(0, beams, dtype=torch.float32)
+        logits = logits[:, None].expand(n, beams, logits.shape[-1])
+        scores = torch.full((n, beams), float("-inf"), device=logits.device)
+        scores[:, 0] = 0.0  # (the beams of a sequence are alike still)
+        ids = torch.zeros(n * beams, new_tokens, dtype=torch.int64, device=logits.device)
+        first, done = beams * torch.arange(n, device=logits.device)[:, None], None
+        try:
+            for step in range(new_tokens):
+                scores, parents, tokens = ops.beam_select(logits, scores, beams, done, end, stay=True)
+                ops.reorder_rows([ids], (first + parents).reshape(-1))
+                ids[:, step] = tokens.reshape(-1)
+                done = None if end is None else tokens == end
+                if step + 1 == new_tokens:
+                    break
+                if not groups:
+                    for s in sequences:
+                        groups.append([])
+                        for _ in range(beams):  # (one by one: what there are is known if the pages do not suffice)
+                            groups[-1].append(self.fork(s))
+                else:
+                    for group, of in zip(groups, parents.tolist()):
+                        self._replace(group, of)
+                new = [s for group in groups for s in group]
+                out = self.forward({s: tokens.view(-1)[i:i + 1] for i, s in enumerate(new)})
+                logits = torch.stack([out[s] for s in new]).view(n, beams, -1)
+        finally:
+            for group in groups:
+                for s in group:
+                    if s is not None:
+                        self.free(s)
+        scores, order = scores.sort(dim=-1, descending=True, stable=True)
+        return ids.view(n, beams, -1).gather(1, order[:, :, None].expand(-1, -1, new_tokens)), scores
+
+    def _replace(self, group: List[int], parents: List[int]) -> None:
+        """The beams of a sequence become those of their parents: where a beam is not its own, it has no children."""
+        moved = [i for i, p in enumerate(parents) if i != p]
+        for i in moved:
+            self.free(group[i])
+            group[i] = None
+        for i in moved:
+            group[i] = self.fork(group[parents[i]])
 
     def score(self, ids: torch.Tensor, chunk: int = 512):
         """(log probabilities, entropies) [len(ids) - 1] of the tokens of a text after its first, each given those before it, read
