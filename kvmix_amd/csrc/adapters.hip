@@ -3,14 +3,18 @@
 // Bound by memory: the weights of the adapters in use and the activations are read once, two operations for a value of them and rank.
 // Two launches, because every value of y wants all of x:
 //   shrink   u = A x.  A tile is up to 64 tokens of one adapter (kvmix_adapter_plan deals them out, whichever sequences they are of), a
-//            block a tile and a stretch of k, its four waves a quarter of that each.  Ranks are the rows of v_mfma_f32_16x16x32, tokens
-//            its columns, so that a lane has eight k of one row of A and of one token: sixteen bytes, as both lie in memory.  The
-//            waves' sums come together in the LDS, those of the stretches (there are several where there are few tiles) in
-//   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then its waves take 32 columns of y at a time.  u is
-//            kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest to
-//            2^13: next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be off by
-//            2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
+//            block a tile and a stretch of k, its four waves every fourth 64 bytes of that, so that they read rows as they lie.  Ranks
+//            are the rows of v_mfma_f32_16x16x32, tokens its columns, so that a lane has eight k of one row of A and of one token:
+//            sixteen bytes, as both lie in memory.  The waves' sums come together in the LDS, those of the stretches (there are
+//            several where there are few tiles) in
+//   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then its waves take every fourth 32 columns of y.
+//            u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest just
+//            below 2^14 (bf16: 1): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be
+//            off by 2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
 //            columns of one token that follow one another.
+// Both read a step ahead of the one that is multiplied, and expand's first reads go out before it sums u.  8168 tokens of 6 adapters of rank
+// 64, k = n = 4096, bf16: 26 + 38 us, of which reading x alone would take 18 and y with base 35; 1567 tokens of rank 32 from k = 11008
+// to n = 4096: 16 + 12 us.  64 tokens of 40 adapters to n = 12288: 9 us, that is two launches.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
 #include <new>
@@ -25,7 +29,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t *PlanWords;
 
 constexpr int kTile = 64, kSub = 16;       // tokens of a tile, of a column of a matrix product
-constexpr int kTileWords = 4;              // adapter or -1, first of the list, how many, one of no use
+constexpr int kTileWords = 4;              // adapter or -1, first of the list, how many, the first token where they follow one another, else -1
 constexpr int kWaves = 4;
 constexpr int64_t kMostRank = 128;
 
@@ -55,43 +59,67 @@ struct AdapterArgs {
     int rank, padded, k, n, splits, rank_chunks, n_blocks, units;  // units: of 32 columns, of a wave of expand
 };
 
+// Every sixteenth token of a tile from m on (where there is none, the last).
+template <int ST>
+__device__ __forceinline__ void rows_of(int (&row)[ST], const AdapterArgs &p, PlanWords tile, int m)
+{
+    const int last = tile[2] - 1;
+    if (tile[3] >= 0) {
+#pragma unroll
+        for (int s = 0; s < ST; s++) row[s] = tile[3] + min(kSub * s + m, last);
+    } else {
+#pragma unroll
+        for (int s = 0; s < ST; s++) row[s] = p.rows[tile[1] + min(kSub * s + m, last)];
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Ranks [first, first + 16 RT) of a tile of up to 16 ST tokens, over the 32-wide units [from, to) of k.
+// Steps 0 .. count - 1, each read into one of two places while the one before is used; `first` comes after the first reads.
+template <typename L, typename U, typename F>
+__device__ __forceinline__ void in_turn(int count, L load, U use, F first)
+{
+    if (count > 0) load(0, 0);
+    first();
+    int i = 0;
+    for (; i + 3 <= count; i += 2) load(1, i + 1), use(0, i), load(0, i + 2), use(1, i + 1);
+    if (i + 1 < count) load(1, i + 1);
+    if (i < count) use(0, i);
+    if (i + 1 < count) use(1, i + 1);
+}
+
+// Ranks [first, first + 16 RT) of a tile of up to 16 ST tokens, over every fourth of the 32-wide units [begin, to) of k: the waves of a
+// block read what follows one another.  The reads of the next units are under way while one is multiplied.
 template <typename T, int RT, int ST>
-__device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *const (&x)[ST], int from, int to, int k, int g, floatx4 (&acc)[RT][ST])
+__device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *const (&x)[ST], int begin, int to, int k, int g, floatx4 (&acc)[RT][ST])
 {
     typedef typename Vec8<T>::type V;
-    constexpr int UN = RT * ST >= 8 ? 2 : 4;  // units whose reads are in flight together
-    const int whole = min(to, k / 32);
-    int u = from;
-    for (; u + UN <= whole; u += UN) {
-        V av[UN][RT], xv[UN][ST];
-#pragma unroll
-        for (int i = 0; i < UN; i++) {
-#pragma unroll
-            for (int r = 0; r < RT; r++) av[i][r] = *(const V *)(a[r] + 32 * (u + i));
-#pragma unroll
-            for (int s = 0; s < ST; s++) xv[i][s] = *(const V *)(x[s] + 32 * (u + i));
-        }
-#pragma unroll
-        for (int i = 0; i < UN; i++)
-#pragma unroll
-            for (int r = 0; r < RT; r++)
-#pragma unroll
-                for (int s = 0; s < ST; s++) acc[r][s] = product(av[i][r], xv[i][s], acc[r][s]);
-    }
-    for (; u < to; u++) {
-        V av[RT], xv[ST];
-        const bool in = 32 * u + 8 * g < k;  // (k in whole eights)
-#pragma unroll
-        for (int r = 0; r < RT; r++) av[r] = in ? *(const V *)(a[r] + 32 * u) : V{};
-#pragma unroll
-        for (int s = 0; s < ST; s++) xv[s] = in ? *(const V *)(x[s] + 32 * u) : V{};
+    struct Unit {
+        V a[RT], x[ST];
+    } v[2];
+    auto multiply = [&](const Unit &v) {
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
-            for (int s = 0; s < ST; s++) acc[r][s] = product(av[r], xv[s], acc[r][s]);
+            for (int s = 0; s < ST; s++) acc[r][s] = product(v.a[r], v.x[s], acc[r][s]);
+    };
+    const int count = max(0, (min(to, k / 32) - begin + kWaves - 1) / kWaves);
+    auto load = [&](Unit &v, int i) {
+        const int at = 32 * (begin + kWaves * i);
+#pragma unroll
+        for (int r = 0; r < RT; r++) v.a[r] = *(const V *)(a[r] + at);
+#pragma unroll
+        for (int s = 0; s < ST; s++) v.x[s] = *(const V *)(x[s] + at);
+    };
+    in_turn(count, [&](int d, int i) { load(v[d], i); }, [&](int d, int) { multiply(v[d]); }, [] {});
+    const int last = k / 32;
+    if (k % 32 && last < to && last >= begin && (last - begin) % kWaves == 0) {  // (k in whole eights)
+        const bool in = 32 * last + 8 * g < k;
+#pragma unroll
+        for (int r = 0; r < RT; r++) v[0].a[r] = in ? *(const V *)(a[r] + 32 * last) : V{};
+#pragma unroll
+        for (int s = 0; s < ST; s++) v[0].x[s] = in ? *(const V *)(x[s] + 32 * last) : V{};
+        multiply(v[0]);
     }
 }
 
@@ -105,18 +133,19 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
     const int split = blockIdx.x % p.splits, nth = blockIdx.x / p.splits, chunk = nth % p.rank_chunks;
     const PlanWords tile = p.tiles + nth / p.rank_chunks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
-    const int units = (p.k + 31) / 32, begin = (int)((int64_t)units * split / p.splits), length = (int)((int64_t)units * (split + 1) / p.splits) - begin;
-    const int from = begin + length * wave / kWaves, to = begin + length * (wave + 1) / kWaves;
+    const int units = (p.k + 31) / 32, begin = (int)((int64_t)units * split / p.splits), to = (int)((int64_t)units * (split + 1) / p.splits);
     const T *a[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) a[r] = (const T *)p.a + adapter * p.a_as + min((chunk * RT + r) * 16 + m, p.rank - 1) * p.a_rs + 8 * g;  // (what lies beyond is not kept)
     auto run = [&](auto st) {
         constexpr int ST = decltype(st)::value;
         const T *x[ST];
+        int row[ST];
+        rows_of(row, p, tile, m);
 #pragma unroll
-        for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + (int64_t)p.rows[first + min(kSub * s + m, count - 1)] * p.x_ts + 8 * g;
+        for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + row[s] * p.x_ts + 8 * g;
         floatx4 acc[RT][ST] = {};
-        shrink_tile<T, RT, ST>(a, x, from, to, p.k, g, acc);
+        shrink_tile<T, RT, ST>(a, x, begin + wave, to, p.k, g, acc);
 #pragma unroll
         for (int s = 0; s < ST; s++)
             if (s < subs)
@@ -149,76 +178,121 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const PlanWords tile = p.tiles + blockIdx.x / p.n_blocks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
-    const int begin = (blockIdx.x % p.n_blocks * kWaves + wave) * p.units, end = min(begin + p.units, (p.n + 31) / 32);
+    const int begin = blockIdx.x % p.n_blocks * kWaves * p.units, end = min(begin + kWaves * p.units, (p.n + 31) / 32);
     if (adapter < 0) {  // (tokens without one: to be copied)
-        for (int i = begin; i < end; i++) {
+        int row[kTile / kSub];
+        rows_of(row, p, tile, m);
+        for (int i = begin + wave; i < end; i += kWaves) {
             const int column = 32 * i + 8 * g;
-            for (int t = m; t < count && column < p.n; t += 16) {
-                const int64_t row = p.rows[first + t];
-                *(V *)((T *)p.out + row * p.out_ts + column) = *(const V *)((const T *)p.base + row * p.base_ts + column);
-            }
+            if (column >= p.n) break;
+            V y[kTile / kSub];
+#pragma unroll
+            for (int s = 0; s < kTile / kSub; s++) y[s] = *(const V *)((const T *)p.base + row[s] * p.base_ts + column);
+#pragma unroll
+            for (int s = 0; s < kTile / kSub; s++)
+                if (kSub * s + m < count) *(V *)((T *)p.out + row[s] * p.out_ts + column) = y[s];
         }
         return;
     }
-    const int c = threadIdx.x % L;
-    for (int t = threadIdx.x / L; t < subs * kSub; t += 256 / L) {
-        floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (t < count && 4 * c < p.rank) {
-            const float *at = p.part + (int64_t)(first + t) * p.padded + 4 * c;
-            for (int i = 0; i < p.splits; i++) s += *(const floatx4 *)(at + i * p.part_rows * p.padded);
+    auto sum = [&](auto st) {
+        constexpr int kTop = std::is_same<T, _Float16>::value ? 14 : 0;  // (bf16 has all of fp32's exponents: products with B must not leave them)
+        constexpr int P = (decltype(st)::value * kSub * L + 255) / 256, AHEAD = P >= 4 ? 2 : P == 2 ? 4 : 8;  // turns of the block
+        const int c = threadIdx.x % L, t0 = threadIdx.x / L;
+        floatx4 s[P] = {};
+        const float *at[P];
+#pragma unroll
+        for (int j = 0; j < P; j++) at[j] = p.part + (int64_t)(first + min(t0 + 256 / L * j, count - 1)) * p.padded + (4 * c < p.rank ? 4 * c : 0);
+        for (int i = 0; i < p.splits; i += AHEAD) {  // (AHEAD stretches' reads under way; of none: the last one's again, not added)
+            floatx4 q[AHEAD][P];
+#pragma unroll
+            for (int h = 0; h < AHEAD; h++)
+#pragma unroll
+                for (int j = 0; j < P; j++) q[h][j] = *(const floatx4 *)(at[j] + min(i + h, p.splits - 1) * p.part_rows * p.padded);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < AHEAD; h++)
+#pragma unroll
+                for (int j = 0; j < P; j++) s[j] += i + h < p.splits ? q[h][j] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(s[j]) < __builtin_inff() ? fabsf(s[j]) : 0.0f);
+        for (int j = 0; j < P; j++)
+            if (t0 + 256 / L * j >= count || 4 * c >= p.rank) s[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int o = L / 2; o; o /= 2) most = fmaxf(most, __shfl_xor(most, o));
-        // (the power of numbers below 2^-100 is that of 2^-100; infinities go through as they are, and their second part is nothing)
-        const int e = (most > 0.0f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0) - 14;
-        typedef T four __attribute__((ext_vector_type(4)));
-        four high, low;
+        for (int j = 0; j < P; j++) {
+            const int t = t0 + 256 / L * j;
+            float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float v = ldexpf(s[j], -e);
-            const T h = (T)v;
-            high[j] = h, low[j] = fabsf(v) < __builtin_inff() ? (T)(v - (float)h) : (T)0.0f;
+            for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(s[j][r]) < __builtin_inff() ? fabsf(s[j][r]) : 0.0f);
+#pragma unroll
+            for (int o = L / 2; o; o /= 2) most = fmaxf(most, __shfl_xor(most, o));
+            // (the power of numbers below 2^-100 is that of 2^-100; infinities go through as they are, and their second part is nothing)
+            const int e = (most > 0.0f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0) - kTop;
+            typedef T four __attribute__((ext_vector_type(4)));
+            four high, low;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float v = ldexpf(s[j][r], -e);
+                const T h = (T)v;
+                high[r] = h, low[r] = fabsf(v) < __builtin_inff() ? (T)(v - (float)h) : (T)0.0f;
+            }
+            if (t < kTile) {
+                *(four *)&u[t][4 * c] = high;
+                *(four *)&u[t][RX + 4 * c] = low;
+                if (c == 0) power[t] = ldexpf(1.0f, e);
+            }
         }
-        *(four *)&u[t][4 * c] = high;
-        *(four *)&u[t][RX + 4 * c] = low;
-        if (c == 0) power[t] = ldexpf(1.0f, e);
-    }
-    __syncthreads();
+        __syncthreads();
+    };
     const float scale = p.scales ? p.scales[adapter] : 1.0f;
-    const T *b = (const T *)p.b + adapter * p.b_as;
-    for (int i = begin; i < end; i++) {
-        const int n0 = 32 * i, column = n0 + 8 * g;
-        V w[2][NF];
+    auto run = [&](auto st) {
+        constexpr int ST = decltype(st)::value;
+        struct Unit {
+            V w[2][NF], y[ST];  // rows of B, values of base
+        } v[2];
+        const T *from[ST];
+        T *to[ST];
+        int row[ST];
+        rows_of(row, p, tile, m);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int s = 0; s < ST; s++) from[s] = (const T *)p.base + row[s] * p.base_ts + 8 * g, to[s] = (T *)p.out + row[s] * p.out_ts + 8 * g;
+        const int steps = max(0, (end - begin - wave + kWaves - 1) / kWaves);
+        auto load = [&](Unit &v, int i) {
+            const int n0 = 32 * (begin + wave + kWaves * i), column = min(n0 + 8 * g, p.n - 8) - 8 * g;  // (what lies beyond is not kept)
 #pragma unroll
-            for (int f = 0; f < NF; f++) {
-                const int row = min(n0 + 8 * (m / 4) + 4 * h + m % 4, p.n - 1), r = (32 * f + 8 * g) % RX;
-                w[h][f] = r < p.rank ? *(const V *)(b + row * p.b_ns + r) : V{};
+            for (int s = 0; s < ST; s++) v.y[s] = *(const V *)(from[s] + column);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    const int row = min(n0 + 8 * (m / 4) + 4 * h + m % 4, p.n - 1), r = (32 * f + 8 * g) % RX;
+                    v.w[h][f] = *(const V *)((const T *)p.b + adapter * p.b_as + row * p.b_ns + (r < p.rank ? r : 0));  // (of u beyond the rank: nothing)
+                }
+        };
+        auto store = [&](Unit &v, int i) {
+            const int n0 = 32 * (begin + wave + kWaves * i);
+#pragma unroll
+            for (int s = 0; s < ST; s++) {
+                const int t = kSub * s + m;
+                floatx4 acc[2] = {};
+#pragma unroll
+                for (int f = 0; f < RX / 16; f++) {
+                    const V x = *(const V *)&u[t][32 * f + 8 * g];
+                    acc[0] = product(v.w[0][f % NF], x, acc[0]);
+                    acc[1] = product(v.w[1][f % NF], x, acc[1]);
+                }
+                if (t >= count || n0 + 8 * g >= p.n) continue;
+                const float two = power[t];
+                V y = v.y[s];
+#pragma unroll
+                for (int c = 0; c < 8; c++) y[c] = (T)fmaf(acc[c / 4][c % 4] * two, scale, (float)y[c]);
+                *(V *)(to[s] + n0) = y;
             }
-        for (int s = 0; s < subs; s++) {
-            const int t = kSub * s + m;
-            const bool in = t < count && column < p.n;
-            int64_t row = 0;
-            V y{};
-            if (in) row = p.rows[first + t], y = *(const V *)((const T *)p.base + row * p.base_ts + column);
-            floatx4 acc[2] = {};
-#pragma unroll
-            for (int f = 0; f < RX / 16; f++) {
-                const V v = *(const V *)&u[t][32 * f + 8 * g];
-                acc[0] = product(w[0][f % NF], v, acc[0]);
-                acc[1] = product(w[1][f % NF], v, acc[1]);
-            }
-            if (!in) continue;
-            const float two = power[t];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = (T)fmaf(acc[j / 4][j % 4] * two, scale, (float)y[j]);
-            *(V *)((T *)p.out + row * p.out_ts + column) = y;
-        }
-    }
+        };
+        in_turn(steps, [&](int d, int i) { load(v[d], i); }, [&](int d, int i) { store(v[d], i); }, [&] { sum(st); });
+    };
+    if (subs == 1) run(std::integral_constant<int, 1>());
+    else if (subs == 2) run(std::integral_constant<int, 2>());
+    else run(std::integral_constant<int, 4>());
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -256,7 +330,7 @@ int make_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t se
         next[i] = plan->rows_at + first;
         const int64_t tiles = (of[i] + kTile - 1) / kTile, even = tiles ? ((of[i] + tiles - 1) / tiles + kSub - 1) / kSub * kSub : 0;
         for (int64_t t = 0; t < tiles; t++, tile += kTileWords) {
-            tile[0] = i < n_adapters ? (int32_t)i : -1, tile[1] = (int32_t)(first + t * even), tile[3] = 0;
+            tile[0] = i < n_adapters ? (int32_t)i : -1, tile[1] = (int32_t)(first + t * even);
             tile[2] = (int32_t)std::min(even, of[i] - t * even);
         }
         first += of[i];
@@ -264,6 +338,10 @@ int make_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t se
     int32_t token = 0;
     for (int64_t s = 0; s < sequences; s++)
         for (int64_t t = 0; t < counts[s]; t++) words[next[adapters[s] < 0 ? n_adapters : adapters[s]]++] = token++;
+    for (tile = words; tile < words + plan->rows_at; tile += kTileWords) {
+        const int32_t *rows = words + plan->rows_at + tile[1];
+        tile[3] = rows[tile[2] - 1] - rows[0] == tile[2] - 1 ? rows[0] : -1;  // (they ascend)
+    }
     return KVMIX_OK;
 }
 
@@ -271,11 +349,14 @@ int64_t padded_rank(int64_t rank) { return (rank + 15) / 16 * 16; }
 
 int64_t rank_chunks(int64_t rank) { return (rank + 63) / 64; }
 
-// Stretches of k: blocks enough for all CUs, but no less than four units to a wave.
+// Stretches of k: a block for every CU, but no less than four units to a wave.  Twice as many blocks read x no faster (64 x rank 64 over
+// k 4096, 8168 tokens: 25.3 and 26.2 us), and the sums that expand has to gather are twice as many (41.0 and 38.3 us).
+constexpr int64_t kStretches = 256;
+
 int64_t splits_of(const kvmix_adapter_plan_t *plan, int64_t rank, int64_t k)
 {
     const int64_t blocks = std::max<int64_t>(plan->tiles * rank_chunks(rank), 1);
-    return std::max<int64_t>(1, std::min<int64_t>({(512 + blocks - 1) / blocks, k / 512, 16}));
+    return std::max<int64_t>(1, std::min<int64_t>({(kStretches + blocks - 1) / blocks, k / 512, 16}));
 }
 
 bool whole(int64_t v) { return v % 8 == 0; }

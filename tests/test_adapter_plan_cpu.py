@@ -28,6 +28,16 @@ def test_every_token_once(adapters, counts, n):
     assert at == len(tokens)
 
 
+@pytest.mark.parametrize("adapters,counts,n", [([0], [200], 1), ([0, 1, 0], [3, 2, 70], 2), ([-1, 0, -1], [1, 100, 1], 1), ([0, 1] * 40, [1] * 80, 2)])
+def test_pieces_of_tokens_that_follow_one_another(adapters, counts, n):
+    """Their first token, by which they are found without the list, or -1."""
+    plan, words = _lib.adapter_plan(adapters, counts, n)
+    for t in range(plan["tiles"] + plan["bare"]):
+        _, first, count, at = words[4 * t:4 * t + 4]
+        rows = words[plan["rows_at"] + first:plan["rows_at"] + first + count]
+        assert at == (rows[0] if rows == list(range(rows[0], rows[0] + count)) else -1)
+
+
 @pytest.mark.parametrize("adapters,counts,n,code", [([3], [1], 3, -19), ([0], [-1], 1, -8), ([0, 0], [1 << 30, 1], 1, -9), ([0], [1], -1, -8), ([0], [1], (1 << 20) + 1, -9)])
 def test_plans_that_are_refused(adapters, counts, n, code):
     plan = _lib.AdapterPlan()
