@@ -188,3 +188,22 @@ def test_captured_and_on_another_stream(dev):
         torch.cuda.synchronize()
         for j, (_, x, out) in enumerate(graphs):
             assert all(torch.equal(a, b) for a, b in zip(out, ops.beam_select(x, scores, stay=True)))
+
+
+@pytest.mark.parametrize("R,W,V,count,dtype", [
+    (1, 20, 40000, 20, torch.float32),          # some hundred parts of a request, more than a block reads at once
+    (2, 3, 40000, 2, torch.float32),            # few of them, and more than are compared by all threads
+    (1, 64, 33000, 3, torch.float16),
+    (1, 2, 1 << 20, 5, torch.float32),          # more parts to a beam than lanes
+    (1, 32, 1 << 20, 2, torch.bfloat16),        # the largest
+    (1, 3, 5000, 1, torch.float16),
+])
+def test_many_parts(dev, R, W, V, count, dtype):
+    from kvmix_amd import ops
+
+    logits, scores = random(R, W, V, dtype, dev, seed=V)
+    logits[:, :, V // 3:V // 3 + 5] = 25.0  # the best ones are equal, and in one part
+    scores[:, 1:] = scores[:, :1]
+    done = torch.rand(R, W, generator=torch.Generator().manual_seed(3)) < 0.3
+    check(ops.beam_select(logits, scores, count), plain(logits, scores, count))
+    check(ops.beam_select(logits, scores, count, done.to(dev), 7), plain(logits, scores, count, done, 7))
