@@ -56,6 +56,21 @@ def test_any_index(dev, B, kind):
         assert torch.equal(a, b), i
 
 
+@pytest.mark.parametrize("kind", INDEXES)
+@pytest.mark.parametrize("B", [16, 32, 63, 64, 65])
+def test_rows_of_a_wave(dev, B, kind):
+    """As many as lanes, one more, and as many as registers hold; some of them gone round, some copied, in requests of their own."""
+    from kvmix_amd import ops
+
+    index = INDEXES[kind](B, torch.Generator().manual_seed(B + 1))
+    eights = (torch.arange(B) // 8 * 8 + index % 8).clamp(max=B - 1)
+    for i in (index.to(dev), eights.to(dev)):
+        views, _ = tensors(B, dev, seed=1)
+        want = [t[i].clone() for t in views]
+        ops.reorder_rows(views, i)
+        assert all(torch.equal(a, b) for a, b in zip(views, want))
+
+
 def test_many_tensors_and_large_ones(dev):
     """More than one launch takes, an entry beyond 2^31 bytes from the first, NaN and infinities as they are."""
     from kvmix_amd import ops
