@@ -683,7 +683,8 @@ int kvmix_adapter_plan(const int64_t *adapters, const int64_t *counts, int64_t s
  * x [tokens, k], a [adapters, rank, k], b [adapters, n, rank], base, out [tokens, n]: fp16 or bf16 (KVMIX_BF16), unit stride along
  * the last dimension, sizes and strides in whole eights, 16-byte aligned; k and n up to 2^24, rank up to 128.  scales [adapters] fp32,
  * or NULL for 1.  out may be base (the tokens without an adapter are left alone then), but not overlap it otherwise.  Sums in fp32; u = A x
- * is held to 2^-22 (bf16: 2^-16) of the token's largest for the second product; out is rounded once.
+ * is held to 2^-22 (bf16: 2^-16) of the token's largest for the second product; out is rounded once.  Infinite values and NaN of x and base
+ * reach their own token; an infinite one in b may become NaN in its column, of the tokens with that adapter.
  */
 typedef struct kvmix_adapters {
     const void *x, *a, *b, *base;
@@ -726,7 +727,7 @@ int kvmix_beam_select(const kvmix_beam_select_t *p, void *workspace, int64_t wor
 /*
  * Tensors reordered along their first dimension in place, t[i] = old t[index[i]], all with the same index [rows] in device memory (rows up
  * to 1024; an index outside of [0, rows) leaves its row as it is).  Entry i of a tensor lies batch_stride further on than entry
- * i - 1 and is `outer` times `inner` rows of row_bytes; strides in bytes.  Entries must not overlap, and no two tensors may.
+ * i - 1 and is `outer` times `inner` rows of row_bytes; strides in bytes.  Entries must not overlap, and no two tensors may, nor one the index.
  */
 typedef struct kvmix_reorder {
     void *base;

@@ -31,6 +31,8 @@ class AdapterPool:
             raise RuntimeError(f"targets are some of {TARGETS}")
         h, i = cfg.hidden_size, cfg.intermediate_size
         shapes = {"wqkv": ((cfg.num_heads + 2 * cfg.num_kv_heads) * cfg.head_dim, h), "wo": (h, h), "w_gate_up": (2 * i, h), "w_down": (h, i)}
+        if any(size % 8 for t in targets for size in shapes[t]):
+            raise RuntimeError("the projections' sizes must be multiples of 8")
         self.count, self.rank, self.targets = count, rank, tuple(targets)
         self.scales = torch.ones(count, dtype=torch.float32, device=device)
         self._pool: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]] = {}

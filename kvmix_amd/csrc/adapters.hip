@@ -9,7 +9,7 @@
 //            several where there are few tiles) in
 //   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then its waves take every fourth 32 columns of y.
 //            u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest just
-//            below 2^14 (bf16: 1): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be
+//            below 2^14 (bf16: 2): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be
 //            off by 2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
 //            columns of one token that follow one another.
 // Both read a step ahead of the one that is multiplied, and expand's first reads go out before it sums u.  8168 tokens of 6 adapters of rank
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         return;
     }
     auto sum = [&](auto st) {
-        constexpr int kTop = std::is_same<T, _Float16>::value ? 14 : 0;  // (bf16 has all of fp32's exponents: products with B must not leave them)
+        constexpr int kTop = std::is_same<T, _Float16>::value ? 14 : 1;  // (bf16 has all of fp32's exponents: products with B must not leave them)
         constexpr int P = (decltype(st)::value * kSub * L + 255) / 256, AHEAD = P >= 4 ? 2 : P == 2 ? 4 : 8;  // turns of the block
         const int c = threadIdx.x % L, t0 = threadIdx.x / L;
         floatx4 s[P] = {};

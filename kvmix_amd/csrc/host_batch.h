@@ -27,8 +27,8 @@ bool in_pieces(const Tensor &t)
 
 Tensor pieces_of(const Tensor &t) { return in_pieces(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
-// Whether the rows of `a` and what `b` spans have no memory in common: columns beside one another of the same wider rows are apart.
-bool apart(const Tensor &a, const Tensor &b)
+// Whether what two tensors span has no byte in common.
+bool spans_apart(const Tensor &a, const Tensor &b)
 {
     if (!a.numel() || !b.numel()) return true;
     auto span = [](const Tensor &t) {
@@ -37,7 +37,14 @@ bool apart(const Tensor &a, const Tensor &b)
         return n * (int64_t)t.element_size();
     };
     const int64_t from_a = (int64_t)a.data_ptr(), from_b = (int64_t)b.data_ptr();
-    if (from_a + span(a) <= from_b || from_b + span(b) <= from_a) return true;
+    return from_a + span(a) <= from_b || from_b + span(b) <= from_a;
+}
+
+// Whether the rows of `a` and what `b` spans have no memory in common: columns beside one another of the same wider rows are apart.
+bool apart(const Tensor &a, const Tensor &b)
+{
+    if (spans_apart(a, b)) return true;
+    const int64_t from_a = (int64_t)a.data_ptr(), from_b = (int64_t)b.data_ptr();
     const Tensor c = b.dim() == 2 ? b : b.dim() == 3 && (b.size(0) == 1 || b.size(1) == 1) ? b.squeeze(b.size(1) == 1 ? 1 : 0) : Tensor();
     if (!c.defined() || a.size(0) == 1 || c.size(0) == 1 || a.stride(0) != c.stride(0) || a.stride(1) != 1 || c.stride(1) != 1 || a.stride(0) < a.size(1)) return false;
     const int64_t row = a.stride(0) * a.element_size(), off = ((from_b - from_a) % row + row) % row;
@@ -86,7 +93,7 @@ Tensor add_adapters(const Tensor &base_in, const Tensor &x_in, const Tensor &a_i
     if (out_in) {
         const bool in_place = out.data_ptr() == base_in.data_ptr() && out.strides() == base_in.strides();
         if (!in_place && !apart(rows, base_in)) fail("add_adapters: out may be base, but not overlap it otherwise");
-        if (!apart(rows, x_in) || !apart(rows, a_in) || !apart(rows, b_in)) fail("add_adapters: out must not overlap what is read");
+        if (!apart(rows, x_in) || !apart(rows, a_in) || !apart(rows, b_in) || (scales_in && !spans_apart(rows, *scales_in))) fail("add_adapters: out must not overlap what is read");
     }
     const Tensor base = out.data_ptr() == base_in.data_ptr() ? rows : pieces_of(as_rows(base_in)), x = pieces_of(as_rows(x_in));
     const Tensor a = pieces_of(a_in), b = pieces_of(b_in), scales = scales_in ? scales_in->contiguous() : Tensor();
@@ -195,7 +202,12 @@ void reorder_rows(const std::vector<Tensor> &tensors, const Tensor &index_in)
     for (const auto &item : items) bases.push_back(item.base);
     std::sort(bases.begin(), bases.end());
     if (std::adjacent_find(bases.begin(), bases.end()) != bases.end()) fail("reorder_rows: no two tensors may overlap");
-    const Tensor index = index_in.contiguous();
+    Tensor index = index_in.contiguous();
+    for (const Tensor &t : tensors)  // (it is read while they are written)
+        if (!spans_apart(t, index)) {
+            index = index.clone();
+            break;
+        }
     const c10::DeviceGuard guard(index.device());
     check(api.reorder_rows(items.data(), (int64_t)items.size(), index.data_ptr<int64_t>(), rows, stream_of(index)));
 }

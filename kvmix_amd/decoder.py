@@ -172,6 +172,14 @@ def head_logits(x: torch.Tensor, weights: dict, eps: float) -> torch.Tensor:
     return F.linear(rms_norm(x[:, 0], weights["norm"], eps), w).to(torch.float32)
 
 
+def check_beams(beams: int, end: Optional[int], vocab: int) -> None:
+    """What ops.beam_select would refuse in a later step."""
+    if not 1 <= beams <= min(64, vocab):
+        raise RuntimeError("beam_search: between 1 and 64 beams, not more than there are tokens")
+    if end is not None and not 0 <= end < vocab:
+        raise RuntimeError("beam_search: the token that ends a beam is one of the vocabulary")
+
+
 class Decoder:
     """weights: the dict of init_weights; attention: one callable per layer with the signature
     attention(q [B,nh,Q,D], k [B,nkv,Q,D], v [B,nkv,Q,D], cache, attention_mask=..., need_weights=False) ->
@@ -258,8 +266,9 @@ class Decoder:
         from . import ops
         from .cache import reorder_caches
 
-        if beams < 1 or new_tokens < 1 or self.position:
-            raise RuntimeError("beam_search: a beam and a new token at least, from a prompt that nothing is cached of")
+        if new_tokens < 1 or self.position or not prompt_ids.numel():
+            raise RuntimeError("beam_search: a new token at least, from prompts that nothing is cached of")
+        check_beams(beams, end, self.cfg.vocab_size)
         B = prompt_ids.shape[0]
         logits = self.forward(prompt_ids.repeat_interleave(beams, 0))
         ids = prompt_ids.new_zeros(B * beams, new_tokens)

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .adapters import AdapterPool
-from .decoder import DecoderConfig, add_mlp, add_projection, head_logits, rms_norm, rope_tables
+from .decoder import DecoderConfig, add_mlp, add_projection, check_beams, head_logits, rms_norm, rope_tables
 from .paged import PagedKVCache
 
 
@@ -129,8 +129,11 @@ class PagedDecoder:
         """Beam search from sequences and the logits [n, vocab] of their last tokens: (token ids [n, beams, new_tokens], sums of
         their log probabilities [n, beams]), the best first.  A beam ends with the token `end`, which then fills it up.  The
         sequences stay as they are; the beams are forks of them, which share pages for as long as they agree, and end with the call."""
-        if beams < 1 or new_tokens < 1 or len(set(sequences)) != len(sequences) or logits.shape[:-1] != (len(sequences),):
-            raise RuntimeError("beam_search: a beam and a new token at least, sequences that are different, and a row of logits for each")
+        if new_tokens < 1 or len(set(sequences)) != len(sequences) or logits.dim() != 2 or logits.shape[0] != len(sequences):
+            raise RuntimeError("beam_search: a new token at least, sequences that are different, and a row of logits for each")
+        check_beams(beams, end, logits.shape[1])
+        for s in sequences:
+            self.cache.length(s)  # (refuses what is no sequence)
         n, groups = len(sequences), []
         if not n:
             return logits.new_empty(0, beams, new_tokens, dtype=torch.int64), logits.new_empty(0, beams, dtype=torch.float32)
@@ -199,7 +202,7 @@ class PagedDecoder:
 
 def main() -> None:
     """A server in small, on random weights: prompts that arrive in chunks beside sequences that are being answered, several
-    answers from one prompt, and what the quantized cache makes of a text's likelihoods."""
+    answers from one prompt, beams, adapters, and what the quantized cache makes of a text's likelihoods."""
     import argparse
     import time
 
@@ -247,12 +250,26 @@ def main() -> None:
         _, _, _, top = ops.token_logprobs(last[s], last[s].argmax(), top=args.answers)  # each answer begins with another token
         first += list(top)
     ids = timed("answers", len(answers) * (args.new - 1), lambda: model.generate(answers, torch.stack(first), args.new))
+    some = list(texts)[:2]
+    best, scores = timed("beams", len(some) * args.answers * args.new, lambda: model.beam_search(
+        some, torch.stack([model.forward({s: texts[s][-1:]})[s] for s in some]), args.answers, args.new))
+    print("best beams' log probabilities:", [round(float(x), 3) for x in scores[:, 0]])
     print("pages free (fp16, packed):", model.cache.free_pages())
     for s in answers:
         model.free(s)
     text = torch.cat([next(iter(texts.values())), ids[0]])
     lp, entropy = timed("likelihoods", text.numel() - 1, lambda: model.score(text, args.chunk))
     print(f"mean log probability {lp.mean():.4f}, mean entropy {entropy.mean():.4f}")
+    pool = AdapterPool(cfg, 2, 16)
+    for i in range(2):
+        pool.load(i, {(layer, "wo"): (torch.randn(16, cfg.hidden_size, device="cuda") / 64, torch.randn(cfg.hidden_size, 16, device="cuda") / 4)
+                      for layer in range(cfg.num_layers)}, scale=0.1)
+    tuned = PagedDecoder(cfg, weights, bits, bits, adapters=pool)
+    users = [tuned.add(), tuned.add(adapter=0), tuned.add(adapter=1)]
+    prompt = next(iter(texts.values()))[:args.chunk]
+    last = tuned.forward({s: prompt for s in users})
+    ids = timed("answers with adapters", len(users) * (args.new - 1), lambda: tuned.generate(users, torch.stack([last[s].argmax() for s in users]), args.new))
+    print("adapters' answers that differ from the plain one:", int((ids[1:] != ids[:1]).any(-1).sum()))
 
 
 __all__ = ["PagedDecoder"]

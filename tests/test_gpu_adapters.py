@@ -110,6 +110,28 @@ def test_infinities_and_large_values(dev):
         assert torch.equal(torch.isnan(got[7]).cpu(), torch.isnan(plain)) and torch.equal(got[7].double().cpu()[~torch.isnan(plain)], plain[~torch.isnan(plain)])
 
 
+def test_values_at_the_ends_of_the_types(dev):
+    """u as large as fp32 holds and as small as counts, beside weights that bring it back into the type."""
+    from kvmix_amd import ops
+
+    big = torch.finfo(torch.bfloat16).max
+    for xs, a_s, b_s in ((big / 2, 1.0, 1e-36), (2.0 ** 64, 2.0 ** 62, 2.0 ** -120), (2.0 ** -60, 2.0 ** -60, 2.0 ** 118), (2.0 ** -40, 1.0, 2.0 ** 100)):
+        base, x, a, b, _ = _inputs(dev, [20], 1, 8, 8, 16, torch.bfloat16)
+        x, a, b = torch.zeros_like(x), torch.zeros_like(a), b.sign() * b_s
+        x[:, 0], a[0, :, 0] = xs, torch.linspace(0.5, 1, 8) * a_s
+        b, base = b.bfloat16(), base * 0
+        plan = ops.adapter_plan([0], [20], 1, dev)
+        want, tol = _want(base, x, a, b, None, [0], [20])
+        got = ops.add_adapters(base, x, a, b, plan).double().cpu()
+        assert torch.isfinite(want).all() and ((got - want).abs() <= tol).all()
+    base, x, a, b, _ = _inputs(dev, [20], 1, 8, 8, 16, torch.float16)
+    plan = ops.adapter_plan([0], [20], 1, dev)
+    for f in (2.0 ** -14, 2.0 ** -20):  # subnormal x and a: products down to 2^-48
+        want, tol = _want(base * 0, (x * f).half(), (a * f).half(), b, None, [0], [20])
+        got = ops.add_adapters(base * 0, (x * f).half(), (a * f).half(), b, plan).double().cpu()
+        assert ((got - want).abs() <= tol).all()
+
+
 def test_strides_and_shapes(dev):
     """Columns of a wider projection in place, three dimensions, weights that are views, rows that sixteen bytes do not fit."""
     from kvmix_amd import ops

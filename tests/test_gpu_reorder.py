@@ -102,6 +102,17 @@ def test_an_index_that_is_none(dev):
     ops.reorder_rows([torch.empty(0, 5, device=dev)], torch.zeros(0, dtype=torch.int64, device=dev))
 
 
+def test_the_index_among_the_tensors(dev):
+    from kvmix_amd import ops
+
+    for B in (40, 300):
+        index = torch.randperm(B, generator=torch.Generator().manual_seed(B)).to(dev)
+        many = [torch.arange(B, device=dev)[:, None].expand(B, 3000).contiguous(), index, torch.arange(B, device=dev)]
+        want = [t[index] for t in many]
+        ops.reorder_rows(many, index)
+        assert all(torch.equal(a, b) for a, b in zip(many, want))
+
+
 def test_refusals(dev):
     from kvmix_amd import ops
 
