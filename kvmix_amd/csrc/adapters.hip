@@ -3,18 +3,21 @@
 // Bound by memory: the weights of the adapters in use and the activations are read once, two operations for a value of them and rank.
 // Two launches, because every value of y wants all of x:
 //   shrink   u = A x.  A tile is up to 64 tokens of one adapter (kvmix_adapter_plan deals them out, whichever sequences they are of), a
-//            block a tile and a stretch of k, its four waves every fourth 64 bytes of that, so that they read rows as they lie.  Ranks
-//            are the rows of v_mfma_f32_16x16x32, tokens its columns, so that a lane has eight k of one row of A and of one token:
-//            sixteen bytes, as both lie in memory.  The waves' sums come together in the LDS, those of the stretches (there are
-//            several where there are few tiles) in
-//   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then its waves take every fourth 32 columns of y.
-//            u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest just
-//            below 2^14 (bf16: 2): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would be
-//            off by 2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
-//            columns of one token that follow one another.
-// Both read a step ahead of the one that is multiplied, and expand's first reads go out before it sums u.  8168 tokens of 6 adapters of rank
-// 64, k = n = 4096, bf16: 26 + 38 us, of which reading x alone would take 18 and y with base 35; 1567 tokens of rank 32 from k = 11008
-// to n = 4096: 16 + 12 us.  64 tokens of 40 adapters to n = 12288: 9 us, that is two launches.
+//            block a tile and a stretch of k.  Ranks are the rows of v_mfma_f32_16x16x32, tokens its columns, so that a lane has eight k
+//            of one row of A and of one token, sixteen bytes.  The four waves read 256 bytes of each row at once, exchange them in
+//            the LDS and multiply a quarter of these each.  (Sixteen tokens at most: each wave its own quarter, without the LDS,
+//            which latency gains from.)  The waves' sums come together in the LDS, those of the stretches (there are several
+//            where there are few tiles) in
+//   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then takes 128 columns of y at a time, a quarter of them
+//            to a wave.  u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest
+//            just below 2^14 (bf16: 2): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would
+//            be off by 2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
+//            columns of one token that follow one another; through the LDS they come to where 256 bytes of a row of base are.
+// Reads of rows in runs of 256 bytes by a wave are what counts: as the matrix products take them, 64 bytes of each of sixteen rows, the
+// same bytes take 26 us instead of 19 (x) and 38 instead of 28 (base and y).  Both kernels read a step ahead of the one that is multiplied,
+// and expand's first reads go out before it sums u.
+// 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 53 us, 3.8 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
+// k = 11008 to n = 4096: 22 us; 64 tokens of 40 adapters to n = 12288: 8.6 us, that is two launches.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
 #include <new>
@@ -30,7 +33,7 @@ typedef const __attribute__((address_space(4))) int32_t *PlanWords;
 
 constexpr int kTile = 64, kSub = 16;       // tokens of a tile, of a column of a matrix product
 constexpr int kTileWords = 4;              // adapter or -1, first of the list, how many, the first token where they follow one another, else -1
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kStep = 32 * kWaves;  // (values of a row in a step of a block)
 constexpr int64_t kMostRank = 128;
 
 template <typename T>
@@ -59,23 +62,32 @@ struct AdapterArgs {
     int rank, padded, k, n, splits, rank_chunks, n_blocks, units;  // units: of 32 columns, of a wave of expand
 };
 
-// Every sixteenth token of a tile from m on (where there is none, the last).
+// Every `step`th token of a tile from `from` on (where there is none, the last).
 template <int ST>
-__device__ __forceinline__ void rows_of(int (&row)[ST], const AdapterArgs &p, PlanWords tile, int m)
+__device__ __forceinline__ void rows_of(int (&row)[ST], const AdapterArgs &p, PlanWords tile, int from, int step)
 {
     const int last = tile[2] - 1;
     if (tile[3] >= 0) {
 #pragma unroll
-        for (int s = 0; s < ST; s++) row[s] = tile[3] + min(kSub * s + m, last);
+        for (int s = 0; s < ST; s++) row[s] = tile[3] + min(step * s + from, last);
     } else {
 #pragma unroll
-        for (int s = 0; s < ST; s++) row[s] = p.rows[tile[1] + min(kSub * s + m, last)];
+        for (int s = 0; s < ST; s++) row[s] = p.rows[tile[1] + min(step * s + from, last)];
     }
+}
+
+// Waves meet; what each has written to the LDS is seen by all.  Reads of memory stay under way.
+__device__ __forceinline__ void meet()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Steps 0 .. count - 1, each read into one of two places while the one before is used; `first` comes after the first reads.
+// Steps 0 .. count - 1, each read into one of two places while the one before is used; `first` comes after the first reads.  (Three or
+// four places gained nothing.)
 template <typename L, typename U, typename F>
 __device__ __forceinline__ void in_turn(int count, L load, U use, F first)
 {
@@ -105,7 +117,7 @@ __device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *co
     };
     const int count = max(0, (min(to, k / 32) - begin + kWaves - 1) / kWaves);
     auto load = [&](Unit &v, int i) {
-        const int at = 32 * (begin + kWaves * i);
+        const int at = 32 * (begin + kWaves * i) + 8 * g;
 #pragma unroll
         for (int r = 0; r < RT; r++) v.a[r] = *(const V *)(a[r] + at);
 #pragma unroll
@@ -116,36 +128,92 @@ __device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *co
     if (k % 32 && last < to && last >= begin && (last - begin) % kWaves == 0) {  // (k in whole eights)
         const bool in = 32 * last + 8 * g < k;
 #pragma unroll
-        for (int r = 0; r < RT; r++) v[0].a[r] = in ? *(const V *)(a[r] + 32 * last) : V{};
+        for (int r = 0; r < RT; r++) v[0].a[r] = in ? *(const V *)(a[r] + 32 * last + 8 * g) : V{};
 #pragma unroll
-        for (int s = 0; s < ST; s++) v[0].x[s] = in ? *(const V *)(x[s] + 32 * last) : V{};
+        for (int s = 0; s < ST; s++) v[0].x[s] = in ? *(const V *)(x[s] + 32 * last + 8 * g) : V{};
         multiply(v[0]);
     }
+}
+
+// The same over whole steps of kStep of k through the LDS: a wave reads a quarter of the rows of A and x, 256 bytes of each at once, and
+// multiplies one of a step's four units.  A row's pieces of sixteen bytes are exchanged by its number, so that no lanes meet in a bank.
+template <typename T, int RT, int ST>
+__device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *const (&x)[ST], void *lds, int begin, int to, int k, int wave, int m,
+                                              int g, floatx4 (&acc)[RT][ST])
+{
+    typedef typename Vec8<T>::type V;
+    typedef V Rows[16];
+    Rows *buffer = (Rows *)lds;  // two steps: rows of A, then of x
+    struct Step {
+        V a[RT], x[ST];
+    } v[2];
+    auto load = [&](Step &v, int i) {
+        const int at = begin + kStep * i + 8 * m;
+#pragma unroll
+        for (int r = 0; r < RT; r++) v.a[r] = *(const V *)(a[r] + min(at, k - 8));
+#pragma unroll
+        for (int s = 0; s < ST; s++) v.x[s] = *(const V *)(x[s] + min(at, k - 8));
+        if (begin + kStep * i + kStep > k && at >= k) {  // (k in whole eights)
+#pragma unroll
+            for (int r = 0; r < RT; r++) v.a[r] = V{};
+#pragma unroll
+            for (int s = 0; s < ST; s++) v.x[s] = V{};
+        }
+    };
+    auto multiply = [&](const Step &v, int i) {
+        Rows *rows_a = buffer + i % 2 * 16 * (RT + ST), *rows_x = rows_a + 16 * RT;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const int row = wave * 4 * RT + g + 4 * r;
+            rows_a[row][m ^ row % 16] = v.a[r];
+        }
+#pragma unroll
+        for (int s = 0; s < ST; s++) {
+            const int row = wave * 4 * ST + g + 4 * s;
+            rows_x[row][m ^ row % 16] = v.x[s];
+        }
+        meet();  // (who is here has multiplied what lay in the other half)
+        V xv[ST];
+#pragma unroll
+        for (int s = 0; s < ST; s++) xv[s] = rows_x[16 * s + m][4 * wave + g ^ m];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const V av = rows_a[16 * r + m][4 * wave + g ^ m];
+#pragma unroll
+            for (int s = 0; s < ST; s++) acc[r][s] = product(av, xv[s], acc[r][s]);
+        }
+    };
+    in_turn((to - begin + kStep - 1) / kStep, [&](int d, int i) { load(v[d], i); }, [&](int d, int i) { multiply(v[d], i); }, [] {});
+    meet();  // (the LDS is wanted for the sums)
 }
 
 template <typename T, int RT>
 __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 {
     constexpr int LD = RT * 16, Q = RT * 4;
-    extern __shared__ float sums[];  // [waves][tokens][ranks]; the fours of ranks of token t in an order of its own, so that lanes meet in no bank
+    // [waves][tokens][ranks]; the fours of ranks of token t in an order of its own, so that lanes meet in no bank
+    extern __shared__ __attribute__((aligned(16))) float sums[];
     auto place = [](int row, int t, int four) { return row * LD + 4 * (four ^ t % Q); };
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const int split = blockIdx.x % p.splits, nth = blockIdx.x / p.splits, chunk = nth % p.rank_chunks;
     const PlanWords tile = p.tiles + nth / p.rank_chunks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
-    const int units = (p.k + 31) / 32, begin = (int)((int64_t)units * split / p.splits), to = (int)((int64_t)units * (split + 1) / p.splits);
-    const T *a[RT];
-#pragma unroll
-    for (int r = 0; r < RT; r++) a[r] = (const T *)p.a + adapter * p.a_as + min((chunk * RT + r) * 16 + m, p.rank - 1) * p.a_rs + 8 * g;  // (what lies beyond is not kept)
+    const int steps = (p.k + kStep - 1) / kStep;
+    const int begin = steps * split / p.splits * kStep, to = steps * (split + 1) / p.splits * kStep;  // (2^17 steps, 16 stretches at most)
     auto run = [&](auto st) {
         constexpr int ST = decltype(st)::value;
-        const T *x[ST];
+        const T *a[RT], *x[ST];
         int row[ST];
-        rows_of(row, p, tile, m);
-#pragma unroll
-        for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + row[s] * p.x_ts + 8 * g;
         floatx4 acc[RT][ST] = {};
-        shrink_tile<T, RT, ST>(a, x, begin + wave, to, p.k, g, acc);
+        const bool staged = ST > 1;
+        rows_of(row, p, tile, staged ? wave * 4 * ST + g : m, staged ? 4 : kSub);
+#pragma unroll
+        for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + row[s] * p.x_ts;
+#pragma unroll
+        for (int r = 0; r < RT; r++)  // (what lies beyond the rank is not kept)
+            a[r] = (const T *)p.a + adapter * p.a_as + min(chunk * RT * 16 + (staged ? wave * 4 * RT + g + 4 * r : 16 * r + m), p.rank - 1) * p.a_rs;
+        if constexpr (ST > 1) shrink_staged<T, RT, ST>(a, x, sums, begin, to, p.k, wave, m, g, acc);
+        else shrink_tile<T, RT, ST>(a, x, begin / 32 + wave, min(to, p.k + 31) / 32, p.k, g, acc);
 #pragma unroll
         for (int s = 0; s < ST; s++)
             if (s < subs)
@@ -173,24 +241,27 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 {
     typedef typename Vec8<T>::type V;
     constexpr int NF = RX >= 32 ? RX / 32 : 1, LD = 2 * RX + 8, L = RX / 4;  // pieces of a row of B; of u: its two parts; lanes to a token
+    constexpr int COLUMNS = 32 * kWaves;                                     // of y, in a step of the block
     __shared__ alignas(16) T u[kTile][LD];
     __shared__ float power[kTile];
+    __shared__ alignas(16) float sums[kTile][COLUMNS + 4];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const PlanWords tile = p.tiles + blockIdx.x / p.n_blocks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
-    const int begin = blockIdx.x % p.n_blocks * kWaves * p.units, end = min(begin + kWaves * p.units, (p.n + 31) / 32);
+    const int begin = blockIdx.x % p.n_blocks * p.units * COLUMNS, steps = (min(p.n - begin, p.units * COLUMNS) + COLUMNS - 1) / COLUMNS;
     if (adapter < 0) {  // (tokens without one: to be copied)
-        int row[kTile / kSub];
-        rows_of(row, p, tile, m);
-        for (int i = begin + wave; i < end; i += kWaves) {
-            const int column = 32 * i + 8 * g;
+        constexpr int ST = kTile / kSub;
+        int row[ST];
+        rows_of(row, p, tile, wave * 4 * ST + g, 4);
+        for (int i = 0; i < steps; i++) {
+            const int column = begin + COLUMNS * i + 8 * m;
             if (column >= p.n) break;
-            V y[kTile / kSub];
+            V y[ST];
 #pragma unroll
-            for (int s = 0; s < kTile / kSub; s++) y[s] = *(const V *)((const T *)p.base + row[s] * p.base_ts + column);
+            for (int s = 0; s < ST; s++) y[s] = *(const V *)((const T *)p.base + row[s] * p.base_ts + column);
 #pragma unroll
-            for (int s = 0; s < kTile / kSub; s++)
-                if (kSub * s + m < count) *(V *)((T *)p.out + row[s] * p.out_ts + column) = y[s];
+            for (int s = 0; s < ST; s++)
+                if (wave * 4 * ST + g + 4 * s < count) *(V *)((T *)p.out + row[s] * p.out_ts + column) = y[s];
         }
         return;
     }
@@ -241,7 +312,7 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
                 if (c == 0) power[t] = ldexpf(1.0f, e);
             }
         }
-        __syncthreads();
+        meet();
     };
     const float scale = p.scales ? p.scales[adapter] : 1.0f;
     auto run = [&](auto st) {
@@ -252,24 +323,23 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         const T *from[ST];
         T *to[ST];
         int row[ST];
-        rows_of(row, p, tile, m);
+        const int t0 = wave * 4 * ST + g;  // a wave reads and writes every fourth of 4 ST tokens, 256 bytes of each at once
+        rows_of(row, p, tile, t0, 4);
 #pragma unroll
-        for (int s = 0; s < ST; s++) from[s] = (const T *)p.base + row[s] * p.base_ts + 8 * g, to[s] = (T *)p.out + row[s] * p.out_ts + 8 * g;
-        const int steps = max(0, (end - begin - wave + kWaves - 1) / kWaves);
+        for (int s = 0; s < ST; s++) from[s] = (const T *)p.base + row[s] * p.base_ts, to[s] = (T *)p.out + row[s] * p.out_ts;
         auto load = [&](Unit &v, int i) {
-            const int n0 = 32 * (begin + wave + kWaves * i), column = min(n0 + 8 * g, p.n - 8) - 8 * g;  // (what lies beyond is not kept)
-#pragma unroll
-            for (int s = 0; s < ST; s++) v.y[s] = *(const V *)(from[s] + column);
+            const int column = begin + COLUMNS * i;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    const int row = min(n0 + 8 * (m / 4) + 4 * h + m % 4, p.n - 1), r = (32 * f + 8 * g) % RX;
-                    v.w[h][f] = *(const V *)((const T *)p.b + adapter * p.b_as + row * p.b_ns + (r < p.rank ? r : 0));  // (of u beyond the rank: nothing)
+                for (int f = 0; f < NF; f++) {  // (what lies beyond is not kept; of u beyond the rank: nothing)
+                    const int row = min(column + 32 * wave + 8 * (m / 4) + 4 * h + m % 4, p.n - 1), r = (32 * f + 8 * g) % RX;
+                    v.w[h][f] = *(const V *)((const T *)p.b + adapter * p.b_as + row * p.b_ns + (r < p.rank ? r : 0));
                 }
+#pragma unroll
+            for (int s = 0; s < ST; s++) v.y[s] = *(const V *)(from[s] + min(column + 8 * m, p.n - 8));
         };
         auto store = [&](Unit &v, int i) {
-            const int n0 = 32 * (begin + wave + kWaves * i);
 #pragma unroll
             for (int s = 0; s < ST; s++) {
                 const int t = kSub * s + m;
@@ -280,13 +350,25 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
                     acc[0] = product(v.w[0][f % NF], x, acc[0]);
                     acc[1] = product(v.w[1][f % NF], x, acc[1]);
                 }
-                if (t >= count || n0 + 8 * g >= p.n) continue;
                 const float two = power[t];
+#pragma unroll
+                for (int h = 0; h < 2; h++) *(floatx4 *)&sums[t][32 * wave + 8 * g + 4 * h] = acc[h] * two;
+            }
+            meet();
+            const int column = begin + COLUMNS * i + 8 * m;
+#pragma unroll
+            for (int s = 0; s < ST; s++) {
+                const int t = t0 + 4 * s;
                 V y = v.y[s];
 #pragma unroll
-                for (int c = 0; c < 8; c++) y[c] = (T)fmaf(acc[c / 4][c % 4] * two, scale, (float)y[c]);
-                *(V *)(to[s] + n0) = y;
+                for (int h = 0; h < 2; h++) {
+                    const floatx4 d = *(const floatx4 *)&sums[t][8 * m + 4 * h];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) y[4 * h + c] = (T)fmaf(d[c], scale, (float)y[4 * h + c]);
+                }
+                if (t < count && column < p.n) *(V *)(to[s] + column) = y;
             }
+            meet();
         };
         in_turn(steps, [&](int d, int i) { load(v[d], i); }, [&](int d, int i) { store(v[d], i); }, [&] { sum(st); });
     };
@@ -349,14 +431,14 @@ int64_t padded_rank(int64_t rank) { return (rank + 15) / 16 * 16; }
 
 int64_t rank_chunks(int64_t rank) { return (rank + 63) / 64; }
 
-// Stretches of k: a block for every CU, but no less than four units to a wave.  Twice as many blocks read x no faster (64 x rank 64 over
-// k 4096, 8168 tokens: 25.3 and 26.2 us), and the sums that expand has to gather are twice as many (41.0 and 38.3 us).
+// Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
+// gather are twice as many (expand of 8168 tokens at rank 64: 41.0 and 38.3 us before its rows were read in runs).
 constexpr int64_t kStretches = 256;
 
 int64_t splits_of(const kvmix_adapter_plan_t *plan, int64_t rank, int64_t k)
 {
     const int64_t blocks = std::max<int64_t>(plan->tiles * rank_chunks(rank), 1);
-    return std::max<int64_t>(1, std::min<int64_t>({(kStretches + blocks - 1) / blocks, k / 512, 16}));
+    return std::max<int64_t>(1, std::min<int64_t>({kStretches / blocks, k / 512, 16}));
 }
 
 bool whole(int64_t v) { return v % 8 == 0; }
@@ -426,7 +508,7 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
     p.rank = (int)c->rank, p.padded = (int)padded_rank(c->rank), p.k = (int)c->k, p.n = (int)c->n;
     p.splits = (int)splits_of(plan, c->rank, c->k), p.rank_chunks = (int)rank_chunks(c->rank);
     const int64_t shrink = plan->tiles * p.rank_chunks * p.splits, tiles = plan->tiles + (in_place ? 0 : plan->bare), columns = (c->n + 31) / 32;
-    p.units = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * columns / (kWaves * 512)));
+    p.units = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * columns / (kWaves * 384)));
     p.n_blocks = (int)((columns + kWaves * p.units - 1) / (kWaves * p.units));
     if (shrink > kMostBlocks || tiles * p.n_blocks > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
@@ -434,7 +516,8 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
         using T = decltype(zero);
         with_rank(c->rank, [&](auto RX) {
             constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
-            const size_t lds = (size_t)kWaves * ((plan->most + kSub - 1) / kSub) * kSub * (RT * 16) * sizeof(float);
+            const size_t subs = (plan->most + kSub - 1) / kSub, sums = kWaves * subs * kSub * (RT * 16) * sizeof(float);
+            const size_t staged = subs == 1 ? 0 : 2 * kSub * (RT + (subs == 2 ? 2 : 4)) * 256, lds = std::max(sums, staged);
             if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
             if (tiles) adapter_expand<T, RX.value><<<(unsigned)(tiles * p.n_blocks), 256, 0, st>>>(p);
         });
