@@ -50,6 +50,9 @@ CASES = [
     ([1] * 3, [17, 15, 65], 2, 72, 40, 24),
     ([-1, -1], [5, 100], 1, 16, 64, 72),
     ([0] * 130, [1] * 130, 1, 8, 11008, 96),
+    ([0, 1, 2], [20, 31, 17], 3, 8, 136, 136),      # tiles of two sixteens, k a little more than a step
+    ([1, 0], [64, 300], 2, 48, 5000, 1160),         # stretches of k that are not alike, the last step cut off
+    ([0, 0, 0], [40, 1, 60], 1, 16, 128, 128),
 ]
 
 
