@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests beside a projection that they share:  y_t = base_t + s_i B_i (A_i x_t), i the adapter of token t.
 //
 // Bound by memory: the weights of the adapters in use and the activations are read once, two operations for a value of them and rank.
-// Two launches, because every value of y wants all of x:
+// Two launches, because every value of y wants all of x (and one where that is little):
 //   shrink   u = A x.  A tile is up to 64 tokens of one adapter (kvmix_adapter_plan deals them out, whichever sequences they are of), a
 //            block a tile and a stretch of k.  Ranks are the rows of v_mfma_f32_16x16x32, tokens its columns, so that a lane has eight k
 //            of one row of A and of one token, sixteen bytes.  The four waves read 256 bytes of each row at once, exchange them in
@@ -16,6 +16,7 @@
 // Reads of rows in runs of 256 bytes by a wave are what counts: as the matrix products take them, 64 bytes of each of sixteen rows, the
 // same bytes take 26 us instead of 19 (x) and 38 instead of 28 (base and y).  Both kernels read a step ahead of the one that is multiplied,
 // and expand's first reads go out before it sums u.
+// One token with an adapter of rank 8, k = n = 4096: 6.0 us, one launch and the reads of A by each of its 32 blocks.
 // 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 53 us, 3.8 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
 // k = 11008 to n = 4096: 22 us; 64 tokens of 40 adapters to n = 12288: 8.6 us, that is two launches.
 // Sums in fp32; y is rounded once.
@@ -100,42 +101,41 @@ __device__ __forceinline__ void in_turn(int count, L load, U use, F first)
     if (i + 1 < count) use(1, i + 1);
 }
 
-// Ranks [first, first + 16 RT) of a tile of up to 16 ST tokens, over every fourth of the 32-wide units [begin, to) of k: the waves of a
-// block read what follows one another.  The reads of the next units are under way while one is multiplied.
-template <typename T, int RT, int ST>
-__device__ __forceinline__ void shrink_tile(const T *const (&a)[RT], const T *const (&x)[ST], int begin, int to, int k, int g, floatx4 (&acc)[RT][ST])
+// Ranks [first, first + 16 RT) of a tile of up to sixteen tokens, over a quarter of the 32-wide units [begin, to) of k: every fourth UN of them,
+// which are read at once.
+template <int UN, typename T, int RT>
+__device__ __forceinline__ void shrink_few(const T *const (&a)[RT], const T *x, int begin, int to, int k, int wave, int g, floatx4 (&acc)[RT][1])
 {
     typedef typename Vec8<T>::type V;
-    struct Unit {
-        V a[RT], x[ST];
+    struct Units {
+        V a[UN][RT], x[UN];
     } v[2];
-    auto multiply = [&](const Unit &v) {
+    const int groups = max(0, (min(to, k / 32) - begin) / UN);
+    auto load = [&](Units &v, int i) {
+        const int at = 32 * (begin + UN * (wave + kWaves * i)) + 8 * g;
 #pragma unroll
-        for (int r = 0; r < RT; r++)
+        for (int j = 0; j < UN; j++) {
+            v.x[j] = *(const V *)(x + at + 32 * j);
 #pragma unroll
-            for (int s = 0; s < ST; s++) acc[r][s] = product(v.a[r], v.x[s], acc[r][s]);
+            for (int r = 0; r < RT; r++) v.a[j][r] = *(const V *)(a[r] + at + 32 * j);
+        }
     };
-    const int count = max(0, (min(to, k / 32) - begin + kWaves - 1) / kWaves);
-    auto load = [&](Unit &v, int i) {
-        const int at = 32 * (begin + kWaves * i) + 8 * g;
+    auto multiply = [&](const Units &v) {
 #pragma unroll
-        for (int r = 0; r < RT; r++) v.a[r] = *(const V *)(a[r] + at);
+        for (int j = 0; j < UN; j++)
 #pragma unroll
-        for (int s = 0; s < ST; s++) v.x[s] = *(const V *)(x[s] + at);
+            for (int r = 0; r < RT; r++) acc[r][0] = product(v.a[j][r], v.x[j], acc[r][0]);
     };
-    in_turn(count, [&](int d, int i) { load(v[d], i); }, [&](int d, int) { multiply(v[d]); }, [] {});
-    const int last = k / 32;
-    if (k % 32 && last < to && last >= begin && (last - begin) % kWaves == 0) {  // (k in whole eights)
-        const bool in = 32 * last + 8 * g < k;
+    in_turn((groups - wave + kWaves - 1) / kWaves, [&](int d, int i) { load(v[d], i); }, [&](int d, int) { multiply(v[d]); }, [] {});
+    for (int u = begin + UN * groups + wave; u < to; u += kWaves) {
+        const bool in = 32 * u + 8 * g < k;  // (k in whole eights)
+        const V xv = in ? *(const V *)(x + 32 * u + 8 * g) : V{};
 #pragma unroll
-        for (int r = 0; r < RT; r++) v[0].a[r] = in ? *(const V *)(a[r] + 32 * last + 8 * g) : V{};
-#pragma unroll
-        for (int s = 0; s < ST; s++) v[0].x[s] = in ? *(const V *)(x[s] + 32 * last + 8 * g) : V{};
-        multiply(v[0]);
+        for (int r = 0; r < RT; r++) acc[r][0] = product(in ? *(const V *)(a[r] + 32 * u + 8 * g) : V{}, xv, acc[r][0]);
     }
 }
 
-// The same over whole steps of kStep of k through the LDS: a wave reads a quarter of the rows of A and x, 256 bytes of each at once, and
+// The same of more tokens, over whole steps of kStep of k through the LDS: a wave reads a quarter of the rows of A and x, 256 bytes of each at once, and
 // multiplies one of a step's four units.  A row's pieces of sixteen bytes are exchanged by its number, so that no lanes meet in a bank.
 template <typename T, int RT, int ST>
 __device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *const (&x)[ST], void *lds, int begin, int to, int k, int wave, int m,
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
         for (int r = 0; r < RT; r++)  // (what lies beyond the rank is not kept)
             a[r] = (const T *)p.a + adapter * p.a_as + min(chunk * RT * 16 + (staged ? wave * 4 * RT + g + 4 * r : 16 * r + m), p.rank - 1) * p.a_rs;
         if constexpr (ST > 1) shrink_staged<T, RT, ST>(a, x, sums, begin, to, p.k, wave, m, g, acc);
-        else shrink_tile<T, RT, ST>(a, x, begin / 32 + wave, min(to, p.k + 31) / 32, p.k, g, acc);
+        else shrink_few<RT <= 2 ? 4 : 2>(a, x[0], begin / 32, min(to, p.k + 31) / 32, p.k, wave, g, acc);
 #pragma unroll
         for (int s = 0; s < ST; s++)
             if (s < subs)
@@ -235,8 +235,9 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-// RX: the rank, rounded up to 16, 32, 64 or 128.
-template <typename T, int RX>
+// RX: the rank, rounded up to 16, 32, 64 or 128.  WHOLE: every block makes all of u itself, of tiles of up to sixteen tokens, and there is no
+// other launch.
+template <typename T, int RX, bool WHOLE>
 __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 {
     typedef typename Vec8<T>::type V;
@@ -270,20 +271,36 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         constexpr int P = (decltype(st)::value * kSub * L + 255) / 256, AHEAD = P >= 4 ? 2 : P == 2 ? 4 : 8;  // turns of the block
         const int c = threadIdx.x % L, t0 = threadIdx.x / L;
         floatx4 s[P] = {};
-        const float *at[P];
+        if constexpr (WHOLE) {
+            constexpr int RT = RX / 16;
+            const T *a[RT];
+            int row[1];
+            rows_of(row, p, tile, m, kSub);
 #pragma unroll
-        for (int j = 0; j < P; j++) at[j] = p.part + (int64_t)(first + min(t0 + 256 / L * j, count - 1)) * p.padded + (4 * c < p.rank ? 4 * c : 0);
-        for (int i = 0; i < p.splits; i += AHEAD) {  // (AHEAD stretches' reads under way; of none: the last one's again, not added)
-            floatx4 q[AHEAD][P];
+            for (int r = 0; r < RT; r++) a[r] = (const T *)p.a + adapter * p.a_as + min(16 * r + m, p.rank - 1) * p.a_rs;
+            floatx4 acc[RT][1] = {};
+            shrink_few<RT <= 2 ? 4 : 2>(a, (const T *)p.x + row[0] * p.x_ts, 0, (p.k + 31) / 32, p.k, wave, g, acc);
 #pragma unroll
-            for (int h = 0; h < AHEAD; h++)
+            for (int r = 0; r < RT; r++) *(floatx4 *)&sums[wave * kSub + m][16 * r + 4 * g] = acc[r][0];
+            meet();
 #pragma unroll
-                for (int j = 0; j < P; j++) q[h][j] = *(const floatx4 *)(at[j] + min(i + h, p.splits - 1) * p.part_rows * p.padded);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int w = 0; w < kWaves; w++) s[0] += *(const floatx4 *)&sums[w * kSub + t0 % kSub][4 * c];
+        } else {
+            const float *at[P];
 #pragma unroll
-            for (int h = 0; h < AHEAD; h++)
+            for (int j = 0; j < P; j++) at[j] = p.part + (int64_t)(first + min(t0 + 256 / L * j, count - 1)) * p.padded + (4 * c < p.rank ? 4 * c : 0);
+            for (int i = 0; i < p.splits; i += AHEAD) {  // (AHEAD stretches' reads under way; of none: the last one's again, not added)
+                floatx4 q[AHEAD][P];
 #pragma unroll
-                for (int j = 0; j < P; j++) s[j] += i + h < p.splits ? q[h][j] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int h = 0; h < AHEAD; h++)
+#pragma unroll
+                    for (int j = 0; j < P; j++) q[h][j] = *(const floatx4 *)(at[j] + min(i + h, p.splits - 1) * p.part_rows * p.padded);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < AHEAD; h++)
+#pragma unroll
+                    for (int j = 0; j < P; j++) s[j] += i + h < p.splits ? q[h][j] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
         }
 #pragma unroll
         for (int j = 0; j < P; j++)
@@ -372,9 +389,11 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         };
         in_turn(steps, [&](int d, int i) { load(v[d], i); }, [&](int d, int i) { store(v[d], i); }, [&] { sum(st); });
     };
-    if (subs == 1) run(std::integral_constant<int, 1>());
-    else if (subs == 2) run(std::integral_constant<int, 2>());
-    else run(std::integral_constant<int, 4>());
+    if (WHOLE || subs == 1) run(std::integral_constant<int, 1>());
+    else if constexpr (!WHOLE) {
+        if (subs == 2) run(std::integral_constant<int, 2>());
+        else run(std::integral_constant<int, 4>());
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -431,6 +450,27 @@ int64_t padded_rank(int64_t rank) { return (rank + 15) / 16 * 16; }
 
 int64_t rank_chunks(int64_t rank) { return (rank + 63) / 64; }
 
+// Pieces of the columns of y, and how many steps each has.
+struct ExpandPlan {
+    int64_t tiles, units, blocks;
+};
+
+ExpandPlan expand_plan(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
+{
+    const int64_t tiles = plan->tiles + (c->out == c->base ? 0 : plan->bare), columns = (c->n + 31) / 32;
+    const int64_t units = std::max<int64_t>(1, std::min<int64_t>(8, tiles * columns / (kWaves * 384)));
+    return {tiles, units, (columns + kWaves * units - 1) / (kWaves * units)};
+}
+
+// One launch instead of two: where the tiles are of few tokens, a block finds a CU of its own and has at most 128 KB of A to read (4096 of
+// rank 16).  One to eight tokens, k = n = 4096: 6.0 us instead of 8.5 launched one after the other, 5.8 instead of 5.4 in a graph; k 2048:
+// 4.3 instead of 5.4 there; k 11008: 10.7 instead of 6.0; twice as many blocks as CUs: 9 instead of 5.8.
+bool whole_u(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
+{
+    const int64_t blocks = (plan->tiles + plan->bare) * ((c->n + 32 * kWaves - 1) / (32 * kWaves));
+    return plan->tiles && plan->most <= kSub && c->rank <= 64 && c->k * padded_rank(c->rank) <= 65536 && blocks <= 256;
+}
+
 // Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
 // gather are twice as many (expand of 8168 tokens at rank 64: 41.0 and 38.3 us before its rows were read in runs).
 constexpr int64_t kStretches = 256;
@@ -485,7 +525,7 @@ extern "C" int kvmix_adapter_plan(const int64_t *adapters, const int64_t *counts
 
 extern "C" int64_t kvmix_add_adapters_workspace_bytes(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
 {
-    if (adapters_check(plan, c) != KVMIX_OK) return 0;
+    if (adapters_check(plan, c) != KVMIX_OK || whole_u(plan, c)) return 0;
     return splits_of(plan, c->rank, c->k) * plan->rows * padded_rank(c->rank) * (int64_t)sizeof(float);
 }
 
@@ -496,8 +536,7 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
     if (rc != KVMIX_OK) return rc;
     if (plan->tokens == 0) return KVMIX_OK;
     if (!c->x || !c->base || !c->out || !list || (plan->rows && (!c->a || !c->b))) return KVMIX_ERR_NULL;
-    const bool in_place = c->out == c->base;
-    if (in_place && c->out_token_stride != c->base_token_stride) return KVMIX_ERR_SHAPE;
+    if (c->out == c->base && c->out_token_stride != c->base_token_stride) return KVMIX_ERR_SHAPE;
     const int64_t need = kvmix_add_adapters_workspace_bytes(plan, c);
     if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return KVMIX_ERR_WORKSPACE;
     AdapterArgs p{};
@@ -507,10 +546,10 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
     p.tiles = (PlanWords)list, p.rows = (PlanWords)list + plan->rows_at, p.part_rows = plan->rows;
     p.rank = (int)c->rank, p.padded = (int)padded_rank(c->rank), p.k = (int)c->k, p.n = (int)c->n;
     p.splits = (int)splits_of(plan, c->rank, c->k), p.rank_chunks = (int)rank_chunks(c->rank);
-    const int64_t shrink = plan->tiles * p.rank_chunks * p.splits, tiles = plan->tiles + (in_place ? 0 : plan->bare), columns = (c->n + 31) / 32;
-    p.units = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * columns / (kWaves * 384)));
-    p.n_blocks = (int)((columns + kWaves * p.units - 1) / (kWaves * p.units));
-    if (shrink > kMostBlocks || tiles * p.n_blocks > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
+    const ExpandPlan e = expand_plan(plan, c);
+    p.units = (int)e.units, p.n_blocks = (int)e.blocks;
+    const int64_t shrink = plan->tiles * p.rank_chunks * p.splits, expand = e.tiles * e.blocks;
+    if (shrink > kMostBlocks || expand > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
     hipStream_t st = (hipStream_t)stream;
     auto run = [&](auto zero) {
         using T = decltype(zero);
@@ -518,8 +557,14 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
             constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
             const size_t subs = (plan->most + kSub - 1) / kSub, sums = kWaves * subs * kSub * (RT * 16) * sizeof(float);
             const size_t staged = subs == 1 ? 0 : 2 * kSub * (RT + (subs == 2 ? 2 : 4)) * 256, lds = std::max(sums, staged);
+            if constexpr (RX.value <= 64) {  // (a rank of more than 64 would need k of 512 at most)
+                if (whole_u(plan, c)) {
+                    adapter_expand<T, RX.value, true><<<(unsigned)expand, 256, 0, st>>>(p);
+                    return;
+                }
+            }
             if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
-            if (tiles) adapter_expand<T, RX.value><<<(unsigned)(tiles * p.n_blocks), 256, 0, st>>>(p);
+            if (expand) adapter_expand<T, RX.value, false><<<(unsigned)expand, 256, 0, st>>>(p);
         });
     };
     if (c->dtype == KVMIX_F16) run((_Float16)0);

@@ -53,6 +53,11 @@ CASES = [
     ([0, 1, 2], [20, 31, 17], 3, 8, 136, 136),      # tiles of two sixteens, k a little more than a step
     ([1, 0], [64, 300], 2, 48, 5000, 1160),         # stretches of k that are not alike, the last step cut off
     ([0, 0, 0], [40, 1, 60], 1, 16, 128, 128),
+    ([0, 1], [1, 3], 2, 64, 4096, 264),             # few tokens, much to read
+    ([0], [5], 1, 8, 11008, 1000),
+    ([1, -1, 0], [16, 20, 2], 2, 32, 2048, 2056),   # few tokens and little to read, to the last of it
+    ([0, 2, 1], [1, 1, 1], 3, 64, 1024, 520),
+    ([0, 1, 0], [3, 1, 2], 2, 8, 4232, 40),
 ]
 
 
