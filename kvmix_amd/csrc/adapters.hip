@@ -5,9 +5,8 @@
 //   shrink   u = A x.  A tile is up to 64 tokens of one adapter (kvmix_adapter_plan deals them out, whichever sequences they are of), a
 //            block a tile and a stretch of k.  Ranks are the rows of v_mfma_f32_16x16x32, tokens its columns, so that a lane has eight k
 //            of one row of A and of one token, sixteen bytes.  The four waves read 256 bytes of each row at once, exchange them in
-//            the LDS and multiply a quarter of these each.  (Sixteen tokens at most: each wave its own quarter, without the LDS,
-//            which latency gains from.)  The waves' sums come together in the LDS, those of the stretches (there are several
-//            where there are few tiles) in
+//            the LDS and multiply a quarter of these each.  (Few tokens and ranks: each wave its own quarter, without the LDS.)  The
+//            waves' sums come together in the LDS, those of the stretches (there are several where there are few tiles) in
 //   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then takes 128 columns of y at a time, a quarter of them
 //            to a wave.  u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest
 //            just below 2^14 (bf16: 2): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would
@@ -18,7 +17,7 @@
 // and expand's first reads go out before it sums u.
 // One token with an adapter of rank 8, k = n = 4096: 6.0 us, one launch and the reads of A by each of its 32 blocks.
 // 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 53 us, 3.8 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
-// k = 11008 to n = 4096: 22 us; 64 tokens of 40 adapters to n = 12288: 8.6 us, that is two launches.
+// k = 11008 to n = 4096: 20 us; 64 tokens of 40 adapters to n = 12288: 8.6 us, that is two launches.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
 #include <new>
@@ -187,6 +186,10 @@ __device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *
     meet();  // (the LDS is wanted for the sums)
 }
 
+// Not of sixteen tokens of a rank of 32 at most, which wait for the LDS longer than for their rows (40 tiles of rank 8, k 11008: 8.5 instead of
+// 10.9 us with the other kernel; one of rank 64, k 4096: 7.2 and 6.6).
+constexpr bool through_lds(int RT, int ST) { return RT > 2 || ST > 1; }
+
 template <typename T, int RT>
 __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 {
@@ -205,15 +208,15 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
         const T *a[RT], *x[ST];
         int row[ST];
         floatx4 acc[RT][ST] = {};
-        const bool staged = ST > 1;
+        constexpr bool staged = through_lds(RT, ST);
         rows_of(row, p, tile, staged ? wave * 4 * ST + g : m, staged ? 4 : kSub);
 #pragma unroll
         for (int s = 0; s < ST; s++) x[s] = (const T *)p.x + row[s] * p.x_ts;
 #pragma unroll
         for (int r = 0; r < RT; r++)  // (what lies beyond the rank is not kept)
             a[r] = (const T *)p.a + adapter * p.a_as + min(chunk * RT * 16 + (staged ? wave * 4 * RT + g + 4 * r : 16 * r + m), p.rank - 1) * p.a_rs;
-        if constexpr (ST > 1) shrink_staged<T, RT, ST>(a, x, sums, begin, to, p.k, wave, m, g, acc);
-        else shrink_few<RT <= 2 ? 4 : 2>(a, x[0], begin / 32, min(to, p.k + 31) / 32, p.k, wave, g, acc);
+        if constexpr (staged) shrink_staged<T, RT, ST>(a, x, sums, begin, to, p.k, wave, m, g, acc);
+        else shrink_few<4>(a, x[0], begin / 32, min(to, p.k + 31) / 32, p.k, wave, g, acc);
 #pragma unroll
         for (int s = 0; s < ST; s++)
             if (s < subs)
@@ -462,13 +465,13 @@ ExpandPlan expand_plan(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t 
     return {tiles, units, (columns + kWaves * units - 1) / (kWaves * units)};
 }
 
-// One launch instead of two: where the tiles are of few tokens, a block finds a CU of its own and has at most 128 KB of A to read (4096 of
-// rank 16).  One to eight tokens, k = n = 4096: 6.0 us instead of 8.5 launched one after the other, 5.8 instead of 5.4 in a graph; k 2048:
-// 4.3 instead of 5.4 there; k 11008: 10.7 instead of 6.0; twice as many blocks as CUs: 9 instead of 5.8.
+// One launch instead of two: where the tiles are of few tokens, a block finds a CU of its own and has at most 64 KB of A to read (4096 of
+// rank 8).  One to eight tokens, n = 4096: 6.0 us instead of 8.5 launched one after the other, 5.8 instead of 5.4 in a graph; k 2048,
+// rank 16: 4.9 instead of 5.4 there; k 4096, rank 16: 7.1 instead of 5.5; twice as many blocks as CUs: 9 instead of 5.8.
 bool whole_u(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
 {
     const int64_t blocks = (plan->tiles + plan->bare) * ((c->n + 32 * kWaves - 1) / (32 * kWaves));
-    return plan->tiles && plan->most <= kSub && c->rank <= 64 && c->k * padded_rank(c->rank) <= 65536 && blocks <= 256;
+    return plan->tiles && plan->most <= kSub && c->rank <= 64 && c->k * c->rank <= 32768 && blocks <= 256;
 }
 
 // Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
@@ -556,8 +559,9 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
         with_rank(c->rank, [&](auto RX) {
             constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
             const size_t subs = (plan->most + kSub - 1) / kSub, sums = kWaves * subs * kSub * (RT * 16) * sizeof(float);
-            const size_t staged = subs == 1 ? 0 : 2 * kSub * (RT + (subs == 2 ? 2 : 4)) * 256, lds = std::max(sums, staged);
-            if constexpr (RX.value <= 64) {  // (a rank of more than 64 would need k of 512 at most)
+            const int ST = subs == 1 ? 1 : subs == 2 ? 2 : 4;
+            const size_t lds = std::max(sums, through_lds(RT, ST) ? 2 * kSub * (RT + ST) * 256 : size_t(0));
+            if constexpr (RX.value <= 64) {  // (a larger rank would need k of 448 at most)
                 if (whole_u(plan, c)) {
                     adapter_expand<T, RX.value, true><<<(unsigned)expand, 256, 0, st>>>(p);
                     return;

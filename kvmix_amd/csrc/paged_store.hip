@@ -96,9 +96,10 @@ __global__ void __launch_bounds__(256) paged_append(AppendArgs a)
 // rotated append: the fused projection of the new tokens, [tokens][heads + 2 kv_heads][D].  The first blocks of the launch rotate
 // queries (to a tensor of their own) and keys (to their pages), the last ones turn the values round as in paged_append.
 // With u = x[d], w = x[d + D / 2]:  u cos_d - w sin_d  and  w cos_d' + u sin_d', d' = d + D / 2.
-// Bound by memory.  A wave takes one token: its lanes are the pairs of pieces of several heads (eight of 128 channels), a turn of the
-// loop as many heads again, so that a lane reads its four pieces of the tables once for all turns, and a turn's reads are 2 KB that follow
-// one another.  Where there are few tokens a wave takes one turn only: latency is what counts, and the chip is not full.
+// Bound by memory.  A wave takes one token and as many heads as it has lanes for (eight of 128 channels): its lanes are the pairs of
+// pieces of a head, so that its reads are 2 KB that follow one another.  (Several such turns of a wave, with its part of the tables
+// read once, gained nothing: 79.9 and 77.9 us, 20 and 19.6.)  8 x 1021 tokens of 32 heads, fp32 tables: 78 to 80 us, 410 MB, 5.1 TB/s;
+// rotated with tensors and appended 979.  64 tokens of 32 heads over 8: 4.8 us, a launch.
 
 template <typename T>
 struct TablePieces {  // eight channels of the first half, eight of the second
@@ -155,8 +156,7 @@ struct RopeStoreArgs {
     int parts, rotating;                            // waves to a token; blocks of the launch that rotate
 };
 
-// TURNS: turns of a wave at most.
-template <int D, typename T, int TURNS>
+template <int D, typename T>
 __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
 {
     constexpr int C = D / 8, HALF = C / 2;
@@ -169,31 +169,17 @@ __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
         const int slot = a.slots[token], at = 8 * (lane % HALF), total = a.heads + a.kv_heads;
         const T *cos = (const T *)a.cos + token * a.cos_ts + at, *sin = (const T *)a.sin + token * a.sin_ts + at;
         const _Float16 *x = a.qkv + token * a.x_ts + at;
-        const int first = part * TURNS * (kWave / HALF) + lane / HALF;
-        half8v u[TURNS], w[TURNS];
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) {
-            const int head = first + i * (kWave / HALF);
-            if (head < total) {
-                u[i] = *(const half8v *)(x + head * a.x_hs);
-                w[i] = *(const half8v *)(x + head * a.x_hs + D / 2);
-            }
-        }
+        const int head = part * (kWave / HALF) + lane / HALF;
+        if (head >= total) return;
+        half8v u = *(const half8v *)(x + head * a.x_hs), w = *(const half8v *)(x + head * a.x_hs + D / 2);
         TablePieces<T> t;
         load_table(t.c1, cos), load_table(t.c2, cos + D / 2), load_table(t.s1, sin), load_table(t.s2, sin + D / 2);
-        _Float16 *q = a.q + token * a.q_ts + at;
+        rotate_pieces(u, w, t);
         const int page = slot >> a.page_log2, place = slot & ((1 << a.page_log2) - 1);
-        _Float16 *keys = a.rows + ((((int64_t)page * a.kv_heads) * 2) << a.page_log2) * D + (int64_t)place * D + at;
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) {
-            const int head = first + i * (kWave / HALF);
-            if (head < total) {
-                rotate_pieces(u[i], w[i], t);
-                _Float16 *to = head < a.heads ? q + head * a.q_hs : keys + (((int64_t)(head - a.heads) * 2) << a.page_log2) * D;
-                *(half8v *)to = u[i];
-                *(half8v *)(to + D / 2) = w[i];
-            }
-        }
+        _Float16 *to = a.q + token * a.q_ts + head * a.q_hs + at;
+        if (head >= a.heads) to = a.rows + ((((int64_t)page * a.kv_heads + head - a.heads) * 2) << a.page_log2) * D + (int64_t)place * D + at;
+        *(half8v *)to = u;
+        *(half8v *)(to + D / 2) = w;
         return;
     }
     const int unit = (blockIdx.x - a.rotating) * 4 + wave;
@@ -574,10 +560,7 @@ extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_
         return KVMIX_ERR_UNSUPPORTED;
     if (plan->tokens == 0) return KVMIX_OK;
     if (!c->qkv || !c->cos || !c->sin || !c->q || !list || !p->rows) return KVMIX_ERR_NULL;
-    // Four turns to a wave once that leaves every CU two waves for each of its SIMDs.
-    const int64_t turns = ((plan->heads + p->kv_heads) * (p->head_dim / 16) + kWave - 1) / kWave;
-    const bool many = plan->tokens * ((turns + 3) / 4) >= 2048;
-    const int64_t parts = many ? (turns + 3) / 4 : turns;
+    const int64_t parts = ((plan->heads + p->kv_heads) * (p->head_dim / 16) + kWave - 1) / kWave;
     const __int128 rotating = ((__int128)plan->tokens * parts + 3) / 4, turning = ((__int128)plan->stores * p->kv_heads + 3) / 4;
     if (rotating + turning > kMostBlocks) return KVMIX_ERR_UNSUPPORTED;
     const RopeStoreArgs a = {(const _Float16 *)c->qkv, c->qkv_token_stride, c->qkv_head_stride, c->cos, c->sin, c->cos_token_stride, c->sin_token_stride,
@@ -586,13 +569,8 @@ extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_
                              __builtin_ctzll((uint64_t)p->page_size), (int)parts, (int)rotating};
     const unsigned grid = (unsigned)(rotating + turning);
     with_dim(p->head_dim, [&](auto D) {
-        if (c->table_dtype == KVMIX_F16) {
-            if (many) paged_rope_append<D.value, _Float16, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-            else paged_rope_append<D.value, _Float16, 1><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-        } else {
-            if (many) paged_rope_append<D.value, float, 4><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-            else paged_rope_append<D.value, float, 1><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-        }
+        if (c->table_dtype == KVMIX_F16) paged_rope_append<D.value, _Float16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        else paged_rope_append<D.value, float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     });
     return launch_status();
 }
