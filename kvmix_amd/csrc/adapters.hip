@@ -540,6 +540,7 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
     if (plan->tokens == 0) return KVMIX_OK;
     if (!c->x || !c->base || !c->out || !list || (plan->rows && (!c->a || !c->b))) return KVMIX_ERR_NULL;
     if (c->out == c->base && c->out_token_stride != c->base_token_stride) return KVMIX_ERR_SHAPE;
+    if (plan->tokens > 1 && c->out_token_stride < c->n) return KVMIX_ERR_SHAPE;
     const int64_t need = kvmix_add_adapters_workspace_bytes(plan, c);
     if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return KVMIX_ERR_WORKSPACE;
     AdapterArgs p{};

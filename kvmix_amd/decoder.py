@@ -172,10 +172,12 @@ def head_logits(x: torch.Tensor, weights: dict, eps: float) -> torch.Tensor:
     return F.linear(rms_norm(x[:, 0], weights["norm"], eps), w).to(torch.float32)
 
 
-def check_beams(beams: int, end: Optional[int], vocab: int) -> None:
-    """What ops.beam_select would refuse in a later step."""
+def check_beams(requests: int, beams: int, end: Optional[int], vocab: int) -> None:
+    """What ops.beam_select and ops.reorder_rows would refuse in a later step."""
     if not 1 <= beams <= min(64, vocab):
         raise RuntimeError("beam_search: between 1 and 64 beams, not more than there are tokens")
+    if requests * beams > 1024:
+        raise RuntimeError("beam_search: at most 1024 beams in all")
     if end is not None and not 0 <= end < vocab:
         raise RuntimeError("beam_search: the token that ends a beam is one of the vocabulary")
 
@@ -268,8 +270,8 @@ class Decoder:
 
         if new_tokens < 1 or self.position or not prompt_ids.numel():
             raise RuntimeError("beam_search: a new token at least, from prompts that nothing is cached of")
-        check_beams(beams, end, self.cfg.vocab_size)
         B = prompt_ids.shape[0]
+        check_beams(B, beams, end, self.cfg.vocab_size)
         logits = self.forward(prompt_ids.repeat_interleave(beams, 0))
         ids = prompt_ids.new_zeros(B * beams, new_tokens)
         scores = torch.full((B, beams), float("-inf"), device=ids.device)

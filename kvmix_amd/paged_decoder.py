@@ -131,7 +131,7 @@ class PagedDecoder:
         sequences stay as they are; the beams are forks of them, which share pages for as long as they agree, and end with the call."""
         if new_tokens < 1 or len(set(sequences)) != len(sequences) or logits.dim() != 2 or logits.shape[0] != len(sequences):
             raise RuntimeError("beam_search: a new token at least, sequences that are different, and a row of logits for each")
-        check_beams(beams, end, logits.shape[1])
+        check_beams(len(sequences), beams, end, logits.shape[1])
         for s in sequences:
             self.cache.length(s)  # (refuses what is no sequence)
         n, groups = len(sequences), []

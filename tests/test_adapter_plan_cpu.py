@@ -61,7 +61,7 @@ def call(**kw):
 @pytest.mark.parametrize("change,code", [
     ({"dtype": 1}, -6), ({"rank": 0}, -8), ({"rank": 20}, -9), ({"rank": 136}, -9), ({"k": 4100}, -9), ({"n": 1 << 25}, -9), ({"adapters": 2}, -19),
     ({"x": (1 << 20) + 2}, -9), ({"x_token_stride": 4097}, -9), ({"b_row_stride": 20}, -9), ({"out_token_stride": 2048, "out": 1 << 20}, -8), ({"x": None}, -7),
-    ({"a": None}, -7), ({"scales": None}, -11),
+    ({"a": None}, -7), ({"out_token_stride": 1016, "out": 1 << 21}, -8), ({"scales": None}, -11),
 ])
 def test_calls_that_are_refused(change, code):
     """With a plan of three adapters and no workspace, which the last one gets to."""

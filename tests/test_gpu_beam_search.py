@@ -174,9 +174,13 @@ def test_refusals(dev):
                         (([a], logits[0], 2, 3), "row"), (([a], logits, 2, 3, 1000), "vocabulary"), (([a], logits, 2, 3, -1), "vocabulary"), (([a + 5], logits, 2, 3), "no sequence")]:
         with pytest.raises(RuntimeError, match=match):
             model.beam_search(*args)
+    many = [model.add() for _ in range(20)]
+    with pytest.raises(RuntimeError, match="1024 beams"):
+        model.beam_search(many, logits.expand(20, -1), 64, 2)
     assert model.beam_search([], logits[:0], 2, 3)[0].shape == (0, 2, 3) and model.cache.length(a) == 9
     dense = Decoder(cfg, w, *kvmix_layers(cfg, [4] * 3, [4] * 3, residual_length=64))
-    for args in ((torch.arange(5, device=dev)[None], 2, 0), (torch.zeros(1, 0, dtype=torch.long, device=dev), 2, 3), (torch.arange(5, device=dev)[None], 65, 3)):
+    for args in ((torch.arange(5, device=dev)[None], 2, 0), (torch.zeros(1, 0, dtype=torch.long, device=dev), 2, 3), (torch.arange(5, device=dev)[None], 65, 3),
+                 (torch.zeros(17, 5, dtype=torch.long, device=dev), 64, 3)):
         with pytest.raises(RuntimeError, match="beam_search"):
             dense.beam_search(*args)
     dense.forward(torch.arange(5, device=dev)[None])
