@@ -596,8 +596,8 @@ int kvmix_paged_append(const kvmix_paged_pool_t *pool, const kvmix_paged_plan_t 
  * head_dim] fp16, queries first, then keys, then values.  Queries and keys are rotated,
  *   y[d] = x[d] cos[d] - x[d + head_dim / 2] sin[d]  (d < head_dim / 2),   y[d] = x[d] cos[d] + x[d - head_dim / 2] sin[d]  (d beyond),
  * queries go to q [plan.tokens, heads, head_dim], keys and values into their pages.
- *   cos, sin [plan.tokens, head_dim]: fp16 (each product and the sum rounded to fp16, as kvmix_rope_append does) or fp32 (one
- *   rounding at the end).  Strides in elements, tokens' ones of the tables may be 0; all in whole pieces of 16 bytes, which the
+ *   cos, sin [plan.tokens, head_dim]: fp16 or fp32; computed in 32 bits and rounded once, or, with fp16 tables and as_tensors, each product
+ *   and the sum rounded to fp16, as kvmix_rope_append does.  Strides in elements, tokens' ones of the tables may be 0; all in whole pieces of 16 bytes, which the
  *   pointers are aligned to, and unit stride along head_dim.
  */
 typedef struct kvmix_paged_rope {
@@ -606,6 +606,7 @@ typedef struct kvmix_paged_rope {
     const void *cos, *sin;
     int64_t cos_token_stride, sin_token_stride;
     int table_dtype;  /* KVMIX_F16 or KVMIX_F32 */
+    int as_tensors;
     void *q;
     int64_t q_token_stride, q_head_stride;
 } kvmix_paged_rope_t;

@@ -155,7 +155,7 @@ Tensor table_pieces(const Tensor &t_in, int64_t tokens, int64_t head_dim)
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-Tensor paged_rope_append(const Tensor &qkv_in, const Tensor &cos_in, const Tensor &sin_in, const Tensor &rows, const PagedPlan &plan)
+Tensor paged_rope_append(const Tensor &qkv_in, const Tensor &cos_in, const Tensor &sin_in, const Tensor &rows, const PagedPlan &plan, bool as_tensors)
 {
     need_no_record("paged_rope_append", {&qkv_in, &cos_in, &sin_in, &rows});
     kvmix_paged_pool_t p{};
@@ -167,13 +167,14 @@ Tensor paged_rope_append(const Tensor &qkv_in, const Tensor &cos_in, const Tenso
     if (plan.c.kv_heads != p.kv_heads || plan.c.page_size != p.page_size || plan.c.head_dim != p.head_dim)
         fail("paged_rope_append: the plan is for pages of another shape");
     if (cos_in.scalar_type() != sin_in.scalar_type()) fail("paged_rope_append: cos and sin must be of one type");
+    if (as_tensors && cos_in.scalar_type() == at::kFloat) fail("paged_rope_append: only with float16 tables can it round as tensors of float16 do");
     if (plan.c.row_pages > p.row_pages) check(KVMIX_ERR_PAGE);
     const Tensor qkv = pieces3(qkv_in), cos = table_pieces(cos_in, plan.c.tokens, p.head_dim), sin = table_pieces(sin_in, plan.c.tokens, p.head_dim);
     Tensor q = at::empty({plan.c.tokens, plan.c.heads, p.head_dim}, qkv.options());
     kvmix_paged_rope_t c{};
     c.qkv = qkv.data_ptr(), c.qkv_token_stride = stride_of(qkv, 0), c.qkv_head_stride = stride_of(qkv, 1);
     c.cos = cos.data_ptr(), c.cos_token_stride = stride_of(cos, 0), c.sin = sin.data_ptr(), c.sin_token_stride = stride_of(sin, 0);
-    c.table_dtype = dtype_tag(cos);
+    c.table_dtype = dtype_tag(cos), c.as_tensors = as_tensors;
     c.q = q.data_ptr(), c.q_token_stride = q.stride(0), c.q_head_stride = q.stride(1);
     const c10::DeviceGuard guard(rows.device());
     check(api.paged_rope_append(&p, &plan.c, plan.words(), &c, stream_of(rows)));

@@ -120,9 +120,8 @@ __device__ __forceinline__ void load_table(float (&to)[8], const float *at)
     for (int j = 0; j < 4; j++) to[j] = a[j], to[4 + j] = b[j];
 }
 
-// fp16 tables: as the fp16 tensor expression rounds, each product and the sum (kvmix_rope_append does the same).  fp32 tables: one
-// rounding at the end.
-__device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TablePieces<_Float16> &t)
+// As the fp16 tensor expression rounds, each product and the sum (kvmix_rope_append does the same).
+__device__ __forceinline__ void rotate_as_tensors(half8v &u, half8v &w, const TablePieces<_Float16> &t)
 {
     typedef uint16_t bits8 __attribute__((ext_vector_type(8)));
     const bits8 x = __builtin_bit_cast(bits8, u), y = __builtin_bit_cast(bits8, w);
@@ -133,13 +132,15 @@ __device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TableP
     u = __builtin_bit_cast(half8v, a), w = __builtin_bit_cast(half8v, b);
 }
 
-__device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TablePieces<float> &t)
+// In 32 bits, rounded once.
+template <typename T>
+__device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TablePieces<T> &t)
 {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float x = (float)u[j], y = (float)w[j];
-        u[j] = (_Float16)fmaf(x, t.c1[j], -(y * t.s1[j]));
-        w[j] = (_Float16)fmaf(y, t.c2[j], x * t.s2[j]);
+        u[j] = (_Float16)fmaf(x, (float)t.c1[j], -(y * (float)t.s1[j]));
+        w[j] = (_Float16)fmaf(y, (float)t.c2[j], x * (float)t.s2[j]);
     }
 }
 
@@ -156,7 +157,8 @@ struct RopeStoreArgs {
     int parts, rotating;                            // waves to a token; blocks of the launch that rotate
 };
 
-template <int D, typename T>
+// T: of the tables.  TENSORS: rounded as the fp16 tensor expression is.
+template <int D, typename T, bool TENSORS>
 __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
 {
     constexpr int C = D / 8, HALF = C / 2;
@@ -174,7 +176,8 @@ __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
         half8v u = *(const half8v *)(x + head * a.x_hs), w = *(const half8v *)(x + head * a.x_hs + D / 2);
         TablePieces<T> t;
         load_table(t.c1, cos), load_table(t.c2, cos + D / 2), load_table(t.s1, sin), load_table(t.s2, sin + D / 2);
-        rotate_pieces(u, w, t);
+        if constexpr (TENSORS) rotate_as_tensors(u, w, t);
+        else rotate_pieces(u, w, t);
         const int page = slot >> a.page_log2, place = slot & ((1 << a.page_log2) - 1);
         _Float16 *to = a.q + token * a.q_ts + head * a.q_hs + at;
         if (head >= a.heads) to = a.rows + ((((int64_t)page * a.kv_heads + head - a.heads) * 2) << a.page_log2) * D + (int64_t)place * D + at;
@@ -554,6 +557,7 @@ extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_
     if (plan->page_size != p->page_size || plan->kv_heads != p->kv_heads || plan->head_dim != p->head_dim) return KVMIX_ERR_SHAPE;
     if (plan->row_pages > p->row_pages) return KVMIX_ERR_PAGE;
     if (c->table_dtype != KVMIX_F16 && c->table_dtype != KVMIX_F32) return KVMIX_ERR_DTYPE;
+    if (c->as_tensors && c->table_dtype != KVMIX_F16) return KVMIX_ERR_DTYPE;
     const int64_t per = c->table_dtype == KVMIX_F16 ? 8 : 4;
     if (c->qkv_token_stride % 8 || c->qkv_head_stride % 8 || c->q_token_stride % 8 || c->q_head_stride % 8 || c->cos_token_stride % per ||
         c->sin_token_stride % per || ((uintptr_t)c->qkv | (uintptr_t)c->cos | (uintptr_t)c->sin | (uintptr_t)c->q) % 16)
@@ -569,8 +573,9 @@ extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_
                              __builtin_ctzll((uint64_t)p->page_size), (int)parts, (int)rotating};
     const unsigned grid = (unsigned)(rotating + turning);
     with_dim(p->head_dim, [&](auto D) {
-        if (c->table_dtype == KVMIX_F16) paged_rope_append<D.value, _Float16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-        else paged_rope_append<D.value, float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        if (c->table_dtype == KVMIX_F32) paged_rope_append<D.value, float, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        else if (c->as_tensors) paged_rope_append<D.value, _Float16, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        else paged_rope_append<D.value, _Float16, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     });
     return launch_status();
 }

@@ -495,12 +495,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, plan) -> 
     _host().paged_append(k, v, rows, plan)
 
 
-def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rows: torch.Tensor, plan) -> torch.Tensor:
+def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rows: torch.Tensor, plan, as_tensors: bool = False) -> torch.Tensor:
     """The projection qkv [plan.tokens, heads + 2 kv_heads, head_dim] fp16 of a step's new tokens: its queries and keys rotated
     (x * cos + rotate_half(x) * sin), keys and values into the fp16 pages as paged_append does, in one launch; returns the rotated
-    queries [plan.tokens, heads, head_dim].  cos, sin [plan.tokens, head_dim], or one row for all: fp16 tables give what the fp16
-    tensor expression gives, bit for bit; fp32 ones are rounded once, at the end."""
-    return _host().paged_rope_append(qkv, cos, sin, rows, plan)
+    queries [plan.tokens, heads, head_dim].  cos, sin [plan.tokens, head_dim], or one row for all, fp16 or fp32: computed in 32 bits and
+    rounded once.  as_tensors=True, with fp16 tables, gives what the fp16 tensor expression gives, bit for bit (its products are
+    rounded to fp16 too), as rope_append does."""
+    return _host().paged_rope_append(qkv, cos, sin, rows, plan, as_tensors)
 
 
 def paged_quantize(rows: torch.Tensor, packed: torch.Tensor, pairs: torch.Tensor, k_bits: int, v_bits: int) -> None:

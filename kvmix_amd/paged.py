@@ -294,10 +294,10 @@ class PagedKVCache:
         """The new tokens' keys and values [tokens, kv_heads, head_dim], sequence after sequence."""
         ops.paged_append(k, v, self.rows[layer], self._plan(step))
 
-    def append_rotated(self, layer: int, step: Step, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def append_rotated(self, layer: int, step: Step, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, as_tensors: bool = False) -> torch.Tensor:
         """The same from the new tokens' projection [tokens, heads + 2 kv_heads, head_dim], queries and keys rotated on the way with the
         tables [tokens, head_dim]; returns the queries (ops.paged_rope_append)."""
-        return ops.paged_rope_append(qkv, cos, sin, self.rows[layer], self._plan(step))
+        return ops.paged_rope_append(qkv, cos, sin, self.rows[layer], self._plan(step), as_tensors)
 
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float = None) -> torch.Tensor:
         """Attention of the new tokens' queries [tokens, heads, head_dim] over their sequences, themselves included."""

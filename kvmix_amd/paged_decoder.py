@@ -86,7 +86,7 @@ class PagedDecoder:
         plan = ops.adapter_plan(of, [i.numel() for i in new_ids.values()], self.adapters.count, device) if max(of) >= 0 else None
         for layer, lw in enumerate(self.w["layers"]):
             def attend(qkv):
-                q = cache.append_rotated(layer, step, qkv.view(-1, nh + 2 * nkv, cfg.head_dim), cos, sin)
+                q = cache.append_rotated(layer, step, qkv.view(-1, nh + 2 * nkv, cfg.head_dim), cos, sin, as_tensors=True)
                 return cache.attend(layer, step, q).reshape(-1, 1, cfg.hidden_size)
 
             if plan is not None:

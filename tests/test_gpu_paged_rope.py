@@ -41,9 +41,9 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("dtype,as_tensors", [(torch.float16, False), (torch.float16, True), (torch.float32, False)])
 @pytest.mark.parametrize("lens,new,heads,kv_heads,D,page", SHAPES)
-def test_against_64_bits(dev, lens, new, heads, kv_heads, D, page, dtype):
+def test_against_64_bits(dev, lens, new, heads, kv_heads, D, page, dtype, as_tensors):
     from kvmix_amd import ops
 
     rows, plan, slots = _case(dev, lens, new, heads, kv_heads, D, page)
@@ -53,17 +53,17 @@ def test_against_64_bits(dev, lens, new, heads, kv_heads, D, page, dtype):
     qkv = wide[:, 1:] if heads % 2 else wide[:, :-1].contiguous()
     cos, sin = _tables(tokens, D, dtype, dev)
     before = rows.clone()
-    q = ops.paged_rope_append(qkv, cos, sin, rows, plan)
+    q = ops.paged_rope_append(qkv, cos, sin, rows, plan, as_tensors)
     assert q.shape == (tokens, heads, D) and q.dtype == torch.float16
     x = qkv[:, :heads + kv_heads].double().cpu()
     turned = torch.cat([-x[..., D // 2:], x[..., :D // 2]], -1)
     c, s = cos.double().cpu()[:, None], sin.double().cpu()[:, None]
     want = x * c + turned * s
     # one rounding to fp16 (2^-11 of the value, 2^-25 where it is subnormal) after fp32 arithmetic (two operations of 2^-24 each of
-    # the products); with fp16 tables each product rounds to fp16 as well, and the sum of what they became
+    # the products); rounded as tensors are, each product rounds to fp16 as well, and the sum of what they became
     size = (x * c).abs() + (turned * s).abs()
     tol = 2.0 ** -11 * want.abs() + 2.0 ** -22 * size + 2.0 ** -25
-    if dtype == torch.float16:
+    if as_tensors:
         tol = 2.0 ** -11 * (want.abs() + size * (1 + 2.0 ** -11)) + 2.0 ** -22 * size + 3 * 2.0 ** -25
     assert ((q.double().cpu() - want[:, :heads]).abs() <= tol[:, :heads]).all()
     k, v = unpack_rows(rows)
@@ -80,7 +80,7 @@ def test_against_64_bits(dev, lens, new, heads, kv_heads, D, page, dtype):
 
 @pytest.mark.parametrize("lens,new,heads,kv_heads,D,page", SHAPES)
 def test_as_the_tensor_expression_and_the_plain_append(dev, lens, new, heads, kv_heads, D, page):
-    """With fp16 tables the same bits as rotating with tensors and appending, infinities and NaN among them."""
+    """Where it is asked for, the same bits as rotating with tensors and appending, infinities and NaN among them."""
     from kvmix_amd import ops
     from kvmix_amd.decoder import apply_rope
 
@@ -94,7 +94,7 @@ def test_as_the_tensor_expression_and_the_plain_append(dev, lens, new, heads, kv
     other = rows.clone()
     qk = apply_rope(qkv[:, :heads + kv_heads], cos[:, None], sin[:, None])
     ops.paged_append(qk[:, heads:], qkv[:, heads + kv_heads:], other, plan)
-    q = ops.paged_rope_append(qkv, cos, sin, rows, plan)
+    q = ops.paged_rope_append(qkv, cos, sin, rows, plan, as_tensors=True)
     nan = torch.isnan(qk[:, :heads])
     assert torch.equal(torch.isnan(q), nan) and torch.equal(q[~nan], qk[:, :heads][~nan])
     nan = torch.isnan(other)
@@ -132,7 +132,8 @@ def test_refusals(dev):
                        ((qkv, cos[:, :64], sin, rows, plan), "head_dim"), ((qkv, cos, sin.half(), rows, plan), "one type"),
                        ((qkv, cos.double(), sin.double(), rows, plan), "float16 or float32"), ((qkv, cos.cpu(), sin, rows, plan), "device|cpu"),
                        ((qkv.cpu(), cos, sin, rows, plan), "GPU|cpu"), ((qkv, cos, sin, rows[:, :1].contiguous(), plan), "another shape"),
-                       ((qkv, cos, sin, rows[:1], plan), "page"), ((qkv.clone().requires_grad_(), cos, sin, rows, plan), "no derivative")):
+                       ((qkv, cos, sin, rows[:1], plan), "page"), ((qkv.clone().requires_grad_(), cos, sin, rows, plan), "no derivative"),
+                       ((qkv, cos, sin, rows, plan, True), "float16 tables")):
         with pytest.raises(RuntimeError, match=match):
             ops.paged_rope_append(*bad)
     assert torch.equal(rows, before)
