@@ -17,7 +17,7 @@
 // and expand's first reads go out before it sums u.
 // One token with an adapter of rank 8, k = n = 4096: 6.0 us, one launch and the reads of A by each of its 32 blocks.
 // 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 53 us, 3.8 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
-// k = 11008 to n = 4096: 20 us; 64 tokens of 40 adapters to n = 12288: 8.6 us, that is two launches.
+// k = 11008 to n = 4096: 20 us; 64 tokens of 8 adapters of rank 16 to n = 12288: 8.6 us, that is two launches.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
 #include <new>
