@@ -60,6 +60,7 @@ struct AdapterArgs {
     PlanWords tiles, rows;  // tiles; their tokens
     int64_t part_rows;
     int rank, padded, k, n, splits, rank_chunks, n_blocks, units;  // units: of 32 columns, of a wave of expand
+    int tokens;                                                    // of a tile at most: 16, 32 or 64
 };
 
 // Every `step`th token of a tile from `from` on (where there is none, the last).
@@ -246,9 +247,10 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
     typedef typename Vec8<T>::type V;
     constexpr int NF = RX >= 32 ? RX / 32 : 1, LD = 2 * RX + 8, L = RX / 4;  // pieces of a row of B; of u: its two parts; lanes to a token
     constexpr int COLUMNS = 32 * kWaves;                                     // of y, in a step of the block
-    __shared__ alignas(16) T u[kTile][LD];
-    __shared__ float power[kTile];
-    __shared__ alignas(16) float sums[kTile][COLUMNS + 4];
+    extern __shared__ __attribute__((aligned(16))) char shared[];            // (of no more tokens than the plan's tiles have)
+    float(*sums)[COLUMNS + 4] = (float(*)[COLUMNS + 4]) shared;
+    T(*u)[LD] = (T(*)[LD])(sums + (WHOLE ? kWaves * kSub : p.tokens));
+    float *power = (float *)(u + p.tokens);
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const PlanWords tile = p.tiles + blockIdx.x / p.n_blocks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
                 const T h = (T)v;
                 high[r] = h, low[r] = fabsf(v) < __builtin_inff() ? (T)(v - (float)h) : (T)0.0f;
             }
-            if (t < kTile) {
+            if (t < kSub * decltype(st)::value) {
                 *(four *)&u[t][4 * c] = high;
                 *(four *)&u[t][RX + 4 * c] = low;
                 if (c == 0) power[t] = ldexpf(1.0f, e);
@@ -560,16 +562,18 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
         with_rank(c->rank, [&](auto RX) {
             constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
             const size_t subs = (plan->most + kSub - 1) / kSub, sums = kWaves * subs * kSub * (RT * 16) * sizeof(float);
-            const int ST = subs == 1 ? 1 : subs == 2 ? 2 : 4;
+            const int ST = subs <= 1 ? 1 : subs == 2 ? 2 : 4;
+            auto expand_lds = [&](int rows) { return rows * (32 * kWaves + 4) * sizeof(float) + kSub * ST * ((2 * RX.value + 8) * sizeof(T) + sizeof(float)); };
+            p.tokens = kSub * ST;
             const size_t lds = std::max(sums, through_lds(RT, ST) ? 2 * kSub * (RT + ST) * 256 : size_t(0));
             if constexpr (RX.value <= 64) {  // (a larger rank would need k of 448 at most)
                 if (whole_u(plan, c)) {
-                    adapter_expand<T, RX.value, true><<<(unsigned)expand, 256, 0, st>>>(p);
+                    adapter_expand<T, RX.value, true><<<(unsigned)expand, 256, expand_lds(kWaves * kSub), st>>>(p);
                     return;
                 }
             }
             if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
-            if (expand) adapter_expand<T, RX.value, false><<<(unsigned)expand, 256, 0, st>>>(p);
+            if (expand) adapter_expand<T, RX.value, false><<<(unsigned)expand, 256, expand_lds(kSub * ST), st>>>(p);
         });
     };
     if (c->dtype == KVMIX_F16) run((_Float16)0);
