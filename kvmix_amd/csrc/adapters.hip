@@ -60,7 +60,6 @@ struct AdapterArgs {
     PlanWords tiles, rows;  // tiles; their tokens
     int64_t part_rows;
     int rank, padded, k, n, splits, rank_chunks, n_blocks, units;  // units: of 32 columns, of a wave of expand
-    int tokens;                                                    // of a tile at most: 16, 32 or 64
 };
 
 // Every `step`th token of a tile from `from` on (where there is none, the last).
@@ -239,18 +238,18 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-// RX: the rank, rounded up to 16, 32, 64 or 128.  WHOLE: every block makes all of u itself, of tiles of up to sixteen tokens, and there is no
-// other launch.
-template <typename T, int RX, bool WHOLE>
+// RX: the rank, rounded up to 16, 32, 64 or 128.  TOKENS: of a tile at most, 16 or 64 (what the LDS holds says how many blocks a CU takes: 40
+// adapters of rank 64 to n = 22016, one token each, 34 instead of 38 us).  WHOLE: every block makes all of u itself, of tiles of up to
+// sixteen tokens, and there is no other launch.
+template <typename T, int RX, int TOKENS, bool WHOLE>
 __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 {
     typedef typename Vec8<T>::type V;
     constexpr int NF = RX >= 32 ? RX / 32 : 1, LD = 2 * RX + 8, L = RX / 4;  // pieces of a row of B; of u: its two parts; lanes to a token
     constexpr int COLUMNS = 32 * kWaves;                                     // of y, in a step of the block
-    extern __shared__ __attribute__((aligned(16))) char shared[];            // (of no more tokens than the plan's tiles have)
-    float(*sums)[COLUMNS + 4] = (float(*)[COLUMNS + 4]) shared;
-    T(*u)[LD] = (T(*)[LD])(sums + (WHOLE ? kWaves * kSub : p.tokens));
-    float *power = (float *)(u + p.tokens);
+    __shared__ alignas(16) T u[TOKENS][LD];
+    __shared__ float power[TOKENS];
+    __shared__ alignas(16) float sums[WHOLE ? kWaves * kSub : TOKENS][COLUMNS + 4];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), m = lane % 16, g = lane / 16;
     const PlanWords tile = p.tiles + blockIdx.x / p.n_blocks * kTileWords;
     const int adapter = tile[0], first = tile[1], count = tile[2], subs = (count + kSub - 1) / kSub;
@@ -394,8 +393,8 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         };
         in_turn(steps, [&](int d, int i) { load(v[d], i); }, [&](int d, int i) { store(v[d], i); }, [&] { sum(st); });
     };
-    if (WHOLE || subs == 1) run(std::integral_constant<int, 1>());
-    else if constexpr (!WHOLE) {
+    if (TOKENS == kSub || subs == 1) run(std::integral_constant<int, 1>());
+    else if constexpr (TOKENS > kSub) {
         if (subs == 2) run(std::integral_constant<int, 2>());
         else run(std::integral_constant<int, 4>());
     }
@@ -563,17 +562,17 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
             constexpr int RT = RX.value >= 64 ? 4 : RX.value / 16;
             const size_t subs = (plan->most + kSub - 1) / kSub, sums = kWaves * subs * kSub * (RT * 16) * sizeof(float);
             const int ST = subs <= 1 ? 1 : subs == 2 ? 2 : 4;
-            auto expand_lds = [&](int rows) { return rows * (32 * kWaves + 4) * sizeof(float) + kSub * ST * ((2 * RX.value + 8) * sizeof(T) + sizeof(float)); };
-            p.tokens = kSub * ST;
             const size_t lds = std::max(sums, through_lds(RT, ST) ? 2 * kSub * (RT + ST) * 256 : size_t(0));
             if constexpr (RX.value <= 64) {  // (a larger rank would need k of 448 at most)
                 if (whole_u(plan, c)) {
-                    adapter_expand<T, RX.value, true><<<(unsigned)expand, 256, expand_lds(kWaves * kSub), st>>>(p);
+                    adapter_expand<T, RX.value, kSub, true><<<(unsigned)expand, 256, 0, st>>>(p);
                     return;
                 }
             }
             if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
-            if (expand) adapter_expand<T, RX.value, false><<<(unsigned)expand, 256, expand_lds(kSub * ST), st>>>(p);
+            if (!expand) return;
+            if (ST == 1) adapter_expand<T, RX.value, kSub, false><<<(unsigned)expand, 256, 0, st>>>(p);
+            else adapter_expand<T, RX.value, kTile, false><<<(unsigned)expand, 256, 0, st>>>(p);
         });
     };
     if (c->dtype == KVMIX_F16) run((_Float16)0);
