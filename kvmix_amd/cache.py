@@ -12,7 +12,7 @@ Flush policy: `flush_length` below, the reference's ratio rule or a fixed fp16 w
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -289,6 +289,22 @@ class PackedKVCache:
         self._packed_views = (None,) * 6
         self._flushed_ahead = False
 
+    def fit(self, batch: int) -> None:
+        """An empty cache lets go of buffers that were of another batch."""
+        tail = self._k_tail.buf
+        if self.kv_seq_len == 0 and tail is not None and tail.shape[0] != batch:
+            self._k_tail, self._v_tail = _Tail(), _Tail()
+            self._k = self._v = None
+
+    def repeat(self, times: int) -> None:
+        """Every sequence of the batch `times` times, one after the other (copies)."""
+        if times == 1:
+            return
+        for tail in (self._k_tail, self._v_tail):
+            tail.buf = None if tail.buf is None else tail.buf.repeat_interleave(times, 0)
+        self._k, self._v = (None if p is None else tuple(t.repeat_interleave(times, 0) for t in p) for p in (self._k, self._v))
+        self._flush_done(0, 0, direct=True)  # (the views)
+
     def reorder(self, index: torch.Tensor) -> None:
         """The batch's sequences reordered in place, sequence i from what sequence index[i] was (reorder_caches below, which takes
         the caches of all layers at once)."""
@@ -332,6 +348,18 @@ def flush_ahead(caches) -> int:
             c._flush_done(nk, nv, direct=False)
             c._flushed_ahead = True
     return len(todo)
+
+
+def repeat_caches(caches, times: int) -> List:
+    """Caches (PackedKVCache, or the reference's 9-tuple, or None) with every sequence of the batch `times` times, one after the other."""
+    out = []
+    for c in caches:
+        if isinstance(c, PackedKVCache):
+            c.repeat(times)
+        elif c is not None:
+            c = tuple(t.repeat_interleave(times, 0) if torch.is_tensor(t) else t for t in c)
+        out.append(c)
+    return out
 
 
 def reorder_caches(caches, index: torch.Tensor, *others: torch.Tensor) -> None:

@@ -263,28 +263,33 @@ class Decoder:
 
     def beam_search(self, prompt_ids: torch.Tensor, beams: int, new_tokens: int, end: Optional[int] = None):
         """Beam search from prompts [B,Q], nothing cached before: (token ids [B, beams, new_tokens], sums of their log probabilities
-        [B, beams]), the best first.  A beam ends with the token `end`, which then fills it up.  The beams' caches are reordered
-        in place between the steps; nothing waits for the GPU."""
+        [B, beams]), the best first.  A beam ends with the token `end`, which then fills it up.  The prompts are read once, then their
+        caches are repeated for the beams and reordered in place between the steps (afterwards they hold all beams but for their last
+        tokens); nothing waits for the GPU."""
         from . import ops
-        from .cache import reorder_caches
+        from .cache import PackedKVCache, reorder_caches, repeat_caches
 
         if new_tokens < 1 or self.position or not prompt_ids.numel():
             raise RuntimeError("beam_search: a new token at least, from prompts that nothing is cached of")
         B = prompt_ids.shape[0]
         check_beams(B, beams, end, self.cfg.vocab_size)
-        logits = self.forward(prompt_ids.repeat_interleave(beams, 0))
+        for c in self.caches:
+            if isinstance(c, PackedKVCache):
+                c.fit(B)
+        logits = self.forward(prompt_ids)[:, None].expand(-1, beams, -1)
+        self.caches = repeat_caches(self.caches, beams)
         ids = prompt_ids.new_zeros(B * beams, new_tokens)
         scores = torch.full((B, beams), float("-inf"), device=ids.device)
         scores[:, 0] = 0.0  # (the beams of a request are alike still)
         first, done = beams * torch.arange(B, device=ids.device)[:, None], None
         for step in range(new_tokens):
-            scores, parents, tokens = ops.beam_select(logits.view(B, beams, -1), scores, beams, done, end, stay=True)
+            scores, parents, tokens = ops.beam_select(logits, scores, beams, done, end, stay=True)
             last = step + 1 == new_tokens
             reorder_caches([] if last else self.caches, (first + parents).reshape(-1), ids)
             ids[:, step] = tokens.reshape(-1)
             done = None if end is None else tokens == end
             if not last:
-                logits = self.forward(tokens.reshape(-1, 1))
+                logits = self.forward(tokens.reshape(-1, 1)).view(B, beams, -1)
         scores, order = scores.sort(dim=-1, descending=True, stable=True)
         return ids.view(B, beams, -1).gather(1, order[:, :, None].expand(-1, -1, new_tokens)), scores
 
@@ -387,7 +392,7 @@ class GraphDecoder(Decoder):
 
     def _capture(self, ids: torch.Tensor) -> None:
         dev = ids.device
-        if self._ids is None:
+        if self._ids is None or self._ids.shape != ids.shape:
             self._ids = torch.zeros_like(ids)
         self._ids.copy_(ids)
         if self.caches[0].residual_length is None:

@@ -109,6 +109,28 @@ def test_beams_of_the_decoders(dev):
     assert torch.equal(one[:, 0], greedy)
 
 
+def test_one_decoder_again_and_again(dev):
+    """A decoder whose caches are reset searches as a new one does, with as many prompts and beams as it likes, and generates."""
+    from kvmix_amd.decoder import Decoder, GraphDecoder, kvmix_layers
+
+    cfg, w = small(dev, 2)
+    prompts = torch.randint(0, cfg.vocab_size, (3, 90), generator=torch.Generator().manual_seed(5)).to(dev)
+    for kind in (Decoder, GraphDecoder):
+        new = lambda: kind(cfg, w, *kvmix_layers(cfg, [4, 2, 3], [2, 4, 4], residual_length=40, capacity=64))
+        used = new()
+        for rows, beams, steps in ((2, 3, 9), (1, 4, 50), (3, 1, 5), (2, 3, 9)):
+            assert used.position == 0
+            got, want = (d.beam_search(prompts[:rows], beams, steps) for d in (used, new()))
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            assert all(c.kv_seq_len == 90 + steps - 1 and c.as_tuple()[1].shape[0] == rows * beams for c in used.caches)
+            for c in used.caches:
+                c.reset()
+            used.position = 0
+        for c in used.caches:
+            c.fit(3)
+        assert torch.equal(used.generate(prompts, 7), new().generate(prompts, 7))
+
+
 @pytest.mark.parametrize("window", [32, 4096])
 def test_every_continuation(dev, window):
     """With as many beams as there are continuations of all but the last token, the best one of all is found."""
@@ -191,7 +213,7 @@ def test_refusals(dev):
 @pytest.mark.parametrize("in_place", [True, False])
 def test_caches_that_are_reordered(dev, in_place):
     """Every entry of every layer, through the cache's own call and for all layers at once, and steps afterwards."""
-    from kvmix_amd.cache import PackedKVCache, reorder_caches
+    from kvmix_amd.cache import PackedKVCache, reorder_caches, repeat_caches
 
     g = torch.Generator().manual_seed(2)
     caches = [PackedKVCache(b, c, residual_length=40) for b, c in ((4, 2), (1, 4))]
@@ -208,8 +230,15 @@ def test_caches_that_are_reordered(dev, in_place):
     for c, was in zip(caches, before):
         for a, b in zip([t for t in c.as_tuple() if torch.is_tensor(t)], was):
             assert torch.equal(a, b[index])
+    twice = [[t.clone() for t in c.as_tuple() if torch.is_tensor(t)] for c in caches]
     more = [torch.randn(6, 2, 1, 128, generator=g).half().to(dev) for _ in range(2)]
     caches[0].append(*more)
     tail = caches[0].as_tuple()[1]  # of the keys: the new token behind what is left of the others
     n = tail.shape[2] - 1
     assert n > 0 and torch.equal(tail[:, :, n:], more[0]) and torch.equal(tail[:, :, :n], before[0][1][index][:, :, -n:])
+    # and repeated, the second cache, which has had no more tokens
+    assert repeat_caches([None, caches[1], (more[0], None, 7)], 3)[2][0].shape[0] == 18
+    for a, b in zip([t for t in caches[1].as_tuple() if torch.is_tensor(t)], twice[1]):
+        assert torch.equal(a, b.repeat_interleave(3, 0))
+    caches[1].append(*(t.repeat_interleave(3, 0) for t in more))
+    assert torch.equal(caches[1].as_tuple()[5][:, :, -1:], more[1].repeat_interleave(3, 0))
