@@ -16,7 +16,7 @@
 // same bytes take 26 us instead of 19 (x) and 38 instead of 28 (base and y).  Both kernels read a step ahead of the one that is multiplied,
 // and expand's first reads go out before it sums u.
 // One token with an adapter of rank 8, k = n = 4096: 6.0 us, one launch and the reads of A by each of its 32 blocks.
-// 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 53 us, 3.8 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
+// 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 44.6 us, 4.5 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
 // k = 11008 to n = 4096: 20 us; 64 tokens of 8 adapters of rank 16 to n = 12288: 8.6 us, that is two launches.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
@@ -240,8 +240,9 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 
 // RX: the rank, rounded up to 16, 32, 64 or 128.  TOKENS: of a tile at most, 16 or 64 (what the LDS holds says how many blocks a CU takes: 40
 // adapters of rank 64 to n = 22016, one token each, 34 instead of 38 us).  WHOLE: every block makes all of u itself, of tiles of up to
-// sixteen tokens, and there is no other launch.
-template <typename T, int RX, int TOKENS, bool WHOLE>
+// sixteen tokens, and there is no other launch.  STREAM: base and y are more than the caches of the dies keep, and are read and written as
+// what nobody wants again soon.
+template <typename T, int RX, int TOKENS, bool WHOLE, bool STREAM>
 __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 {
     typedef typename Vec8<T>::type V;
@@ -358,7 +359,10 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
                     v.w[h][f] = *(const V *)((const T *)p.b + adapter * p.b_as + row * p.b_ns + (r < p.rank ? r : 0));
                 }
 #pragma unroll
-            for (int s = 0; s < ST; s++) v.y[s] = *(const V *)(from[s] + min(column + 8 * m, p.n - 8));
+            for (int s = 0; s < ST; s++) {
+                const V *at = (const V *)(from[s] + min(column + 8 * m, p.n - 8));
+                v.y[s] = STREAM ? __builtin_nontemporal_load(at) : *at;
+            }
         };
         auto store = [&](Unit &v, int i) {
 #pragma unroll
@@ -387,7 +391,9 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 #pragma unroll
                     for (int c = 0; c < 4; c++) y[4 * h + c] = (T)fmaf(d[c], scale, (float)y[4 * h + c]);
                 }
-                if (t < count && column < p.n) *(V *)(to[s] + column) = y;
+                if (t >= count || column >= p.n) continue;
+                if constexpr (STREAM) __builtin_nontemporal_store(y, (V *)(to[s] + column));
+                else *(V *)(to[s] + column) = y;
             }
             meet();
         };
@@ -474,6 +480,11 @@ bool whole_u(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
     const int64_t blocks = (plan->tiles + plan->bare) * ((c->n + 32 * kWaves - 1) / (32 * kWaves));
     return plan->tiles && plan->most <= kSub && c->rank <= 64 && c->k * c->rank <= 32768 && blocks <= 256;
 }
+
+// y of more than the eight dies' caches hold (32 MB) goes by them.  8168 tokens at rank 64 (k = n = 4096): 44.5 instead of 53 us among calls with
+// other inputs, 55.7 instead of 53.8 between a kernel that writes base and one that reads y; n = 12288: 95 instead of 101 there.  12 MB
+// of y: 20.6 instead of 19.9.
+bool streams(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c) { return plan->tokens > ((1 << 25) / 2) / c->n; }
 
 // Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
 // gather are twice as many (expand of 8168 tokens at rank 64: 41.0 and 38.3 us before its rows were read in runs).
@@ -565,14 +576,15 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
             const size_t lds = std::max(sums, through_lds(RT, ST) ? 2 * kSub * (RT + ST) * 256 : size_t(0));
             if constexpr (RX.value <= 64) {  // (a larger rank would need k of 448 at most)
                 if (whole_u(plan, c)) {
-                    adapter_expand<T, RX.value, kSub, true><<<(unsigned)expand, 256, 0, st>>>(p);
+                    adapter_expand<T, RX.value, kSub, true, false><<<(unsigned)expand, 256, 0, st>>>(p);
                     return;
                 }
             }
             if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
             if (!expand) return;
-            if (ST == 1) adapter_expand<T, RX.value, kSub, false><<<(unsigned)expand, 256, 0, st>>>(p);
-            else adapter_expand<T, RX.value, kTile, false><<<(unsigned)expand, 256, 0, st>>>(p);
+            if (ST == 1) adapter_expand<T, RX.value, kSub, false, false><<<(unsigned)expand, 256, 0, st>>>(p);
+            else if (streams(plan, c)) adapter_expand<T, RX.value, kTile, false, true><<<(unsigned)expand, 256, 0, st>>>(p);
+            else adapter_expand<T, RX.value, kTile, false, false><<<(unsigned)expand, 256, 0, st>>>(p);
         });
     };
     if (c->dtype == KVMIX_F16) run((_Float16)0);

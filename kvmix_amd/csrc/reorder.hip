@@ -8,7 +8,7 @@
 // where not, up to 32 rows' old values are in registers before the first is written.  Otherwise old values that are still wanted
 // when their place is written are put in the LDS first, each by the thread that will want it; where they are too many for
 // all threads of a block, fewer take a turn.
-// 1.1 GB read and written each way where half of 32 rows stay: 480 us (4.6 TB/s); all 32 moved round, 1.2 GB: 0.97 ms, through the LDS 3.7.
+// 1.1 GB read and written each way where half of 32 rows stay: 440 us (5.0 TB/s); all 32 moved round, 1.2 GB: 0.9 ms, through the LDS 3.7.
 #include "copy_rows.h"
 
 namespace kvmix {
@@ -38,10 +38,12 @@ typedef uint16_t half1 __attribute__((aligned(1)));
 
 typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
 
-// Sixteen bytes, or the first n of them, piece by piece: the last of a row is followed by what another thread writes.
+// Sixteen bytes, or the first n of them, piece by piece: the last of a row is followed by what another thread writes.  STREAM: whole ones
+// as what nobody wants again soon.
+template <bool STREAM>
 __device__ __forceinline__ Bytes16 load_bytes(const uint8_t *p, int n)
 {
-    if (n == 16) return *(const word4 *)p;
+    if (n == 16) return STREAM ? __builtin_nontemporal_load((const word4 *)p) : *(const word4 *)p;
     uint32_t first[2] = {0, 0}, four = 0, tail = 0;
     if (n & 8) {
         const word2 x = *(const word2 *)p;
@@ -53,10 +55,12 @@ __device__ __forceinline__ Bytes16 load_bytes(const uint8_t *p, int n)
     return Bytes16{first[0], first[1], four, tail};
 }
 
+template <bool STREAM>
 __device__ __forceinline__ void store_bytes(uint8_t *p, Bytes16 v, int n)
 {
     if (n == 16) {
-        *(word4 *)p = v;
+        if constexpr (STREAM) __builtin_nontemporal_store((word4)v, (word4 *)p);
+        else *(word4 *)p = v;
         return;
     }
     if (n & 8) *(word2 *)p = word2{v[0], v[1]};
@@ -79,7 +83,7 @@ __device__ __forceinline__ Piece16 piece_of(const ReorderItem &it, uint32_t p)
 }
 
 // Rows `change` (a bit each) become their sources, N at once: every old value of these is read before the first is written.
-template <int N>
+template <int N, bool STREAM>
 __device__ __forceinline__ void move_rows(uint8_t *at, int64_t batch, int bytes, uint64_t change, int source)
 {
     while (change) {
@@ -88,20 +92,21 @@ __device__ __forceinline__ void move_rows(uint8_t *at, int64_t batch, int bytes,
 #pragma unroll
         for (int j = 0; j < N; j++)
             if (left) {
-                v[j] = load_bytes(at + __builtin_amdgcn_readlane(source, __builtin_ctzll(left)) * batch, bytes);
+                v[j] = load_bytes<STREAM>(at + __builtin_amdgcn_readlane(source, __builtin_ctzll(left)) * batch, bytes);
                 left &= left - 1;
             }
         left = change;
 #pragma unroll
         for (int j = 0; j < N; j++)
             if (left) {
-                store_bytes(at + __builtin_ctzll(left) * batch, v[j], bytes);
+                store_bytes<STREAM>(at + __builtin_ctzll(left) * batch, v[j], bytes);
                 left &= left - 1;
             }
         change = left;
     }
 }
 
+template <bool STREAM>
 __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
 {
     const int t = threadIdx.x, lane = t % kWave;
@@ -123,9 +128,9 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
             if (begin + t >= end) return;
             const Piece16 piece = piece_of(it, begin + t);
             auto move = [&](int bytes) {
-                if (__popcll(change) <= 8) move_rows<8>(piece.at, piece.batch, bytes, change, source);
-                else if (apart) move_rows<16>(piece.at, piece.batch, bytes, change, source);
-                else move_rows<32>(piece.at, piece.batch, bytes, change, source);
+                if (__popcll(change) <= 8) move_rows<8, STREAM>(piece.at, piece.batch, bytes, change, source);
+                else if (apart) move_rows<16, STREAM>(piece.at, piece.batch, bytes, change, source);
+                else move_rows<32, STREAM>(piece.at, piece.batch, bytes, change, source);
             };
             if (__all(piece.bytes == 16)) move(16);
             else move(piece.bytes);
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
         for (int i = 0; i < staged; i += kReorderAhead) {
 #pragma unroll
             for (int j = 0; j < kReorderAhead; j++)
-                if (i + j < staged) v[j] = load_bytes(piece.at + uniform(early[i + j]) * piece.batch, piece.bytes);
+                if (i + j < staged) v[j] = load_bytes<STREAM>(piece.at + uniform(early[i + j]) * piece.batch, piece.bytes);
 #pragma unroll
             for (int j = 0; j < kReorderAhead; j++)
                 if (i + j < staged) stage[(i + j) * at_once + t] = v[j];
@@ -180,12 +185,12 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
             for (int j = 0; j < kReorderAhead; j++) {
                 if (i + j < n) {
                     const int from = uniform(source[uniform(change[i + j])]), s = uniform(slot[from]);
-                    v[j] = s >= 0 ? stage[s * at_once + t] : load_bytes(piece.at + from * piece.batch, piece.bytes);
+                    v[j] = s >= 0 ? stage[s * at_once + t] : load_bytes<STREAM>(piece.at + from * piece.batch, piece.bytes);
                 }
             }
 #pragma unroll
             for (int j = 0; j < kReorderAhead; j++)
-                if (i + j < n) store_bytes(piece.at + uniform(change[i + j]) * piece.batch, v[j], piece.bytes);
+                if (i + j < n) store_bytes<STREAM>(piece.at + uniform(change[i + j]) * piece.batch, v[j], piece.bytes);
         }
     }
 }
@@ -212,6 +217,11 @@ extern "C" int kvmix_reorder_rows(const kvmix_reorder_t *items, int64_t count, c
     }
     if (rows <= 1 || count == 0) return KVMIX_OK;  // (one row is itself)
     if (!index) return KVMIX_ERR_NULL;
+    // Tensors of more than the 256 MB that the cache before the memory holds go by the caches.  Half of 32 rows, 1 GB in all: 189 instead of 204 us,
+    // 181 instead of 198 before a kernel that reads them; 256 MB: 46 instead of 39, 128 MB before one that reads them 33 instead of 22.
+    __int128 total = 0;
+    for (int64_t i = 0; i < count; i++) total += empty(items[i]) ? 0 : (__int128)rows * items[i].outer * items[i].inner * items[i].row_bytes;
+    const bool stream_by = total > 1 << 28;
     int rc = KVMIX_OK;
     for (int64_t i = 0; i < count;) {
         ReorderArgs a{};
@@ -229,7 +239,9 @@ extern "C" int kvmix_reorder_rows(const kvmix_reorder_t *items, int64_t count, c
             a.count++;
         }
         if (!a.count) continue;
-        reorder_rows<<<a.first[a.count], kReorderThreads, (size_t)rows * 5 * sizeof(int16_t), (hipStream_t)stream>>>(a);
+        const size_t lists = (size_t)rows * 5 * sizeof(int16_t);
+        if (stream_by) reorder_rows<true><<<a.first[a.count], kReorderThreads, lists, (hipStream_t)stream>>>(a);
+        else reorder_rows<false><<<a.first[a.count], kReorderThreads, lists, (hipStream_t)stream>>>(a);
         rc = launch_status();
         if (rc != KVMIX_OK) break;
     }

@@ -140,6 +140,23 @@ def test_values_at_the_ends_of_the_types(dev):
         assert ((got - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_results_beyond_the_caches(dev, dtype):
+    """More than 32 MB of them, to the last columns and tokens: as in parts, and against 64 bits."""
+    from kvmix_amd import ops
+
+    counts, adapters, n = [700, 33, 1, 1400], [0, -1, 1, 0], 8200
+    base, x, a, b, scales = _inputs(dev, counts, 2, 24, 72, n, dtype)
+    plan = ops.adapter_plan(adapters, counts, 2, dev)
+    out = ops.add_adapters(base, x, a, b, plan, scales)
+    want, tol = _want(base, x, a, b, scales, adapters, counts)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+    for at in (0, 4096):
+        part = slice(at, min(at + 4096, n))
+        assert torch.equal(ops.add_adapters(base[:, part], x, a, b[:, part], plan, scales), out[:, part])
+    assert torch.equal(ops.add_adapters(base, x, a, b, plan, scales, out=base), out)
+
+
 def test_strides_and_shapes(dev):
     """Columns of a wider projection in place, three dimensions, weights that are views, rows that sixteen bytes do not fit."""
     from kvmix_amd import ops
