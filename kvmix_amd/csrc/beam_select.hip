@@ -44,7 +44,8 @@ struct BeamArgs {
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 
-template <typename T>
+// STREAM: the logits are more than the caches of the dies keep, and are read as what nobody wants again soon.
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows(BeamArgs a)
 {
     constexpr int PER = 16 / sizeof(T), NT = kBeamThreads, W = NT / kWave;
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows(BeamArgs a)
         const int i = (r * NT + (int)threadIdx.x) * PER;
         if (r * NT * PER < length) {
             if (i + PER <= length) {
-                x[r].raw = *(const uint4u *)(at + i);
+                x[r].raw = STREAM ? __builtin_nontemporal_load((const uint4u *)(at + i)) : *(const uint4u *)(at + i);
             } else {
                 x[r].raw = uint4v{none, none, none, none};
 #pragma unroll
@@ -389,7 +390,14 @@ extern "C" int kvmix_beam_select(const kvmix_beam_select_t *p, void *workspace, 
     a.part = (BeamPart *)workspace, a.keys = (uint64_t *)((BeamPart *)workspace + parts);
     a.out_scores = p->out_scores, a.parents = p->parents, a.tokens = p->tokens;
     hipStream_t st = (hipStream_t)stream;
-    with_type(p->dtype, [&](auto zero) { beam_rows<decltype(zero)><<<(unsigned)parts, kBeamThreads, 0, st>>>(a); });
+    // Logits of more than the eight dies' caches hold (32 MB): 16.3 instead of 18.1 us behind a kernel that writes 64 x 8 rows of 32000 in fp32, 84
+    // instead of 143 of 64 x 16 of 128000; 5 MB in fp16 11.4 instead of 10.4.
+    const bool stream_by = p->requests * p->beams * p->vocab > (1 << 25) / (p->dtype == KVMIX_F32 ? 4 : 2);
+    with_type(p->dtype, [&](auto zero) {
+        using T = decltype(zero);
+        if (stream_by) beam_rows<T, true><<<(unsigned)parts, kBeamThreads, 0, st>>>(a);
+        else beam_rows<T, false><<<(unsigned)parts, kBeamThreads, 0, st>>>(a);
+    });
     beam_join<<<(unsigned)p->requests, kBeamThreads, 0, st>>>(a);
     return launch_status();
 }

@@ -207,3 +207,15 @@ def test_many_parts(dev, R, W, V, count, dtype):
     done = torch.rand(R, W, generator=torch.Generator().manual_seed(3)) < 0.3
     check(ops.beam_select(logits, scores, count), plain(logits, scores, count))
     check(ops.beam_select(logits, scores, count, done.to(dev), 7), plain(logits, scores, count, done, 7))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_logits_beyond_the_caches(dev, dtype):
+    """More than 32 MB of them, at odd offsets."""
+    from kvmix_amd import ops
+
+    R, W, V = 70, 8, 32003
+    logits, scores = random(R, W, V, dtype, dev, seed=8)
+    got = ops.beam_select(logits, scores, 10)
+    for r in (*range(0, R, 9), R - 1):
+        check([x[r:r + 1] for x in got], plain(logits[r:r + 1], scores[r:r + 1], 10))
