@@ -136,7 +136,7 @@ __device__ __forceinline__ void shrink_few(const T *const (&a)[RT], const T *x, 
 
 // The same of more tokens, over whole steps of kStep of k through the LDS: a wave reads a quarter of the rows of A and x, 256 bytes of each at once, and
 // multiplies one of a step's four units.  A row's pieces of sixteen bytes are exchanged by its number, so that no lanes meet in a bank.
-template <typename T, int RT, int ST>
+template <bool STREAM, typename T, int RT, int ST>
 __device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *const (&x)[ST], void *lds, int begin, int to, int k, int wave, int m,
                                               int g, floatx4 (&acc)[RT][ST])
 {
@@ -151,7 +151,10 @@ __device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *
 #pragma unroll
         for (int r = 0; r < RT; r++) v.a[r] = *(const V *)(a[r] + min(at, k - 8));
 #pragma unroll
-        for (int s = 0; s < ST; s++) v.x[s] = *(const V *)(x[s] + min(at, k - 8));
+        for (int s = 0; s < ST; s++) {
+            const V *from = (const V *)(x[s] + min(at, k - 8));
+            v.x[s] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
         if (begin + kStep * i + kStep > k && at >= k) {  // (k in whole eights)
 #pragma unroll
             for (int r = 0; r < RT; r++) v.a[r] = V{};
@@ -190,7 +193,8 @@ __device__ __forceinline__ void shrink_staged(const T *const (&a)[RT], const T *
 // 10.9 us with the other kernel; one of rank 64, k 4096: 7.2 and 6.6).
 constexpr bool through_lds(int RT, int ST) { return RT > 2 || ST > 1; }
 
-template <typename T, int RT>
+// STREAM: x is more than the caches of the dies keep.
+template <typename T, int RT, bool STREAM>
 __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 {
     constexpr int LD = RT * 16, Q = RT * 4;
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(256) adapter_shrink(AdapterArgs p)
 #pragma unroll
         for (int r = 0; r < RT; r++)  // (what lies beyond the rank is not kept)
             a[r] = (const T *)p.a + adapter * p.a_as + min(chunk * RT * 16 + (staged ? wave * 4 * RT + g + 4 * r : 16 * r + m), p.rank - 1) * p.a_rs;
-        if constexpr (staged) shrink_staged<T, RT, ST>(a, x, sums, begin, to, p.k, wave, m, g, acc);
+        if constexpr (staged) shrink_staged<STREAM>(a, x, sums, begin, to, p.k, wave, m, g, acc);
         else shrink_few<4>(a, x[0], begin / 32, min(to, p.k + 31) / 32, p.k, wave, g, acc);
 #pragma unroll
         for (int s = 0; s < ST; s++)
@@ -486,6 +490,10 @@ bool whole_u(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
 // of y: 20.6 instead of 19.9.
 bool streams(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c) { return plan->tokens > ((1 << 25) / 2) / c->n; }
 
+// x of more than twice that: 4096 tokens of k = 11008 (90 MB) 46 instead of 49.7 us between a kernel that writes base and one that reads y, 16384 of
+// 4096 (134 MB) 96 instead of 108; 8168 of 4096 (67 MB) 55 instead of 57, but 47.6 instead of 44.6 among calls with other inputs.
+bool streams_x(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c) { return plan->tokens > ((1 << 26) / 2) / c->k; }
+
 // Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
 // gather are twice as many (expand of 8168 tokens at rank 64: 41.0 and 38.3 us before its rows were read in runs).
 constexpr int64_t kStretches = 256;
@@ -580,7 +588,8 @@ extern "C" int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_
                     return;
                 }
             }
-            if (shrink) adapter_shrink<T, RT><<<(unsigned)shrink, 256, lds, st>>>(p);
+            if (shrink && streams_x(plan, c)) adapter_shrink<T, RT, true><<<(unsigned)shrink, 256, lds, st>>>(p);
+            else if (shrink) adapter_shrink<T, RT, false><<<(unsigned)shrink, 256, lds, st>>>(p);
             if (!expand) return;
             if (ST == 1) adapter_expand<T, RX.value, kSub, false, false><<<(unsigned)expand, 256, 0, st>>>(p);
             else if (streams(plan, c)) adapter_expand<T, RX.value, kTile, false, true><<<(unsigned)expand, 256, 0, st>>>(p);

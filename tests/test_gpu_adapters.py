@@ -157,6 +157,26 @@ def test_results_beyond_the_caches(dev, dtype):
     assert torch.equal(ops.add_adapters(base, x, a, b, plan, scales, out=base), out)
 
 
+def test_inputs_beyond_the_caches(dev):
+    """More than 64 MB of x, of two adapters' tokens and of none's, against 64 bits."""
+    from kvmix_amd import ops
+
+    k, counts, adapters = 11016, [2900, 17, 260], [1, -1, 0]
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(3177, k, generator=g, device=dev).half()
+    a, b = (torch.randn(2, 40, k, generator=g, device=dev) * k ** -0.5).half(), torch.randn(2, 48, 40, generator=g, device=dev).half()
+    base = torch.randn(3177, 48, generator=g, device=dev).half()
+    out = ops.add_adapters(base, x, a, b, ops.adapter_plan(adapters, counts, 2, dev))
+    for at in range(0, 3177, 353):  # (in 64 bits, some rows at a time)
+        i = torch.tensor([1 if t < 2900 else 0 for t in range(at, at + 353)], device=dev)
+        u = torch.stack([x[at:at + 353].double() @ a[j].double().t() for j in range(2)])[i, torch.arange(353, device=dev)]
+        size = torch.stack([x[at:at + 353].double().abs() @ a[j].double().abs().t() for j in range(2)])[i, torch.arange(353, device=dev)]
+        y = base[at:at + 353].double() + (u[:, None] * b[i].double()).sum(-1) * torch.tensor([0.0 if 2900 <= t < 2917 else 1.0 for t in range(at, at + 353)], device=dev)[:, None]
+        off = k * 2.0 ** -24 * size + u.abs().amax(-1, keepdim=True) * 2.0 ** -22
+        e = (off[:, None] * b[i].double().abs()).sum(-1) + 80 * 2.0 ** -24 * (u.abs()[:, None] * b[i].double().abs()).sum(-1)
+        assert ((out[at:at + 353].double() - y).abs() <= e + 2.0 ** -11 * (y.abs() + e) + 2.0 ** -25 + 2.0 ** -23 * (y.abs() + base[at:at + 353].double().abs())).all()
+
+
 def test_strides_and_shapes(dev):
     """Columns of a wider projection in place, three dimensions, weights that are views, rows that sixteen bytes do not fit."""
     from kvmix_amd import ops
