@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) paged_append(AppendArgs a)
 // With u = x[d], w = x[d + D / 2]:  u cos_d - w sin_d  and  w cos_d' + u sin_d', d' = d + D / 2.
 // Bound by memory.  A wave takes one token and as many heads as it has lanes for (eight of 128 channels): its lanes are the pairs of
 // pieces of a head, so that its reads are 2 KB that follow one another.  (Several such turns of a wave, with its part of the tables
-// read once, gained nothing: 79.9 and 77.9 us, 20 and 19.6.)  8 x 1021 tokens of 32 heads, fp32 tables: 78 to 80 us, 410 MB, 5.1 TB/s;
+// read once, gained nothing: 79.9 and 77.9 us, 20 and 19.6.)  8 x 1021 tokens of 32 heads, fp32 tables: 69 to 71 us, 410 MB, 5.8 TB/s;
 // rotated with tensors and appended 979.  64 tokens of 32 heads over 8: 4.8 us, a launch.
 
 template <typename T>
@@ -144,6 +144,19 @@ __device__ __forceinline__ void rotate_pieces(half8v &u, half8v &w, const TableP
     }
 }
 
+template <bool STREAM>
+__device__ __forceinline__ half8v load_piece(const _Float16 *at)
+{
+    return STREAM ? __builtin_nontemporal_load((const half8v *)at) : *(const half8v *)at;
+}
+
+template <bool STREAM>
+__device__ __forceinline__ void store_piece(_Float16 *at, half8v v)
+{
+    if constexpr (STREAM) __builtin_nontemporal_store(v, (half8v *)at);
+    else *(half8v *)at = v;
+}
+
 struct RopeStoreArgs {
     const _Float16 *qkv;
     int64_t x_ts, x_hs;
@@ -157,8 +170,9 @@ struct RopeStoreArgs {
     int parts, rotating;                            // waves to a token; blocks of the launch that rotate
 };
 
-// T: of the tables.  TENSORS: rounded as the fp16 tensor expression is.
-template <int D, typename T, bool TENSORS>
+// T: of the tables.  TENSORS: rounded as the fp16 tensor expression is.  STREAM: the projection is read, queries and keys are written
+// as what nobody wants again soon.
+template <int D, typename T, bool TENSORS, bool STREAM>
 __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
 {
     constexpr int C = D / 8, HALF = C / 2;
@@ -173,7 +187,7 @@ __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
         const _Float16 *x = a.qkv + token * a.x_ts + at;
         const int head = part * (kWave / HALF) + lane / HALF;
         if (head >= total) return;
-        half8v u = *(const half8v *)(x + head * a.x_hs), w = *(const half8v *)(x + head * a.x_hs + D / 2);
+        half8v u = load_piece<STREAM>(x + head * a.x_hs), w = load_piece<STREAM>(x + head * a.x_hs + D / 2);
         TablePieces<T> t;
         load_table(t.c1, cos), load_table(t.c2, cos + D / 2), load_table(t.s1, sin), load_table(t.s2, sin + D / 2);
         if constexpr (TENSORS) rotate_as_tensors(u, w, t);
@@ -181,8 +195,8 @@ __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
         const int page = slot >> a.page_log2, place = slot & ((1 << a.page_log2) - 1);
         _Float16 *to = a.q + token * a.q_ts + head * a.q_hs + at;
         if (head >= a.heads) to = a.rows + ((((int64_t)page * a.kv_heads + head - a.heads) * 2) << a.page_log2) * D + (int64_t)place * D + at;
-        *(half8v *)to = u;
-        *(half8v *)(to + D / 2) = w;
+        store_piece<STREAM>(to, u);
+        store_piece<STREAM>(to + D / 2, w);
         return;
     }
     const int unit = (blockIdx.x - a.rotating) * 4 + wave;
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(256) paged_rope_append(RopeStoreArgs a)
 #pragma unroll
     for (int i = 0; i < kTurns; i++) {
         const int t = (i * kWave + lane) / C, c = (i * kWave + lane) % C;
-        if (t < n) value[i] = *(const half8v *)(v + t * a.x_ts + 8 * c);
+        if (t < n) value[i] = load_piece<STREAM>(v + t * a.x_ts + 8 * c);
     }
 #pragma unroll
     for (int i = 0; i < kTurns; i++) {
@@ -572,10 +586,20 @@ extern "C" int kvmix_paged_rope_append(const kvmix_paged_pool_t *p, const kvmix_
                              (PlanWords)list + plan->store_at, (int)plan->tokens, (int)plan->heads, (int)p->kv_heads, (int)(plan->stores * p->kv_heads),
                              __builtin_ctzll((uint64_t)p->page_size), (int)parts, (int)rotating};
     const unsigned grid = (unsigned)(rotating + turning);
+    // A projection of more than 128 MB: 201 MB 71 instead of 78 us, 69 instead of 83 between a kernel that writes it and ones that read queries and
+    // pages; 402 MB 145 instead of 152, 141 instead of 152 there; 100 MB 38 instead of 39, but 42 instead of 36.5 there.
+    const bool stream_by = plan->tokens * (plan->heads + 2 * p->kv_heads) > (1 << 27) / (2 * p->head_dim);
     with_dim(p->head_dim, [&](auto D) {
-        if (c->table_dtype == KVMIX_F32) paged_rope_append<D.value, float, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-        else if (c->as_tensors) paged_rope_append<D.value, _Float16, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-        else paged_rope_append<D.value, _Float16, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        auto run = [&](auto table, auto tensors, auto by) {
+            paged_rope_append<D.value, decltype(table), tensors.value, by.value><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+        };
+        auto with = [&](auto by) {
+            if (c->table_dtype == KVMIX_F32) run(0.0f, std::false_type(), by);
+            else if (c->as_tensors) run((_Float16)0, std::true_type(), by);
+            else run((_Float16)0, std::false_type(), by);
+        };
+        if (stream_by) with(std::true_type());
+        else with(std::false_type());
     });
     return launch_status();
 }

@@ -58,3 +58,29 @@ def test_logits_far_apart(dev, dtype):
     scores = torch.linspace(-9, -1, R, device=dev)[:, None].contiguous()
     for a, b in zip(ops.beam_select(big[:, :, 5:3006], scores, 3), ops.beam_select(near, scores, 3)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind,as_tensors", [(torch.float32, False), (torch.float16, False), (torch.float16, True)])
+def test_a_projection_beyond_the_caches(dev, kind, as_tensors):
+    """More than 128 MB of it: as sequence by sequence."""
+    from kvmix_amd import ops
+
+    H, KV, D, P, lens = 48, 16, 128, 64, [4000, 1, 3301]
+    T = sum(lens)
+    qkv = torch.randn(T, H + 2 * KV, D, generator=torch.Generator(device=dev).manual_seed(5), device=dev).half()
+    angle = torch.rand(T, D, generator=torch.Generator().manual_seed(6)).to(dev)
+    cos, sin = angle.cos().to(kind), angle.sin().to(kind)
+    need = [-(-n // P) for n in lens]
+    table = torch.full((3, max(need)), -1, dtype=torch.int32)
+    ids = torch.randperm(sum(need), generator=torch.Generator().manual_seed(7)).int().split(need)
+    for row, i in zip(table, ids):
+        row[:len(i)] = i
+    rows, apart = (torch.zeros(sum(need), KV, 2, P, D, dtype=torch.float16, device=dev) for _ in range(2))
+    q = ops.paged_rope_append(qkv, cos, sin, rows, ops.paged_plan(table, lens, [0] * 3, lens, H, KV, D, P, dev), as_tensors)
+    at = 0
+    for s, n in enumerate(lens):
+        part = slice(at, at + n)
+        plan = ops.paged_plan(table[s:s + 1], [n], [0], [n], H, KV, D, P, dev)
+        assert torch.equal(ops.paged_rope_append(qkv[part], cos[part], sin[part], apart, plan, as_tensors), q[part])
+        at += n
+    assert torch.equal(rows, apart)
