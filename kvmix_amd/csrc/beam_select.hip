@@ -22,7 +22,11 @@
 namespace kvmix {
 
 constexpr int kBeamThreads = 256, kBeamPieces = 8;  // of sixteen bytes, of a thread
-constexpr int kBeamsMost = 64, kListsMost = 4096;   // (of 2^25 values in 32 bits)
+constexpr int64_t kBeamValues = int64_t(1) << 25;   // of all beams of a request
+constexpr int kBeamsMost = 64;
+// Parts of a request at most: what a block holds in 32 bits to each, and one that is not full to a beam.
+constexpr int kListsMost = kBeamValues / (kBeamThreads * kBeamPieces * 4) + kBeamsMost;
+static_assert(kListsMost >= kTopMost * kTopMost && kListsMost >= 1024, "the join keeps as many candidates; beam_plan makes as many parts of few values");
 
 typedef uint32_t uint4u __attribute__((ext_vector_type(4), aligned(2)));  // (rows are aligned as their values are)
 
@@ -339,7 +343,7 @@ struct BeamPlan {
 };
 
 // Parts of a row: as many as a block can hold at most, and shorter ones, down to two pieces to a thread, as long as the chip is not full of
-// blocks (or a request has more lists than the join takes): 512 or 2048 blocks take the same time as 1024.
+// blocks: 512 or 2048 blocks take the same time as 1024.
 BeamPlan beam_plan(const kvmix_beam_select_t *p)
 {
     const int64_t rows = std::max<int64_t>(p->requests * p->beams, 1), per = p->dtype == KVMIX_F32 ? 4 : 8, piece = kBeamThreads * per;
@@ -356,7 +360,7 @@ int beam_check(const kvmix_beam_select_t *p)
     if (p->requests < 0 || p->beams <= 0 || p->vocab <= 0 || p->count <= 0 || p->row_stride < 0 || (p->done && (p->end < 0 || p->end >= p->vocab)) ||
         (p->stay && p->count != p->beams))
         return KVMIX_ERR_SHAPE;
-    if (p->beams > kBeamsMost || p->count > kTopMost || p->count > p->vocab || p->vocab > (1 << kTokenBits) || p->beams * p->vocab > (1 << 25))
+    if (p->beams > kBeamsMost || p->count > kTopMost || p->count > p->vocab || p->vocab > (1 << kTokenBits) || p->beams * p->vocab > kBeamValues)
         return KVMIX_ERR_UNSUPPORTED;
     if ((__int128)p->requests * p->beams * ((p->vocab + 2047) / 2048 + 1) >= 1 << 24) return KVMIX_ERR_UNSUPPORTED;  // (blocks of 256 threads)
     return KVMIX_OK;
