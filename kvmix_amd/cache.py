@@ -64,6 +64,9 @@ class _Tail:
         B, H, n, D = new.shape
         if self.buf is None:
             self.buf = torch.zeros((B, H, max(reserve, n), D), dtype=new.dtype, device=new.device)
+        elif (self.buf.shape[0], self.buf.shape[1], self.buf.shape[3]) != (B, H, D):  # (a copy would repeat one sequence for all)
+            raise RuntimeError(f"the cache holds {self.buf.shape[0]} sequences of {self.buf.shape[1]} heads of {self.buf.shape[3]}, the new tokens "
+                               f"are of {B} of {H} of {D}")
         self.room(n).copy_(new)
         self.len += n
 
@@ -188,6 +191,7 @@ class PackedKVCache:
         if not key_states.is_cuda:
             raise RuntimeError("KVmix operators run on the GPU only: got a tensor on " + str(key_states.device))
         key_states, value_states = key_states.detach(), value_states.detach()  # the cache is not part of any autograd graph
+        self.fit(key_states.shape[0])
         n = key_states.shape[2]
         steady = max((self.residual_length or 0) + self.Vgroup_size, 2 * self.Vgroup_size)  # a tail between two flushes
         # Many tokens onto empty tails (a prompt): what the policy flushes is quantized straight from
@@ -280,7 +284,7 @@ class PackedKVCache:
         self._flushed_ahead = False
 
     def reset(self) -> None:
-        """Forget every token; the buffers stay allocated and are reused by the next prompt."""
+        """Forget every token; the buffers stay allocated and are reused by the next prompt of as many sequences."""
         self.kv_seq_len = self.k_tokens = self.v_tokens = 0
         for tail in (self._k_tail, self._v_tail):
             tail.start = tail.len = 0
@@ -290,7 +294,7 @@ class PackedKVCache:
         self._flushed_ahead = False
 
     def fit(self, batch: int) -> None:
-        """An empty cache lets go of buffers that were of another batch."""
+        """An empty cache lets go of buffers that were of another batch (append does so by itself)."""
         tail = self._k_tail.buf
         if self.kv_seq_len == 0 and tail is not None and tail.shape[0] != batch:
             self._k_tail, self._v_tail = _Tail(), _Tail()

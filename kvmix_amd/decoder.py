@@ -267,15 +267,12 @@ class Decoder:
         caches are repeated for the beams and reordered in place between the steps (afterwards they hold all beams but for their last
         tokens); nothing waits for the GPU."""
         from . import ops
-        from .cache import PackedKVCache, reorder_caches, repeat_caches
+        from .cache import reorder_caches, repeat_caches
 
         if new_tokens < 1 or self.position or not prompt_ids.numel():
             raise RuntimeError("beam_search: a new token at least, from prompts that nothing is cached of")
         B = prompt_ids.shape[0]
         check_beams(B, beams, end, self.cfg.vocab_size)
-        for c in self.caches:
-            if isinstance(c, PackedKVCache):
-                c.fit(B)
         logits = self.forward(prompt_ids)[:, None].expand(-1, beams, -1)
         self.caches = repeat_caches(self.caches, beams)
         ids = prompt_ids.new_zeros(B * beams, new_tokens)
