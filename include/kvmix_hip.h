@@ -52,6 +52,7 @@ extern "C" {
 #define KVMIX_ERR_LENGTHS (-17)    /* kvmix_paged_plan: lengths that do not fit one another or the table */
 #define KVMIX_ERR_MEMORY (-18)     /* host memory could not be had */
 #define KVMIX_ERR_ADAPTER (-19)    /* an adapter's number outside its pool */
+#define KVMIX_ERR_OVERLAP (-20)    /* kvmix_reorder_rows: two tensors with memory in common */
 
 #define KVMIX_F16 0
 #define KVMIX_F32 1
@@ -728,7 +729,9 @@ int kvmix_beam_select(const kvmix_beam_select_t *p, void *workspace, int64_t wor
 /*
  * Tensors reordered along their first dimension in place, t[i] = old t[index[i]], all with the same index [rows] in device memory (rows up
  * to 1024; an index outside of [0, rows) leaves its row as it is).  Entry i of a tensor lies batch_stride further on than entry
- * i - 1 and is `outer` times `inner` rows of row_bytes; strides in bytes.  Entries must not overlap, and no two tensors may, nor one the index.
+ * i - 1 and is `outer` times `inner` rows of row_bytes; strides in bytes.  Entries must not overlap, nor a tensor the index.
+ * Two tensors with a byte in common are refused (ones that lie between one another's rows have none; ones whose rows follow one
+ * another at different strides, so that it takes more than 65536 comparisons of a row to tell, are refused too).
  */
 typedef struct kvmix_reorder {
     void *base;

@@ -35,6 +35,7 @@ extern "C" const char *kvmix_strerror(int code)
                "not packed, pages for all tokens in the table";
     case KVMIX_ERR_MEMORY: return "host memory could not be had";
     case KVMIX_ERR_ADAPTER: return "an adapter's number lies outside the pool of adapters";
+    case KVMIX_ERR_OVERLAP: return "no two tensors may overlap: what one writes the other reads";
     default: return "unknown kvmix error";
     }
 }

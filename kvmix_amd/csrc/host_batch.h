@@ -198,10 +198,6 @@ void reorder_rows(const std::vector<Tensor> &tensors, const Tensor &index_in)
         if (t.numel() == 0) continue;
         items.push_back(reorder_item(t));
     }
-    std::vector<const void *> bases;
-    for (const auto &item : items) bases.push_back(item.base);
-    std::sort(bases.begin(), bases.end());
-    if (std::adjacent_find(bases.begin(), bases.end()) != bases.end()) fail("reorder_rows: no two tensors may overlap");
     Tensor index = index_in.contiguous();
     for (const Tensor &t : tensors)  // (it is read while they are written)
         if (!spans_apart(t, index)) {

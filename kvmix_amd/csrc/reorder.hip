@@ -9,6 +9,10 @@
 // when their place is written are put in the LDS first, each by the thread that will want it; where they are too many for
 // all threads of a block, fewer take a turn.
 // 1.1 GB read and written each way where half of 32 rows stay: 440 us (5.0 TB/s); all 32 moved round, 1.2 GB: 0.9 ms, through the LDS 3.7.
+#include <algorithm>
+#include <numeric>
+#include <vector>
+
 #include "copy_rows.h"
 
 namespace kvmix {
@@ -195,6 +199,94 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
     }
 }
 
+namespace {
+
+// What a tensor takes of memory: runs of bytes, every stride[i] bytes of each dimension, larger strides first.
+struct Layout {
+    int64_t at;              // of the first byte
+    int64_t size[3], stride[3];
+    int64_t extent[4];       // what is left of it from dimension i on spans; the last: a run
+    int dims;
+};
+
+// Bytes from the first to behind the last.
+__int128 extent_of(const kvmix_reorder_t &p, int64_t rows)
+{
+    return (__int128)(rows - 1) * p.batch_stride + (__int128)(p.outer - 1) * p.outer_stride + (__int128)(p.inner - 1) * p.inner_stride + p.row_bytes;
+}
+
+Layout layout_of(const kvmix_reorder_t &p, int64_t rows)
+{
+    struct Dim {
+        int64_t size, stride;
+    } dim[3] = {{rows, p.batch_stride}, {p.outer, p.outer_stride}, {p.inner, p.inner_stride}};
+    std::sort(dim, dim + 3, [](const Dim &a, const Dim &b) { return a.stride > b.stride; });
+    Layout l{};
+    l.at = (int64_t)p.base;
+    for (const Dim &d : dim)
+        if (d.size > 1) l.size[l.dims] = d.size, l.stride[l.dims++] = d.stride;
+    l.extent[l.dims] = p.row_bytes;
+    for (int i = l.dims - 1; i >= 0; i--) l.extent[i] = (l.size[i] - 1) * l.stride[i] + l.extent[i + 1];
+    return l;
+}
+
+int64_t down(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Columns beside one another of the same wider rows: the runs of both begin at one place each of a stride that all of theirs are multiples
+// of, and fit beside one another there.
+bool columns_apart(const Layout &a, int i, const Layout &b, int j, int64_t d)
+{
+    int64_t stride = 0;
+    while (i < a.dims) stride = std::gcd(stride, a.stride[i++]);
+    while (j < b.dims) stride = std::gcd(stride, b.stride[j++]);
+    d = (d % stride + stride) % stride;
+    return d >= a.extent[a.dims] && d + b.extent[b.dims] <= stride;
+}
+
+// Whether what is left of a from dimension i on and of b from j on, which begins `d` bytes after a's, have a byte in common.  Where their strides
+// are alike only the distance of their indexes matters, and few distances bring them near one another; where not, the larger
+// stride's entries are looked at one by one.  That ends after `steps`: then they count as meeting.
+bool meet(const Layout &a, int i, const Layout &b, int j, int64_t d, int &steps)
+{
+    if (d >= a.extent[i] || -d >= b.extent[j]) return false;
+    if ((i == a.dims && j == b.dims) || --steps < 0) return true;
+    const bool both = i < a.dims && j < b.dims && a.stride[i] == b.stride[j], of_a = both || j == b.dims || (i < a.dims && a.stride[i] > b.stride[j]);
+    const bool of_b = both || !of_a;
+    if (!both && i < a.dims && j < b.dims && columns_apart(a, i, b, j, d)) return false;
+    const int64_t stride = of_a ? a.stride[i] : b.stride[j], ea = a.extent[i + of_a], eb = b.extent[j + of_b];
+    const int64_t least = of_a ? -(a.size[i] - 1) : 0, most = of_b ? b.size[j] - 1 : 0;  // of the index of b less that of a
+    for (int64_t m = std::max(least, down(-eb - d, stride) + 1); m <= std::min(most, down(ea - d - 1, stride)); m++)
+        if (meet(a, i + of_a, b, j + of_b, d + m * stride, steps)) return true;
+    return false;
+}
+
+// Whether two of the tensors have memory in common, or a code of its own.
+int check_apart(const kvmix_reorder_t *items, int64_t count, int64_t rows)
+{
+    struct Span {
+        int64_t from, to;
+        const kvmix_reorder_t *item;
+    };
+    std::vector<Span> all;
+    all.reserve(count);
+    for (int64_t i = 0; i < count; i++) {
+        const kvmix_reorder_t &p = items[i];
+        if (p.outer == 0 || p.inner == 0 || p.row_bytes == 0) continue;
+        const __int128 extent = extent_of(p, rows);
+        if (extent < 0 || extent > (int64_t)1 << 60) return KVMIX_ERR_UNSUPPORTED;  // (nothing that an address space could hold)
+        all.push_back({(int64_t)p.base, (int64_t)p.base + (int64_t)extent, &p});
+    }
+    std::sort(all.begin(), all.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    for (size_t i = 0; i < all.size(); i++)
+        for (size_t j = i + 1; j < all.size() && all[j].from < all[i].to; j++) {
+            const Layout a = layout_of(*all[i].item, rows), b = layout_of(*all[j].item, rows);
+            int steps = 1 << 16;
+            if (meet(a, 0, b, 0, b.at - a.at, steps)) return KVMIX_ERR_OVERLAP;
+        }
+    return KVMIX_OK;
+}
+
+}  // namespace
 }  // namespace kvmix
 
 using namespace kvmix;
@@ -216,13 +308,19 @@ extern "C" int kvmix_reorder_rows(const kvmix_reorder_t *items, int64_t count, c
             return KVMIX_ERR_UNSUPPORTED;
     }
     if (rows <= 1 || count == 0) return KVMIX_OK;  // (one row is itself)
+    int rc = KVMIX_OK;
+    try {
+        rc = check_apart(items, count, rows);
+    } catch (...) {  // (what a vector throws)
+        return KVMIX_ERR_MEMORY;
+    }
+    if (rc != KVMIX_OK) return rc;
     if (!index) return KVMIX_ERR_NULL;
     // Tensors of more than the 256 MB that the cache before the memory holds go by the caches.  Half of 32 rows, 1 GB in all: 189 instead of 204 us,
     // 181 instead of 198 before a kernel that reads them; 256 MB: 46 instead of 39, 128 MB before one that reads them 33 instead of 22.
     __int128 total = 0;
     for (int64_t i = 0; i < count; i++) total += empty(items[i]) ? 0 : (__int128)rows * items[i].outer * items[i].inner * items[i].row_bytes;
     const bool stream_by = total > 1 << 28;
-    int rc = KVMIX_OK;
     for (int64_t i = 0; i < count;) {
         ReorderArgs a{};
         a.index = index, a.rows = (int)rows;
