@@ -8,10 +8,12 @@
 //            the LDS and multiply a quarter of these each.  (Few tokens and ranks: each wave its own quarter, without the LDS.)  The
 //            waves' sums come together in the LDS, those of the stretches (there are several where there are few tiles) in
 //   expand   y = base + s B u.  A block sums u of its tile and keeps it in the LDS, then takes 128 columns of y at a time, a quarter of them
-//            to a wave.  u is kept as the sum of two numbers of 16 bits, of each token times a power of two that brings its largest
-//            just below 2^14 (bf16: 2): next to its largest, u is exact to 2^-22 (bf16: 2^-16), where it rounds to fp16 alone it would
-//            be off by 2^-11 before the sum over the ranks.  Rows of B are dealt to two matrix products so that a lane ends with eight
-//            columns of one token that follow one another; through the LDS they come to where 256 bytes of a row of base are.
+//            to a wave.  u is kept as the sum of two numbers of 16 bits: next to a token's largest it is exact to 2^-22 (bf16: 2^-16), where it
+//            rounds to fp16 alone it would be off by 2^-11 before the sum over the ranks.  In fp16 it is kept times a power of two that
+//            brings the token's largest just below 2^14.  bf16 has all of fp32's exponents: what is below 2^-8 is brought up to there, so that
+//            second parts keep their digits and 128 products with the largest of B stay below 2^128, and what is beyond 2^126, which could
+//            round to an infinity, down to there.  Rows of B are dealt to two matrix products so that a lane ends with eight columns of
+//            one token that follow one another; through the LDS they come to where 256 bytes of a row of base are.
 // Reads of rows in runs of 256 bytes by a wave are what counts: as the matrix products take them, 64 bytes of each of sixteen rows, the
 // same bytes take 26 us instead of 19 (x) and 38 instead of 28 (base and y).  Both kernels read a step ahead of the one that is multiplied,
 // and expand's first reads go out before it sums u.
@@ -276,7 +278,6 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
         return;
     }
     auto sum = [&](auto st) {
-        constexpr int kTop = std::is_same<T, _Float16>::value ? 14 : 1;  // (bf16 has all of fp32's exponents: products with B must not leave them)
         constexpr int P = (decltype(st)::value * kSub * L + 255) / 256, AHEAD = P >= 4 ? 2 : P == 2 ? 4 : 8;  // turns of the block
         const int c = threadIdx.x % L, t0 = threadIdx.x / L;
         floatx4 s[P] = {};
@@ -323,7 +324,8 @@ __global__ void __launch_bounds__(256) adapter_expand(AdapterArgs p)
 #pragma unroll
             for (int o = L / 2; o; o /= 2) most = fmaxf(most, __shfl_xor(most, o));
             // (the power of numbers below 2^-100 is that of 2^-100; infinities go through as they are, and their second part is nothing)
-            const int e = (most > 0.0f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0) - kTop;
+            const int top = most > 0.0f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0;
+            const int e = std::is_same<T, _Float16>::value ? top - 14 : max(min(top + 8, 0), top - 126);
             typedef T four __attribute__((ext_vector_type(4)));
             four high, low;
 #pragma unroll
