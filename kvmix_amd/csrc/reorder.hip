@@ -86,9 +86,10 @@ __device__ __forceinline__ Piece16 piece_of(const ReorderItem &it, uint32_t p)
     return {it.base + o * it.outer + (row - o * it.rows.d) * it.inner + in, it.batch, (int)(it.row_bytes - in < 16 ? it.row_bytes - in : 16)};
 }
 
-// Rows `change` (a bit each) become their sources, N at once: every old value of these is read before the first is written.
+// Rows `change` (a bit each) become their sources, N at once: every old value of these is read before the first is written.  All lanes
+// come here, since each has the source of a row in its register; those that have no piece of their own (`mine`) write nothing.
 template <int N, bool STREAM>
-__device__ __forceinline__ void move_rows(uint8_t *at, int64_t batch, int bytes, uint64_t change, int source)
+__device__ __forceinline__ void move_rows(uint8_t *at, int64_t batch, int bytes, bool mine, uint64_t change, int source)
 {
     while (change) {
         Bytes16 v[N];
@@ -99,13 +100,15 @@ __device__ __forceinline__ void move_rows(uint8_t *at, int64_t batch, int bytes,
                 v[j] = load_bytes<STREAM>(at + __builtin_amdgcn_readlane(source, __builtin_ctzll(left)) * batch, bytes);
                 left &= left - 1;
             }
-        left = change;
+        if (mine) {
+            uint64_t to = change;
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            if (left) {
-                store_bytes<STREAM>(at + __builtin_ctzll(left) * batch, v[j], bytes);
-                left &= left - 1;
-            }
+            for (int j = 0; j < N; j++)
+                if (to) {
+                    store_bytes<STREAM>(at + __builtin_ctzll(to) * batch, v[j], bytes);
+                    to &= to - 1;
+                }
+        }
         change = left;
     }
 }
@@ -114,7 +117,7 @@ template <bool STREAM>
 __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
 {
     const int t = threadIdx.x, lane = t % kWave;
-    const int64_t mine = a.rows <= kWave && lane < a.rows ? a.index[lane] : lane;
+    const int64_t own = a.rows <= kWave && lane < a.rows ? a.index[lane] : lane;
     const int nth = __popcll(__ballot(lane < a.count && blockIdx.x >= a.first[min(lane, kReorderItems)])) - 1;
     const ReorderItem it = a.item[nth];
     const uint32_t begin = (blockIdx.x - a.first[nth]) * kReorderThreads;
@@ -122,19 +125,20 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_rows(ReorderArgs a)
 
     if (a.rows <= kWave) {
         // every wave has all rows in its lanes
-        const int source = mine >= 0 && mine < a.rows ? (int)mine : lane;  // (an index that is none changes nothing)
+        const int source = own >= 0 && own < a.rows ? (int)own : lane;  // (an index that is none changes nothing)
         const uint64_t change = __ballot(source != lane);
         if (!change) return;
         uint64_t wanted = 0;
         for (uint64_t left = change; left; left &= left - 1) wanted |= 1ull << __builtin_amdgcn_readlane(source, __builtin_ctzll(left));
         const bool apart = !(wanted & change);  // nothing that is written is read
         if (apart || __popcll(change) <= 32) {
-            if (begin + t >= end) return;
-            const Piece16 piece = piece_of(it, begin + t);
+            if (begin + __builtin_amdgcn_readfirstlane(t - lane) >= end) return;  // (a wave in which no lane has a piece)
+            const bool mine = begin + t < end;
+            const Piece16 piece = piece_of(it, mine ? begin + t : end - 1);
             auto move = [&](int bytes) {
-                if (__popcll(change) <= 8) move_rows<8, STREAM>(piece.at, piece.batch, bytes, change, source);
-                else if (apart) move_rows<16, STREAM>(piece.at, piece.batch, bytes, change, source);
-                else move_rows<32, STREAM>(piece.at, piece.batch, bytes, change, source);
+                if (__popcll(change) <= 8) move_rows<8, STREAM>(piece.at, piece.batch, bytes, mine, change, source);
+                else if (apart) move_rows<16, STREAM>(piece.at, piece.batch, bytes, mine, change, source);
+                else move_rows<32, STREAM>(piece.at, piece.batch, bytes, mine, change, source);
             };
             if (__all(piece.bytes == 16)) move(16);
             else move(piece.bytes);
