@@ -176,6 +176,8 @@ def check_beams(requests: int, beams: int, end: Optional[int], vocab: int) -> No
     """What ops.beam_select and ops.reorder_rows would refuse in a later step."""
     if not 1 <= beams <= min(64, vocab):
         raise RuntimeError("beam_search: between 1 and 64 beams, not more than there are tokens")
+    if vocab > 1 << 20 or beams * vocab > 1 << 25:
+        raise RuntimeError("beam_search: a vocabulary of at most 2^20 tokens, 2^25 with all beams of a request")
     if requests * beams > 1024:
         raise RuntimeError("beam_search: at most 1024 beams in all")
     if end is not None and not 0 <= end < vocab:
