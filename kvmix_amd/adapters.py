@@ -41,6 +41,17 @@ class AdapterPool:
                 n, k = shapes[t]
                 self._pool[layer, t] = (torch.zeros(count, rank, k, dtype=dtype, device=device), torch.zeros(count, n, rank, dtype=dtype, device=device))
 
+    def check(self, weights: dict) -> None:
+        """Refuses a decoder's weights (decoder.init_weights) that these adapters are not for: other layers, sizes, types or devices."""
+        layers = {layer for layer, _ in self._pool}
+        if len(layers) != len(weights["layers"]):
+            raise RuntimeError(f"the adapters are for {len(layers)} layers, the weights have {len(weights['layers'])}")
+        for (layer, t), (a, b) in self._pool.items():
+            w = weights["layers"][layer][t]
+            if tuple(w.shape) != (b.shape[1], a.shape[2]) or w.dtype != a.dtype or w.device != a.device:
+                raise RuntimeError(f"the adapters' projection {(layer, t)} is [{b.shape[1]}, {a.shape[2]}], {a.dtype}, on {a.device}; the weights' "
+                                   f"is {list(w.shape)}, {w.dtype}, on {w.device}")
+
     def load(self, i: int, weights: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0) -> None:
         """Adapter i becomes {(layer, projection): (a [r, k], b [n, r])}, r up to the pool's rank, times scale; zero elsewhere."""
         if not 0 <= i < self.count:

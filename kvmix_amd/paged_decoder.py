@@ -32,6 +32,8 @@ class PagedDecoder:
 
     def __init__(self, cfg: DecoderConfig, weights: dict, k_bits: Sequence[int], v_bits: Sequence[int], row_pages: int = 256,
                  packed_pages: int = 1024, page_size: int = 64, window: int = 128, adapters: Optional[AdapterPool] = None):
+        if adapters is not None:
+            adapters.check(weights)
         self.cfg, self.w, self.adapters = cfg, weights, adapters
         self._adapter_of: Dict[int, int] = {}  # of the sequences that have one
         self.cache = PagedKVCache(k_bits, v_bits, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, row_pages, packed_pages, page_size, window,
