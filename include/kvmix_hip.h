@@ -706,7 +706,9 @@ int kvmix_add_adapters(const kvmix_adapter_plan_t *plan, const int32_t *list, co
  * equal ones in the order of (w, v), with their beams and tokens, the best first.  A beam that has ended (done) has one continuation,
  * `end` at its own score.  Where nothing can be computed (a score that is not finite; a row with NaN or +inf, or of -inf only), a beam's
  * continuations count as -inf.  With `stay` (count = beams) a request's results are put in the places of beams: the best
- * child of a beam where that beam was, the others where beams have none, best first.  Sums in fp32 over parts of a row, the rest in 64 bits.
+ * child of a beam where that beam was, the others where beams have none, best first.  Sums in fp32 over parts of a row, the rest in 64 bits:
+ * continuations that differ by less than the sums' error, 2^-17 at most, may stand in either order, and how a row is cut into parts goes by the
+ * number of requests.
  *   logits [requests * beams, vocab] fp16, bf16 or fp32, rows row_stride elements apart; vocab up to 2^20, beams times
  *   vocab up to 2^25;  scores [requests * beams];  done NULL or [requests * beams], 0 or 1;  beams and count up to 64, count up to vocab
  *   out_scores, parents (0 .. beams - 1), tokens [requests, count]

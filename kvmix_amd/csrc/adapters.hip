@@ -19,7 +19,7 @@
 // and expand's first reads go out before it sums u.
 // One token with an adapter of rank 8, k = n = 4096: 6.0 us, one launch and the reads of A by each of its 32 blocks.
 // 8168 tokens of 6 adapters of rank 64, k = n = 4096, bf16: 44.6 us, 4.5 TB/s (a copy of as many bytes: 40); 1567 tokens of rank 32 from
-// k = 11008 to n = 4096: 20 us; 64 tokens of 8 adapters of rank 16 to n = 12288: 8.6 us, that is two launches.
+// k = 11008 to n = 4096: 20 us; 64 tokens of 8 adapters of rank 16 to n = 12288: 8.6 us, that is two launches; of 40 adapters 11.4, of 64 11.9.
 // Sums in fp32; y is rounded once.
 #include <algorithm>
 #include <new>
@@ -479,8 +479,9 @@ ExpandPlan expand_plan(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t 
 }
 
 // One launch instead of two: where the tiles are of few tokens, a block finds a CU of its own and has at most 64 KB of A to read (4096 of
-// rank 8).  One to eight tokens, n = 4096: 6.0 us instead of 8.5 launched one after the other, 5.8 instead of 5.4 in a graph; k 2048,
-// rank 16: 4.9 instead of 5.4 there; k 4096, rank 16: 7.1 instead of 5.5; twice as many blocks as CUs: 9 instead of 5.8.
+// rank 8): up to there a call gains more than a graph's node loses.  One token, n = 4096, called one after the other and in a graph: k 2048,
+// rank 16 5.0 instead of 7.4 us, 5.0 instead of 5.6; k 4096, rank 8 5.9 instead of 7.0, 5.8 instead of 5.5; k 4096, rank 16 7.1 instead of 7.3,
+// 7.1 instead of 5.7 (eight tokens 7.7 instead of 7.4).  Twice as many blocks as CUs: 9 instead of 5.8 in a graph.
 bool whole_u(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c)
 {
     const int64_t blocks = (plan->tiles + plan->bare) * ((c->n + 32 * kWaves - 1) / (32 * kWaves));
@@ -497,7 +498,8 @@ bool streams(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c) { retu
 bool streams_x(const kvmix_adapter_plan_t *plan, const kvmix_adapters_t *c) { return plan->tokens > ((1 << 26) / 2) / c->k; }
 
 // Stretches of k: a block for every CU, but no less than four steps.  Twice as many blocks read x no faster, and the sums that expand has to
-// gather are twice as many (expand of 8168 tokens at rank 64: 41.0 and 38.3 us before its rows were read in runs).
+// gather are twice as many: 128, 256 and 512 blocks take 24.9, 21.6 and 24.0 us for 1546 tokens of rank 32 from k = 11008, 54.0, 47.7 and
+// 49.7 for 7972 of rank 64 from 4096.
 constexpr int64_t kStretches = 256;
 
 int64_t splits_of(const kvmix_adapter_plan_t *plan, int64_t rank, int64_t k)

@@ -9,7 +9,7 @@
 // worse than the count-th best beginning.  That block has little to do and waits for everything it does, so it reads all there is at its
 // start (where that is up to eight keys to a thread), sums a beam's parts with a lane to a part, and shares the comparisons of few
 // lists or candidates among all threads: 6 us, where a thread to a beam and to a list took 12 to 17.
-// 64 x 8 beams of 32000 in fp32, a quarter of them ended: 19.1 us, of which 12 to 14 for the 50 MB of rows; 16 x 5 in fp16, 10 of each: 12.4 us;
+// 64 x 8 beams of 32000 in fp32, a quarter of them ended: 19.1 us, of which 12 to 14 for the 50 MB of rows; 16 x 5 in fp16, 10 of each: 12.4 to 14 us;
 // 4 beams: 10.6 us.
 //
 // Order is decided by 64-bit scores made of sums in 32 bits over parts that begin at multiples of eight values whatever the rows'

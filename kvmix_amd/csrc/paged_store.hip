@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) paged_append(AppendArgs a)
 // Bound by memory.  A wave takes one token and as many heads as it has lanes for (eight of 128 channels): its lanes are the pairs of
 // pieces of a head, so that its reads are 2 KB that follow one another.  (Several such turns of a wave, with its part of the tables
 // read once, gained nothing: 79.9 and 77.9 us, 20 and 19.6.)  8 x 1021 tokens of 32 heads, fp32 tables: 69 to 71 us, 410 MB, 5.8 TB/s;
-// rotated with tensors and appended 979.  64 tokens of 32 heads over 8: 4.8 us, a launch.
+// rotated with tensors and appended 979; rounded as tensors are, the same (73.3 and 73.7 us side by side).  64 tokens of 32 heads over 8: 4.8 us, a launch.
 
 template <typename T>
 struct TablePieces {  // eight channels of the first half, eight of the second

@@ -8,7 +8,8 @@
 // where not, up to 32 rows' old values are in registers before the first is written.  Otherwise old values that are still wanted
 // when their place is written are put in the LDS first, each by the thread that will want it; where they are too many for
 // all threads of a block, fewer take a turn.
-// 1.1 GB read and written each way where half of 32 rows stay: 440 us (5.0 TB/s); all 32 moved round, 1.2 GB: 0.9 ms, through the LDS 3.7.
+// 2.2 GB of states in 32 rows: 440 us where half of them stay (1.1 GB read, 1.1 written, 5.0 TB/s), 895 us where all are moved round (2.2 GB each,
+// 4.9 TB/s).  Through the LDS less: 40 rows of 1.4 GB moved round 1.6 ms (1.8 TB/s), 128 of 1.3 GB 4.1 ms.
 #include <algorithm>
 #include <numeric>
 #include <vector>

@@ -552,13 +552,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int = None, d
     scores + log_softmax(logits), the best first, equal ones in the order of (beam, token).  A beam that has ended (done, bool) goes on as
     it is: its one continuation is the token `end` at its own score.  stay=True puts the best child of a beam in that beam's place and
     the others, best first, where beams have no children: then the states of few beams have to be moved (reorder_rows).  Beams whose
-    score is not finite, or whose logits have NaN, +inf or nothing but -inf, go on at -inf, after all others."""
+    score is not finite, or whose logits have NaN, +inf or nothing but -inf, go on at -inf, after all others.  Sums over a row are in fp32: what
+    differs by less than their error, 2^-17 at most, may stand in either order, and not in the same one among other requests."""
     return _host().beam_select(logits, scores, count, done, end, stay)
 
 
 def reorder_rows(tensors, index: torch.Tensor) -> None:
-    """t[:] = t[index] for each of the tensors, in place: index int64 [rows] on the device, any types and strides of tensors [rows,
-    ...] that do not overlap (kvmix_reorder_rows).  Rows that stay are not touched; an index outside of the rows leaves its row as it is."""
+    """t[:] = t[index] for each of the tensors, in place: index int64 [rows] on the device, tensors [rows, ...] of any type, an entry of which
+    is rows of memory in at most two dimensions (what lies together counts as one).  No two may have memory in common; views that
+    lie between one another's rows have none (kvmix_reorder_rows).  Rows that stay are not touched; an index outside of the rows
+    leaves its row as it is."""
     _host().reorder_rows(list(tensors), index)
 
 
