@@ -282,12 +282,33 @@ int check_apart(const kvmix_reorder_t *items, int64_t count, int64_t rows)
         all.push_back({(int64_t)p.base, (int64_t)p.base + (int64_t)extent, &p});
     }
     std::sort(all.begin(), all.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    bool apart = true;
+    for (size_t i = 0; i + 1 < all.size(); i++) apart = apart && all[i].to <= all[i + 1].from;
+    if (apart) return KVMIX_OK;
+
+    std::vector<Layout> l;
+    l.reserve(all.size());
+    for (const Span &span : all) l.push_back(layout_of(*span.item, rows));
+    auto in_common = [&](size_t i, size_t j) {
+        int steps = 1 << 16;
+        return meet(l[i], 0, l[j], 0, l[j].at - l[i].at, steps);
+    };
+    const int64_t stride = l[0].stride[0];
+    if (std::all_of(l.begin(), l.end(), [&](const Layout &a) { return a.stride[0] == stride && a.extent[1] <= stride; })) {
+        // Views of one storage, or of several alike: each is near those alone that begin in its part of the stride.
+        std::sort(l.begin(), l.end(), [&](const Layout &a, const Layout &b) { return a.at % stride < b.at % stride; });
+        for (size_t i = 0; i < l.size(); i++)
+            for (size_t k = 1; k < l.size(); k++) {
+                const size_t j = (i + k) % l.size();
+                const int64_t off = l[j].at % stride - l[i].at % stride;
+                if ((j < i ? off + stride : off) >= l[i].extent[1]) break;
+                if (in_common(i, j)) return KVMIX_ERR_OVERLAP;
+            }
+        return KVMIX_OK;
+    }
     for (size_t i = 0; i < all.size(); i++)
-        for (size_t j = i + 1; j < all.size() && all[j].from < all[i].to; j++) {
-            const Layout a = layout_of(*all[i].item, rows), b = layout_of(*all[j].item, rows);
-            int steps = 1 << 16;
-            if (meet(a, 0, b, 0, b.at - a.at, steps)) return KVMIX_ERR_OVERLAP;
-        }
+        for (size_t j = i + 1; j < all.size() && all[j].from < all[i].to; j++)
+            if (in_common(i, j)) return KVMIX_ERR_OVERLAP;
     return KVMIX_OK;
 }
 

@@ -80,3 +80,23 @@ def test_many_tensors():
     for bad in (item(48 * 65 * 9 * 2 + 48 * 65 * 8 + 48 * 64 + 47, 1, 1 << 20), item(48 * 30 + 20, 48, 1 << 20)):
         assert reorder(9, *items[:40], bad, *items[40:], index=None) == OVERLAP
     assert "overlap" in _lib.strerror(OVERLAP)
+
+
+def test_any_views_of_one_storage(seed=1):
+    """Several of alike strides, some of them in a storage of their own."""
+    rng = random.Random(seed)
+    seen = {APART: 0, OVERLAP: 0}
+    for _ in range(2000):
+        rows, items = rng.randint(2, 5), []
+        inner_stride = rng.choice([4, 7, 16])
+        outer_stride = inner_stride * rng.randint(1, 4) + rng.choice([0, 3])
+        batch = outer_stride * rng.randint(1, 4) + rng.choice([0, 5, 40])
+        for _ in range(rng.randint(2, 6)):
+            p = item(rng.randint(0, batch) + rng.choice([0, 0, 0, 1000, 3 * batch]), rng.randint(1, max(1, inner_stride // 2)), batch, rng.randint(1, max(1, batch // outer_stride)),
+                     outer_stride, rng.randint(1, max(1, outer_stride // inner_stride)), inner_stride)
+            items.append(p)
+        bytes_of = [np.unique(taken(rows, p)) for p in items]
+        want = OVERLAP if sum(b.size for b in bytes_of) > np.unique(np.concatenate(bytes_of)).size else APART
+        assert reorder(rows, *items, index=None) == want, items
+        seen[want] += 1
+    assert min(seen.values()) > 200
