@@ -534,7 +534,8 @@ def paged_attention(q: torch.Tensor, rows: torch.Tensor, packed: torch.Tensor, p
 def adapter_plan(adapters, counts, n_adapters: int, device="cuda"):
     """Which token of a batch has which adapter, for every projection of a step (kvmix_adapter_plan): adapters [sequences], each a
     number below n_adapters, or negative for none; counts [sequences]: the new tokens of each, sequence after sequence.  As paged_plan's it is
-    copied to `device` on the current stream, can be used on any, and cannot be made while a graph is captured."""
+    copied to `device` on the current stream, can be used on any, and cannot be made while a graph is captured; a graph in which it is
+    used needs it as long as the graph is replayed."""
     return _host().adapter_plan(list(adapters), list(counts), n_adapters, _cuda(device))
 
 
